@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libgdnx.so")
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F64 = 2      # gdnx_check_finite only
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _c_int, _c_ll, _vp, _c_float = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_float
 
@@ -79,6 +79,19 @@ SIGNATURES = {
     "gdnx_rls_fwd": (_c_int, [_vp] * 11 + [_c_int] * 7 + [_c_float, _c_int, _c_int, _c_float, _vp]),
     "gdnx_rls_bwd_workspace_bytes": (_c_ll, [_c_int] * 6),
     "gdnx_rls_bwd": (_c_int, [_vp] * 18 + [_c_int] * 7 + [_c_float, _c_int, _c_int, _c_float, _c_int, _vp, _vp]),
+    "gdnx_win_attn_bwd_workspace_bytes": (_c_ll, [_c_int] * 9),
+    "gdnx_win_attn_fwd": (_c_int, [_vp] * 6 + [_c_ll] * 9 + [_c_int] * 8 + [_c_float, _c_int, _vp]),
+    "gdnx_win_attn_bwd": (_c_int, [_vp] * 11 + [_c_ll] * 9 + [_c_int] * 8 + [_c_float, _c_int, _vp]),
+    "gdnx_paged_attn_workspace_bytes": (_c_ll, [_c_int] * 9),
+    "gdnx_paged_attn_step": (_c_int, [_vp] * 10 + [_c_int] * 10 + [_c_float, _c_int, _vp]),
+    "gdnx_pages_workspace_bytes": (_c_ll, [_c_int] * 2),
+    "gdnx_pages_reserve": (_c_int, [_vp] * 7 + [_c_int] * 6 + [_vp]),
+    "gdnx_pages_write": (_c_int, [_vp] * 7 + [_c_int] * 10 + [_vp]),
+    "gdnx_pages_copy": (_c_int, [_vp] * 4 + [_c_int] * 7 + [_vp]),
+    "gdnx_pages_fork": (_c_int, [_vp] * 9 + [_c_int] * 9 + [_vp]),
+    "gdnx_pages_free": (_c_int, [_vp] * 4 + [_c_int] * 4 + [_vp]),
+    "gdnx_pages_trim": (_c_int, [_vp] * 4 + [_c_int] * 7 + [_vp]),
+    "gdnx_pages_compact": (_c_int, [_vp] * 7 + [_c_int] * 8 + [_vp]),
 }
 
 

@@ -1,0 +1,176 @@
+"""Softmax attention for the layers of a hybrid model that are not recurrent.
+
+``window_attention`` is differentiable attention over a sliding window of the
+last tokens and the first few ones (sinks), for training and prompts;
+``paged_attention_step`` serves one token per sequence from a paged key-value
+cache (``gdnx_amd.pages``) under the same visibility rule.  Grouped heads:
+query head h reads key head h // (Hq // Hkv).  The kernels are
+csrc/attn_win.hip and csrc/attn_paged.hip (gdnx_win_attn_*,
+gdnx_paged_attn_step in include/gdnx.h).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ops import _need, empty_result
+
+
+def _window(window, sinks):
+    window, sinks = 0 if window is None else int(window), int(sinks)
+    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+    return min(window, 1 << 30), min(sinks, 1 << 30)
+
+
+def _rows16(t):
+    """t with D contiguous and every other stride a multiple of 16 bytes, as the
+    kernels read it (views of a fused projection are taken as they are)."""
+    unit = 16 // t.element_size()
+    if t.stride(-1) == 1 and all(s % unit == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _check(q, k, v, lengths):
+    _need(q.is_cuda, "gdnx ops need CUDA (HIP) tensors")
+    _need(q.dim() == 4 and k.dim() == 4 and k.shape == v.shape, "q must be [B,Tq,Hq,D], k and v [B,Tk,Hkv,D]")
+    _need(q.dtype == k.dtype == v.dtype, "q, k, v must share dtype")
+    _need(k.device == q.device and v.device == q.device, "inputs must be on one device")
+    B, Tq, Hq, D = q.shape
+    Tk, Hkv = k.shape[1:3]
+    _need(k.shape[0] == B and k.shape[3] == D, "q, k, v must share batch and head dim")
+    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key heads ({Hkv})")
+    if lengths is not None:
+        _need(tuple(lengths.shape) == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous()
+              and lengths.device == q.device, "lengths must be contiguous int32 [B] on q's device")
+    return B, Tq, Tk, Hq, Hkv, D
+
+
+def _forward(q, k, v, window, sinks, scale, lengths, want_lse):
+    lib = _lib.load()
+    B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
+    code = _lib.dtype_code(q.dtype)
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    y = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if want_lse else None
+    with torch.cuda.device(q.device):
+        rc = lib.gdnx_win_attn_fwd(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(lengths), _lib.ptr(y),
+                                   _lib.ptr(lse), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq,
+                                   Hkv, D, window, sinks, scale, code, _lib.stream_of(q))
+    _lib.check(rc, "gdnx_win_attn_fwd")
+    return q, k, v, y, lse
+
+
+class WindowAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale, lengths):
+        q, k, v, y, lse = _forward(q, k, v, window, sinks, scale, lengths, True)
+        ctx.save_for_backward(q, k, v, lengths, y, lse)
+        ctx.args = (window, sinks, scale)
+        ctx.mark_non_differentiable(lse)
+        return y, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _):
+        q, k, v, lengths, y, lse = ctx.saved_tensors
+        window, sinks, scale = ctx.args
+        lib = _lib.load()
+        B, Tq, Hq, D = q.shape
+        Tk, Hkv = k.shape[1:3]
+        code = _lib.dtype_code(q.dtype)
+        dy = _rows16(dy.to(q.dtype).contiguous())
+        dq = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty(B, Tk, Hkv, D, dtype=q.dtype, device=q.device) for _ in range(2))
+        nws = lib.gdnx_win_attn_bwd_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
+        _need(nws >= 0, "invalid sizes")
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+        with torch.cuda.device(q.device):
+            rc = lib.gdnx_win_attn_bwd(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(lengths), _lib.ptr(y),
+                                       _lib.ptr(lse), _lib.ptr(dy), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
+                                       _lib.ptr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk,
+                                       Hq, Hkv, D, window, sinks, scale, code, _lib.stream_of(q))
+        _lib.check(rc, "gdnx_win_attn_bwd")
+        return dq, dk, dv, None, None, None, None
+
+
+def window_attention(q, k, v, window=None, sinks=0, *, scale=None, lengths=None, return_lse=False):
+    """Attention of q [B,Tq,Hq,D] over k, v [B,Tk,Hkv,D] (bfloat16 or float32,
+    D 64 or 128, any strides), differentiable in q, k and v.
+
+    Query i stands at position p = i + Tk - Tq and sees key j if j <= p and
+    p - j < window or j < sinks (window None: every earlier key).  lengths
+    (int32 [B]): tokens at or beyond a row's length are padding, whatever they
+    hold; their outputs and gradients are zero, as are those of queries before
+    position 0.  scale defaults to 1/sqrt(D).  Returns y [B,Tq,Hq,D], with
+    return_lse also the log-sum-exp of each query's scores [B,Hq,Tq] (float32,
+    -inf where nothing is seen, not differentiable)."""
+    window, sinks = _window(window, sinks)
+    B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
+    if B == 0 or Tq == 0 or Tk == 0:
+        y = empty_result((B, Tq, Hq, D), q.dtype, q.device, q, k, v)
+        return (y, torch.full((B, Hq, Tq), float("-inf"), device=q.device)) if return_lse else y
+    scale = D ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        y, lse = WindowAttentionFunction.apply(q, k, v, window, sinks, scale, lengths)
+    else:
+        y, lse = _forward(q, k, v, window, sinks, scale, lengths, return_lse)[3:]
+    return (y, lse) if return_lse else y
+
+
+def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=None, window=None, sinks=0, scale=None,
+                         out=None):
+    """One served token for every row: q [NS,Hq,D] over the row's cached tokens.
+
+    k_pages, v_pages [n_pages,Hkv,page,D], table [rows,width] and lengths
+    [rows] (int32) as ``gdnx_amd.pages`` keeps them; row s is table row
+    slots[s] (int32 [NS]; outside the table: an empty row, y = 0), or s.  The
+    token stands at position length - 1.  k, v [NS,Hkv,D] are its key and
+    value, which the call also writes to their page; None where they are there
+    already.  window, sinks and scale as in ``window_attention``.  Returns y
+    [NS,Hq,D] (or ``out``)."""
+    lib = _lib.load()
+    window, sinks = _window(window, sinks)
+    _need(q.is_cuda and q.dim() == 3, "q must be a CUDA (HIP) tensor [NS,Hq,D]")
+    NS, Hq, D = q.shape
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == D,
+          "k_pages and v_pages must share shape [n_pages,Hkv,page,D]")
+    n_pages, Hkv, page, _ = k_pages.shape
+    _need(Hkv > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key heads ({Hkv})")
+    _need(table.dim() == 2 and tuple(lengths.shape) == (table.shape[0],), "table must be [rows,width], lengths [rows]")
+    rows, width = table.shape
+    _need((k is None) == (v is None), "k and v must be given together")
+    new = () if k is None else (k, v)
+    for t in new:
+        _need(tuple(t.shape) == (NS, Hkv, D), "k and v must be [NS,Hkv,D]")
+    ints = (table, lengths) if slots is None else (table, lengths, slots)
+    if slots is None:
+        _need(NS <= rows, f"{NS} rows for a table of {rows}")
+    else:
+        _need(tuple(slots.shape) == (NS,), "slots must be [NS]")
+    for t in ints:
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == q.device,
+              "table, lengths and slots must be contiguous int32 on q's device")
+    for t in (k_pages, v_pages, *new):
+        _need(t.dtype == q.dtype and t.device == q.device, "q, k, v and the pages must share dtype and device")
+    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), "k_pages and v_pages must be contiguous")
+    code = _lib.dtype_code(q.dtype)
+    if out is None:
+        out = torch.empty(NS, Hq, D, dtype=q.dtype, device=q.device)
+    else:
+        _need(tuple(out.shape) == (NS, Hq, D) and out.dtype == q.dtype and out.is_contiguous()
+              and out.device == q.device, "out must be contiguous [NS,Hq,D] of q's dtype")
+    if NS == 0:
+        return out
+    q = _rows16(q.contiguous())
+    if new:
+        k, v = _rows16(k.contiguous()), _rows16(v.contiguous())
+    nws = lib.gdnx_paged_attn_workspace_bytes(NS, width, page, Hq, Hkv, D, window, sinks, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
+    with torch.cuda.device(q.device):
+        rc = lib.gdnx_paged_attn_step(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(k_pages), _lib.ptr(v_pages),
+                                      _lib.ptr(table), _lib.ptr(lengths), _lib.ptr(slots), _lib.ptr(out), _lib.ptr(ws),
+                                      NS, rows, width, n_pages, page, Hq, Hkv, D, window, sinks,
+                                      D ** -0.5 if scale is None else float(scale), code, _lib.stream_of(q))
+    _lib.check(rc, "gdnx_paged_attn_step")
+    return out

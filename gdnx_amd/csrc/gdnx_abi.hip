@@ -1120,3 +1120,276 @@ extern "C" int gdnx_rls_bwd(const float* q, const float* K, const float* V, cons
                             {d_state0, (size_t)B * H * value_dim * key_dim, GDNX_DTYPE_F32}};
   return finite_outputs(outs, 8, (hipStream_t)stream);
 }
+
+// ---- attention layers of a hybrid model and their page cache ----
+
+namespace gdnx {
+
+// (every grid below has at most 2^24 - 1 workgroups of 256 threads)
+constexpr long long kMaxGroups = (1LL << 24) - 1;
+
+static int check_attn_sizes(int Hq, int Hkv, int D, int window, int sinks, int dtype) {
+  if (dtype != GDNX_DTYPE_F32 && dtype != GDNX_DTYPE_BF16)
+    return set_error(GDNX_ERR_ARG, "dtype %d is not GDNX_DTYPE_F32/BF16", dtype);
+  if (D != 64 && D != 128) return set_error(GDNX_ERR_SHAPE, "head_dim %d unsupported (64 or 128)", D);
+  if (Hq < 1 || Hkv < 1 || Hq > 65536 || Hq % Hkv != 0)
+    return set_error(GDNX_ERR_SHAPE, "query heads %d are no multiple of %d key heads", Hq, Hkv);
+  if (window < 0 || sinks < 0) return set_error(GDNX_ERR_SHAPE, "window %d or sinks %d is negative", window, sinks);
+  return GDNX_OK;
+}
+
+static int check_win(int B, int Tq, int Tk, int Hq, int Hkv, int D, int window, int sinks, int dtype) {
+  const int rc = check_attn_sizes(Hq, Hkv, D, window, sinks, dtype);
+  if (rc) return rc;
+  if (B < 1 || Tq < 1 || Tk < 1 || Tq >= kNoWindow || Tk >= kNoWindow)
+    return set_error(GDNX_ERR_SHAPE, "bad sizes B=%d Tq=%d Tk=%d", B, Tq, Tk);
+  if (!prod_le(kMaxGroups, {B, Hq, ((Tq > Tk ? Tq : Tk) + 63) / 64}))
+    return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
+  return GDNX_OK;
+}
+
+static int check_strides(const long long* st, int dtype, const char* name) {
+  const int unit = dtype == GDNX_DTYPE_BF16 ? 8 : 4;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] % unit != 0 || st[i] > (1LL << 40))
+      return set_error(GDNX_ERR_SHAPE, "%s: strides must be non-negative multiples of 16 bytes", name);
+  return GDNX_OK;
+}
+
+static long long win_bwd_delta_bytes(int B, int Tq, int Hq) { return ((long long)B * Tq * Hq * 4 + 255) / 256 * 256; }
+
+static bool page_ok(int page) { return page >= 1 && page <= (1 << 20) && (page & (page - 1)) == 0; }
+
+static int check_pool(int rows, int width, int n_pages, int page) {
+  if (!page_ok(page)) return set_error(GDNX_ERR_SHAPE, "page %d is no power of two up to 2^20", page);
+  if (rows < 1 || width < 1 || n_pages < 1 || n_pages > (1 << 30) || !prod_le((1LL << 31) - 1, {rows, width}) ||
+      !prod_le(kNoWindow - 1, {width, page}))
+    return set_error(GDNX_ERR_SHAPE, "bad sizes rows=%d width=%d n_pages=%d", rows, width, n_pages);
+  return GDNX_OK;
+}
+
+static int check_pool_data(const void* k, const void* v, int layers, int Hkv, int page, int D, int dtype, PagesArgs& a) {
+  int rc = check_attn_sizes(Hkv, Hkv, D, 0, 0, dtype);
+  if (rc) return rc;
+  if (layers < 1 || layers > 65536) return set_error(GDNX_ERR_SHAPE, "bad number of layers %d", layers);
+  if (!k || !v) return set_error(GDNX_ERR_ARG, "k_pages and v_pages must be non-null");
+  if (!aligned16(k) || !aligned16(v)) return set_error(GDNX_ERR_ARG, "k_pages and v_pages must be 16-byte aligned");
+  a.layers = layers;
+  a.Hkv = Hkv;
+  a.row_bytes = D * (dtype == GDNX_DTYPE_BF16 ? 2 : 4);
+  a.page_bytes = (long long)Hkv * page * a.row_bytes;
+  if (!prod_le(1LL << 50, {layers, a.n_pages, a.page_bytes})) return set_error(GDNX_ERR_SHAPE, "page pool too large");
+  return GDNX_OK;
+}
+
+}  // namespace gdnx
+
+extern "C" long long gdnx_win_attn_bwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
+                                                       int sinks, int dtype) {
+  if (check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype)) return -1;
+  return win_bwd_delta_bytes(B, Tq, Hq);
+}
+
+extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, float* lse,
+                                 long long q_b, long long q_t, long long q_h, long long k_b, long long k_t,
+                                 long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk,
+                                 int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
+                                 void* stream) {
+  g_err[0] = 0;
+  int rc = check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype);
+  if (rc) return rc;
+  if (!q || !k || !v || !y) return set_error(GDNX_ERR_ARG, "q, k, v, y must be non-null");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(y))
+    return set_error(GDNX_ERR_ARG, "q, k, v, y must be 16-byte aligned");
+  WinAttnArgs a{q, k, v, lengths, y, lse, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv,
+                head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype};
+  if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
+      (rc = check_strides(a.vs, dtype, "v")))
+    return rc;
+  if ((rc = win_attn_fwd_dispatch(a, (hipStream_t)stream))) return rc;
+  const FiniteBuf outs[] = {{y, (size_t)B * Tq * Hq * head_dim, dtype}};
+  return finite_outputs(outs, 1, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, const int* lengths, const void* y,
+                                 const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                                 long long q_b, long long q_t, long long q_h, long long k_b, long long k_t,
+                                 long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk,
+                                 int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
+                                 void* stream) {
+  g_err[0] = 0;
+  int rc = check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype);
+  if (rc) return rc;
+  if (!q || !k || !v || !y || !lse || !dy || !dq || !dk || !dv)
+    return set_error(GDNX_ERR_ARG, "all pointers but lengths must be non-null");
+  if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  for (const void* p : {q, k, v, y, dy, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
+    if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
+  WinAttnBwdArgs a{q, k, v, lengths, y, lse, dy, dq, dk, dv, (float*)workspace, {q_b, q_t, q_h}, {k_b, k_t, k_h},
+                   {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim,
+                   window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype};
+  if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
+      (rc = check_strides(a.vs, dtype, "v")))
+    return rc;
+  if ((rc = win_attn_bwd_dispatch(a, (hipStream_t)stream))) return rc;
+  const size_t nq = (size_t)B * Tq * Hq * head_dim, nk = (size_t)B * Tk * Hkv * head_dim;
+  const FiniteBuf outs[] = {{dq, nq, dtype}, {dk, nk, dtype}, {dv, nk, dtype}};
+  return finite_outputs(outs, 3, (hipStream_t)stream);
+}
+
+static long long paged_keys(int width, int page, int window, int sinks) {
+  const long long all = (long long)width * page;
+  return window > 0 && (long long)window + sinks < all ? (long long)window + sinks : all;
+}
+
+extern "C" long long gdnx_paged_attn_workspace_bytes(int NS, int width, int page, int Hq, int Hkv, int head_dim,
+                                                     int window, int sinks, int dtype) {
+  if (check_attn_sizes(Hq, Hkv, head_dim, window, sinks, dtype) || NS < 1 || NS > (1 << 20) || width < 1 ||
+      !page_ok(page) || !prod_le(kNoWindow - 1, {width, page}))
+    return -1;
+  const long long sp = paged_attn_spans(NS, Hq, Hkv, paged_keys(width, page, window, sinks), dtype);
+  return sp > 1 ? (long long)NS * Hq * sp * (head_dim + 2) * 4 : 0;
+}
+
+extern "C" int gdnx_paged_attn_step(const void* q, const void* k, const void* v, void* k_pages, void* v_pages,
+                                    const int* table, const int* lengths, const int* slots, void* y, void* workspace,
+                                    int NS, int rows, int width, int n_pages, int page, int Hq, int Hkv, int head_dim,
+                                    int window, int sinks, float scale, int dtype, void* stream) {
+  g_err[0] = 0;
+  int rc = check_attn_sizes(Hq, Hkv, head_dim, window, sinks, dtype);
+  if (rc) return rc;
+  if ((rc = check_pool(rows, width, n_pages, page))) return rc;
+  if (NS < 1 || NS > (1 << 20) || (!slots && NS > rows))
+    return set_error(GDNX_ERR_SHAPE, "bad number of rows %d (table rows %d)", NS, rows);
+  if (!q || !k_pages || !v_pages || !table || !lengths || !y)
+    return set_error(GDNX_ERR_ARG, "all pointers but k, v, slots and workspace must be non-null");
+  if (!k != !v) return set_error(GDNX_ERR_ARG, "k and v must be given together");
+  for (const void* p : {q, k, v, (const void*)k_pages, (const void*)v_pages, (const void*)y, (const void*)workspace})
+    if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
+  const int sp = paged_attn_spans(NS, Hq, Hkv, paged_keys(width, page, window, sinks), dtype);
+  if (sp > 1 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  if (!prod_le(kMaxGroups, {NS, Hkv, (Hq / Hkv + 15) / 16, sp}))
+    return set_error(GDNX_ERR_SHAPE, "too many rows and heads in one call");
+  int lg = 0;
+  while ((1 << lg) < page) ++lg;
+  PagedAttnArgs a{q, k, v, k_pages, v_pages, table, lengths, slots, y, (float*)workspace, NS, rows, width, n_pages, lg,
+                  Hq, Hkv, head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype, sp};
+  if ((rc = paged_attn_dispatch(a, (hipStream_t)stream))) return rc;
+  const FiniteBuf outs[] = {{y, (size_t)NS * Hq * head_dim, dtype}};
+  return finite_outputs(outs, 1, (hipStream_t)stream);
+}
+
+extern "C" long long gdnx_pages_workspace_bytes(int n, int n_pages) {
+  if (n < 0 || n > (1 << 24) || n_pages < 1 || n_pages > (1 << 30)) return -1;
+  return 4 * (5LL * n + 2LL * n_pages + 8);
+}
+
+extern "C" int gdnx_pages_reserve(int* table, int* lengths, int* refs, const int* slots, int* start, int* status,
+                                  void* workspace, int n, int n_new, int rows, int width, int n_pages, int page,
+                                  void* stream) {
+  g_err[0] = 0;
+  int rc = check_pool(rows, width, n_pages, page);
+  if (rc) return rc;
+  if (n < 1 || n > (1 << 24) || n_new < 0 || n_new >= kNoWindow || !prod_le((1LL << 31) - 1, {n, width}))
+    return set_error(GDNX_ERR_SHAPE, "bad sizes n=%d n_new=%d", n, n_new);
+  if (!table || !lengths || !refs || !slots || !start || !status)
+    return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  PagesArgs a{};
+  a.table = table; a.lengths = lengths; a.refs = refs; a.slots = slots; a.start = start; a.status = status;
+  a.n = n; a.n_new = n_new; a.rows = rows; a.width = width; a.n_pages = n_pages; a.page = page;
+  return pages_reserve_dispatch(a, (int*)workspace, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_pages_write(const void* k_new, const void* v_new, void* k_pages, void* v_pages, const int* table,
+                                const int* slots, const int* start, int layers, int n, int n_new, int rows, int width,
+                                int n_pages, int page, int Hkv, int head_dim, int dtype, void* stream) {
+  g_err[0] = 0;
+  PagesArgs a{};
+  a.n_pages = n_pages;
+  int rc = check_pool(rows, width, n_pages, page);
+  if (rc) return rc;
+  if ((rc = check_pool_data(k_pages, v_pages, layers, Hkv, page, head_dim, dtype, a))) return rc;
+  if (n < 1 || n > (1 << 24) || n_new < 1 || n_new >= kNoWindow || !prod_le(1LL << 50, {layers, n, n_new, Hkv, a.row_bytes}))
+    return set_error(GDNX_ERR_SHAPE, "bad sizes n=%d n_new=%d", n, n_new);
+  if (!k_new || !v_new || !table || !slots || !start) return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  if (!aligned16(k_new) || !aligned16(v_new)) return set_error(GDNX_ERR_ARG, "k_new and v_new must be 16-byte aligned");
+  a.k_pages = k_pages; a.v_pages = v_pages; a.k_new = k_new; a.v_new = v_new;
+  a.table = const_cast<int*>(table); a.slots = slots; a.start = const_cast<int*>(start);
+  a.n = n; a.n_new = n_new; a.rows = rows; a.width = width; a.page = page;
+  return pages_write_dispatch(a, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_pages_copy(void* k_pages, void* v_pages, const int* src, const int* dst, int layers, int n,
+                               int n_pages, int page, int Hkv, int head_dim, int dtype, void* stream) {
+  g_err[0] = 0;
+  PagesArgs a{};
+  a.n_pages = n_pages;
+  int rc = check_pool(1, 1, n_pages, page);
+  if (rc) return rc;
+  if ((rc = check_pool_data(k_pages, v_pages, layers, Hkv, page, head_dim, dtype, a))) return rc;
+  if (n < 1 || n > (1 << 24)) return set_error(GDNX_ERR_SHAPE, "bad number of pages %d", n);
+  if (!src || !dst) return set_error(GDNX_ERR_ARG, "src and dst must be non-null");
+  a.k_pages = k_pages; a.v_pages = v_pages; a.n = n; a.page = page;
+  return pages_copy_dispatch(a, src, dst, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_pages_fork(void* k_pages, void* v_pages, int* table, int* lengths, int* refs, const int* parents,
+                               const int* children, int* status, void* workspace, int layers, int n, int rows, int width,
+                               int n_pages, int page, int Hkv, int head_dim, int dtype, void* stream) {
+  g_err[0] = 0;
+  PagesArgs a{};
+  a.n_pages = n_pages;
+  int rc = check_pool(rows, width, n_pages, page);
+  if (rc) return rc;
+  if ((rc = check_pool_data(k_pages, v_pages, layers, Hkv, page, head_dim, dtype, a))) return rc;
+  if (n < 1 || n > (1 << 24)) return set_error(GDNX_ERR_SHAPE, "bad number of pairs %d", n);
+  if (!table || !lengths || !refs || !parents || !children || !status)
+    return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  a.k_pages = k_pages; a.v_pages = v_pages; a.table = table; a.lengths = lengths; a.refs = refs;
+  a.slots = parents; a.start = const_cast<int*>(children); a.status = status;
+  a.n = n; a.rows = rows; a.width = width; a.page = page;
+  return pages_fork_dispatch(a, (int*)workspace, (hipStream_t)stream);
+}
+
+static int pages_free_common(int* table, int* lengths, int* refs, const int* slots, int n, int rows, int width,
+                             int n_pages, int page, int window, int sinks, int trim, void* stream) {
+  g_err[0] = 0;
+  const int rc = check_pool(rows, width, n_pages, page);
+  if (rc) return rc;
+  if (n < 1 || n > (1 << 23)) return set_error(GDNX_ERR_SHAPE, "bad number of rows %d", n);
+  if (trim && (window < 1 || sinks < 0 || sinks >= kNoWindow))
+    return set_error(GDNX_ERR_SHAPE, "bad window %d or sinks %d", window, sinks);
+  if (!table || !lengths || !refs || !slots) return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  PagesArgs a{};
+  a.table = table; a.lengths = lengths; a.refs = refs; a.slots = slots; a.n = n; a.rows = rows; a.width = width;
+  a.n_pages = n_pages; a.page = page; a.window = window; a.sinks = sinks; a.trim = trim;
+  return pages_free_dispatch(a, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_pages_free(int* table, int* lengths, int* refs, const int* slots, int n, int rows, int width,
+                               int n_pages, void* stream) {
+  return pages_free_common(table, lengths, refs, slots, n, rows, width, n_pages, 1, 1, 0, 0, stream);
+}
+
+extern "C" int gdnx_pages_trim(int* table, int* lengths, int* refs, const int* slots, int window, int sinks, int n,
+                               int rows, int width, int n_pages, int page, void* stream) {
+  return pages_free_common(table, lengths, refs, slots, n, rows, width, n_pages, page, window, sinks, 1, stream);
+}
+
+extern "C" int gdnx_pages_compact(void* k_pages, void* v_pages, const int* table, const int* refs, int* table_out,
+                                  int* refs_out, void* workspace, int layers, int rows, int width, int n_pages, int page,
+                                  int Hkv, int head_dim, int dtype, void* stream) {
+  g_err[0] = 0;
+  PagesArgs a{};
+  a.n_pages = n_pages;
+  int rc = check_pool(rows, width, n_pages, page);
+  if (rc) return rc;
+  if ((rc = check_pool_data(k_pages, v_pages, layers, Hkv, page, head_dim, dtype, a))) return rc;
+  if (!table || !refs || !table_out || !refs_out) return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  a.k_pages = k_pages; a.v_pages = v_pages; a.table = const_cast<int*>(table); a.refs = const_cast<int*>(refs);
+  a.table_out = table_out; a.refs_out = refs_out; a.rows = rows; a.width = width; a.page = page;
+  return pages_compact_dispatch(a, (int*)workspace, (hipStream_t)stream);
+}

@@ -446,4 +446,82 @@ size_t chan_fwd_workspace_bytes(int nchains, int T, int D);
 int delta_chunk_size(int D, int dtype);
 int delta_train_chunk_size(int D, int dtype);
 
+// Attention with a sliding window and sinks.  Strides (batch, token, head) in
+// elements; y, dy and the gradients are contiguous, lse and delta [B,Hq,Tq].
+constexpr int kNoWindow = 1 << 30;      // every earlier key (lengths stay below it)
+struct WinAttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int* lengths;   // [B] valid tokens of a row, or null
+  void* y;
+  float* lse;
+  long long qs[3], ks[3], vs[3];
+  int B, Tq, Tk, Hq, Hkv, D, window, sinks;
+  float scale;
+  int dtype;
+};
+struct WinAttnBwdArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int* lengths;
+  const void* y;
+  const float* lse;
+  const void* dy;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* delta;
+  long long qs[3], ks[3], vs[3];
+  int B, Tq, Tk, Hq, Hkv, D, window, sinks;
+  float scale;
+  int dtype;
+};
+int win_attn_fwd_dispatch(const WinAttnArgs& a, hipStream_t stream);
+int win_attn_bwd_dispatch(const WinAttnBwdArgs& a, hipStream_t stream);
+
+// One new token over a paged key-value cache.
+struct PagedAttnArgs {
+  const void* q;        // [NS,Hq,D]
+  const void* k;        // [NS,Hkv,D] the new token, or null (in its page already)
+  const void* v;
+  void* k_pages;        // [n_pages,Hkv,page,D]
+  void* v_pages;
+  const int* table;     // [rows,width]
+  const int* lengths;   // [rows]
+  const int* slots;     // [NS] table row of each row, or null
+  void* y;
+  float* part;          // [NS*Hq][spans][D] outputs, then [NS*Hq][spans][2] maximum and sum
+  int NS, rows, width, n_pages, page_log, Hq, Hkv, D, window, sinks;
+  float scale;
+  int dtype, spans;
+};
+int paged_attn_spans(int NS, int Hq, int Hkv, long long keys, int dtype);
+int paged_attn_dispatch(const PagedAttnArgs& a, hipStream_t stream);
+
+// The page pool's operations.
+struct PagesArgs {
+  void* k_pages;        // [layers,n_pages,Hkv,page,D]
+  void* v_pages;
+  const void* k_new;    // [layers,n,n_new,Hkv,D]
+  const void* v_new;
+  int* table;
+  int* lengths;
+  int* refs;            // [n_pages]
+  int* table_out;
+  int* refs_out;
+  const int* slots;     // [n]
+  int* start;           // [n] (fork: the children)
+  int* status;          // [2]
+  long long page_bytes;
+  int row_bytes, layers, n, n_new, rows, width, n_pages, page, Hkv, window, sinks, trim;
+};
+int pages_reserve_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
+int pages_fork_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
+int pages_copy_dispatch(const PagesArgs& a, const int* src, const int* dst, hipStream_t stream);
+int pages_compact_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
+int pages_free_dispatch(const PagesArgs& a, hipStream_t stream);
+int pages_write_dispatch(const PagesArgs& a, hipStream_t stream);
+
 }  // namespace gdnx

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define GDNX_ABI_VERSION 12
+#define GDNX_ABI_VERSION 13
 
 enum { GDNX_DTYPE_F32 = 0, GDNX_DTYPE_BF16 = 1, GDNX_DTYPE_F64 = 2 /* gdnx_check_finite only */ };
 
@@ -598,6 +598,107 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
                  float* da, float* d_out_mix_seq, float* d_state0, int B, int T, int H, int R,
                  int R_out, int key_dim, int value_dim, float eps, int compact_P, int compact_R,
                  float slow_decay, int straight_through, void* workspace, void* stream);
+
+/* ---- attention layers of a hybrid model, and the pages they are served from ----
+ *
+ * Attention with a sliding window and sinks.  q [B,Tq,Hq,D], k and v
+ * [B,Tk,Hkv,D] in the io dtype with any element strides (batch, token, head)
+ * that are multiples of 16 bytes, D contiguous; Hq a multiple of Hkv, query
+ * head h reading key head h / (Hq / Hkv); D = 64 or 128.  Query i stands at
+ * position p = i + Tk - Tq and sees key j if
+ *     j <= p,  p < lengths[b],  and  p - j < window or j < sinks
+ * (lengths null: Tk; window 0: every earlier key).  A query that sees
+ * nothing gives y = 0, lse = -infinity and no gradient.  Keys at or beyond
+ * lengths[b] are never read.
+ *   y   [B,Tq,Hq,D] io dtype, contiguous: softmax(scale q.k) v
+ *   lse [B,Hq,Tq] float32 (may be null): log of the softmax's denominator */
+int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, float* lse,
+                      long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
+                      long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
+                      int head_dim, int window, int sinks, float scale, int dtype, void* stream);
+
+/* Its gradients from dy [B,Tq,Hq,D] (contiguous) and the forward's y and lse:
+ * dq, dk, dv contiguous in the io dtype, dk and dv summed over a key head's
+ * query heads in float32.  workspace: gdnx_win_attn_bwd_workspace_bytes (-1 if
+ * the sizes are invalid). */
+long long gdnx_win_attn_bwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
+                                            int sinks, int dtype);
+int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, const int* lengths, const void* y,
+                      const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                      long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
+                      long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
+                      int head_dim, int window, int sinks, float scale, int dtype, void* stream);
+
+/* One served token over a paged key-value cache.  Row s (0 <= s < NS) is table
+ * row r = slots[s] (slots null: s; outside [0, rows): an empty row, y = 0);
+ * its token stands at position lengths[r] - 1 and sees the last `window` tokens
+ * (0: all) and the first `sinks` ones.  Token j lies in page
+ * table[r][j / page], place j % page; page is a power of two.
+ *   q, y [NS,Hq,D];  k, v [NS,Hkv,D] the new token's key and value, written to
+ *   their page by the call, or both null where they are there already;
+ *   k_pages, v_pages [n_pages,Hkv,page,D];  table [rows,width] int32, an entry
+ *   outside [0, n_pages) meaning that the row has no such page: its tokens are
+ *   not seen;  lengths [rows] int32.
+ * workspace: gdnx_paged_attn_workspace_bytes bytes (-1 if the sizes are
+ * invalid; null where that is 0).  Two rows of a call must not share a slot
+ * when k and v are given. */
+long long gdnx_paged_attn_workspace_bytes(int NS, int width, int page, int Hq, int Hkv, int head_dim, int window,
+                                          int sinks, int dtype);
+int gdnx_paged_attn_step(const void* q, const void* k, const void* v, void* k_pages, void* v_pages,
+                         const int* table, const int* lengths, const int* slots, void* y, void* workspace, int NS,
+                         int rows, int width, int n_pages, int page, int Hq, int Hkv, int head_dim, int window,
+                         int sinks, float scale, int dtype, void* stream);
+
+/* The page pool: k_pages, v_pages [layers,n_pages,Hkv,page,D], one table
+ * [rows,width], lengths [rows] and reference counts refs [n_pages] (int32, 0:
+ * free) for all layers.  Free pages are taken lowest index first, in the
+ * order of the call's rows.  slots, start, parents, children are int32 of n;
+ * a slot outside [0, rows) is an empty row.  No slot may be named twice in a
+ * call (free and trim: it may).  status [2] int32 is written only by a
+ * reserve or fork that could not be served and then changed nothing else:
+ * the pages that were missing, and the rows whose table row is too short.
+ * workspace: gdnx_pages_workspace_bytes(n, n_pages). */
+long long gdnx_pages_workspace_bytes(int n, int n_pages);
+
+/* Every row of slots gets the pages of its next n_new tokens and is that much
+ * longer; start gets the old lengths (-1: an empty row, or nothing was done). */
+int gdnx_pages_reserve(int* table, int* lengths, int* refs, const int* slots, int* start, int* status,
+                       void* workspace, int n, int n_new, int rows, int width, int n_pages, int page, void* stream);
+
+/* Keys and values k_new, v_new [layers,n,n_new,Hkv,D] to the positions
+ * start[i] .. start[i] + n_new - 1 of table row slots[i] (start < 0: none). */
+int gdnx_pages_write(const void* k_new, const void* v_new, void* k_pages, void* v_pages, const int* table,
+                     const int* slots, const int* start, int layers, int n, int n_new, int rows, int width,
+                     int n_pages, int page, int Hkv, int head_dim, int dtype, void* stream);
+
+/* Page src[i] onto page dst[i] in every layer (either outside [0, n_pages):
+ * nothing).  No page may be both a source and a destination. */
+int gdnx_pages_copy(void* k_pages, void* v_pages, const int* src, const int* dst, int layers, int n, int n_pages,
+                    int page, int Hkv, int head_dim, int dtype, void* stream);
+
+/* Row children[i], which must be empty, becomes a copy of row parents[i]: the
+ * full pages are shared (a reference more each), a started last page is
+ * copied to a free one.  A pair whose child is not empty, or whose rows do not
+ * exist, is left out. */
+int gdnx_pages_fork(void* k_pages, void* v_pages, int* table, int* lengths, int* refs, const int* parents,
+                    const int* children, int* status, void* workspace, int layers, int n, int rows, int width,
+                    int n_pages, int page, int Hkv, int head_dim, int dtype, void* stream);
+
+/* The rows' references are given back and the rows are empty. */
+int gdnx_pages_free(int* table, int* lengths, int* refs, const int* slots, int n, int rows, int width, int n_pages,
+                    void* stream);
+
+/* The rows give back the pages that hold no sink and lie wholly before the
+ * last `window` tokens; the rows keep their lengths. */
+int gdnx_pages_trim(int* table, int* lengths, int* refs, const int* slots, int window, int sinks, int n, int rows,
+                    int width, int n_pages, int page, void* stream);
+
+/* The used pages at or beyond the number of used pages move, in order, into
+ * the free pages below it, so that the pages in use are the pool's first;
+ * table_out and refs_out (which may be table and refs) follow. */
+int gdnx_pages_compact(void* k_pages, void* v_pages, const int* table, const int* refs, int* table_out,
+                       int* refs_out, void* workspace, int layers, int rows, int width, int n_pages, int page,
+                       int Hkv, int head_dim, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
