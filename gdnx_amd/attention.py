@@ -26,7 +26,8 @@ def _rows16(t):
     """t with D contiguous and every other stride a multiple of 16 bytes, as the
     kernels read it (views of a fused projection are taken as they are)."""
     unit = 16 // t.element_size()
-    if t.stride(-1) == 1 and all(s % unit == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
+    if (t.stride(-1) == 1 and all(s % unit == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+            and (t.dim() < 4 or t.stride(1) <= 1 << 24)):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
@@ -53,9 +54,11 @@ def _forward(q, k, v, window, sinks, scale, lengths, want_lse):
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     y = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if want_lse else None
+    nws = lib.gdnx_win_attn_fwd_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
     with torch.cuda.device(q.device):
         rc = lib.gdnx_win_attn_fwd(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(lengths), _lib.ptr(y),
-                                   _lib.ptr(lse), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq,
+                                   _lib.ptr(lse), _lib.ptr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq,
                                    Hkv, D, window, sinks, scale, code, _lib.stream_of(q))
     _lib.check(rc, "gdnx_win_attn_fwd")
     return q, k, v, y, lse

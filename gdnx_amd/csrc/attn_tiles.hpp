@@ -1,0 +1,138 @@
+// Tiles in LDS and 32 x 32 x 16 matrix operands of the bf16 attention kernels.
+//
+// v_mfma_f32_32x32x16_bf16, lane l = 32 h + n (checked on gfx950):
+//   A: lane supplies A[m = n][k in set(h)], B: B[k in set(h)][n], 8 values;
+//   D: element e of the lane is D[8 (e / 4) + 4 h + e % 4][n].
+// The k set of a lane is the same permutation for A and B.  Operands whose k
+// runs along a row take 8 contiguous values (8 h + i); those contracted over
+// accumulator rows take the rows 16 c + 4 h + {0..3} and + 8, as the
+// accumulators hold them, read transposed from row-major tiles
+// (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16 columns, a lane gets a
+// column of 4).
+//
+// A tile row is D values; its 16-byte units are permuted by an xor with the
+// row's bits, so that both reads are free of bank conflicts: 16 rows of one
+// unit fall into different units, and 4 rows of 4 units into different
+// quarters.
+#pragma once
+#include "attn_common.hpp"
+
+namespace gdnx {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ void mma32(f32x16& acc, const bf16x8& a, const bf16x8& b) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zero16() {
+  return (f32x16){0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+// Rows 16 c .. 16 c + 15 of an accumulator tile as an operand over them.
+__device__ __forceinline__ bf16x8 acc_frag32(const f32x16& s, int c) {
+  return (bf16x8){(bf16)s[8 * c], (bf16)s[8 * c + 1], (bf16)s[8 * c + 2], (bf16)s[8 * c + 3],
+                  (bf16)s[8 * c + 4], (bf16)s[8 * c + 5], (bf16)s[8 * c + 6], (bf16)s[8 * c + 7]};
+}
+// Maximum / sum over the lanes n and n + 32.
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int D> struct Tile {
+  static constexpr int RB = 2 * D, UPR = D / 8;      // bytes and 16-byte units of a row
+  static constexpr int NS = D / 16, ND = D / 32;     // k steps along a row, 32-column blocks
+  __device__ static __forceinline__ int swz(int r) {
+    return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  }
+  __device__ static __forceinline__ int at(int r, int unit) { return r * RB + ((unit ^ swz(r)) << 4); }
+};
+
+// A lane's places in a tile of 32 rows.
+template <int D> struct LaneMap {
+  using T = Tile<D>;
+  int row0, rsw, col[T::ND][2], n, h;
+  __device__ __forceinline__ LaneMap(int lane) {
+    n = lane & 31;
+    h = lane >> 5;
+    row0 = n * T::RB;
+    rsw = (T::swz(n) ^ h) << 4;
+    const int i = lane & 15, c2 = (lane >> 4) & 1;
+#pragma unroll
+    for (int t = 0; t < T::ND; ++t)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) col[t][q] = T::at(4 * h + (i >> 2) + 8 * q, 4 * t + 2 * c2 + ((i & 3) >> 1)) + 8 * (i & 1);
+  }
+  // row n, k step c
+  __device__ __forceinline__ bf16x8 row(const char* tile, int c) const {
+    return *(const bf16x8*)(tile + row0 + ((c << 5) ^ rsw));
+  }
+  // columns 32 t + n over the 16 rows that start at `tile`
+  __device__ __forceinline__ bf16x8 cols(const char* tile, int t) const {
+    typedef __attribute__((address_space(3))) bf16x4 Lds4;
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + col[t][0]));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + col[t][1]));
+    return (bf16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+  // a transposed accumulator [D][32 rows], times f, as 32 rows of bf16
+  __device__ __forceinline__ void put(char* tile, const f32x16* o, float f) const {
+#pragma unroll
+    for (int t = 0; t < T::ND; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        st4((bf16*)(tile + T::at(n, 4 * t + i) + 8 * h), o[t][4 * i] * f, o[t][4 * i + 1] * f, o[t][4 * i + 2] * f,
+            o[t][4 * i + 3] * f);
+  }
+};
+
+// Rows of one key head: (query, head of the group) pairs, heads fastest; row r
+// of a tile that starts at row `first`.
+struct RowMap {
+  int i0, rem, G;
+  unsigned magic;       // ceil(2^32 / G): exact for the small numbers of a tile
+  __device__ __forceinline__ RowMap(long long first, int G_, unsigned magic_) : G(G_), magic(magic_) {
+    i0 = (int)(first / G);
+    rem = (int)(first - (long long)i0 * G);
+  }
+  __device__ __forceinline__ int div(int x) const { return G == 1 ? x : (int)__umulhi((unsigned)x, magic); }
+  __device__ __forceinline__ void at(int r, int* i, int* g) const {
+    const int x = r + rem, q = div(x);
+    *i = i0 + q;
+    *g = x - q * G;
+  }
+  __device__ __forceinline__ int last(int r) const { return i0 + div(r + rem); }      // the query of row r
+};
+
+// A tile of BK rows of two matrices, by way of registers: 256 threads, rows
+// clamped to the last valid one (what lies beyond is masked).  Offsets within
+// a tile are 32-bit: token strides stay below 2^24 elements.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <int D, int BK> struct Stage {
+  using T = Tile<D>;
+  static constexpr int N = BK * T::UPR / 256, STEP = 256 / T::UPR;
+  u32x4 x[N], y[N];
+  int row, unit;
+  __device__ __forceinline__ Stage(int tid) : row(tid / T::UPR), unit(tid % T::UPR) {}
+  // a, b: the tile's first rows; last: the last valid row of the tile (>= 0)
+  __device__ __forceinline__ void load(const bf16* a, int as, const bf16* b, int bs, int last) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned r = min(row + i * STEP, last);
+      x[i] = *(const u32x4*)((const char*)a + (r * (unsigned)as + 8 * unit) * 2);
+      y[i] = *(const u32x4*)((const char*)b + (r * (unsigned)bs + 8 * unit) * 2);
+    }
+  }
+  __device__ __forceinline__ void store(char* ta, char* tb) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = T::at(row + i * STEP, unit);
+      *(u32x4*)(ta + o) = x[i];
+      *(u32x4*)(tb + o) = y[i];
+    }
+  }
+};
+
+}  // namespace gdnx

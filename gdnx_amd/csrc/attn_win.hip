@@ -302,7 +302,7 @@ template <typename CT, int D> static int launch_bwd(const WinAttnBwdArgs& a, hip
 }
 
 int win_attn_fwd_dispatch(const WinAttnArgs& a, hipStream_t stream) {
-  if (a.dtype == GDNX_DTYPE_BF16) return a.D == 128 ? launch_fwd<bf16, 128>(a, stream) : launch_fwd<bf16, 64>(a, stream);
+  if (a.dtype == GDNX_DTYPE_BF16) return win_fwd_bf16_dispatch(a, stream);
   return a.D == 128 ? launch_fwd<float, 128>(a, stream) : launch_fwd<float, 64>(a, stream);
 }
 

@@ -1,0 +1,227 @@
+// Windowed attention with sinks for bf16 (gfx950): forward.  Forms and rules
+// as in attn_win.hip, on the 32 x 32 x 16 matrix instruction.
+#include "attn_tiles.hpp"
+
+namespace gdnx {
+
+// Forward.  A workgroup of four waves takes 128 rows of one key head, a row
+// being a (query, query head of the group) pair with the heads fastest, so
+// that grouped heads share the key tiles and the tile's queries span few
+// positions; a wave owns 32 rows.  Key tiles of 64 go through registers into
+// LDS, double-buffered, one barrier a tile.
+//   S^T = K Q^T   a lane holds 32 scores of one row
+//   O^T += V^T P^T   the score accumulators, as bf16, are the operand
+// The running maximum is raised only when a score exceeds it by 2^8: the
+// output is then rescaled (P stays below 256, its relative rounding does not
+// change), which spares the rescaling of 64 accumulators on most tiles.
+template <int D>
+__global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
+  using T = Tile<D>;
+  constexpr int BK = 64, BYTES = BK * T::RB;
+  __shared__ __attribute__((aligned(16))) char smem[4 * BYTES];   // two buffers of K, V
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, nt = (int)(((long long)a.Tq * G + 127) / 128);
+  // heads fastest (a head's tiles share an XCD's L2 where 8 divides the heads), the longest rows of keys first
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B; w /= a.B;
+  const int part = w % a.parts, tile = nt - 1 - w / a.parts;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
+  const RowMap rm(tile * 128LL, G, a.g_magic);
+  const bf16* kb = (const bf16*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const bf16* vb = (const bf16*)a.v + b * a.vs[0] + hk * a.vs[2];
+
+  // the wave's rows
+  int qi, qh;
+  rm.at(wave * 32 + n, &qi, &qh);
+  qh += hk * G;
+  const int p = qi < a.Tq && qi + off < len ? qi + off : -1;
+  bf16x8 qf[T::NS];
+  {
+    const bf16* qp = (const bf16*)a.q + b * a.qs[0] + (long long)(p >= 0 ? qi : 0) * a.qs[1] + (long long)(p >= 0 ? qh : 0) * a.qs[2];
+#pragma unroll
+    for (int c = 0; c < T::NS; ++c) {
+      qf[c] = *(const bf16x8*)(qp + 16 * c + 8 * h);
+      if (a.scale < 0.f) qf[c] = -qf[c];
+    }
+  }
+  const float sc = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+  // positions of the workgroup's and of the wave's rows
+  const int wg0 = rm.i0 + off, wg1 = min(rm.last(127), a.Tq - 1) + off;
+  const int wv0 = rm.last(wave * 32) + off, wv1 = min(min(rm.last(wave * 32 + 31), a.Tq - 1) + off, len - 1);
+  const bool rows_ok = rm.last(wave * 32 + 31) < a.Tq && rm.last(wave * 32 + 31) + off < len && wv0 >= 0;
+  const KeyTiles<BK> kt(wg0, wg1, len, a.window, a.sinks);
+  const int per = (kt.count + a.parts - 1) / a.parts, t0 = part * per, t1 = min(kt.count, t0 + per);
+
+  f32x16 o[T::ND];
+#pragma unroll
+  for (int t = 0; t < T::ND; ++t) o[t] = zero16();
+  float m = -INFINITY, l = 0.f;
+
+  Stage<D, BK> st(tid);
+  const LaneMap<D> lm(lane);
+  const auto load = [&](int it) {
+    const int j0 = kt.start(it);
+    st.load(kb + j0 * a.ks[1], (int)a.ks[1], vb + j0 * a.vs[1], (int)a.vs[1], len - 1 - j0);
+  };
+  if (t0 < t1) {
+    load(t0);
+    st.store(smem, smem + BYTES);
+  }
+  lds_barrier();
+  for (int it = t0; it < t1; ++it) {
+    const int j0 = kt.start(it);
+    char* buf = smem + ((it - t0) & 1) * 2 * BYTES;
+    load(min(it + 1, t1 - 1));
+    // whether the wave sees anything of the tile, and all of it
+    const bool some = j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    if (some) {
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = zero16();
+#pragma unroll
+        for (int c = 0; c < T::NS; ++c) mma32(s[u], lm.row(buf + u * 32 * T::RB, c), qf[c]);
+      }
+      const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
+      if (!all) {
+        const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = 32 * u + 8 * (e >> 2) + (e & 3);
+            s[u][e] = (c <= d) & ((d - c < a.window) | (c < ds)) ? s[u][e] : -INFINITY;
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
+      mx = half_max(mx) * sc;
+      if (__any(mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < T::ND; ++t) o[t] *= f;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], sc, -ms));
+          sum += s[u][e];
+        }
+      l += sum;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const bf16x8 pf = acc_frag32(s[u], c);
+#pragma unroll
+          for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(buf + BYTES + (32 * u + 16 * c) * T::RB, t), pf);
+        }
+    }
+    char* next = smem + ((it - t0 + 1) & 1) * 2 * BYTES;
+    st.store(next, next + BYTES);
+    lds_barrier();
+  }
+  l = half_sum(l);
+
+  if (a.parts > 1) {                       // a span of the keys: unnormalised, joined by win_join_kernel
+    const long long rows = (long long)a.B * a.Hq * a.Tq;
+    if (qi < a.Tq) {
+      const long long r = (long long)part * rows + ((long long)b * a.Tq + qi) * a.Hq + qh;
+      float* po = a.part + r * D + 4 * h;
+#pragma unroll
+      for (int t = 0; t < T::ND; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(f32x4*)(po + 32 * t + 8 * i) = (f32x4){o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+      if (h == 0) {
+        float* ml = a.part + (long long)a.parts * rows * D + 2 * r;
+        ml[0] = m;
+        ml[1] = l;
+      }
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (h == 0 && a.lse && qi < a.Tq)
+    a.lse[((long long)b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  // the output by way of LDS, so that whole rows are stored
+  lm.put(smem + wave * 32 * T::RB, o, inv);
+  __syncthreads();
+  bf16* yb = (bf16*)a.y + (long long)b * a.Tq * a.Hq * D;
+#pragma unroll
+  for (int u = tid; u < 128 * T::UPR; u += 256) {
+    const int r = u / T::UPR, c = u % T::UPR;
+    int i, g;
+    rm.at(r, &i, &g);
+    if (i < a.Tq) *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)(smem + T::at(r, c));
+  }
+}
+
+// One wave a row: its spans of the keys joined in order.
+template <int D> __global__ void __launch_bounds__(256) win_join_kernel(WinAttnArgs a) {
+  constexpr int E = D / 64;
+  const long long rows = (long long)a.B * a.Hq * a.Tq, r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const float* ml = a.part + (long long)a.parts * rows * D;
+  float mm = -INFINITY;
+  for (int i = 0; i < a.parts; ++i) mm = fmaxf(mm, ml[2 * (i * rows + r)]);
+  const float ms = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int i = 0; i < a.parts; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * (i * rows + r)] - ms);
+    ll += ml[2 * (i * rows + r) + 1] * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += a.part[(i * rows + r) * D + lane * E + e] * f;
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+  for (int e = 0; e < E; ++e) ((bf16*)a.y)[r * D + lane * E + e] = (bf16)(acc[e] * inv);
+  if (lane == 0 && a.lse) {
+    const int h = (int)(r % a.Hq);
+    const long long bi = r / a.Hq;
+    a.lse[((bi / a.Tq) * a.Hq + h) * a.Tq + bi % a.Tq] = ll == 0.f ? -INFINITY : mm * kLn2 + logf(ll);
+  }
+}
+
+// Spans that the rows' keys are cut into: one, unless the workgroups would not
+// give every CU its two; then as many as do, each of at least four tiles.
+int win_attn_fwd_parts(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype) {
+  if (dtype != GDNX_DTYPE_BF16) return 1;
+  const int G = Hq / Hkv;
+  const long long base = (((long long)Tq * G + 127) / 128) * B * Hkv;
+  long long keys = Tk;
+  if (window > 0 && (long long)window + sinks + 127 / G + 1 < keys) keys = (long long)window + sinks + 127 / G + 1;
+  const long long tiles = (keys + 63) / 64;
+  long long parts = 512 / base;
+  if (parts > tiles / 4) parts = tiles / 4;
+  return parts < 1 ? 1 : (int)parts;
+}
+
+template <int D> static int launch(const WinAttnArgs& a, hipStream_t stream) {
+  const long long nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 127) / 128;
+  hipLaunchKernelGGL((win_fwd_bf16_kernel<D>), dim3((unsigned)(nt * a.B * a.Hkv * a.parts)), dim3(256), 0, stream, a);
+  int rc = check_launch("win_fwd_bf16_kernel");
+  if (rc || a.parts == 1) return rc;
+  const long long rows = (long long)a.B * a.Hq * a.Tq;
+  hipLaunchKernelGGL((win_join_kernel<D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  return check_launch("win_join_kernel");
+}
+
+int win_fwd_bf16_dispatch(const WinAttnArgs& a, hipStream_t stream) {
+  return a.D == 128 ? launch<128>(a, stream) : launch<64>(a, stream);
+}
+
+}  // namespace gdnx

@@ -1132,7 +1132,7 @@ static int check_attn_sizes(int Hq, int Hkv, int D, int window, int sinks, int d
   if (dtype != GDNX_DTYPE_F32 && dtype != GDNX_DTYPE_BF16)
     return set_error(GDNX_ERR_ARG, "dtype %d is not GDNX_DTYPE_F32/BF16", dtype);
   if (D != 64 && D != 128) return set_error(GDNX_ERR_SHAPE, "head_dim %d unsupported (64 or 128)", D);
-  if (Hq < 1 || Hkv < 1 || Hq > 65536 || Hq % Hkv != 0)
+  if (Hq < 1 || Hkv < 1 || Hq > 32768 || Hq % Hkv != 0)
     return set_error(GDNX_ERR_SHAPE, "query heads %d are no multiple of %d key heads", Hq, Hkv);
   if (window < 0 || sinks < 0) return set_error(GDNX_ERR_SHAPE, "window %d or sinks %d is negative", window, sinks);
   return GDNX_OK;
@@ -1151,8 +1151,9 @@ static int check_win(int B, int Tq, int Tk, int Hq, int Hkv, int D, int window, 
 static int check_strides(const long long* st, int dtype, const char* name) {
   const int unit = dtype == GDNX_DTYPE_BF16 ? 8 : 4;
   for (int i = 0; i < 3; ++i)
-    if (st[i] < 0 || st[i] % unit != 0 || st[i] > (1LL << 40))
-      return set_error(GDNX_ERR_SHAPE, "%s: strides must be non-negative multiples of 16 bytes", name);
+    if (st[i] < 0 || st[i] % unit != 0 || st[i] > (i == 1 ? 1LL << 24 : 1LL << 40))
+      return set_error(GDNX_ERR_SHAPE, "%s: strides must be non-negative multiples of 16 bytes (a token's up to 2^24 elements)",
+                       name);
   return GDNX_OK;
 }
 
@@ -1190,7 +1191,17 @@ extern "C" long long gdnx_win_attn_bwd_workspace_bytes(int B, int Tq, int Tk, in
   return win_bwd_delta_bytes(B, Tq, Hq);
 }
 
+static unsigned group_magic(int G) { return G > 1 ? (unsigned)(((1ULL << 32) + G - 1) / G) : 0; }
+
+extern "C" long long gdnx_win_attn_fwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
+                                                       int sinks, int dtype) {
+  if (check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype)) return -1;
+  const long long parts = win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
+  return parts > 1 ? parts * B * Tq * Hq * (head_dim + 2) * 4 : 0;
+}
+
 extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, float* lse,
+                                 void* workspace,
                                  long long q_b, long long q_t, long long q_h, long long k_b, long long k_t,
                                  long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk,
                                  int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
@@ -1201,8 +1212,12 @@ extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, co
   if (!q || !k || !v || !y) return set_error(GDNX_ERR_ARG, "q, k, v, y must be non-null");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(y))
     return set_error(GDNX_ERR_ARG, "q, k, v, y must be 16-byte aligned");
+  if (!aligned16(workspace)) return set_error(GDNX_ERR_ARG, "workspace must be 16-byte aligned");
+  const int parts = win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
+  if (parts > 1 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
   WinAttnArgs a{q, k, v, lengths, y, lse, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv,
-                head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype};
+                head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype,
+                group_magic(Hq / Hkv), parts, (float*)workspace};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
       (rc = check_strides(a.vs, dtype, "v")))
     return rc;

@@ -460,6 +460,9 @@ struct WinAttnArgs {
   int B, Tq, Tk, Hq, Hkv, D, window, sinks;
   float scale;
   int dtype;
+  unsigned g_magic;     // ceil(2^32 / (Hq / Hkv))
+  int parts;            // spans that a row's keys are cut into
+  float* part;          // their outputs [parts][B,Tq,Hq][D], then [parts][B,Tq,Hq][2] maximum (log2) and sum
 };
 struct WinAttnBwdArgs {
   const void* q;
@@ -479,6 +482,8 @@ struct WinAttnBwdArgs {
   int dtype;
 };
 int win_attn_fwd_dispatch(const WinAttnArgs& a, hipStream_t stream);
+int win_fwd_bf16_dispatch(const WinAttnArgs& a, hipStream_t stream);
+int win_attn_fwd_parts(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype);
 int win_attn_bwd_dispatch(const WinAttnBwdArgs& a, hipStream_t stream);
 
 // One new token over a paged key-value cache.

@@ -603,7 +603,7 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
  *
  * Attention with a sliding window and sinks.  q [B,Tq,Hq,D], k and v
  * [B,Tk,Hkv,D] in the io dtype with any element strides (batch, token, head)
- * that are multiples of 16 bytes, D contiguous; Hq a multiple of Hkv, query
+ * that are multiples of 16 bytes (a token's at most 2^24), D contiguous; Hq a multiple of Hkv, query
  * head h reading key head h / (Hq / Hkv); D = 64 or 128.  Query i stands at
  * position p = i + Tk - Tq and sees key j if
  *     j <= p,  p < lengths[b],  and  p - j < window or j < sinks
@@ -611,9 +611,14 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
  * nothing gives y = 0, lse = -infinity and no gradient.  Keys at or beyond
  * lengths[b] are never read.
  *   y   [B,Tq,Hq,D] io dtype, contiguous: softmax(scale q.k) v
- *   lse [B,Hq,Tq] float32 (may be null): log of the softmax's denominator */
+ *   lse [B,Hq,Tq] float32 (may be null): log of the softmax's denominator
+ * workspace: gdnx_win_attn_fwd_workspace_bytes bytes (-1 if the sizes are
+ * invalid; null where that is 0): few rows of queries against many keys are
+ * split over the keys and joined. */
+long long gdnx_win_attn_fwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
+                                            int sinks, int dtype);
 int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, float* lse,
-                      long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
+                      void* workspace, long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
                       long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
                       int head_dim, int window, int sinks, float scale, int dtype, void* stream);
 

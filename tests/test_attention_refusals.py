@@ -15,7 +15,7 @@ def _win(over, bwd=False):
     a.update(over)
     lib = _lib.load()
     ints = [a[n] for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D", "window", "sinks")]
-    names = ("q", "k", "v", "lengths", "y", "lse") + (("dy", "dq", "dk", "dv", "ws") if bwd else ())
+    names = ("q", "k", "v", "lengths", "y", "lse") + (("dy", "dq", "dk", "dv", "ws") if bwd else ("ws",))
     fn = lib.gdnx_win_attn_bwd if bwd else lib.gdnx_win_attn_fwd
     return fn(*(VP(a[n]) for n in names), *a["st"], *ints, a["scale"], a["dt"], None), lib.gdnx_last_error().decode()
 
@@ -31,8 +31,10 @@ def test_window_attention_refuses(over, code, msg, bwd):
     assert rc == code and msg in err
 
 
-def test_window_backward_needs_its_workspace():
+def test_window_attention_needs_its_workspace():
     rc, err = _win(dict(ws=None), True)
+    assert rc == -3 and "workspace" in err
+    rc, err = _win(dict(ws=None, Tk=1 << 20))            # few queries, many keys: split over the keys
     assert rc == -3 and "workspace" in err
     lib = _lib.load()
     assert lib.gdnx_win_attn_bwd_workspace_bytes(2, 100, 100, 4, 2, 64, 10, 2, _lib.DTYPE_BF16) >= 2 * 100 * 4 * 4
