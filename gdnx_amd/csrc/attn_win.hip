@@ -307,7 +307,7 @@ int win_attn_fwd_dispatch(const WinAttnArgs& a, hipStream_t stream) {
 }
 
 int win_attn_bwd_dispatch(const WinAttnBwdArgs& a, hipStream_t stream) {
-  if (a.dtype == GDNX_DTYPE_BF16) return a.D == 128 ? launch_bwd<bf16, 128>(a, stream) : launch_bwd<bf16, 64>(a, stream);
+  if (a.dtype == GDNX_DTYPE_BF16) return win_bwd_bf16_dispatch(a, stream);
   return a.D == 128 ? launch_bwd<float, 128>(a, stream) : launch_bwd<float, 64>(a, stream);
 }
 

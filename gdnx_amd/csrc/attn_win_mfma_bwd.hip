@@ -1,0 +1,389 @@
+// Windowed attention with sinks for bf16 (gfx950): backward.  Forms and rules
+// as in attn_win.hip, tiles and operands as in attn_tiles.hpp, rows packed as
+// in the forward (attn_win_mfma.hip).
+#include "attn_tiles.hpp"
+
+namespace gdnx {
+
+// dQ, and delta for dK: the forward's walk over the key tiles, per 32 x 32
+// scores
+//   S^T = K Q^T,  dP^T = V dY^T,  dS^T = P^T o (dP^T - delta),  dQ^T += K^T dS^T
+template <int D>
+__global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
+  using T = Tile<D>;
+  constexpr int BK = 32, BYTES = BK * T::RB;
+  __shared__ __attribute__((aligned(16))) char smem[4 * BYTES];   // two buffers of K, V (then the output's 128 rows)
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, nt = (int)(((long long)a.Tq * G + 127) / 128);
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B, tile = nt - 1 - w / a.B;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
+  const RowMap rm(tile * 128LL, G, a.g_magic);
+  const bf16* kb = (const bf16*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const bf16* vb = (const bf16*)a.v + b * a.vs[0] + hk * a.vs[2];
+
+  int qi, qh;
+  rm.at(wave * 32 + n, &qi, &qh);
+  qh += hk * G;
+  const int p = qi < a.Tq && qi + off < len ? qi + off : -1;
+  bf16x8 qf[T::NS], gf[T::NS];
+  float delta = 0.f, lse = 0.f;
+  {
+    const int i = p >= 0 ? qi : 0, g = p >= 0 ? qh : 0;
+    const bf16* qp = (const bf16*)a.q + b * a.qs[0] + (long long)i * a.qs[1] + (long long)g * a.qs[2];
+    const long long row = (((long long)b * a.Tq + i) * a.Hq + g) * D;
+    const long long srow = ((long long)b * a.Hq + g) * a.Tq + i;
+#pragma unroll
+    for (int c = 0; c < T::NS; ++c) {
+      qf[c] = *(const bf16x8*)(qp + 16 * c + 8 * h);
+      gf[c] = *(const bf16x8*)((const bf16*)a.dy + row + 16 * c + 8 * h);
+      const bf16x8 yf = *(const bf16x8*)((const bf16*)a.y + row + 16 * c + 8 * h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta += (float)gf[c][e] * (float)yf[e];
+    }
+    delta = half_sum(delta);
+    if (p >= 0) {
+      lse = a.lse[srow] * kLog2e;
+      if (h == 0) a.delta[srow] = delta;
+    }
+  }
+  const float sc = a.scale * kLog2e;
+  const int wg0 = rm.i0 + off, wg1 = min(rm.last(127), a.Tq - 1) + off;
+  const int wv0 = rm.last(wave * 32) + off, wv1 = min(min(rm.last(wave * 32 + 31), a.Tq - 1) + off, len - 1);
+  const bool rows_ok = rm.last(wave * 32 + 31) < a.Tq && rm.last(wave * 32 + 31) + off < len && wv0 >= 0;
+  const KeyTiles<BK> kt(wg0, wg1, len, a.window, a.sinks);
+
+  f32x16 o[T::ND];
+#pragma unroll
+  for (int t = 0; t < T::ND; ++t) o[t] = zero16();
+  Stage<D, BK> st(tid);
+  const LaneMap<D> lm(lane);
+  const auto load = [&](int it) {
+    const int j0 = kt.start(it);
+    st.load(kb + j0 * a.ks[1], (int)a.ks[1], vb + j0 * a.vs[1], (int)a.vs[1], len - 1 - j0);
+  };
+  if (kt.count > 0) {
+    load(0);
+    st.store(smem, smem + BYTES);
+  }
+  lds_barrier();
+  for (int it = 0; it < kt.count; ++it) {
+    const int j0 = kt.start(it);
+    const char* buf = smem + (it & 1) * 2 * BYTES;
+    load(min(it + 1, kt.count - 1));
+    const bool some = j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    if (some) {
+      const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
+#pragma unroll
+      for (int u = 0; u < BK / 32; ++u) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(buf + u * 32 * T::RB, c), qf[c]);
+#pragma unroll
+        for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(buf + BYTES + u * 32 * T::RB, c), gf[c]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sc, -lse)) * (dp[e] - delta);
+        if (!all) {
+          const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = 32 * u + 8 * (e >> 2) + (e & 3);
+            s[e] = (c <= d) & ((d - c < a.window) | (c < ds)) ? s[e] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const bf16x8 f = acc_frag32(s, c);
+#pragma unroll
+          for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(buf + (32 * u + 16 * c) * T::RB, t), f);
+        }
+      }
+    }
+    char* next = smem + ((it + 1) & 1) * 2 * BYTES;
+    st.store(next, next + BYTES);
+    lds_barrier();
+  }
+  lm.put(smem + wave * 32 * T::RB, o, a.scale);
+  __syncthreads();
+  bf16* qo = (bf16*)a.dq + (long long)b * a.Tq * a.Hq * D;
+#pragma unroll
+  for (int u = tid; u < 128 * T::UPR; u += 256) {
+    const int r = u / T::UPR, c = u % T::UPR;
+    int i, g;
+    rm.at(r, &i, &g);
+    if (i < a.Tq) *(uint4*)(qo + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)(smem + T::at(r, c));
+  }
+}
+
+// The 64-row steps that the 128 keys from k0 take, and how they are shared:
+// spans of at most `span` steps each.
+struct KeySpan {
+  int i0;              // the first query
+  long long rows;      // rows (query, head) from there on
+  int steps, parts;
+  __device__ __forceinline__ KeySpan(const WinAttnBwdArgs& a, int k0, int len) {
+    const int off = a.Tk - a.Tq, p0 = max(k0, off), pe = k0 < len ? last_query<128>(k0, len, a.window, a.sinks) : 0;
+    i0 = p0 - off;
+    rows = pe > p0 ? (long long)(pe - p0) * (a.Hq / a.Hkv) : 0;
+    steps = (int)((rows + 63) / 64);
+    parts = max(1, (steps + a.span - 1) / a.span);
+  }
+};
+
+// dK, dV of 128 keys of one key head over a span of the rows that see them; a
+// wave owns 32 keys.  Per 32 rows
+//   S = Q K^T,  dP = dY V^T,  dV^T += dY^T P,  dK^T += Q^T dS
+// K stays in registers, V in LDS; 64 rows of Q and dY a step, double-buffered.
+template <int D>
+__global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) {
+  using T = Tile<D>;
+  constexpr int BR = 32, BYTES = BR * T::RB, VB = 128 * T::RB;
+  __shared__ __attribute__((aligned(16))) char smem[4 * BYTES + VB];
+  __shared__ __attribute__((aligned(16))) float s_lse[2][BR], s_del[2][BR];
+  __shared__ __attribute__((aligned(16))) int s_pos[2][BR];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, off = a.Tk - a.Tq;
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B; w /= a.B;
+  // the tiles that hold sinks first, then the others, each with its most parts
+  const int ns = a.sink_tiles, sp = a.sink_parts;
+  const int kt = w < ns * sp ? w / sp : ns + (w - ns * sp) / a.tile_parts;
+  const int part = w < ns * sp ? w % sp : (w - ns * sp) % a.tile_parts;
+  const int k0 = kt * 128;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+  const KeySpan ks(a, k0, len);
+  if (part >= ks.parts) return;
+  const int t0 = part * a.span * (64 / BR), t1 = min((part + 1) * a.span * (64 / BR), (int)((ks.rows + BR - 1) / BR));
+
+  const int kw = k0 + wave * 32, j = kw + n;
+  bf16x8 kf[T::NS];
+  {
+    const bf16* kp = (const bf16*)a.k + b * a.ks[0] + hk * a.ks[2] + (long long)max(0, min(j, len - 1)) * a.ks[1];
+    const bf16* vp = (const bf16*)a.v + b * a.vs[0] + hk * a.vs[2];
+#pragma unroll
+    for (int c = 0; c < T::NS; ++c) kf[c] = *(const bf16x8*)(kp + 16 * c + 8 * h);
+#pragma unroll
+    for (int u = tid; u < 128 * T::UPR; u += 256) {
+      const int r = u / T::UPR, c = u % T::UPR;
+      *(u32x4*)(smem + 4 * BYTES + T::at(r, c)) =
+          *(const u32x4*)(vp + (long long)max(0, min(k0 + r, len - 1)) * a.vs[1] + 8 * c);
+    }
+  }
+  const float sc = a.scale * kLog2e;
+  f32x16 ok[T::ND], ov[T::ND];
+#pragma unroll
+  for (int t = 0; t < T::ND; ++t) ok[t] = ov[t] = zero16();
+  const bf16* qb = (const bf16*)a.q + b * a.qs[0] + (long long)hk * G * a.qs[2];
+  const bf16* gb = (const bf16*)a.dy + ((long long)b * a.Tq * a.Hq + hk * G) * D;
+  const LaneMap<D> lm(lane);
+
+  constexpr int N = BR * T::UPR / 256, STEP = 256 / T::UPR;
+  u32x4 xq[N], xg[N];
+  float x_lse = 0.f, x_del = 0.f;
+  int x_pos = -1;
+  const int srow = tid / T::UPR, sunit = tid % T::UPR;
+  // step t: rows BR t .. of the span's rows, clamped to the last one
+  const auto load = [&](int t) {
+    const long long last = ks.rows - 1;
+    const RowMap rm((long long)t * BR, G, a.g_magic);
+    int li, lg;
+    rm.at((int)min((long long)BR - 1, last - (long long)t * BR), &li, &lg);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int qi, qg;
+      rm.at(srow + i * STEP, &qi, &qg);
+      const bool in = (long long)t * BR + srow + i * STEP <= last;
+      qi = (in ? qi : li) + ks.i0;
+      qg = in ? qg : lg;
+      xq[i] = *(const u32x4*)(qb + qi * a.qs[1] + qg * a.qs[2] + 8 * sunit);
+      xg[i] = *(const u32x4*)(gb + (long long)qi * a.Hq * D + qg * D + 8 * sunit);
+    }
+    if (tid < BR) {
+      int qi, qg;
+      rm.at(tid, &qi, &qg);
+      const bool in = (long long)t * BR + tid <= last;
+      qi = (in ? qi : li) + ks.i0;
+      qg = in ? qg : lg;
+      const long long sr = ((long long)b * a.Hq + hk * G + qg) * a.Tq + qi;
+      x_lse = a.lse[sr] * kLog2e;
+      x_del = a.delta[sr];
+      x_pos = in ? qi + off : -1;
+    }
+  };
+  const auto store = [&](int s) {
+    char* buf = smem + s * 2 * BYTES;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = T::at(srow + i * STEP, sunit);
+      *(u32x4*)(buf + o) = xq[i];
+      *(u32x4*)(buf + BYTES + o) = xg[i];
+    }
+    if (tid < BR) {
+      s_lse[s][tid] = x_lse;
+      s_del[s][tid] = x_del;
+      s_pos[s][tid] = x_pos;
+    }
+  };
+  if (t0 < t1) {
+    load(t0);
+    store(0);
+  }
+  lds_barrier();
+  const char* vt = smem + 4 * BYTES + wave * 32 * T::RB;
+  for (int t = t0; t < t1; ++t) {
+    const int s_i = (t - t0) & 1;
+    const char* buf = smem + s_i * 2 * BYTES;
+    load(min(t + 1, t1 - 1));
+    // positions of the step's rows (uniform)
+    const RowMap rm((long long)t * BR, G, a.g_magic);
+    const int tp0 = rm.i0 + ks.i0 + off, tp1 = rm.last(BR - 1) + ks.i0 + off;
+    const bool some = tp1 >= kw && (tp0 - a.window < kw + 31 || kw < a.sinks);
+    if (some) {
+      const bool all = (long long)(t + 1) * BR <= ks.rows && tp0 >= kw + 31 && (tp1 - kw < a.window || kw + 32 <= a.sinks);
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(buf, c), kf[c]);
+#pragma unroll
+      for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(buf + BYTES, c), lm.row(vt, c));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 ls = *(const f32x4*)&s_lse[s_i][8 * q + 4 * h], dl = *(const f32x4*)&s_del[s_i][8 * q + 4 * h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pr = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], sc, -ls[e]));
+          s[4 * q + e] = pr;
+          dp[4 * q + e] = pr * (dp[4 * q + e] - dl[e]);
+        }
+      }
+      if (!all) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int* ps = &s_pos[s_i][8 * q + 4 * h];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int p = ps[e];
+            const bool vis = (j <= p) & ((p - j < a.window) | (j < a.sinks));
+            s[4 * q + e] = vis ? s[4 * q + e] : 0.f;
+            dp[4 * q + e] = vis ? dp[4 * q + e] : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const bf16x8 pf = acc_frag32(s, c), df = acc_frag32(dp, c);
+#pragma unroll
+        for (int t2 = 0; t2 < T::ND; ++t2) {
+          mma32(ov[t2], lm.cols(buf + BYTES + 16 * c * T::RB, t2), pf);
+          mma32(ok[t2], lm.cols(buf + 16 * c * T::RB, t2), df);
+        }
+      }
+    }
+    store(s_i ^ 1);
+    lds_barrier();
+  }
+
+  if (ks.parts > 1) {                       // a span: float32 sums, joined by win_dkv_join_kernel
+    const long long slots = (long long)ns * sp + (long long)((a.Tk + 127) / 128 - ns) * a.tile_parts;
+    const long long slot = ((long long)b * a.Hkv + hk) * slots + w;
+    float* pk = a.part + (slot * 2 * 128 + wave * 32 + n) * D + 4 * h;
+#pragma unroll
+    for (int t = 0; t < T::ND; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        *(f32x4*)(pk + 32 * t + 8 * i) = (f32x4){ok[t][4 * i], ok[t][4 * i + 1], ok[t][4 * i + 2], ok[t][4 * i + 3]};
+        *(f32x4*)(pk + 128 * D + 32 * t + 8 * i) = (f32x4){ov[t][4 * i], ov[t][4 * i + 1], ov[t][4 * i + 2], ov[t][4 * i + 3]};
+      }
+    return;
+  }
+  // by way of LDS (Q and dY tiles, then V's), so that whole rows are stored
+  bf16* outs[2] = {(bf16*)a.dk, (bf16*)a.dv};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    __syncthreads();
+    lm.put(smem + wave * 32 * T::RB, m ? ov : ok, m ? 1.f : a.scale);
+    __syncthreads();
+#pragma unroll
+    for (int u = tid; u < 128 * T::UPR; u += 256) {
+      const int r = u / T::UPR, c = u % T::UPR;
+      if (k0 + r < a.Tk)
+        *(uint4*)(outs[m] + (((long long)b * a.Tk + k0 + r) * a.Hkv + hk) * D + 8 * c) = *(const uint4*)(smem + T::at(r, c));
+    }
+  }
+}
+
+// The spans of 128 keys' gradients summed in order: four keys' rows a workgroup of 256.
+template <int D> __global__ void __launch_bounds__(256) win_dkv_join_kernel(WinAttnBwdArgs a) {
+  constexpr int V = D / 4, RPW = 256 / V;         // threads of a row, rows a pass
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B; w /= a.B;
+  const int blk = w % 4, kt = w / 4;              // 32 keys a workgroup
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+  const KeySpan ks(a, kt * 128, len);
+  if (ks.parts <= 1) return;
+  const int ns = a.sink_tiles, sp = a.sink_parts;
+  const long long slots = (long long)ns * sp + (long long)((a.Tk + 127) / 128 - ns) * a.tile_parts;
+  const long long slot = ((long long)b * a.Hkv + hk) * slots + (kt < ns ? (long long)kt * sp : (long long)ns * sp + (long long)(kt - ns) * a.tile_parts);
+  const int d = 4 * (threadIdx.x % V);
+  for (int r = blk * 32 + threadIdx.x / V; r < blk * 32 + 32; r += RPW) {
+    if (kt * 128 + r >= a.Tk) break;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      f32x4 x = zero4();
+      for (int p = 0; p < ks.parts; ++p) x += *(const f32x4*)(a.part + ((slot + p) * 2 * 128 + m * 128 + r) * D + d);
+      if (m == 0) x *= a.scale;
+      st4((bf16*)(m ? a.dv : a.dk) + (((long long)b * a.Tk + kt * 128 + r) * a.Hkv + hk) * D + d, x[0], x[1], x[2], x[3]);
+    }
+  }
+}
+
+// Steps a span may take, and the most spans of a tile with and without sinks.
+// Tiles see (128 + window) positions' rows, those with sinks every later one.
+// Ordinary tiles are cut only where the workgroups are too few to give every
+// CU its two; the sinks' tiles, as long as the whole row, into spans of an
+// ordinary tile's length.
+WinBwdPlan win_attn_bwd_plan(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks) {
+  const long long G = Hq / Hkv, tiles = (Tk + 127) / 128, heads = (long long)B * Hkv;
+  const bool win = window > 0 && (long long)window + 128 < Tk;
+  const long long full = ((long long)Tq * G + 63) / 64;
+  long long one = win ? (((long long)window + 127) * G + 63) / 64 : full;
+  if (one > full) one = full;
+  const long long ns = sinks > 0 && win ? ((long long)sinks + 127) / 128 : 0;
+  WinBwdPlan p;
+  p.sink_tiles = (int)(ns < tiles ? ns : tiles);
+  // all heads' steps: a triangle without a window
+  const long long total = heads * (win ? (tiles - p.sink_tiles) * one + p.sink_tiles * full : tiles * full / 2);
+  long long span = (total + 767) / 768;
+  if (span < 8) span = 8;
+  if (win && one <= 2 * span) span = span > one ? span : one;
+  p.span = (int)span;
+  p.tile_parts = (int)((one + span - 1) / span);
+  p.sink_parts = (int)((full + span - 1) / span);
+  return p;
+}
+
+template <int D> static int launch(const WinAttnBwdArgs& a, hipStream_t stream) {
+  const long long heads = (long long)a.B * a.Hkv, nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 127) / 128;
+  hipLaunchKernelGGL((win_dq_bf16_kernel<D>), dim3((unsigned)(nt * heads)), dim3(256), 0, stream, a);
+  int rc = check_launch("win_dq_bf16_kernel");
+  if (rc) return rc;
+  const long long tiles = (a.Tk + 127) / 128;
+  const long long slots = (long long)a.sink_tiles * a.sink_parts + (tiles - a.sink_tiles) * a.tile_parts;
+  hipLaunchKernelGGL((win_dkv_bf16_kernel<D>), dim3((unsigned)(slots * heads)), dim3(256), 0, stream, a);
+  rc = check_launch("win_dkv_bf16_kernel");
+  if (rc || (a.tile_parts == 1 && (a.sink_tiles == 0 || a.sink_parts == 1))) return rc;
+  // (without a window every tile may have several spans; with one, often only the sinks')
+  const long long joined = a.tile_parts > 1 ? tiles : a.sink_tiles;
+  hipLaunchKernelGGL((win_dkv_join_kernel<D>), dim3((unsigned)(joined * 4 * heads)), dim3(256), 0, stream, a);
+  return check_launch("win_dkv_join_kernel");
+}
+
+int win_bwd_bf16_dispatch(const WinAttnBwdArgs& a, hipStream_t stream) {
+  return a.D == 128 ? launch<128>(a, stream) : launch<64>(a, stream);
+}
+
+}  // namespace gdnx
