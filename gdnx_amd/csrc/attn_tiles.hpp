@@ -93,9 +93,14 @@ template <int D> struct LaneMap {
 struct RowMap {
   int i0, rem, G;
   unsigned magic;       // ceil(2^32 / G): exact for the small numbers of a tile
-  __device__ __forceinline__ RowMap(long long first, int G_, unsigned magic_) : G(G_), magic(magic_) {
-    i0 = (int)(first / G);
-    rem = (int)(first - (long long)i0 * G);
+  __device__ __forceinline__ RowMap(int first, int G_, unsigned magic_) : G(G_), magic(magic_) {
+    i0 = first / G;
+    rem = first - i0 * G;
+  }
+  __device__ __forceinline__ void advance(int rows) {
+    const int q = div(rem + rows);
+    i0 += q;
+    rem += rows - q * G;
   }
   __device__ __forceinline__ int div(int x) const { return G == 1 ? x : (int)__umulhi((unsigned)x, magic); }
   __device__ __forceinline__ void at(int r, int* i, int* g) const {

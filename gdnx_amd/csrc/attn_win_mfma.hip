@@ -21,14 +21,14 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[4 * BYTES];   // two buffers of K, V
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = a.Hq / a.Hkv, nt = (int)(((long long)a.Tq * G + 127) / 128);
+  const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 127) / 128;
   // heads fastest (a head's tiles share an XCD's L2 where 8 divides the heads), the longest rows of keys first
   int w = blockIdx.x;
   const int hk = w % a.Hkv; w /= a.Hkv;
   const int b = w % a.B; w /= a.B;
   const int part = w % a.parts, tile = nt - 1 - w / a.parts;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
-  const RowMap rm(tile * 128LL, G, a.g_magic);
+  const RowMap rm(tile * 128, G, a.g_magic);
   const bf16* kb = (const bf16*)a.k + b * a.ks[0] + hk * a.ks[2];
   const bf16* vb = (const bf16*)a.v + b * a.vs[0] + hk * a.vs[2];
 

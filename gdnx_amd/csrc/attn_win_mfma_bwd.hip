@@ -15,12 +15,12 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[4 * BYTES];   // two buffers of K, V (then the output's 128 rows)
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = a.Hq / a.Hkv, nt = (int)(((long long)a.Tq * G + 127) / 128);
+  const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 127) / 128;
   int w = blockIdx.x;
   const int hk = w % a.Hkv; w /= a.Hkv;
   const int b = w % a.B, tile = nt - 1 - w / a.B;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
-  const RowMap rm(tile * 128LL, G, a.g_magic);
+  const RowMap rm(tile * 128, G, a.g_magic);
   const bf16* kb = (const bf16*)a.k + b * a.ks[0] + hk * a.ks[2];
   const bf16* vb = (const bf16*)a.v + b * a.vs[0] + hk * a.vs[2];
 
@@ -121,13 +121,13 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
 // spans of at most `span` steps each.
 struct KeySpan {
   int i0;              // the first query
-  long long rows;      // rows (query, head) from there on
+  int rows;            // rows (query, head) from there on
   int steps, parts;
   __device__ __forceinline__ KeySpan(const WinAttnBwdArgs& a, int k0, int len) {
     const int off = a.Tk - a.Tq, p0 = max(k0, off), pe = k0 < len ? last_query<128>(k0, len, a.window, a.sinks) : 0;
     i0 = p0 - off;
-    rows = pe > p0 ? (long long)(pe - p0) * (a.Hq / a.Hkv) : 0;
-    steps = (int)((rows + 63) / 64);
+    rows = pe > p0 ? (pe - p0) * (a.Hq / a.Hkv) : 0;
+    steps = (rows + 63) / 64;
     parts = max(1, (steps + a.span - 1) / a.span);
   }
 };
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
   const KeySpan ks(a, k0, len);
   if (part >= ks.parts) return;
-  const int t0 = part * a.span * (64 / BR), t1 = min((part + 1) * a.span * (64 / BR), (int)((ks.rows + BR - 1) / BR));
+  const int t0 = part * a.span * (64 / BR), t1 = min((part + 1) * a.span * (64 / BR), (ks.rows + BR - 1) / BR);
 
   const int kw = k0 + wave * 32, j = kw + n;
   bf16x8 kf[T::NS];
@@ -186,32 +186,25 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   float x_lse = 0.f, x_del = 0.f;
   int x_pos = -1;
   const int srow = tid / T::UPR, sunit = tid % T::UPR;
-  // step t: rows BR t .. of the span's rows, clamped to the last one
-  const auto load = [&](int t) {
-    const long long last = ks.rows - 1;
-    const RowMap rm((long long)t * BR, G, a.g_magic);
-    int li, lg;
-    rm.at((int)min((long long)BR - 1, last - (long long)t * BR), &li, &lg);
+  // step t: rows BR t .. of the keys' rows, clamped to the last one
+  const auto load = [&](const RowMap& rm, int t) {
+    const int last = ks.rows - 1 - t * BR;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       int qi, qg;
-      rm.at(srow + i * STEP, &qi, &qg);
-      const bool in = (long long)t * BR + srow + i * STEP <= last;
-      qi = (in ? qi : li) + ks.i0;
-      qg = in ? qg : lg;
+      rm.at(min(srow + i * STEP, last), &qi, &qg);
+      qi += ks.i0;
       xq[i] = *(const u32x4*)(qb + qi * a.qs[1] + qg * a.qs[2] + 8 * sunit);
       xg[i] = *(const u32x4*)(gb + (long long)qi * a.Hq * D + qg * D + 8 * sunit);
     }
     if (tid < BR) {
       int qi, qg;
-      rm.at(tid, &qi, &qg);
-      const bool in = (long long)t * BR + tid <= last;
-      qi = (in ? qi : li) + ks.i0;
-      qg = in ? qg : lg;
+      rm.at(min(tid, last), &qi, &qg);
+      qi += ks.i0;
       const long long sr = ((long long)b * a.Hq + hk * G + qg) * a.Tq + qi;
-      x_lse = a.lse[sr] * kLog2e;
+      x_lse = a.lse[sr];
       x_del = a.delta[sr];
-      x_pos = in ? qi + off : -1;
+      x_pos = tid <= last ? qi + off : -1;
     }
   };
   const auto store = [&](int s) {
@@ -223,13 +216,14 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
       *(u32x4*)(buf + BYTES + o) = xg[i];
     }
     if (tid < BR) {
-      s_lse[s][tid] = x_lse;
+      s_lse[s][tid] = x_lse * kLog2e;
       s_del[s][tid] = x_del;
       s_pos[s][tid] = x_pos;
     }
   };
+  RowMap rm(t0 * BR, G, a.g_magic);          // of the step at hand
   if (t0 < t1) {
-    load(t0);
+    load(rm, t0);
     store(0);
   }
   lds_barrier();
@@ -237,18 +231,18 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   for (int t = t0; t < t1; ++t) {
     const int s_i = (t - t0) & 1;
     const char* buf = smem + s_i * 2 * BYTES;
-    load(min(t + 1, t1 - 1));
     // positions of the step's rows (uniform)
-    const RowMap rm((long long)t * BR, G, a.g_magic);
     const int tp0 = rm.i0 + ks.i0 + off, tp1 = rm.last(BR - 1) + ks.i0 + off;
     const bool some = tp1 >= kw && (tp0 - a.window < kw + 31 || kw < a.sinks);
+    bf16x8 pf[2], df[2];
     if (some) {
-      const bool all = (long long)(t + 1) * BR <= ks.rows && tp0 >= kw + 31 && (tp1 - kw < a.window || kw + 32 <= a.sinks);
+      const bool all = (t + 1) * BR <= ks.rows && tp0 >= kw + 31 && (tp1 - kw < a.window || kw + 32 <= a.sinks);
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(buf, c), kf[c]);
 #pragma unroll
       for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(buf + BYTES, c), lm.row(vt, c));
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const f32x4 ls = *(const f32x4*)&s_lse[s_i][8 * q + 4 * h], dl = *(const f32x4*)&s_del[s_i][8 * q + 4 * h];
@@ -274,13 +268,23 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const bf16x8 pf = acc_frag32(s, c), df = acc_frag32(dp, c);
+        pf[c] = acc_frag32(s, c);
+        df[c] = acc_frag32(dp, c);
+      }
+    }
+    // the next rows are asked for once the scores' accumulators are free
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 1 < t1) rm.advance(BR);
+    load(rm, min(t + 1, t1 - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    if (some) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int t2 = 0; t2 < T::ND; ++t2) {
-          mma32(ov[t2], lm.cols(buf + BYTES + 16 * c * T::RB, t2), pf);
-          mma32(ok[t2], lm.cols(buf + 16 * c * T::RB, t2), df);
+          mma32(ov[t2], lm.cols(buf + BYTES + 16 * c * T::RB, t2), pf[c]);
+          mma32(ok[t2], lm.cols(buf + 16 * c * T::RB, t2), df[c]);
         }
-      }
     }
     store(s_i ^ 1);
     lds_barrier();

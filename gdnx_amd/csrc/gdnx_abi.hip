@@ -1143,7 +1143,7 @@ static int check_win(int B, int Tq, int Tk, int Hq, int Hkv, int D, int window, 
   if (rc) return rc;
   if (B < 1 || Tq < 1 || Tk < 1 || Tq >= kNoWindow || Tk >= kNoWindow)
     return set_error(GDNX_ERR_SHAPE, "bad sizes B=%d Tq=%d Tk=%d", B, Tq, Tk);
-  if (!prod_le(kMaxGroups, {B, Hq, ((Tq > Tk ? Tq : Tk) + 63) / 64}))
+  if (!prod_le(kMaxGroups, {B, Hq, ((Tq > Tk ? Tq : Tk) + 63) / 64}) || !prod_le(kNoWindow, {Hq, Tq}))
     return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
   return GDNX_OK;
 }
