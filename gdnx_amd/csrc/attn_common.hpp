@@ -10,6 +10,8 @@
 
 namespace gdnx {
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

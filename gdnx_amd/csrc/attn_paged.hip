@@ -40,6 +40,13 @@ struct Seen {                                     // a row's visible keys
 // spans that a row of n key tiles is cut into: at least four tiles each
 __device__ __forceinline__ int spans(int tiles, int max_spans) { return min(max_spans, (tiles + 3) / 4); }
 
+// (a choice between pointers is read as memory of any kind, LDS included,
+// unless it is said to be global: its loads would then wait for LDS too)
+typedef const __attribute__((address_space(1))) char* GlobalBytes;
+template <typename V> __device__ __forceinline__ V ld_global(GlobalBytes p) {
+  return *(const __attribute__((address_space(1))) V*)p;
+}
+
 typedef __bf16 LdsB4 __attribute__((ext_vector_type(4)));
 
 // V^T operand of a 16-wide column block: the lane's column 16 t + n, its keys
@@ -82,7 +89,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[4 * (STAGE > OUT ? STAGE : OUT)];
   __shared__ long long s_off[4][BT];
   __shared__ float s_m[4][16], s_l[4][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.Hq / a.Hkv, gb = (G + 15) / 16;
   int w = blockIdx.x;
   const int span = w % a.spans; w /= a.spans;
@@ -126,7 +134,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
     return table[j >> a.page_log];
   };
   Frag kr[NU][NKS];
-  uint4 vr[NV];
+  u32x4 vr[NV];
   bool live[NU];                       // whether the lane's keys of the tile are visible
   long long* off = s_off[wave];
   CT* stage = (CT*)(smem + wave * STAGE);
@@ -147,17 +155,17 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const long long o = off[16 * u + n];
-      const char* p = o >= 0 ? (const char*)a.k_pages + o : o == -2 ? knew : (const char*)g_zero_row;
+      const GlobalBytes p = (GlobalBytes)(o >= 0 ? (const char*)a.k_pages + o : o == -2 ? knew : (const char*)g_zero_row);
       live[u] = o != -1;
 #pragma unroll
-      for (int c = 0; c < NKS; ++c) kr[u][c] = *(const Frag*)(p + (4 * c + g) * 16);
+      for (int c = 0; c < NKS; ++c) kr[u][c] = ld_global<Frag>(p + (4 * c + g) * 16);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int U = i * 64 + lane, row = U / UPR, u = (U % UPR) ^ v_swizzle<D>((const CT*)nullptr, row);
       const long long o = off[row];
-      const char* p = o >= 0 ? (const char*)a.v_pages + o : o == -2 ? vnew : (const char*)g_zero_row;
-      vr[i] = *(const uint4*)(p + u * 16);
+      const GlobalBytes p = (GlobalBytes)(o >= 0 ? (const char*)a.v_pages + o : o == -2 ? vnew : (const char*)g_zero_row);
+      vr[i] = ld_global<u32x4>(p + u * 16);
     }
   };
 
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
     }
     wave_lds_sync();
 #pragma unroll
-    for (int i = 0; i < NV; ++i) *(uint4*)((char*)stage + (i * 64 + lane) * 16) = vr[i];
+    for (int i = 0; i < NV; ++i) *(u32x4*)((char*)stage + (i * 64 + lane) * 16) = vr[i];
     // which keys of the lane's accumulator rows are visible: lane 4 g + e has key 16 u + 4 g + e
 #pragma unroll
     for (int u = 0; u < NU; ++u) {

@@ -114,7 +114,6 @@ struct RowMap {
 // A tile of BK rows of two matrices, by way of registers: 256 threads, rows
 // clamped to the last valid one (what lies beyond is masked).  Offsets within
 // a tile are 32-bit: token strides stay below 2^24 elements.
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 template <int D, int BK> struct Stage {
   using T = Tile<D>;
   static constexpr int N = BK * T::UPR / 256, STEP = 256 / T::UPR;
