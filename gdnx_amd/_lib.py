@@ -155,6 +155,21 @@ def stream_of(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def call(name: str, device, *args) -> None:
+    """Entry point ``name`` with ``args`` (device pointers as ints) and, last, the
+    current stream of ``device``; raises on an error.  The device is made
+    current only where it is not (a step of a small model is bound by the
+    host: guard and stream objects are 6 of its 20 us)."""
+    fn, index = getattr(_lib or load(), name), device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
+
+
 def dtype_code(dt) -> int:
     if dt == torch.bfloat16:
         return DTYPE_BF16

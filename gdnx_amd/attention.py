@@ -22,6 +22,10 @@ def _window(window, sinks):
     return min(window, 1 << 30), min(sinks, 1 << 30)
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _rows16(t):
     """t with D contiguous and every other stride a multiple of 16 bytes, as the
     kernels read it (views of a fused projection are taken as they are)."""
@@ -56,11 +60,9 @@ def _forward(q, k, v, window, sinks, scale, lengths, want_lse):
     lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if want_lse else None
     nws = lib.gdnx_win_attn_fwd_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
-    with torch.cuda.device(q.device):
-        rc = lib.gdnx_win_attn_fwd(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(lengths), _lib.ptr(y),
-                                   _lib.ptr(lse), _lib.ptr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq,
-                                   Hkv, D, window, sinks, scale, code, _lib.stream_of(q))
-    _lib.check(rc, "gdnx_win_attn_fwd")
+    _lib.call("gdnx_win_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths), y.data_ptr(),
+              _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
+              sinks, scale, code)
     return q, k, v, y, lse
 
 
@@ -88,12 +90,10 @@ class WindowAttentionFunction(torch.autograd.Function):
         nws = lib.gdnx_win_attn_bwd_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
         _need(nws >= 0, "invalid sizes")
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
-        with torch.cuda.device(q.device):
-            rc = lib.gdnx_win_attn_bwd(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(lengths), _lib.ptr(y),
-                                       _lib.ptr(lse), _lib.ptr(dy), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
-                                       _lib.ptr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk,
-                                       Hq, Hkv, D, window, sinks, scale, code, _lib.stream_of(q))
-        _lib.check(rc, "gdnx_win_attn_bwd")
+        _lib.call("gdnx_win_attn_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths),
+                  y.data_ptr(), lse.data_ptr(), dy.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                  ws.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
+                  sinks, scale, code)
         return dq, dk, dv, None, None, None, None
 
 
@@ -170,10 +170,7 @@ def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=Non
         k, v = _rows16(k.contiguous()), _rows16(v.contiguous())
     nws = lib.gdnx_paged_attn_workspace_bytes(NS, width, page, Hq, Hkv, D, window, sinks, code)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
-    with torch.cuda.device(q.device):
-        rc = lib.gdnx_paged_attn_step(_lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(k_pages), _lib.ptr(v_pages),
-                                      _lib.ptr(table), _lib.ptr(lengths), _lib.ptr(slots), _lib.ptr(out), _lib.ptr(ws),
-                                      NS, rows, width, n_pages, page, Hq, Hkv, D, window, sinks,
-                                      D ** -0.5 if scale is None else float(scale), code, _lib.stream_of(q))
-    _lib.check(rc, "gdnx_paged_attn_step")
+    _lib.call("gdnx_paged_attn_step", q.device, q.data_ptr(), _addr(k), _addr(v), k_pages.data_ptr(),
+              v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), _addr(slots), out.data_ptr(), _addr(ws), NS,
+              rows, width, n_pages, page, Hq, Hkv, D, window, sinks, D ** -0.5 if scale is None else float(scale), code)
     return out

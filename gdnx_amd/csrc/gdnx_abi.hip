@@ -1353,6 +1353,8 @@ extern "C" int gdnx_pages_write(const void* k_new, const void* v_new, void* k_pa
   a.k_pages = k_pages; a.v_pages = v_pages; a.k_new = k_new; a.v_new = v_new;
   a.table = const_cast<int*>(table); a.slots = slots; a.start = const_cast<int*>(start);
   a.n = n; a.n_new = n_new; a.rows = rows; a.width = width; a.page = page;
+  if (!prod_le(kMaxGroups, {2, layers, pages_write_groups(a)}))
+    return set_error(GDNX_ERR_SHAPE, "too many tokens in one call");
   return pages_write_dispatch(a, (hipStream_t)stream);
 }
 
@@ -1379,7 +1381,7 @@ extern "C" int gdnx_pages_fork(void* k_pages, void* v_pages, int* table, int* le
   int rc = check_pool(rows, width, n_pages, page);
   if (rc) return rc;
   if ((rc = check_pool_data(k_pages, v_pages, layers, Hkv, page, head_dim, dtype, a))) return rc;
-  if (n < 1 || n > (1 << 24)) return set_error(GDNX_ERR_SHAPE, "bad number of pairs %d", n);
+  if (n < 1 || n > (1 << 23)) return set_error(GDNX_ERR_SHAPE, "bad number of pairs %d", n);
   if (!table || !lengths || !refs || !parents || !children || !status)
     return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
   if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");

@@ -537,6 +537,7 @@ int pages_fork_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
 int pages_copy_dispatch(const PagesArgs& a, const int* src, const int* dst, hipStream_t stream);
 int pages_compact_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
 int pages_free_dispatch(const PagesArgs& a, hipStream_t stream);
+long long pages_write_groups(const PagesArgs& a);
 int pages_write_dispatch(const PagesArgs& a, hipStream_t stream);
 
 }  // namespace gdnx

@@ -19,8 +19,7 @@
 // reserve and fork change nothing unless every row can be served: status[0]
 // then holds the pages that were missing, status[1] the rows whose table row
 // is too short.
-#include "gdnx_common.hpp"
-#include "gdnx_internal.hpp"
+#include "attn_common.hpp"
 
 namespace gdnx {
 
@@ -169,37 +168,23 @@ __global__ void __launch_bounds__(PT) pages_fork_kernel(PagesArgs a, int* ws) {
       a.status[0] = need - got;
       a.status[1] = 0;
     }
+    for (int s = threadIdx.x; s < a.n; s += PT) lens[s] = -1;
     return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int s = wave; s < a.n; s += PW) {
+  for (int s = threadIdx.x; s < a.n; s += PT) {
     const int len = lens[s];
-    if (len < 0) continue;
-    const int full = len / a.page;
-    const int* tp = a.table + (size_t)a.slots[s] * a.width;
-    int* tc = a.table + (size_t)a.start[s] * a.width;
-    for (int i = lane; i < full; i += 64) {
-      const int pg = tp[i];
-      tc[i] = pg;
-      if (pg >= 0 && pg < a.n_pages) atomicAdd(&a.refs[pg], 1);
-    }
-    if (lane == 0) {
-      if (len % a.page != 0) {
-        const int pg = list[offs[s]], from = tp[full];
-        tc[full] = pg;
-        a.refs[pg] = 1;
-        src[s] = from;
-        if (from >= 0 && from < a.n_pages) dst[s] = pg;
-      }
-      a.lengths[a.start[s]] = len;
-    }
+    if (len <= 0 || len % a.page == 0) continue;
+    const int pg = list[offs[s]], full = len / a.page, from = a.table[(size_t)a.slots[s] * a.width + full];
+    a.table[(size_t)a.start[s] * a.width + full] = pg;
+    a.refs[pg] = 1;
+    src[s] = from;
+    if (from >= 0 && from < a.n_pages) dst[s] = pg;
   }
 }
 
 // A workgroup's 16 KB run of a page: 4 x 16 bytes a thread.
 constexpr int kRun = 16384;
 __device__ __forceinline__ void copy_run(char* dst, const char* src, long long bytes) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   u32x4 x[4];
   const long long at = 16LL * threadIdx.x;
 #pragma unroll
@@ -229,6 +214,28 @@ __device__ __forceinline__ void copy_pages(const PagesArgs& a, const int* src, c
 
 __global__ void __launch_bounds__(256) pages_copy_kernel(PagesArgs a, const int* src, const int* dst) {
   copy_pages(a, src, dst, a.n, blockIdx.x, gridDim.x);
+}
+
+// The second half of a fork: the first n workgroups share a pair's full pages
+// each (one workgroup's latencies, not one after the other as in the plan's
+// workgroup), the others copy the started ones.
+__global__ void __launch_bounds__(256) pages_share_kernel(PagesArgs a, const int* ws) {
+  const int *src = ws, *dst = ws + a.n, *lens = ws + 3 * a.n;
+  if ((int)blockIdx.x >= a.n) {
+    copy_pages(a, src, dst, a.n, blockIdx.x - a.n, gridDim.x - a.n);
+    return;
+  }
+  const int s = blockIdx.x, len = lens[s];
+  if (len < 0) return;
+  const int full = len / a.page, child = a.start[s];
+  const int* tp = a.table + (size_t)a.slots[s] * a.width;
+  int* tc = a.table + (size_t)child * a.width;
+  for (int i = threadIdx.x; i < full; i += 256) {
+    const int pg = tp[i];
+    tc[i] = pg;
+    if (pg >= 0 && pg < a.n_pages) atomicAdd(&a.refs[pg], 1);
+  }
+  if (threadIdx.x == 0) a.lengths[child] = len;
 }
 
 // ws: moves, then src[n_pages / 2], dst[n_pages / 2], then map[n_pages] (new
@@ -297,28 +304,41 @@ __global__ void __launch_bounds__(256) pages_free_kernel(PagesArgs a) {
   if (!a.trim && threadIdx.x == 0) a.lengths[r] = 0;
 }
 
-// New tokens [layers][n][n_new][Hkv][D] to their pages: 16 bytes a thread and step.
-__global__ void __launch_bounds__(256) pages_write_kernel(PagesArgs a) {
-  const int upr = a.row_bytes / 16;                            // 16-byte units of a head's row
-  const long long per = (long long)a.n * a.n_new * a.Hkv * upr, total = 2 * a.layers * per;
-  for (long long it = (long long)blockIdx.x * 256 + threadIdx.x; it < total; it += (long long)gridDim.x * 256) {
-    const bool is_v = it >= a.layers * per;
-    const long long x = is_v ? it - a.layers * per : it;
-    const int layer = (int)(x / per);
-    long long y = x % per;
-    const int u = (int)(y % upr); y /= upr;
-    const int h = (int)(y % a.Hkv); y /= a.Hkv;
-    const int t = (int)(y % a.n_new), s = (int)(y / a.n_new);
-    const int r = a.slots[s], st = a.start[s];
-    if (r < 0 || r >= a.rows || st < 0) continue;
-    const long long pos = (long long)st + t, col = pos / a.page;
-    if (col >= a.width) continue;
-    const int pg = a.table[(size_t)r * a.width + col];
+// New tokens [layers][n][n_new][Hkv][D] to their pages.  A workgroup takes
+// 1024 of a layer's 16-byte units, four a thread, all loaded before the first
+// is stored; units of a token follow each other, so its place is looked up
+// from small numbers (one wide division a workgroup).
+__global__ void __launch_bounds__(256) pages_write_kernel(PagesArgs a, unsigned per_layer) {
+  const unsigned upr = a.row_bytes / 16, upt = a.Hkv * upr;    // units of a head's row, of a token
+  const unsigned lk = blockIdx.x / per_layer, blk = blockIdx.x % per_layer;
+  const int layer = lk >> 1;
+  const long long tokens = (long long)a.n * a.n_new, first = (long long)blk * 1024;
+  const long long tok0 = first / upt;
+  const unsigned rem = (unsigned)(first - tok0 * upt);
+  const char* from = (const char*)((lk & 1) ? a.v_new : a.k_new) + ((long long)layer * tokens * upt + first) * 16;
+  char* pool = (char*)((lk & 1) ? a.v_pages : a.k_pages) + (long long)layer * a.n_pages * a.page_bytes;
+  const int s0 = (int)(tok0 / a.n_new), tr0 = (int)(tok0 - (long long)s0 * a.n_new);
+  u32x4 x[4];
+  long long to[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned v = e * 256 + threadIdx.x, r = rem + v, dt = r / upt, u = r - dt * upt;
+    to[e] = -1;
+    if (tok0 + dt >= tokens) continue;
+    x[e] = *(const u32x4*)(from + v * 16);
+    const unsigned tt = tr0 + dt, ds = tt / (unsigned)a.n_new;
+    const int s = s0 + ds, t = tt - ds * a.n_new, row = a.slots[s], st = a.start[s];
+    if (row < 0 || row >= a.rows || st < 0) continue;
+    const long long pos = (long long)st + t;
+    if (pos >= (long long)a.width * a.page) continue;
+    const int col = (int)pos / a.page, in = (int)pos - col * a.page, pg = a.table[(size_t)row * a.width + col];
     if (pg < 0 || pg >= a.n_pages) continue;
-    char* pool = (char*)(is_v ? a.v_pages : a.k_pages) + ((long long)layer * a.n_pages + pg) * a.page_bytes;
-    const char* from = (const char*)(is_v ? a.v_new : a.k_new) + x * 16;
-    *(uint4*)(pool + ((long long)h * a.page + pos % a.page) * a.row_bytes + u * 16) = *(const uint4*)from;
+    const unsigned h = u / upr;
+    to[e] = pg * a.page_bytes + ((long long)h * a.page + in) * a.row_bytes + (u - h * upr) * 16;
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (to[e] >= 0) *(u32x4*)(pool + to[e]) = x[e];
 }
 
 int pages_reserve_dispatch(const PagesArgs& a, int* ws, hipStream_t stream) {
@@ -330,7 +350,10 @@ int pages_fork_dispatch(const PagesArgs& a, int* ws, hipStream_t stream) {
   hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(PT), 0, stream, a, ws);
   const int rc = check_launch("pages_fork_kernel");
   if (rc) return rc;
-  return pages_copy_dispatch(a, ws, ws + a.n, stream);
+  const long long items = (long long)a.n * a.layers * 2 * ((a.page_bytes + kRun - 1) / kRun);
+  const unsigned grid = (unsigned)(a.n + (items < 8192 ? items : 8192));
+  hipLaunchKernelGGL(pages_share_kernel, dim3(grid), dim3(256), 0, stream, a, (const int*)ws);
+  return check_launch("pages_share_kernel");
 }
 
 int pages_copy_dispatch(const PagesArgs& a, const int* src, const int* dst, hipStream_t stream) {
@@ -354,9 +377,14 @@ int pages_free_dispatch(const PagesArgs& a, hipStream_t stream) {
 }
 
 int pages_write_dispatch(const PagesArgs& a, hipStream_t stream) {
-  const long long units = 2LL * a.layers * a.n * a.n_new * a.Hkv * (a.row_bytes / 16), wg = (units + 255) / 256;
-  hipLaunchKernelGGL(pages_write_kernel, dim3((unsigned)(wg < 16384 ? wg : 16384)), dim3(256), 0, stream, a);
+  const unsigned per_layer = pages_write_groups(a);
+  hipLaunchKernelGGL(pages_write_kernel, dim3(per_layer * 2 * a.layers), dim3(256), 0, stream, a, per_layer);
   return check_launch("pages_write_kernel");
+}
+
+// workgroups of one layer's keys (or values)
+long long pages_write_groups(const PagesArgs& a) {
+  return ((long long)a.n * a.n_new * a.Hkv * (a.row_bytes / 16) + 1023) / 1024;
 }
 
 }  // namespace gdnx

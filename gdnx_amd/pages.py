@@ -31,12 +31,13 @@ def _state(table, lengths, refs):
     return table.shape[0], table.shape[1], refs.shape[0]
 
 
-def _pools(k_pages, v_pages, n_pages=None):
+def _pools(k_pages, v_pages, ints, n_pages=None):
     """(layers, n_pages, Hkv, page, D, dtype code) of a pool with or without its layer axis."""
     _need(k_pages.is_cuda and k_pages.shape == v_pages.shape and k_pages.dim() in (4, 5)
           and k_pages.dtype == v_pages.dtype and k_pages.is_contiguous() and v_pages.is_contiguous()
-          and k_pages.device == v_pages.device,
-          "k_pages and v_pages must be contiguous CUDA (HIP) tensors of one shape [(layers,)n_pages,Hkv,page,D]")
+          and k_pages.device == v_pages.device == ints.device,
+          "k_pages and v_pages must be contiguous CUDA (HIP) tensors of one shape [(layers,)n_pages,Hkv,page,D], "
+          "on the table's device")
     shape = tuple(k_pages.shape) if k_pages.dim() == 5 else (1, *k_pages.shape)
     _need(n_pages is None or shape[1] == n_pages, f"the pool has {shape[1]} pages, refs {n_pages}")
     return (*shape, _lib.dtype_code(k_pages.dtype))
@@ -59,18 +60,16 @@ def pages_reserve(table, lengths, refs, slots, n_new: int, page: int, status):
     if slots.numel() == 0:
         return start
     ws = _workspace(slots.numel(), n_pages, table.device)
-    with torch.cuda.device(table.device):
-        rc = _lib.load().gdnx_pages_reserve(_lib.ptr(table), _lib.ptr(lengths), _lib.ptr(refs), _lib.ptr(slots),
-                                            _lib.ptr(start), _lib.ptr(status), _lib.ptr(ws), slots.numel(), int(n_new),
-                                            rows, width, n_pages, int(page), _lib.stream_of(table))
-    _lib.check(rc, "gdnx_pages_reserve")
+    _lib.call("gdnx_pages_reserve", table.device, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
+              slots.data_ptr(), start.data_ptr(), status.data_ptr(), ws.data_ptr(), slots.numel(), int(n_new), rows,
+              width, n_pages, int(page))
     return start
 
 
 def pages_write(k, v, k_pages, v_pages, table, slots, start):
     """Keys and values k, v [(layers,)n,T,Hkv,D] to the positions start[i] ..
     start[i] + T - 1 of table row slots[i] (start < 0: none of it)."""
-    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages)
+    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages, table)
     _ints(table, slots, start)
     _need(table.dim() == 2 and slots.dim() == 1 and start.shape == slots.shape,
           "table must be [rows,width], slots and start [n]")
@@ -82,26 +81,21 @@ def pages_write(k, v, k_pages, v_pages, table, slots, start):
     if k.numel() == 0:
         return
     k, v = attention._rows16(k.contiguous()), attention._rows16(v.contiguous())
-    with torch.cuda.device(table.device):
-        rc = _lib.load().gdnx_pages_write(_lib.ptr(k), _lib.ptr(v), _lib.ptr(k_pages), _lib.ptr(v_pages),
-                                          _lib.ptr(table), _lib.ptr(slots), _lib.ptr(start), layers, slots.numel(),
-                                          k.shape[-3], table.shape[0], table.shape[1], n_pages, page, Hkv, D, code,
-                                          _lib.stream_of(table))
-    _lib.check(rc, "gdnx_pages_write")
+    _lib.call("gdnx_pages_write", table.device, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+              table.data_ptr(), slots.data_ptr(), start.data_ptr(), layers, slots.numel(), k.shape[-3],
+              table.shape[0], table.shape[1], n_pages, page, Hkv, D, code)
 
 
 def pages_copy(k_pages, v_pages, src, dst):
     """Page src[i] onto page dst[i] (int32 [n]; either outside the pool:
     nothing) in every layer.  No page may be both a source and a destination."""
-    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages)
+    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages, src)
     _ints(src, dst)
     _need(src.dim() == 1 and src.shape == dst.shape, "src and dst must be [n]")
     if src.numel() == 0:
         return
-    with torch.cuda.device(src.device):
-        rc = _lib.load().gdnx_pages_copy(_lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(src), _lib.ptr(dst), layers,
-                                         src.numel(), n_pages, page, Hkv, D, code, _lib.stream_of(src))
-    _lib.check(rc, "gdnx_pages_copy")
+    _lib.call("gdnx_pages_copy", src.device, k_pages.data_ptr(), v_pages.data_ptr(), src.data_ptr(), dst.data_ptr(),
+              layers, src.numel(), n_pages, page, Hkv, D, code)
 
 
 def pages_fork(k_pages, v_pages, table, lengths, refs, parents, children, status):
@@ -109,7 +103,7 @@ def pages_fork(k_pages, v_pages, table, lengths, refs, parents, children, status
     pages are shared, a started last page is copied to a free one.  If the pool
     lacks pages, nothing changes and status[0] holds how many were missing."""
     rows, width, n_pages = _state(table, lengths, refs)
-    layers, _, Hkv, page, D, code = _pools(k_pages, v_pages, n_pages)
+    layers, _, Hkv, page, D, code = _pools(k_pages, v_pages, table, n_pages)
     _ints(table, parents, children, status)
     _need(parents.dim() == 1 and parents.shape == children.shape and tuple(status.shape) == (2,),
           "parents and children must be [n], status [2]")
@@ -117,12 +111,9 @@ def pages_fork(k_pages, v_pages, table, lengths, refs, parents, children, status
     if n == 0:
         return
     ws = _workspace(n, n_pages, table.device)
-    with torch.cuda.device(table.device):
-        rc = _lib.load().gdnx_pages_fork(_lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(table), _lib.ptr(lengths),
-                                         _lib.ptr(refs), _lib.ptr(parents), _lib.ptr(children), _lib.ptr(status),
-                                         _lib.ptr(ws), layers, n, rows, width, n_pages, page, Hkv, D, code,
-                                         _lib.stream_of(table))
-    _lib.check(rc, "gdnx_pages_fork")
+    _lib.call("gdnx_pages_fork", table.device, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+              lengths.data_ptr(), refs.data_ptr(), parents.data_ptr(), children.data_ptr(), status.data_ptr(),
+              ws.data_ptr(), layers, n, rows, width, n_pages, page, Hkv, D, code)
 
 
 def pages_free(table, lengths, refs, slots):
@@ -131,10 +122,8 @@ def pages_free(table, lengths, refs, slots):
     _ints(table, slots)
     if slots.numel() == 0:
         return
-    with torch.cuda.device(table.device):
-        rc = _lib.load().gdnx_pages_free(_lib.ptr(table), _lib.ptr(lengths), _lib.ptr(refs), _lib.ptr(slots),
-                                         slots.numel(), rows, width, n_pages, _lib.stream_of(table))
-    _lib.check(rc, "gdnx_pages_free")
+    _lib.call("gdnx_pages_free", table.device, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
+              slots.data_ptr(), slots.numel(), rows, width, n_pages)
 
 
 def pages_trim(table, lengths, refs, slots, window: int, sinks: int, page: int):
@@ -144,29 +133,24 @@ def pages_trim(table, lengths, refs, slots, window: int, sinks: int, page: int):
     _ints(table, slots)
     if slots.numel() == 0:
         return
-    with torch.cuda.device(table.device):
-        rc = _lib.load().gdnx_pages_trim(_lib.ptr(table), _lib.ptr(lengths), _lib.ptr(refs), _lib.ptr(slots),
-                                         int(window), int(sinks), slots.numel(), rows, width, n_pages, int(page),
-                                         _lib.stream_of(table))
-    _lib.check(rc, "gdnx_pages_trim")
+    _lib.call("gdnx_pages_trim", table.device, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
+              slots.data_ptr(), int(window), int(sinks), slots.numel(), rows, width, n_pages, int(page))
 
 
 def pages_compact(k_pages, v_pages, table, refs, out=None):
     """Moves the used pages at or beyond the number of used pages, in order, into
     the free pages below it.  Returns (table, refs) as they are then: the
     inputs, changed in place, or the pair of tensors ``out``."""
-    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages, refs.shape[0])
+    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages, table, refs.shape[0])
     _ints(table, refs)
     _need(table.dim() == 2 and refs.dim() == 1, "table must be [rows,width], refs [n_pages]")
     t_out, r_out = (table, refs) if out is None else out
     _ints(table, t_out, r_out)
     _need(t_out.shape == table.shape and r_out.shape == refs.shape, "out must have the shapes of table and refs")
     ws = _workspace(0, n_pages, table.device)
-    with torch.cuda.device(table.device):
-        rc = _lib.load().gdnx_pages_compact(_lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(table), _lib.ptr(refs),
-                                            _lib.ptr(t_out), _lib.ptr(r_out), _lib.ptr(ws), layers, table.shape[0],
-                                            table.shape[1], n_pages, page, Hkv, D, code, _lib.stream_of(table))
-    _lib.check(rc, "gdnx_pages_compact")
+    _lib.call("gdnx_pages_compact", table.device, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+              refs.data_ptr(), t_out.data_ptr(), r_out.data_ptr(), ws.data_ptr(), layers, table.shape[0],
+              table.shape[1], n_pages, page, Hkv, D, code)
     return t_out, r_out
 
 
