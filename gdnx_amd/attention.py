@@ -10,6 +10,8 @@ gdnx_paged_attn_step in include/gdnx.h).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -22,6 +24,12 @@ def _window(window, sinks):
     return min(window, 1 << 30), min(sinks, 1 << 30)
 
 
+@functools.lru_cache(maxsize=4096)
+def _bytes(query, *sizes):
+    """A workspace's bytes: the library's size query, once per sizes."""
+    return getattr(_lib.load(), query)(*sizes)
+
+
 def _addr(t):
     return None if t is None else t.data_ptr()
 
@@ -29,10 +37,12 @@ def _addr(t):
 def _rows16(t):
     """t with D contiguous and every other stride a multiple of 16 bytes, as the
     kernels read it (views of a fused projection are taken as they are)."""
-    unit = 16 // t.element_size()
-    if (t.stride(-1) == 1 and all(s % unit == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
-            and (t.dim() < 4 or t.stride(1) <= 1 << 24)):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t                    # (D is 64 or 128: every row is whole units)
+        unit = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(s % unit == 0 for s in t.stride()[:-1]) and t.stride(1) <= 1 << 24:
+            return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
@@ -44,7 +54,7 @@ def _check(q, k, v, lengths):
     B, Tq, Hq, D = q.shape
     Tk, Hkv = k.shape[1:3]
     _need(k.shape[0] == B and k.shape[3] == D, "q, k, v must share batch and head dim")
-    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key heads ({Hkv})")
+    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, "query heads must be a multiple of key heads")
     if lengths is not None:
         _need(tuple(lengths.shape) == (B,) and lengths.dtype == torch.int32 and lengths.is_contiguous()
               and lengths.device == q.device, "lengths must be contiguous int32 [B] on q's device")
@@ -52,13 +62,12 @@ def _check(q, k, v, lengths):
 
 
 def _forward(q, k, v, window, sinks, scale, lengths, want_lse):
-    lib = _lib.load()
     B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
     code = _lib.dtype_code(q.dtype)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     y = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if want_lse else None
-    nws = lib.gdnx_win_attn_fwd_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
+    nws = _bytes("gdnx_win_attn_fwd_workspace_bytes", B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
     _lib.call("gdnx_win_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths), y.data_ptr(),
               _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
@@ -80,14 +89,13 @@ class WindowAttentionFunction(torch.autograd.Function):
     def backward(ctx, dy, _):
         q, k, v, lengths, y, lse = ctx.saved_tensors
         window, sinks, scale = ctx.args
-        lib = _lib.load()
         B, Tq, Hq, D = q.shape
         Tk, Hkv = k.shape[1:3]
         code = _lib.dtype_code(q.dtype)
         dy = _rows16(dy.to(q.dtype).contiguous())
         dq = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
         dk, dv = (torch.empty(B, Tk, Hkv, D, dtype=q.dtype, device=q.device) for _ in range(2))
-        nws = lib.gdnx_win_attn_bwd_workspace_bytes(B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
+        nws = _bytes("gdnx_win_attn_bwd_workspace_bytes", B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
         _need(nws >= 0, "invalid sizes")
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("gdnx_win_attn_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths),
@@ -132,31 +140,32 @@ def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=Non
     value, which the call also writes to their page; None where they are there
     already.  window, sinks and scale as in ``window_attention``.  Returns y
     [NS,Hq,D] (or ``out``)."""
-    lib = _lib.load()
     window, sinks = _window(window, sinks)
+    dev, dtype = q.device, q.dtype
     _need(q.is_cuda and q.dim() == 3, "q must be a CUDA (HIP) tensor [NS,Hq,D]")
     NS, Hq, D = q.shape
     _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == D,
           "k_pages and v_pages must share shape [n_pages,Hkv,page,D]")
     n_pages, Hkv, page, _ = k_pages.shape
-    _need(Hkv > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key heads ({Hkv})")
-    _need(table.dim() == 2 and tuple(lengths.shape) == (table.shape[0],), "table must be [rows,width], lengths [rows]")
+    _need(Hkv > 0 and Hq % Hkv == 0, "query heads must be a multiple of key heads")
+    _need(table.dim() == 2 and lengths.dim() == 1 and lengths.shape[0] == table.shape[0],
+          "table must be [rows,width], lengths [rows]")
     rows, width = table.shape
     _need((k is None) == (v is None), "k and v must be given together")
-    new = () if k is None else (k, v)
-    for t in new:
-        _need(tuple(t.shape) == (NS, Hkv, D), "k and v must be [NS,Hkv,D]")
-    ints = (table, lengths) if slots is None else (table, lengths, slots)
+    if k is not None:
+        _need(k.shape == v.shape == (NS, Hkv, D) and k.dtype == v.dtype == dtype and k.device == v.device == dev,
+              "k and v must be [NS,Hkv,D] of q's dtype on q's device")
+        k, v = _rows16(k.contiguous()), _rows16(v.contiguous())
     if slots is None:
-        _need(NS <= rows, f"{NS} rows for a table of {rows}")
+        _need(NS <= rows, "more rows than the table has: name their slots")
     else:
-        _need(tuple(slots.shape) == (NS,), "slots must be [NS]")
-    for t in ints:
-        _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == q.device,
-              "table, lengths and slots must be contiguous int32 on q's device")
-    for t in (k_pages, v_pages, *new):
-        _need(t.dtype == q.dtype and t.device == q.device, "q, k, v and the pages must share dtype and device")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), "k_pages and v_pages must be contiguous")
+        _need(slots.shape == (NS,) and slots.dtype == torch.int32 and slots.is_contiguous() and slots.device == dev,
+              "slots must be contiguous int32 [NS] on q's device")
+    _need(table.dtype == lengths.dtype == torch.int32 and table.is_contiguous() and lengths.is_contiguous()
+          and table.device == lengths.device == dev, "table and lengths must be contiguous int32 on q's device")
+    _need(k_pages.dtype == v_pages.dtype == dtype and k_pages.device == v_pages.device == dev
+          and k_pages.is_contiguous() and v_pages.is_contiguous(),
+          "k_pages and v_pages must be contiguous, of q's dtype and device")
     code = _lib.dtype_code(q.dtype)
     if out is None:
         out = torch.empty(NS, Hq, D, dtype=q.dtype, device=q.device)
@@ -166,10 +175,8 @@ def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=Non
     if NS == 0:
         return out
     q = _rows16(q.contiguous())
-    if new:
-        k, v = _rows16(k.contiguous()), _rows16(v.contiguous())
-    nws = lib.gdnx_paged_attn_workspace_bytes(NS, width, page, Hq, Hkv, D, window, sinks, code)
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
+    nws = _bytes("gdnx_paged_attn_workspace_bytes", NS, width, page, Hq, Hkv, D, window, sinks, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
     _lib.call("gdnx_paged_attn_step", q.device, q.data_ptr(), _addr(k), _addr(v), k_pages.data_ptr(),
               v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), _addr(slots), out.data_ptr(), _addr(ws), NS,
               rows, width, n_pages, page, Hq, Hkv, D, window, sinks, D ** -0.5 if scale is None else float(scale), code)
