@@ -88,29 +88,6 @@ template <int D> struct LaneMap {
   }
 };
 
-// Rows of one key head: (query, head of the group) pairs, heads fastest; row r
-// of a tile that starts at row `first`.
-struct RowMap {
-  int i0, rem, G;
-  unsigned magic;       // ceil(2^32 / G): exact for the small numbers of a tile
-  __device__ __forceinline__ RowMap(int first, int G_, unsigned magic_) : G(G_), magic(magic_) {
-    i0 = first / G;
-    rem = first - i0 * G;
-  }
-  __device__ __forceinline__ void advance(int rows) {
-    const int q = div(rem + rows);
-    i0 += q;
-    rem += rows - q * G;
-  }
-  __device__ __forceinline__ int div(int x) const { return G == 1 ? x : (int)__umulhi((unsigned)x, magic); }
-  __device__ __forceinline__ void at(int r, int* i, int* g) const {
-    const int x = r + rem, q = div(x);
-    *i = i0 + q;
-    *g = x - q * G;
-  }
-  __device__ __forceinline__ int last(int r) const { return i0 + div(r + rem); }      // the query of row r
-};
-
 // A tile of BK rows of two matrices, by way of registers: 256 threads, rows
 // clamped to the last valid one (what lies beyond is masked).  Offsets within
 // a tile are 32-bit: token strides stay below 2^24 elements.

@@ -1,314 +1,484 @@
-// Attention with a sliding window and sinks, forward and backward (gfx950):
-// the kernels that serve every type and size.
+// Attention with a sliding window and sinks (gfx950): the rules, the shares of
+// the work, and the float32 kernels.
 //
 //   P_ij = exp(s q_i.k_j - lse_i) over the visible j,  y_i = sum_j P_ij v_j
 //   dV = P^T dY;  dP = dY V^T;  dS = P o (dP - delta),  delta_i = dY_i.Y_i;
 //   dQ = s dS K;  dK = s dS^T Q, both summed over a key head's query heads.
 //
-// One wave owns 16 queries (forward, dq) or 16 keys (dk, dv).  The scores are
-// formed transposed to what they are contracted over next, so that a score
-// tile's accumulators are the next product's operand: S^T = K Q^T feeds
-// O^T = V^T P^T and dQ^T = K^T dS^T; S = Q K^T feeds dV^T = dY^T P and
+// Rows are (query, query head of the group) pairs with the heads fastest, so
+// grouped heads share the key tiles and a tile's rows span few positions.  The
+// scores are formed transposed to what they are contracted over next, so that
+// a score tile's accumulators are the next product's operand: S^T = K Q^T
+// feeds O^T = V^T P^T and dQ^T = K^T dS^T; S = Q K^T feeds dV^T = dY^T P and
 // dK^T = Q^T dS.  Softmax statistics, sums and products are float32.
-#include "attn_common.hpp"
+//
+// Float32: v_mfma_f32_16x16x4_f32, a wave owns 16 rows (forward, dq) or 16
+// keys (dk, dv); tiles of 32 keys (rows) by way of registers into LDS,
+// double-buffered, one barrier a tile.  Rows of a tile are D + 4 words apart,
+// which keeps both reads (16 rows of 4 words, 4 x 16 words) off each other's
+// banks.
+#include "attn_spans.hpp"
 
 namespace gdnx {
 
-// Fragment over rows kb.. of a row-major LDS tile, column c of the lane.
-template <int LD> __device__ __forceinline__ bf16x8 ld_frag_rows(const bf16* t, int kb, int c, int g) {
-  bf16x8 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[i] = t[(kb + 4 * g + i) * LD + c];
-    r[4 + i] = t[(kb + 16 + 4 * g + i) * LD + c];
-  }
-  return r;
-}
-template <int LD> __device__ __forceinline__ f32x4 ld_frag_rows(const float* t, int kb, int c, int g) {
+namespace {
+
+template <int D> struct F32Tile {
+  static constexpr int LD = D + 4, NS = D / 16, BT = 32, WORDS = BT * LD;
+};
+
+// Fragment over rows kb .. kb + 15 of a tile, column c of the lane.
+template <int LD> __device__ __forceinline__ f32x4 ld_cols(const float* t, int kb, int c, int g) {
   f32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = t[(kb + 4 * g + i) * LD + c];
   return r;
 }
 
-// Rows [r0, r0 + N) of a strided [rows][D] matrix into an LDS tile; rows
-// outside [0, end) are zero, so that what padding holds never enters a product.
-template <typename CT, int D, int N, int LD, int TH>
-__device__ __forceinline__ void stage_rows(CT* dst, const CT* src, long long stride, int r0, int end, int tid) {
-  constexpr int EPU = 16 / sizeof(CT), UPR = D / EPU;
+// 32 rows of two matrices by way of registers; a row's places come from
+// at(r, &a, &b), which clamps r to a valid row.
+template <int D> struct F32Stage {
+  static constexpr int UPR = D / 4, N = 32 * UPR / 256, STEP = 256 / UPR;
+  f32x4 x[N], y[N];
+  int row, unit;
+  __device__ __forceinline__ F32Stage(int tid) : row(tid / UPR), unit(tid % UPR) {}
+  template <typename At> __device__ __forceinline__ void load(const At& at) {
 #pragma unroll
-  for (int u = tid; u < N * UPR; u += TH) {
-    const int r = u / UPR, c = (u % UPR) * EPU;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r0 + r >= 0 && r0 + r < end) x = *(const uint4*)(src + (long long)(r0 + r) * stride + c);
-    *(uint4*)(dst + r * LD + c) = x;
+    for (int i = 0; i < N; ++i) {
+      const float *pa, *pb;
+      at(row + i * STEP, &pa, &pb);
+      x[i] = *(const f32x4*)(pa + 4 * unit);
+      y[i] = *(const f32x4*)(pb + 4 * unit);
+    }
   }
-}
-
-// A wave's 16 rows as fragments (row n of the lane); rows outside are zero.
-template <typename CT, int D>
-__device__ __forceinline__ void load_row_frags(typename FragT<CT>::type* f, const CT* src, long long stride, int row,
-                                               bool ok, int g) {
-  constexpr int KS = FragT<CT>::KSTEP;
+  __device__ __forceinline__ void store(float* ta, float* tb) const {
 #pragma unroll
-  for (int s = 0; s < D / KS; ++s) {
-    if (ok) f[s] = ld_frag(src + (long long)row * stride + s * KS, g);
-    else f[s] = typename FragT<CT>::type{};
+    for (int i = 0; i < N; ++i) {
+      const int o = (row + i * STEP) * F32Tile<D>::LD + 4 * unit;
+      *(f32x4*)(ta + o) = x[i];
+      *(f32x4*)(tb + o) = y[i];
+    }
   }
-}
-
-template <typename CT, int D> struct WinTile {
-  static constexpr int BK = 32, NW = 4, BQ = 16 * NW, TH = 64 * NW, LD = D + 16 / (int)sizeof(CT);
-  static constexpr int KS = FragT<CT>::KSTEP, NS = D / KS, TPS = FragT<CT>::TPS, NT = D / 16;
 };
 
-template <typename CT, int D>
-__global__ void __launch_bounds__(256) win_attn_fwd_kernel(WinAttnArgs a) {
-  using W = WinTile<CT, D>;
-  typedef typename FragT<CT>::type Frag;
-  __shared__ __attribute__((aligned(16))) CT sk[W::BK * W::LD], sv[W::BK * W::LD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int nqt = (a.Tq + W::BQ - 1) / W::BQ, G = a.Hq / a.Hkv;
-  // work order: a key head's query heads and tiles are neighbours (one XCD's L2)
-  const int w = xcd_remap(blockIdx.x, gridDim.x);
-  const int h = (w / nqt) % a.Hq, b = w / nqt / a.Hq, i0 = (w % nqt) * W::BQ, hk = h / G;
+// The rows of a workgroup of the forward and dq: 64 rows, a lane's row n of
+// its wave's 16, and the positions that they span.
+struct F32Rows {
+  RowMap rm;
+  int i, h, p, wg0, wg1, wv0, wv1;
+  bool rows_ok;
+  __device__ __forceinline__ F32Rows(int tile, int wave, int n, int hk, int G, unsigned magic, int Tq, int off, int len)
+      : rm(tile * 64, G, magic) {
+    rm.at(wave * 16 + n, &i, &h);
+    h += hk * G;
+    p = i < Tq && i + off < len ? i + off : -1;
+    wg0 = rm.i0 + off;
+    wg1 = min(rm.last(63), Tq - 1) + off;
+    wv0 = rm.last(wave * 16) + off;
+    const int last = rm.last(wave * 16 + 15);
+    wv1 = min(min(last, Tq - 1) + off, len - 1);
+    rows_ok = last < Tq && last + off < len && wv0 >= 0;
+  }
+  __device__ __forceinline__ bool some(int j0, int window, int sinks) const {
+    return j0 <= wv1 && (j0 + 31 > wv0 - window || j0 < sinks);
+  }
+  __device__ __forceinline__ bool all(int j0, int window, int sinks) const {
+    return rows_ok && j0 + 31 <= wv0 && (wv1 - j0 < window || j0 + 32 <= sinks);
+  }
+};
+
+}  // namespace
+
+template <int D> __global__ void __launch_bounds__(256, 2) win_fwd_f32_kernel(WinAttnArgs a) {
+  using T = F32Tile<D>;
+  __shared__ __attribute__((aligned(16))) float smem[4 * T::WORDS];       // two buffers of K, V
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 63) / 64;
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B; w /= a.B;
+  const int part = w % a.parts, tile = nt - 1 - w / a.parts;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
-  const CT* qb = (const CT*)a.q + b * a.qs[0] + h * a.qs[2];
-  const CT* kb = (const CT*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const CT* vb = (const CT*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const int i = i0 + wave * 16 + n;
-  const int p = i < a.Tq && i + off < len ? i + off : -1;
-  Frag qf[W::NS];
-  load_row_frags<CT, D>(qf, qb, a.qs[1], i, p >= 0, g);
+  const F32Rows rows(tile, wave, n, hk, G, a.g_magic, a.Tq, off, len);
+  const float* kb = (const float*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const float* vb = (const float*)a.v + b * a.vs[0] + hk * a.vs[2];
+  f32x4 qf[T::NS];
+  {
+    const float* qp = (const float*)a.q + b * a.qs[0] + (rows.p >= 0 ? rows.i * a.qs[1] + rows.h * a.qs[2] : 0);
+#pragma unroll
+    for (int c = 0; c < T::NS; ++c) qf[c] = *(const f32x4*)(qp + 16 * c + 4 * g);
+  }
   const float sc = a.scale * kLog2e;
-  f32x4 o[W::NT];
-#pragma unroll
-  for (int t = 0; t < W::NT; ++t) o[t] = zero4();
-  float m = -INFINITY, l = 0.f;
-  const KeyTiles<W::BK> kt(i0 + off, min(i0 + W::BQ, a.Tq) - 1 + off, len, a.window, a.sinks);
-  for (int it = 0; it < kt.count; ++it) {
+  const KeyTiles<32> kt(rows.wg0, rows.wg1, len, a.window, a.sinks);
+  const int per = (kt.count + a.parts - 1) / a.parts, t0 = part * per, t1 = min(kt.count, t0 + per);
+  F32Stage<D> st(tid);
+  const auto load = [&](int it) {
     const int j0 = kt.start(it);
-    __syncthreads();
-    stage_rows<CT, D, W::BK, W::LD, W::TH>(sk, kb, a.ks[1], j0, len, tid);
-    stage_rows<CT, D, W::BK, W::LD, W::TH>(sv, vb, a.vs[1], j0, len, tid);
-    __syncthreads();
-    f32x4 s[2];
+    st.load([&](int r, const float** x, const float** y) {
+      const long long j = min(j0 + r, len - 1);
+      *x = kb + j * a.ks[1];
+      *y = vb + j * a.vs[1];
+    });
+  };
+  f32x4 o[T::NS];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = zero4();
+  for (int t = 0; t < T::NS; ++t) o[t] = zero4();
+  float m = -INFINITY, l = 0.f;
+  if (t0 < t1) {
+    load(t0);
+    st.store(smem, smem + T::WORDS);
+  }
+  lds_barrier();
+  for (int it = t0; it < t1; ++it) {
+    const int j0 = kt.start(it);
+    const float *sk = smem + ((it - t0) & 1) * 2 * T::WORDS, *sv = sk + T::WORDS;
+    load(min(it + 1, t1 - 1));
+    if (rows.some(j0, a.window, a.sinks)) {
+      const bool all = rows.all(j0, a.window, a.sinks);
+      f32x4 s[2];
 #pragma unroll
-      for (int c = 0; c < W::NS; ++c) mma(s[u], ld_frag(sk + (16 * u + n) * W::LD + c * W::KS, g), qf[c]);
+      for (int u = 0; u < 2; ++u) {
+        s[u] = zero4();
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        s[u][e] = attn_visible(p, j0 + 16 * u + 4 * g + e, a.window, a.sinks) ? s[u][e] * sc : -INFINITY;
-    }
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
-    const float f = exp2f(m - ms);
-    float sum = 0.f;
+        for (int c = 0; c < T::NS; ++c) mma(s[u], ld_frag(sk + (16 * u + n) * T::LD + 16 * c, g), qf[c]);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[u][e] = exp2f(s[u][e] - ms);
-        sum += s[u][e];
+        for (int e = 0; e < 4; ++e)
+          s[u][e] = all || attn_visible(rows.p, j0 + 16 * u + 4 * g + e, a.window, a.sinks) ? s[u][e] * sc : -INFINITY;
       }
-    l = l * f + sum;
-    m = mn;
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
+      const float f = exp2f(m - ms);
+      float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < W::NT; ++t) {
-      o[t] *= f;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int c = 0; c < W::BK / W::KS; ++c)
-        mma(o[t], ld_frag_rows<W::LD>(sv, c * W::KS, 16 * t + n, g),
-            acc_frag((CT*)nullptr, s[c * W::TPS], s[c * W::TPS + W::TPS - 1]));
+        for (int e = 0; e < 4; ++e) {
+          s[u][e] = exp2f(s[u][e] - ms);
+          sum += s[u][e];
+        }
+      l = l * f + sum;
+      m = mn;
+#pragma unroll
+      for (int t = 0; t < T::NS; ++t) {
+        o[t] *= f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) mma(o[t], ld_cols<T::LD>(sv, 16 * u, 16 * t + n, g), s[u]);
+      }
     }
+    float* next = smem + ((it - t0 + 1) & 1) * 2 * T::WORDS;
+    st.store(next, next + T::WORDS);
+    lds_barrier();
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (i >= a.Tq) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
-  CT* yb = (CT*)a.y + (((long long)b * a.Tq + i) * a.Hq + h) * D;
+  if (rows.i >= a.Tq) return;
+  const long long r = ((long long)b * a.Tq + rows.i) * a.Hq + rows.h;
+  if (a.parts > 1) {
+    float* po = part_out(a, part, r) + 4 * g;
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t)
-    st4(yb + 16 * t + 4 * g, o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv);
-  if (g == 0 && a.lse) a.lse[((long long)b * a.Hq + h) * a.Tq + i] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    for (int t = 0; t < T::NS; ++t) *(f32x4*)(po + 16 * t) = o[t];
+    if (g == 0) {
+      float* ml = part_stats(a, part, r);
+      ml[0] = m;
+      ml[1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int t = 0; t < T::NS; ++t) *(f32x4*)((float*)a.y + r * D + 16 * t + 4 * g) = o[t] * inv;
+  if (g == 0 && a.lse)
+    a.lse[((long long)b * a.Hq + rows.h) * a.Tq + rows.i] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // dq, and delta for the dk / dv kernel
-template <typename CT, int D>
-__global__ void __launch_bounds__(256) win_attn_dq_kernel(WinAttnBwdArgs a) {
-  using W = WinTile<CT, D>;
-  typedef typename FragT<CT>::type Frag;
-  __shared__ __attribute__((aligned(16))) CT sk[W::BK * W::LD], sv[W::BK * W::LD];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int nqt = (a.Tq + W::BQ - 1) / W::BQ, G = a.Hq / a.Hkv;
-  const int w = xcd_remap(blockIdx.x, gridDim.x);
-  const int h = (w / nqt) % a.Hq, b = w / nqt / a.Hq, i0 = (w % nqt) * W::BQ, hk = h / G;
+template <int D> __global__ void __launch_bounds__(256, 2) win_dq_f32_kernel(WinAttnBwdArgs a) {
+  using T = F32Tile<D>;
+  __shared__ __attribute__((aligned(16))) float smem[4 * T::WORDS];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 63) / 64;
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B, tile = nt - 1 - w / a.B;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
-  const CT* kb = (const CT*)a.k + b * a.ks[0] + hk * a.ks[2];
-  const CT* vb = (const CT*)a.v + b * a.vs[0] + hk * a.vs[2];
-  const int i = i0 + wave * 16 + n;
-  const int p = i < a.Tq && i + off < len ? i + off : -1;
-  const long long row = ((long long)b * a.Tq + i) * a.Hq + h, srow = ((long long)b * a.Hq + h) * a.Tq + i;
-  Frag qf[W::NS], gf[W::NS];
-  load_row_frags<CT, D>(qf, (const CT*)a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], i, p >= 0, g);
-  load_row_frags<CT, D>(gf, (const CT*)a.dy + row * D, 0, 0, p >= 0, g);
+  const F32Rows rows(tile, wave, n, hk, G, a.g_magic, a.Tq, off, len);
+  const float* kb = (const float*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const float* vb = (const float*)a.v + b * a.vs[0] + hk * a.vs[2];
+  const long long r = ((long long)b * a.Tq + rows.i) * a.Hq + rows.h;
+  f32x4 qf[T::NS], gf[T::NS];
   float delta = 0.f, lse = 0.f;
   {
-    Frag yf[W::NS];
-    load_row_frags<CT, D>(yf, (const CT*)a.y + row * D, 0, 0, p >= 0, g);
+    const float* qp = (const float*)a.q + b * a.qs[0] + (rows.p >= 0 ? rows.i * a.qs[1] + rows.h * a.qs[2] : 0);
+    const long long row = rows.p >= 0 ? r * D : 0, srow = ((long long)b * a.Hq + rows.h) * a.Tq + rows.i;
 #pragma unroll
-    for (int s = 0; s < W::NS; ++s)
+    for (int c = 0; c < T::NS; ++c) {
+      qf[c] = *(const f32x4*)(qp + 16 * c + 4 * g);
+      gf[c] = *(const f32x4*)((const float*)a.dy + row + 16 * c + 4 * g);
+      const f32x4 yf = *(const f32x4*)((const float*)a.y + row + 16 * c + 4 * g);
 #pragma unroll
-      for (int e = 0; e < (int)(sizeof(Frag) / sizeof(CT)); ++e) delta += to_f(gf[s][e]) * to_f(yf[s][e]);
+      for (int e = 0; e < 4; ++e) delta += gf[c][e] * yf[e];
+    }
     delta += __shfl_xor(delta, 16, 64);
     delta += __shfl_xor(delta, 32, 64);
-    if (g == 0 && i < a.Tq) a.delta[srow] = delta;
-    if (p >= 0) lse = a.lse[srow] * kLog2e;
+    if (rows.p >= 0) {
+      lse = a.lse[srow] * kLog2e;
+      if (g == 0) a.delta[srow] = delta;
+    }
   }
   const float sc = a.scale * kLog2e;
-  f32x4 o[W::NT];
+  const KeyTiles<32> kt(rows.wg0, rows.wg1, len, a.window, a.sinks);
+  F32Stage<D> st(tid);
+  const auto load = [&](int it) {
+    const int j0 = kt.start(it);
+    st.load([&](int x, const float** pk, const float** pv) {
+      const long long j = min(j0 + x, len - 1);
+      *pk = kb + j * a.ks[1];
+      *pv = vb + j * a.vs[1];
+    });
+  };
+  f32x4 o[T::NS];
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t) o[t] = zero4();
-  const KeyTiles<W::BK> kt(i0 + off, min(i0 + W::BQ, a.Tq) - 1 + off, len, a.window, a.sinks);
+  for (int t = 0; t < T::NS; ++t) o[t] = zero4();
+  if (kt.count > 0) {
+    load(0);
+    st.store(smem, smem + T::WORDS);
+  }
+  lds_barrier();
   for (int it = 0; it < kt.count; ++it) {
     const int j0 = kt.start(it);
-    __syncthreads();
-    stage_rows<CT, D, W::BK, W::LD, W::TH>(sk, kb, a.ks[1], j0, len, tid);
-    stage_rows<CT, D, W::BK, W::LD, W::TH>(sv, vb, a.vs[1], j0, len, tid);
-    __syncthreads();
-    f32x4 ds[2];
+    const float *sk = smem + (it & 1) * 2 * T::WORDS, *sv = sk + T::WORDS;
+    load(min(it + 1, kt.count - 1));
+    if (rows.some(j0, a.window, a.sinks)) {
+      const bool all = rows.all(j0, a.window, a.sinks);
+      f32x4 ds[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x4 s = zero4(), dp = zero4();
+      for (int u = 0; u < 2; ++u) {
+        f32x4 s = zero4(), dp = zero4();
 #pragma unroll
-      for (int c = 0; c < W::NS; ++c) {
-        mma(s, ld_frag(sk + (16 * u + n) * W::LD + c * W::KS, g), qf[c]);
-        mma(dp, ld_frag(sv + (16 * u + n) * W::LD + c * W::KS, g), gf[c]);
+        for (int c = 0; c < T::NS; ++c) {
+          mma(s, ld_frag(sk + (16 * u + n) * T::LD + 16 * c, g), qf[c]);
+          mma(dp, ld_frag(sv + (16 * u + n) * T::LD + 16 * c, g), gf[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          ds[u][e] = all || attn_visible(rows.p, j0 + 16 * u + 4 * g + e, a.window, a.sinks)
+                         ? exp2f(s[e] * sc - lse) * (dp[e] - delta) : 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        ds[u][e] = attn_visible(p, j0 + 16 * u + 4 * g + e, a.window, a.sinks)
-                       ? exp2f(s[e] * sc - lse) * (dp[e] - delta) * a.scale : 0.f;
+      for (int t = 0; t < T::NS; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) mma(o[t], ld_cols<T::LD>(sk, 16 * u, 16 * t + n, g), ds[u]);
     }
-#pragma unroll
-    for (int t = 0; t < W::NT; ++t)
-#pragma unroll
-      for (int c = 0; c < W::BK / W::KS; ++c)
-        mma(o[t], ld_frag_rows<W::LD>(sk, c * W::KS, 16 * t + n, g),
-            acc_frag((CT*)nullptr, ds[c * W::TPS], ds[c * W::TPS + W::TPS - 1]));
+    float* next = smem + ((it + 1) & 1) * 2 * T::WORDS;
+    st.store(next, next + T::WORDS);
+    lds_barrier();
   }
-  if (i >= a.Tq) return;
-  CT* qo = (CT*)a.dq + row * D;
+  if (rows.i >= a.Tq) return;
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t) st4(qo + 16 * t + 4 * g, o[t][0], o[t][1], o[t][2], o[t][3]);
+  for (int t = 0; t < T::NS; ++t) *(f32x4*)((float*)a.dq + r * D + 16 * t + 4 * g) = o[t] * a.scale;
 }
 
-// dk, dv of 64 keys: the group's query heads in turn, each over the queries
-// that see some of the keys
-template <typename CT, int D>
-__global__ void __launch_bounds__(256) win_attn_dkv_kernel(WinAttnBwdArgs a) {
-  using W = WinTile<CT, D>;
-  typedef typename FragT<CT>::type Frag;
-  constexpr int BQ = W::BK, BKV = W::BQ;      // 32 queries a step, 64 keys a workgroup
-  __shared__ __attribute__((aligned(16))) CT sq[BQ * W::LD], sg[BQ * W::LD];
-  __shared__ __attribute__((aligned(16))) float slse[BQ], sdel[BQ];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  const int nkt = (a.Tk + BKV - 1) / BKV, G = a.Hq / a.Hkv;
-  const int w = xcd_remap(blockIdx.x, gridDim.x);
-  const int hk = (w / nkt) % a.Hkv, b = w / nkt / a.Hkv, k0 = (w % nkt) * BKV;
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
-  const int j = k0 + wave * 16 + n;
-  Frag kf[W::NS], vf[W::NS];
-  load_row_frags<CT, D>(kf, (const CT*)a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], j, j < len, g);
-  load_row_frags<CT, D>(vf, (const CT*)a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], j, j < len, g);
-  const float sc = a.scale * kLog2e;
-  f32x4 ok[W::NT], ov[W::NT];
+// dk, dv of 64 keys over a span of the rows that see them, 32 rows a step
+template <int D> __global__ void __launch_bounds__(256, 2) win_dkv_f32_kernel(WinAttnBwdArgs a) {
+  using T = F32Tile<D>;
+  constexpr int BR = 32, KT = 64;
+  __shared__ __attribute__((aligned(16))) float smem[4 * T::WORDS];       // two buffers of Q, dY
+  __shared__ __attribute__((aligned(16))) float s_lse[2][BR], s_del[2][BR];
+  __shared__ __attribute__((aligned(16))) int s_pos[2][BR];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, off = a.Tk - a.Tq;
+  int w = blockIdx.x;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B; w /= a.B;
+  const SpanSlot sl(a, w);
+  const int k0 = sl.tile * KT;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+  const KeySpan<KT> ks(a, k0, len);
+  if (sl.part >= ks.parts) return;
+  const int t0 = sl.part * a.span * (64 / BR), t1 = min((sl.part + 1) * a.span * (64 / BR), (ks.rows + BR - 1) / BR);
+  const int kw = k0 + wave * 16, j = kw + n;
+  f32x4 kf[T::NS], vf[T::NS];
+  {
+    const long long jj = max(0, min(j, len - 1));
+    const float* kp = (const float*)a.k + b * a.ks[0] + hk * a.ks[2] + jj * a.ks[1];
+    const float* vp = (const float*)a.v + b * a.vs[0] + hk * a.vs[2] + jj * a.vs[1];
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t) ok[t] = ov[t] = zero4();
-  const int pe = k0 < len ? last_query<BKV>(k0, len, a.window, a.sinks) : 0;
-  for (int hg = 0; hg < G; ++hg) {
-    const int h = hk * G + hg;
-    const CT* qb = (const CT*)a.q + b * a.qs[0] + h * a.qs[2];
-    const CT* gb = (const CT*)a.dy + ((long long)b * a.Tq * a.Hq + h) * D;
-    const float* lb = a.lse + ((long long)b * a.Hq + h) * a.Tq;
-    const float* db = a.delta + ((long long)b * a.Hq + h) * a.Tq;
-    for (int p0 = max(k0, off); p0 < pe; p0 += BQ) {
-      const int i0 = p0 - off;
-      __syncthreads();
-      stage_rows<CT, D, BQ, W::LD, W::TH>(sq, qb, a.qs[1], i0, len - off, tid);
-      stage_rows<CT, D, BQ, W::LD, W::TH>(sg, gb, (long long)a.Hq * D, i0, len - off, tid);
-      if (tid < BQ) {
-        const bool in = i0 + tid < a.Tq && p0 + tid < len;
-        slse[tid] = in ? lb[i0 + tid] * kLog2e : 0.f;
-        sdel[tid] = in ? db[i0 + tid] : 0.f;
-      }
-      __syncthreads();
+    for (int c = 0; c < T::NS; ++c) {
+      kf[c] = *(const f32x4*)(kp + 16 * c + 4 * g);
+      vf[c] = *(const f32x4*)(vp + 16 * c + 4 * g);
+    }
+  }
+  const float sc = a.scale * kLog2e;
+  f32x4 ok[T::NS], ov[T::NS];
+#pragma unroll
+  for (int t = 0; t < T::NS; ++t) ok[t] = ov[t] = zero4();
+  const float* qb = (const float*)a.q + b * a.qs[0] + (long long)hk * G * a.qs[2];
+  const float* gb = (const float*)a.dy + ((long long)b * a.Tq * a.Hq + hk * G) * D;
+  F32Stage<D> st(tid);
+  float x_lse = 0.f, x_del = 0.f;
+  int x_pos = -1;
+  RowMap rm(t0 * BR, G, a.g_magic);
+  const auto load = [&](int t) {
+    const int last = ks.rows - 1 - t * BR;
+    st.load([&](int r, const float** pq, const float** pg) {
+      int qi, qg;
+      rm.at(min(r, last), &qi, &qg);
+      qi += ks.i0;
+      *pq = qb + qi * a.qs[1] + qg * a.qs[2];
+      *pg = gb + ((long long)qi * a.Hq + qg) * D;
+    });
+    if (tid < BR) {
+      int qi, qg;
+      rm.at(min(tid, last), &qi, &qg);
+      qi += ks.i0;
+      const long long sr = ((long long)b * a.Hq + hk * G + qg) * a.Tq + qi;
+      x_lse = a.lse[sr];
+      x_del = a.delta[sr];
+      x_pos = tid <= last ? qi + off : -1;
+    }
+  };
+  const auto store = [&](int s) {
+    st.store(smem + s * 2 * T::WORDS, smem + (s * 2 + 1) * T::WORDS);
+    if (tid < BR) {
+      s_lse[s][tid] = x_lse * kLog2e;
+      s_del[s][tid] = x_del;
+      s_pos[s][tid] = x_pos;
+    }
+  };
+  if (t0 < t1) {
+    load(t0);
+    store(0);
+  }
+  lds_barrier();
+  for (int t = t0; t < t1; ++t) {
+    const int si = (t - t0) & 1;
+    const float *sq = smem + si * 2 * T::WORDS, *sg = sq + T::WORDS;
+    const int tp0 = rm.i0 + ks.i0 + off, tp1 = rm.last(BR - 1) + ks.i0 + off;
+    if (t + 1 < t1) rm.advance(BR);
+    load(min(t + 1, t1 - 1));
+    if (tp1 >= kw && (tp0 - a.window < kw + 15 || kw < a.sinks)) {
+      const bool all = (t + 1) * BR <= ks.rows && tp0 >= kw + 15 && (tp1 - kw < a.window || kw + 16 <= a.sinks);
       f32x4 pr[2], ds[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         f32x4 s = zero4(), dp = zero4();
 #pragma unroll
-        for (int c = 0; c < W::NS; ++c) {
-          mma(s, ld_frag(sq + (16 * u + n) * W::LD + c * W::KS, g), kf[c]);
-          mma(dp, ld_frag(sg + (16 * u + n) * W::LD + c * W::KS, g), vf[c]);
+        for (int c = 0; c < T::NS; ++c) {
+          mma(s, ld_frag(sq + (16 * u + n) * T::LD + 16 * c, g), kf[c]);
+          mma(dp, ld_frag(sg + (16 * u + n) * T::LD + 16 * c, g), vf[c]);
         }
-        const f32x4 ls = *(const f32x4*)&slse[16 * u + 4 * g], dl = *(const f32x4*)&sdel[16 * u + 4 * g];
+        const f32x4 ls = *(const f32x4*)&s_lse[si][16 * u + 4 * g], dl = *(const f32x4*)&s_del[si][16 * u + 4 * g];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int p = p0 + 16 * u + 4 * g + e;
-          const bool vis = attn_visible(p < len ? p : -1, j, a.window, a.sinks);
+          const bool vis = all || attn_visible(s_pos[si][16 * u + 4 * g + e], j, a.window, a.sinks);
           pr[u][e] = vis ? exp2f(s[e] * sc - ls[e]) : 0.f;
-          ds[u][e] = vis ? pr[u][e] * (dp[e] - dl[e]) * a.scale : 0.f;
+          ds[u][e] = vis ? pr[u][e] * (dp[e] - dl[e]) : 0.f;
         }
       }
 #pragma unroll
-      for (int t = 0; t < W::NT; ++t)
+      for (int c = 0; c < T::NS; ++c)
 #pragma unroll
-        for (int c = 0; c < BQ / W::KS; ++c) {
-          mma(ov[t], ld_frag_rows<W::LD>(sg, c * W::KS, 16 * t + n, g),
-              acc_frag((CT*)nullptr, pr[c * W::TPS], pr[c * W::TPS + W::TPS - 1]));
-          mma(ok[t], ld_frag_rows<W::LD>(sq, c * W::KS, 16 * t + n, g),
-              acc_frag((CT*)nullptr, ds[c * W::TPS], ds[c * W::TPS + W::TPS - 1]));
+        for (int u = 0; u < 2; ++u) {
+          mma(ov[c], ld_cols<T::LD>(sg, 16 * u, 16 * c + n, g), pr[u]);
+          mma(ok[c], ld_cols<T::LD>(sq, 16 * u, 16 * c + n, g), ds[u]);
         }
     }
+    store(si ^ 1);
+    lds_barrier();
+  }
+  if (ks.parts > 1) {                        // a span's sums, joined by win_dkv_join_kernel
+    const long long slot = ((long long)b * a.Hkv + hk) * span_slots<KT>(a) + w;
+    float* pk = a.part + (slot * 2 * KT + wave * 16 + n) * D + 4 * g;
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) {
+      *(f32x4*)(pk + 16 * t) = ok[t];
+      *(f32x4*)(pk + KT * D + 16 * t) = ov[t];
+    }
+    return;
   }
   if (j >= a.Tk) return;
   const long long row = ((long long)b * a.Tk + j) * a.Hkv + hk;
 #pragma unroll
-  for (int t = 0; t < W::NT; ++t) {
-    st4((CT*)a.dk + row * D + 16 * t + 4 * g, ok[t][0], ok[t][1], ok[t][2], ok[t][3]);
-    st4((CT*)a.dv + row * D + 16 * t + 4 * g, ov[t][0], ov[t][1], ov[t][2], ov[t][3]);
+  for (int t = 0; t < T::NS; ++t) {
+    *(f32x4*)((float*)a.dk + row * D + 16 * t + 4 * g) = ok[t] * a.scale;
+    *(f32x4*)((float*)a.dv + row * D + 16 * t + 4 * g) = ov[t];
   }
 }
 
-template <typename CT, int D> static int launch_fwd(const WinAttnArgs& a, hipStream_t stream) {
-  const long long nqt = (a.Tq + 63) / 64;
-  hipLaunchKernelGGL((win_attn_fwd_kernel<CT, D>), dim3((unsigned)(nqt * a.B * a.Hq)), dim3(256), 0, stream, a);
-  return check_launch("win_attn_fwd_kernel");
+// ---- shares of the work ----
+// Rows a workgroup takes in the forward, keys a tile holds, workgroups that run at once.
+static int fwd_rows(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 128 : 64; }
+static int fwd_keys(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 64 : 32; }
+int win_dkv_keys(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 128 : 64; }
+
+// Parts that the rows' keys are cut into: one, unless the workgroups would not
+// give every CU its two; then as many as do, each of at least four tiles.
+int win_attn_fwd_parts(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype) {
+  const int G = Hq / Hkv, R = fwd_rows(dtype);
+  const long long base = (((long long)Tq * G + R - 1) / R) * B * Hkv;
+  const long long span = window > 0 ? (long long)window + sinks + (R - 1) / G + 1 : Tk, keys = span < Tk ? span : Tk;
+  const long long tiles = (keys + fwd_keys(dtype) - 1) / fwd_keys(dtype);
+  long long parts = 512 / base;
+  if (parts > tiles / 4) parts = tiles / 4;
+  return parts < 1 ? 1 : (int)parts;
 }
 
-template <typename CT, int D> static int launch_bwd(const WinAttnBwdArgs& a, hipStream_t stream) {
-  const long long nqt = (a.Tq + 63) / 64, nkt = (a.Tk + 63) / 64;
-  hipLaunchKernelGGL((win_attn_dq_kernel<CT, D>), dim3((unsigned)(nqt * a.B * a.Hq)), dim3(256), 0, stream, a);
-  const int rc = check_launch("win_attn_dq_kernel");
+// Tiles of keys see (tile + window) positions' rows, those with sinks every
+// later one.  Ordinary tiles are cut only where the workgroups are too few to
+// give every CU its two; the sinks' tiles, as long as the whole row, into
+// spans of an ordinary tile's length.
+WinBwdPlan win_attn_bwd_plan(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype) {
+  const int KT = win_dkv_keys(dtype);
+  const long long G = Hq / Hkv, tiles = (Tk + KT - 1) / KT, heads = (long long)B * Hkv;
+  const bool win = window > 0 && (long long)window + KT < Tk;
+  const long long full = ((long long)Tq * G + 63) / 64;
+  long long one = win ? (((long long)window + KT - 1) * G + 63) / 64 : full;
+  if (one > full) one = full;
+  const long long ns = sinks > 0 && win ? ((long long)sinks + KT - 1) / KT : 0;
+  WinBwdPlan p;
+  p.sink_tiles = (int)(ns < tiles ? ns : tiles);
+  // all heads' steps: a triangle without a window
+  const long long total = heads * (win ? (tiles - p.sink_tiles) * one + p.sink_tiles * full : tiles * full / 2);
+  long long span = (total + 767) / 768;
+  if (span < 8) span = 8;
+  if (win && one <= 2 * span) span = span > one ? span : one;
+  p.span = (int)span;
+  p.tile_parts = (int)((one + span - 1) / span);
+  p.sink_parts = (int)((full + span - 1) / span);
+  return p;
+}
+
+template <int D> static int launch_fwd(const WinAttnArgs& a, hipStream_t stream) {
+  const long long nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 63) / 64;
+  hipLaunchKernelGGL((win_fwd_f32_kernel<D>), dim3((unsigned)(nt * a.B * a.Hkv * a.parts)), dim3(256), 0, stream, a);
+  const int rc = check_launch("win_fwd_f32_kernel");
+  return rc ? rc : launch_win_join<float, D>(a, stream);
+}
+
+template <int D> static int launch_bwd(const WinAttnBwdArgs& a, hipStream_t stream) {
+  const long long nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 63) / 64, heads = (long long)a.B * a.Hkv;
+  hipLaunchKernelGGL((win_dq_f32_kernel<D>), dim3((unsigned)(nt * heads)), dim3(256), 0, stream, a);
+  int rc = check_launch("win_dq_f32_kernel");
   if (rc) return rc;
-  hipLaunchKernelGGL((win_attn_dkv_kernel<CT, D>), dim3((unsigned)(nkt * a.B * a.Hkv)), dim3(256), 0, stream, a);
-  return check_launch("win_attn_dkv_kernel");
+  hipLaunchKernelGGL((win_dkv_f32_kernel<D>), dim3((unsigned)(span_slots<64>(a) * heads)), dim3(256), 0, stream, a);
+  rc = check_launch("win_dkv_f32_kernel");
+  return rc ? rc : launch_dkv_join<float, D, 64>(a, stream);
 }
 
 int win_attn_fwd_dispatch(const WinAttnArgs& a, hipStream_t stream) {
   if (a.dtype == GDNX_DTYPE_BF16) return win_fwd_bf16_dispatch(a, stream);
-  return a.D == 128 ? launch_fwd<float, 128>(a, stream) : launch_fwd<float, 64>(a, stream);
+  return a.D == 128 ? launch_fwd<128>(a, stream) : launch_fwd<64>(a, stream);
 }
 
 int win_attn_bwd_dispatch(const WinAttnBwdArgs& a, hipStream_t stream) {
   if (a.dtype == GDNX_DTYPE_BF16) return win_bwd_bf16_dispatch(a, stream);
-  return a.D == 128 ? launch_bwd<float, 128>(a, stream) : launch_bwd<float, 64>(a, stream);
+  return a.D == 128 ? launch_bwd<128>(a, stream) : launch_bwd<64>(a, stream);
 }
 
 }  // namespace gdnx

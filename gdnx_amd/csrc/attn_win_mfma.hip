@@ -1,5 +1,6 @@
 // Windowed attention with sinks for bf16 (gfx950): forward.  Forms and rules
 // as in attn_win.hip, on the 32 x 32 x 16 matrix instruction.
+#include "attn_spans.hpp"
 #include "attn_tiles.hpp"
 
 namespace gdnx {
@@ -134,17 +135,16 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   l = half_sum(l);
 
   if (a.parts > 1) {                       // a span of the keys: unnormalised, joined by win_join_kernel
-    const long long rows = (long long)a.B * a.Hq * a.Tq;
     if (qi < a.Tq) {
-      const long long r = (long long)part * rows + ((long long)b * a.Tq + qi) * a.Hq + qh;
-      float* po = a.part + r * D + 4 * h;
+      const long long r = ((long long)b * a.Tq + qi) * a.Hq + qh;
+      float* po = part_out(a, part, r) + 4 * h;
 #pragma unroll
       for (int t = 0; t < T::ND; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *(f32x4*)(po + 32 * t + 8 * i) = (f32x4){o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
       if (h == 0) {
-        float* ml = a.part + (long long)a.parts * rows * D + 2 * r;
+        float* ml = part_stats(a, part, r);
         ml[0] = m;
         ml[1] = l;
       }
@@ -167,57 +167,11 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   }
 }
 
-// One wave a row: its spans of the keys joined in order.
-template <int D> __global__ void __launch_bounds__(256) win_join_kernel(WinAttnArgs a) {
-  constexpr int E = D / 64;
-  const long long rows = (long long)a.B * a.Hq * a.Tq, r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int lane = threadIdx.x & 63;
-  const float* ml = a.part + (long long)a.parts * rows * D;
-  float mm = -INFINITY;
-  for (int i = 0; i < a.parts; ++i) mm = fmaxf(mm, ml[2 * (i * rows + r)]);
-  const float ms = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int i = 0; i < a.parts; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * (i * rows + r)] - ms);
-    ll += ml[2 * (i * rows + r) + 1] * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += a.part[(i * rows + r) * D + lane * E + e] * f;
-  }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll
-  for (int e = 0; e < E; ++e) ((bf16*)a.y)[r * D + lane * E + e] = (bf16)(acc[e] * inv);
-  if (lane == 0 && a.lse) {
-    const int h = (int)(r % a.Hq);
-    const long long bi = r / a.Hq;
-    a.lse[((bi / a.Tq) * a.Hq + h) * a.Tq + bi % a.Tq] = ll == 0.f ? -INFINITY : mm * kLn2 + logf(ll);
-  }
-}
-
-// Spans that the rows' keys are cut into: one, unless the workgroups would not
-// give every CU its two; then as many as do, each of at least four tiles.
-int win_attn_fwd_parts(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype) {
-  if (dtype != GDNX_DTYPE_BF16) return 1;
-  const int G = Hq / Hkv;
-  const long long base = (((long long)Tq * G + 127) / 128) * B * Hkv;
-  long long keys = Tk;
-  if (window > 0 && (long long)window + sinks + 127 / G + 1 < keys) keys = (long long)window + sinks + 127 / G + 1;
-  const long long tiles = (keys + 63) / 64;
-  long long parts = 512 / base;
-  if (parts > tiles / 4) parts = tiles / 4;
-  return parts < 1 ? 1 : (int)parts;
-}
-
 template <int D> static int launch(const WinAttnArgs& a, hipStream_t stream) {
   const long long nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 127) / 128;
   hipLaunchKernelGGL((win_fwd_bf16_kernel<D>), dim3((unsigned)(nt * a.B * a.Hkv * a.parts)), dim3(256), 0, stream, a);
-  int rc = check_launch("win_fwd_bf16_kernel");
-  if (rc || a.parts == 1) return rc;
-  const long long rows = (long long)a.B * a.Hq * a.Tq;
-  hipLaunchKernelGGL((win_join_kernel<D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
-  return check_launch("win_join_kernel");
+  const int rc = check_launch("win_fwd_bf16_kernel");
+  return rc ? rc : launch_win_join<bf16, D>(a, stream);
 }
 
 int win_fwd_bf16_dispatch(const WinAttnArgs& a, hipStream_t stream) {

@@ -1,6 +1,7 @@
 // Windowed attention with sinks for bf16 (gfx950): backward.  Forms and rules
 // as in attn_win.hip, tiles and operands as in attn_tiles.hpp, rows packed as
 // in the forward (attn_win_mfma.hip).
+#include "attn_spans.hpp"
 #include "attn_tiles.hpp"
 
 namespace gdnx {
@@ -117,21 +118,6 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   }
 }
 
-// The 64-row steps that the 128 keys from k0 take, and how they are shared:
-// spans of at most `span` steps each.
-struct KeySpan {
-  int i0;              // the first query
-  int rows;            // rows (query, head) from there on
-  int steps, parts;
-  __device__ __forceinline__ KeySpan(const WinAttnBwdArgs& a, int k0, int len) {
-    const int off = a.Tk - a.Tq, p0 = max(k0, off), pe = k0 < len ? last_query<128>(k0, len, a.window, a.sinks) : 0;
-    i0 = p0 - off;
-    rows = pe > p0 ? (pe - p0) * (a.Hq / a.Hkv) : 0;
-    steps = (rows + 63) / 64;
-    parts = max(1, (steps + a.span - 1) / a.span);
-  }
-};
-
 // dK, dV of 128 keys of one key head over a span of the rows that see them; a
 // wave owns 32 keys.  Per 32 rows
 //   S = Q K^T,  dP = dY V^T,  dV^T += dY^T P,  dK^T += Q^T dS
@@ -149,13 +135,10 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   int w = blockIdx.x;
   const int hk = w % a.Hkv; w /= a.Hkv;
   const int b = w % a.B; w /= a.B;
-  // the tiles that hold sinks first, then the others, each with its most parts
-  const int ns = a.sink_tiles, sp = a.sink_parts;
-  const int kt = w < ns * sp ? w / sp : ns + (w - ns * sp) / a.tile_parts;
-  const int part = w < ns * sp ? w % sp : (w - ns * sp) % a.tile_parts;
-  const int k0 = kt * 128;
+  const SpanSlot sl(a, w);
+  const int part = sl.part, k0 = sl.tile * 128;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
-  const KeySpan ks(a, k0, len);
+  const KeySpan<128> ks(a, k0, len);
   if (part >= ks.parts) return;
   const int t0 = part * a.span * (64 / BR), t1 = min((part + 1) * a.span * (64 / BR), (ks.rows + BR - 1) / BR);
 
@@ -291,8 +274,7 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   }
 
   if (ks.parts > 1) {                       // a span: float32 sums, joined by win_dkv_join_kernel
-    const long long slots = (long long)ns * sp + (long long)((a.Tk + 127) / 128 - ns) * a.tile_parts;
-    const long long slot = ((long long)b * a.Hkv + hk) * slots + w;
+    const long long slot = ((long long)b * a.Hkv + hk) * span_slots<128>(a) + w;
     float* pk = a.part + (slot * 2 * 128 + wave * 32 + n) * D + 4 * h;
 #pragma unroll
     for (int t = 0; t < T::ND; ++t)
@@ -319,71 +301,14 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   }
 }
 
-// The spans of 128 keys' gradients summed in order: four keys' rows a workgroup of 256.
-template <int D> __global__ void __launch_bounds__(256) win_dkv_join_kernel(WinAttnBwdArgs a) {
-  constexpr int V = D / 4, RPW = 256 / V;         // threads of a row, rows a pass
-  int w = blockIdx.x;
-  const int hk = w % a.Hkv; w /= a.Hkv;
-  const int b = w % a.B; w /= a.B;
-  const int blk = w % 4, kt = w / 4;              // 32 keys a workgroup
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
-  const KeySpan ks(a, kt * 128, len);
-  if (ks.parts <= 1) return;
-  const int ns = a.sink_tiles, sp = a.sink_parts;
-  const long long slots = (long long)ns * sp + (long long)((a.Tk + 127) / 128 - ns) * a.tile_parts;
-  const long long slot = ((long long)b * a.Hkv + hk) * slots + (kt < ns ? (long long)kt * sp : (long long)ns * sp + (long long)(kt - ns) * a.tile_parts);
-  const int d = 4 * (threadIdx.x % V);
-  for (int r = blk * 32 + threadIdx.x / V; r < blk * 32 + 32; r += RPW) {
-    if (kt * 128 + r >= a.Tk) break;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      f32x4 x = zero4();
-      for (int p = 0; p < ks.parts; ++p) x += *(const f32x4*)(a.part + ((slot + p) * 2 * 128 + m * 128 + r) * D + d);
-      if (m == 0) x *= a.scale;
-      st4((bf16*)(m ? a.dv : a.dk) + (((long long)b * a.Tk + kt * 128 + r) * a.Hkv + hk) * D + d, x[0], x[1], x[2], x[3]);
-    }
-  }
-}
-
-// Steps a span may take, and the most spans of a tile with and without sinks.
-// Tiles see (128 + window) positions' rows, those with sinks every later one.
-// Ordinary tiles are cut only where the workgroups are too few to give every
-// CU its two; the sinks' tiles, as long as the whole row, into spans of an
-// ordinary tile's length.
-WinBwdPlan win_attn_bwd_plan(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks) {
-  const long long G = Hq / Hkv, tiles = (Tk + 127) / 128, heads = (long long)B * Hkv;
-  const bool win = window > 0 && (long long)window + 128 < Tk;
-  const long long full = ((long long)Tq * G + 63) / 64;
-  long long one = win ? (((long long)window + 127) * G + 63) / 64 : full;
-  if (one > full) one = full;
-  const long long ns = sinks > 0 && win ? ((long long)sinks + 127) / 128 : 0;
-  WinBwdPlan p;
-  p.sink_tiles = (int)(ns < tiles ? ns : tiles);
-  // all heads' steps: a triangle without a window
-  const long long total = heads * (win ? (tiles - p.sink_tiles) * one + p.sink_tiles * full : tiles * full / 2);
-  long long span = (total + 767) / 768;
-  if (span < 8) span = 8;
-  if (win && one <= 2 * span) span = span > one ? span : one;
-  p.span = (int)span;
-  p.tile_parts = (int)((one + span - 1) / span);
-  p.sink_parts = (int)((full + span - 1) / span);
-  return p;
-}
-
 template <int D> static int launch(const WinAttnBwdArgs& a, hipStream_t stream) {
   const long long heads = (long long)a.B * a.Hkv, nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 127) / 128;
   hipLaunchKernelGGL((win_dq_bf16_kernel<D>), dim3((unsigned)(nt * heads)), dim3(256), 0, stream, a);
   int rc = check_launch("win_dq_bf16_kernel");
   if (rc) return rc;
-  const long long tiles = (a.Tk + 127) / 128;
-  const long long slots = (long long)a.sink_tiles * a.sink_parts + (tiles - a.sink_tiles) * a.tile_parts;
-  hipLaunchKernelGGL((win_dkv_bf16_kernel<D>), dim3((unsigned)(slots * heads)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((win_dkv_bf16_kernel<D>), dim3((unsigned)(span_slots<128>(a) * heads)), dim3(256), 0, stream, a);
   rc = check_launch("win_dkv_bf16_kernel");
-  if (rc || (a.tile_parts == 1 && (a.sink_tiles == 0 || a.sink_parts == 1))) return rc;
-  // (without a window every tile may have several spans; with one, often only the sinks')
-  const long long joined = a.tile_parts > 1 ? tiles : a.sink_tiles;
-  hipLaunchKernelGGL((win_dkv_join_kernel<D>), dim3((unsigned)(joined * 4 * heads)), dim3(256), 0, stream, a);
-  return check_launch("win_dkv_join_kernel");
+  return rc ? rc : launch_dkv_join<bf16, D, 128>(a, stream);
 }
 
 int win_bwd_bf16_dispatch(const WinAttnBwdArgs& a, hipStream_t stream) {

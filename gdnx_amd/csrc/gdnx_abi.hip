@@ -1161,10 +1161,11 @@ static int check_strides(const long long* st, int dtype, const char* name) {
 static unsigned group_magic(int G) { return G > 1 ? (unsigned)(((1ULL << 32) + G - 1) / G) : 0; }
 
 // Bytes of the spans' gradients behind delta (-1: too many).
-static long long win_bwd_part_bytes(const WinBwdPlan& p, int B, int Tk, int Hkv, int D) {
-  const long long slots = (long long)p.sink_tiles * p.sink_parts + ((Tk + 127) / 128 - p.sink_tiles) * (long long)p.tile_parts;
+static long long win_bwd_part_bytes(const WinBwdPlan& p, int B, int Tk, int Hkv, int D, int dtype) {
+  const int KT = win_dkv_keys(dtype);
+  const long long slots = (long long)p.sink_tiles * p.sink_parts + ((Tk + KT - 1) / KT - p.sink_tiles) * (long long)p.tile_parts;
   if (!prod_le(kMaxGroups / 4, {B, Hkv, slots})) return -1;
-  return p.tile_parts > 1 || (p.sink_tiles > 0 && p.sink_parts > 1) ? slots * B * Hkv * 2 * 128 * D * 4 : 0;
+  return p.tile_parts > 1 || (p.sink_tiles > 0 && p.sink_parts > 1) ? slots * B * Hkv * 2 * KT * D * 4 : 0;
 }
 
 static long long win_bwd_delta_bytes(int B, int Tq, int Hq) { return ((long long)B * Tq * Hq * 4 + 255) / 256 * 256; }
@@ -1199,8 +1200,8 @@ extern "C" long long gdnx_win_attn_bwd_workspace_bytes(int B, int Tq, int Tk, in
                                                        int sinks, int dtype) {
   if (check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype)) return -1;
   const long long delta = win_bwd_delta_bytes(B, Tq, Hq);
-  if (dtype != GDNX_DTYPE_BF16) return delta;
-  const long long part = win_bwd_part_bytes(win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks), B, Tk, Hkv, head_dim);
+  const long long part =
+      win_bwd_part_bytes(win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks, dtype), B, Tk, Hkv, head_dim, dtype);
   return part < 0 ? -1 : delta + part;
 }
 
@@ -1257,16 +1258,14 @@ extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, co
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
       (rc = check_strides(a.vs, dtype, "v")))
     return rc;
-  if (dtype == GDNX_DTYPE_BF16) {
-    const WinBwdPlan p = win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks);
-    if (win_bwd_part_bytes(p, B, Tk, Hkv, head_dim) < 0)
-      return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
-    a.span = p.span;
-    a.tile_parts = p.tile_parts;
-    a.sink_tiles = p.sink_tiles;
-    a.sink_parts = p.sink_parts;
-    a.part = (float*)((char*)workspace + win_bwd_delta_bytes(B, Tq, Hq));
-  }
+  const WinBwdPlan p = win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
+  if (win_bwd_part_bytes(p, B, Tk, Hkv, head_dim, dtype) < 0)
+    return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
+  a.span = p.span;
+  a.tile_parts = p.tile_parts;
+  a.sink_tiles = p.sink_tiles;
+  a.sink_parts = p.sink_parts;
+  a.part = (float*)((char*)workspace + win_bwd_delta_bytes(B, Tq, Hq));
   if ((rc = win_attn_bwd_dispatch(a, (hipStream_t)stream))) return rc;
   const size_t nq = (size_t)B * Tq * Hq * head_dim, nk = (size_t)B * Tk * Hkv * head_dim;
   const FiniteBuf outs[] = {{dq, nq, dtype}, {dk, nk, dtype}, {dv, nk, dtype}};

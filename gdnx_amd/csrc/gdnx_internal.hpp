@@ -482,14 +482,15 @@ struct WinAttnBwdArgs {
   int dtype;
   unsigned g_magic;     // ceil(2^32 / (Hq / Hkv))
   int span, tile_parts, sink_tiles, sink_parts;     // WinBwdPlan
-  float* part;          // [B,Hkv][slots][dk, dv][128][D]: a slot is a span of a tile of 128 keys
+  float* part;          // [B,Hkv][slots][dk, dv][tile's keys][D]: a slot is a span of a key tile's rows
 };
-// How the dk / dv of bf16 shares the rows: spans of at most `span` 64-row
+// How the dk / dv kernels share the rows: spans of at most `span` 64-row
 // steps; the most spans of a tile without and with sinks.
 struct WinBwdPlan {
   int span, tile_parts, sink_tiles, sink_parts;
 };
-WinBwdPlan win_attn_bwd_plan(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks);
+WinBwdPlan win_attn_bwd_plan(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype);
+int win_dkv_keys(int dtype);      // keys of a tile
 int win_attn_fwd_dispatch(const WinAttnArgs& a, hipStream_t stream);
 int win_fwd_bf16_dispatch(const WinAttnArgs& a, hipStream_t stream);
 int win_attn_fwd_parts(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype);
