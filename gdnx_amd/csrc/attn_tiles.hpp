@@ -88,6 +88,40 @@ template <int D> struct LaneMap {
   }
 };
 
+// 64-row tiles of two matrices straight into LDS, 256 threads, 16 bytes a lane:
+// an instruction fills 1 KB in lane order, so the units' permutation is made by
+// what each lane reads.  Rows beyond the last valid one are read from it.
+template <int D> struct TileLoad {
+  using T = Tile<D>;
+  static constexpr int N = 64 * T::UPR / 256, STEP = 256 / T::UPR;
+  unsigned row, oa, ob, sa, sb, u;
+  int wave;
+  __device__ __forceinline__ TileLoad(int tid, int wave_, int as, int bs) : row(tid / T::UPR), wave(wave_) {
+    u = ((tid % T::UPR) ^ T::swz(row)) * 16;
+    sa = 2 * as;
+    sb = 2 * bs;
+  }
+  __device__ __forceinline__ void load(char* ta, const bf16* a, char* tb, const bf16* b, int last) const {
+    typedef __attribute__((address_space(1))) void* G;
+    typedef __attribute__((address_space(3))) void* L;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const unsigned r = min((int)row + i * STEP, last);
+      __builtin_amdgcn_global_load_lds((G)((const char*)a + (r * sa + u)), (L)(ta + i * 4096 + wave * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((G)((const char*)b + (r * sb + u)), (L)(tb + i * 4096 + wave * 1024), 16, 0, 0);
+    }
+  }
+};
+// A workgroup barrier after which every wave's loads into LDS are there.  The
+// wait (vmcnt 0, lgkmcnt 0) is the builtin, which the compiler counts: it then
+// adds none of its own before the tiles are read.
+__device__ __forceinline__ void loads_done_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // A tile of BK rows of two matrices, by way of registers: 256 threads, rows
 // clamped to the last valid one (what lies beyond is masked).  Offsets within
 // a tile are 32-bit: token strides stay below 2^24 elements.

@@ -19,7 +19,9 @@ template <int D>
 __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   using T = Tile<D>;
   constexpr int BK = 64, BYTES = BK * T::RB;
-  __shared__ __attribute__((aligned(16))) char smem[4 * BYTES];   // two buffers of K, V
+  // two buffers of K and V, each a variable of its own: what is read from one
+  // then does not wait for the loads into the other
+  __shared__ __attribute__((aligned(16))) char k0[BYTES], v0[BYTES], k1[BYTES], v1[BYTES];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 127) / 128;
@@ -60,77 +62,76 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   for (int t = 0; t < T::ND; ++t) o[t] = zero16();
   float m = -INFINITY, l = 0.f;
 
-  Stage<D, BK> st(tid);
   const LaneMap<D> lm(lane);
-  const auto load = [&](int it) {
-    const int j0 = kt.start(it);
-    st.load(kb + j0 * a.ks[1], (int)a.ks[1], vb + j0 * a.vs[1], (int)a.vs[1], len - 1 - j0);
+  const TileLoad<D> tl(tid, wave, (int)a.ks[1], (int)a.vs[1]);
+  const auto load = [&](char* tk, char* tv, int it) {
+    const int j0 = kt.start(min(it, t1 - 1));
+    tl.load(tk, kb + j0 * a.ks[1], tv, vb + j0 * a.vs[1], len - 1 - j0);
   };
-  if (t0 < t1) {
-    load(t0);
-    st.store(smem, smem + BYTES);
-  }
-  lds_barrier();
-  for (int it = t0; it < t1; ++it) {
+  const auto tile_step = [&](const char* tk, const char* tv, int it) {
     const int j0 = kt.start(it);
-    char* buf = smem + ((it - t0) & 1) * 2 * BYTES;
-    load(min(it + 1, t1 - 1));
     // whether the wave sees anything of the tile, and all of it
-    const bool some = j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
-    if (some) {
-      f32x16 s[2];
+    const bool some = it < t1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    if (!some) return;
+    const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
+    f32x16 s[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = zero16();
+    for (int u = 0; u < 2; ++u) {
+      s[u] = zero16();
 #pragma unroll
-        for (int c = 0; c < T::NS; ++c) mma32(s[u], lm.row(buf + u * 32 * T::RB, c), qf[c]);
-      }
-      const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
-      if (!all) {
-        const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int c = 32 * u + 8 * (e >> 2) + (e & 3);
-            s[u][e] = (c <= d) & ((d - c < a.window) | (c < ds)) ? s[u][e] : -INFINITY;
-          }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
-      mx = half_max(mx) * sc;
-      if (__any(mx > m + 8.f)) {
-        const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int t = 0; t < T::ND; ++t) o[t] *= f;
-      }
-      const float ms = m == -INFINITY ? 0.f : m;
-      float sum = 0.f;
+      for (int c = 0; c < T::NS; ++c) mma32(s[u], lm.row(tk + u * 32 * T::RB, c), qf[c]);
+    }
+    if (!all) {
+      const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], sc, -ms));
-          sum += s[u][e];
-        }
-      l += sum;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const bf16x8 pf = acc_frag32(s[u], c);
-#pragma unroll
-          for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(buf + BYTES + (32 * u + 16 * c) * T::RB, t), pf);
+          const int c = 32 * u + 8 * (e >> 2) + (e & 3);
+          s[u][e] = (c <= d) & ((d - c < a.window) | (c < ds)) ? s[u][e] : -INFINITY;
         }
     }
-    char* next = smem + ((it - t0 + 1) & 1) * 2 * BYTES;
-    st.store(next, next + BYTES);
-    lds_barrier();
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
+    mx = half_max(mx) * sc;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < T::ND; ++t) o[t] *= f;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], sc, -ms));
+        sum += s[u][e];
+      }
+    l += sum;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const bf16x8 pf = acc_frag32(s[u], c);
+#pragma unroll
+        for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(tv + (32 * u + 16 * c) * T::RB, t), pf);
+      }
+  };
+  if (t0 < t1) load(k0, v0, t0);
+  loads_done_barrier();
+  for (int it = t0; it < t1; it += 2) {
+    load(k1, v1, it + 1);
+    tile_step(k0, v0, it);
+    loads_done_barrier();
+    load(k0, v0, it + 2);
+    tile_step(k1, v1, it + 1);
+    loads_done_barrier();
   }
   l = half_sum(l);
 
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   if (h == 0 && a.lse && qi < a.Tq)
     a.lse[((long long)b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
   // the output by way of LDS, so that whole rows are stored
-  lm.put(smem + wave * 32 * T::RB, o, inv);
+  lm.put((wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RB, o, inv);
   __syncthreads();
   bf16* yb = (bf16*)a.y + (long long)b * a.Tq * a.Hq * D;
 #pragma unroll
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
     const int r = u / T::UPR, c = u % T::UPR;
     int i, g;
     rm.at(r, &i, &g);
-    if (i < a.Tq) *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)(smem + T::at(r, c));
+    if (i < a.Tq) *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)((r < 64 ? k0 : v0) + T::at(r & 63, c));
   }
 }
 
