@@ -54,17 +54,23 @@ template <int D> struct Tile {
 // A lane's places in a tile of 32 rows.
 template <int D> struct LaneMap {
   using T = Tile<D>;
-  int row0, rsw, col[T::ND][2], n, h;
+  int row0, rsw, col0, n, h;
   __device__ __forceinline__ LaneMap(int lane) {
     n = lane & 31;
     h = lane >> 5;
     row0 = n * T::RB;
     rsw = (T::swz(n) ^ h) << 4;
     const int i = lane & 15, c2 = (lane >> 4) & 1;
-#pragma unroll
-    for (int t = 0; t < T::ND; ++t)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) col[t][q] = T::at(4 * h + (i >> 2) + 8 * q, 4 * t + 2 * c2 + ((i & 3) >> 1)) + 8 * (i & 1);
+    col0 = T::at(4 * h + (i >> 2), 2 * c2 + ((i & 3) >> 1)) + 8 * (i & 1);
+  }
+  // the same places as numbers that the compiler takes for new ones: what is
+  // derived from them is not kept in registers from one step to the next
+  __device__ __forceinline__ LaneMap fresh() const {
+    LaneMap m = *this;
+    m.row0 = opaque(row0);
+    m.rsw = opaque(rsw);
+    m.col0 = opaque(col0);
+    return m;
   }
   // row n, k step c
   __device__ __forceinline__ bf16x8 row(const char* tile, int c) const {
@@ -73,8 +79,9 @@ template <int D> struct LaneMap {
   // columns 32 t + n over the 16 rows that start at `tile`
   __device__ __forceinline__ bf16x8 cols(const char* tile, int t) const {
     typedef __attribute__((address_space(3))) bf16x4 Lds4;
-    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + col[t][0]));
-    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + col[t][1]));
+    // (eight rows on, the units' permutation differs in bit 1)
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + (col0 ^ (64 * t))));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + 8 * T::RB + (col0 ^ (64 * t) ^ 32)));
     return (bf16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
   // a transposed accumulator [D][32 rows], times f, as 32 rows of bf16

@@ -12,8 +12,8 @@ namespace gdnx {
 template <int D>
 __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   using T = Tile<D>;
-  constexpr int BK = 32, BYTES = BK * T::RB;
-  __shared__ __attribute__((aligned(16))) char smem[4 * BYTES];   // two buffers of K, V (then the output's 128 rows)
+  constexpr int BK = 64, BYTES = BK * T::RB;
+  __shared__ __attribute__((aligned(16))) char k0[BYTES], v0[BYTES], k1[BYTES], v1[BYTES];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 127) / 128;
@@ -59,54 +59,53 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   f32x16 o[T::ND];
 #pragma unroll
   for (int t = 0; t < T::ND; ++t) o[t] = zero16();
-  Stage<D, BK> st(tid);
   const LaneMap<D> lm(lane);
-  const auto load = [&](int it) {
-    const int j0 = kt.start(it);
-    st.load(kb + j0 * a.ks[1], (int)a.ks[1], vb + j0 * a.vs[1], (int)a.vs[1], len - 1 - j0);
+  const TileLoad<D> tl(tid, wave, (int)a.ks[1], (int)a.vs[1]);
+  const auto load = [&](char* tk, char* tv, int it) {
+    const int j0 = kt.start(min(it, kt.count - 1));
+    tl.load(tk, kb + j0 * a.ks[1], tv, vb + j0 * a.vs[1], len - 1 - j0);
   };
-  if (kt.count > 0) {
-    load(0);
-    st.store(smem, smem + BYTES);
-  }
-  lds_barrier();
-  for (int it = 0; it < kt.count; ++it) {
+  const auto tile_step = [&](const char* tk, const char* tv, int it) {
     const int j0 = kt.start(it);
-    const char* buf = smem + (it & 1) * 2 * BYTES;
-    load(min(it + 1, kt.count - 1));
-    const bool some = j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
-    if (some) {
-      const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
+    const bool some = it < kt.count && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    if (!some) return;
+    const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
 #pragma unroll
-      for (int u = 0; u < BK / 32; ++u) {
-        f32x16 s = zero16(), dp = zero16();
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-        for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(buf + u * 32 * T::RB, c), qf[c]);
+      for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(tk + u * 32 * T::RB, c), qf[c]);
 #pragma unroll
-        for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(buf + BYTES + u * 32 * T::RB, c), gf[c]);
+      for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(tv + u * 32 * T::RB, c), gf[c]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sc, -lse)) * (dp[e] - delta);
-        if (!all) {
-          const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sc, -lse)) * (dp[e] - delta);
+      if (!all) {
+        const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int c = 32 * u + 8 * (e >> 2) + (e & 3);
-            s[e] = (c <= d) & ((d - c < a.window) | (c < ds)) ? s[e] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const bf16x8 f = acc_frag32(s, c);
-#pragma unroll
-          for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(buf + (32 * u + 16 * c) * T::RB, t), f);
+        for (int e = 0; e < 16; ++e) {
+          const int c = 32 * u + 8 * (e >> 2) + (e & 3);
+          s[e] = (c <= d) & ((d - c < a.window) | (c < ds)) ? s[e] : 0.f;
         }
       }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const bf16x8 f = acc_frag32(s, c);
+#pragma unroll
+        for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(tk + (32 * u + 16 * c) * T::RB, t), f);
+      }
     }
-    char* next = smem + ((it + 1) & 1) * 2 * BYTES;
-    st.store(next, next + BYTES);
-    lds_barrier();
+  };
+  if (kt.count > 0) load(k0, v0, 0);
+  loads_done_barrier();
+  for (int it = 0; it < kt.count; it += 2) {
+    load(k1, v1, it + 1);
+    tile_step(k0, v0, it);
+    loads_done_barrier();
+    load(k0, v0, it + 2);
+    tile_step(k1, v1, it + 1);
+    loads_done_barrier();
   }
-  lm.put(smem + wave * 32 * T::RB, o, a.scale);
+  lm.put((wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RB, o, a.scale);
   __syncthreads();
   bf16* qo = (bf16*)a.dq + (long long)b * a.Tq * a.Hq * D;
 #pragma unroll
@@ -114,7 +113,8 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
     const int r = u / T::UPR, c = u % T::UPR;
     int i, g;
     rm.at(r, &i, &g);
-    if (i < a.Tq) *(uint4*)(qo + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)(smem + T::at(r, c));
+    if (i < a.Tq)
+      *(uint4*)(qo + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)((r < 64 ? k0 : v0) + T::at(r & 63, c));
   }
 }
 
@@ -126,7 +126,7 @@ template <int D>
 __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) {
   using T = Tile<D>;
   constexpr int BR = 32, BYTES = BR * T::RB, VB = 128 * T::RB;
-  __shared__ __attribute__((aligned(16))) char smem[4 * BYTES + VB];
+  __shared__ __attribute__((aligned(16))) char q0[BYTES], g0[BYTES], q1[BYTES], g1[BYTES], vtile[VB];
   __shared__ __attribute__((aligned(16))) float s_lse[2][BR], s_del[2][BR];
   __shared__ __attribute__((aligned(16))) int s_pos[2][BR];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
 #pragma unroll
     for (int u = tid; u < 128 * T::UPR; u += 256) {
       const int r = u / T::UPR, c = u % T::UPR;
-      *(u32x4*)(smem + 4 * BYTES + T::at(r, c)) =
+      *(u32x4*)(vtile + T::at(r, c)) =
           *(const u32x4*)(vp + (long long)max(0, min(k0 + r, len - 1)) * a.vs[1] + 8 * c);
     }
   }
@@ -162,23 +162,27 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   for (int t = 0; t < T::ND; ++t) ok[t] = ov[t] = zero16();
   const bf16* qb = (const bf16*)a.q + b * a.qs[0] + (long long)hk * G * a.qs[2];
   const bf16* gb = (const bf16*)a.dy + ((long long)b * a.Tq * a.Hq + hk * G) * D;
-  const LaneMap<D> lm(lane);
+  const LaneMap<D> lm_(lane);
 
+  // step t: rows BR t .. of the keys' rows, clamped to the last one.  Q and dY
+  // go straight into LDS, an instruction's 1 KB in lane order.
   constexpr int N = BR * T::UPR / 256, STEP = 256 / T::UPR;
-  u32x4 xq[N], xg[N];
+  const int srow = tid / T::UPR, sunit = 8 * ((tid % T::UPR) ^ T::swz(srow));
   float x_lse = 0.f, x_del = 0.f;
   int x_pos = -1;
-  const int srow = tid / T::UPR, sunit = tid % T::UPR;
-  // step t: rows BR t .. of the keys' rows, clamped to the last one
-  const auto load = [&](const RowMap& rm, int t) {
+  const auto load = [&](char* tq, char* tg, const RowMap& rm, int t) {
     const int last = ks.rows - 1 - t * BR;
+    typedef __attribute__((address_space(1))) void* Gp;
+    typedef __attribute__((address_space(3))) void* Lp;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       int qi, qg;
       rm.at(min(srow + i * STEP, last), &qi, &qg);
       qi += ks.i0;
-      xq[i] = *(const u32x4*)(qb + qi * a.qs[1] + qg * a.qs[2] + 8 * sunit);
-      xg[i] = *(const u32x4*)(gb + (long long)qi * a.Hq * D + qg * D + 8 * sunit);
+      __builtin_amdgcn_global_load_lds((Gp)(qb + qi * a.qs[1] + qg * a.qs[2] + sunit), (Lp)(tq + i * 4096 + wave * 1024),
+                                       16, 0, 0);
+      __builtin_amdgcn_global_load_lds((Gp)(gb + ((long long)qi * a.Hq + qg) * D + sunit),
+                                       (Lp)(tg + i * 4096 + wave * 1024), 16, 0, 0);
     }
     if (tid < BR) {
       int qi, qg;
@@ -190,41 +194,32 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
       x_pos = tid <= last ? qi + off : -1;
     }
   };
-  const auto store = [&](int s) {
-    char* buf = smem + s * 2 * BYTES;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int o = T::at(srow + i * STEP, sunit);
-      *(u32x4*)(buf + o) = xq[i];
-      *(u32x4*)(buf + BYTES + o) = xg[i];
-    }
+  const auto store_stats = [&](int s) {
     if (tid < BR) {
       s_lse[s][tid] = x_lse * kLog2e;
       s_del[s][tid] = x_del;
       s_pos[s][tid] = x_pos;
     }
   };
-  RowMap rm(t0 * BR, G, a.g_magic);          // of the step at hand
-  if (t0 < t1) {
-    load(rm, t0);
-    store(0);
-  }
-  lds_barrier();
-  const char* vt = smem + 4 * BYTES + wave * 32 * T::RB;
-  for (int t = t0; t < t1; ++t) {
-    const int s_i = (t - t0) & 1;
-    const char* buf = smem + s_i * 2 * BYTES;
+  const char* vt = vtile + wave * 32 * T::RB;
+  // tq, tg: the step's tiles, rm its rows; asks for the next step's into nq, ng
+  RowMap rm(t0 * BR, G, a.g_magic);
+  const auto row_step = [&](const char* tq, const char* tg, char* nq, char* ng, int t, int s_i) {
+    const LaneMap<D> lm = lm_.fresh();
     // positions of the step's rows (uniform)
     const int tp0 = rm.i0 + ks.i0 + off, tp1 = rm.last(BR - 1) + ks.i0 + off;
+    if (t + 1 < t1) {
+      rm.advance(BR);
+      load(nq, ng, rm, t + 1);
+    }
     const bool some = tp1 >= kw && (tp0 - a.window < kw + 31 || kw < a.sinks);
-    bf16x8 pf[2], df[2];
     if (some) {
       const bool all = (t + 1) * BR <= ks.rows && tp0 >= kw + 31 && (tp1 - kw < a.window || kw + 32 <= a.sinks);
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(buf, c), kf[c]);
+      for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(tq, c), kf[c]);
 #pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(buf + BYTES, c), lm.row(vt, c));
+      for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(tg, c), lm.row(vt, c));
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -251,26 +246,25 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        pf[c] = acc_frag32(s, c);
-        df[c] = acc_frag32(dp, c);
-      }
-    }
-    // the next rows are asked for once the scores' accumulators are free
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 < t1) rm.advance(BR);
-    load(rm, min(t + 1, t1 - 1));
-    __builtin_amdgcn_sched_barrier(0);
-    if (some) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
+        const bf16x8 pf = acc_frag32(s, c), df = acc_frag32(dp, c);
 #pragma unroll
         for (int t2 = 0; t2 < T::ND; ++t2) {
-          mma32(ov[t2], lm.cols(buf + BYTES + 16 * c * T::RB, t2), pf[c]);
-          mma32(ok[t2], lm.cols(buf + 16 * c * T::RB, t2), df[c]);
+          mma32(ov[t2], lm.cols(tg + 16 * c * T::RB, t2), pf);
+          mma32(ok[t2], lm.cols(tq + 16 * c * T::RB, t2), df);
         }
+      }
     }
-    store(s_i ^ 1);
-    lds_barrier();
+    if (t + 1 < t1) store_stats(s_i ^ 1);
+    loads_done_barrier();
+  };
+  if (t0 < t1) {
+    load(q0, g0, rm, t0);
+    store_stats(0);
+  }
+  loads_done_barrier();
+  for (int t = t0; t < t1; t += 2) {
+    row_step(q0, g0, q1, g1, t, 0);
+    if (t + 1 < t1) row_step(q1, g1, q0, g0, t + 1, 1);
   }
 
   if (ks.parts > 1) {                       // a span: float32 sums, joined by win_dkv_join_kernel
@@ -285,18 +279,18 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
       }
     return;
   }
-  // by way of LDS (Q and dY tiles, then V's), so that whole rows are stored
+  // by way of LDS, so that whole rows are stored
   bf16* outs[2] = {(bf16*)a.dk, (bf16*)a.dv};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     __syncthreads();
-    lm.put(smem + wave * 32 * T::RB, m ? ov : ok, m ? 1.f : a.scale);
+    lm_.put(vtile + wave * 32 * T::RB, m ? ov : ok, m ? 1.f : a.scale);
     __syncthreads();
 #pragma unroll
     for (int u = tid; u < 128 * T::UPR; u += 256) {
       const int r = u / T::UPR, c = u % T::UPR;
       if (k0 + r < a.Tk)
-        *(uint4*)(outs[m] + (((long long)b * a.Tk + k0 + r) * a.Hkv + hk) * D + 8 * c) = *(const uint4*)(smem + T::at(r, c));
+        *(uint4*)(outs[m] + (((long long)b * a.Tk + k0 + r) * a.Hkv + hk) * D + 8 * c) = *(const uint4*)(vtile + T::at(r, c));
     }
   }
 }
