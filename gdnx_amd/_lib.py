@@ -81,8 +81,8 @@ SIGNATURES = {
     "gdnx_rls_bwd": (_c_int, [_vp] * 18 + [_c_int] * 7 + [_c_float, _c_int, _c_int, _c_float, _c_int, _vp, _vp]),
     "gdnx_win_attn_bwd_workspace_bytes": (_c_ll, [_c_int] * 9),
     "gdnx_win_attn_fwd_workspace_bytes": (_c_ll, [_c_int] * 9),
-    "gdnx_win_attn_fwd": (_c_int, [_vp] * 7 + [_c_ll] * 9 + [_c_int] * 8 + [_c_float, _c_int, _vp]),
-    "gdnx_win_attn_bwd": (_c_int, [_vp] * 11 + [_c_ll] * 9 + [_c_int] * 8 + [_c_float, _c_int, _vp]),
+    "gdnx_win_attn_fwd": (_c_int, [_vp] * 8 + [_c_ll] * 9 + [_c_int] * 8 + [_c_float, _c_int, _vp]),
+    "gdnx_win_attn_bwd": (_c_int, [_vp] * 12 + [_c_ll] * 9 + [_c_int] * 8 + [_c_float, _c_int, _vp]),
     "gdnx_paged_attn_workspace_bytes": (_c_ll, [_c_int] * 9),
     "gdnx_paged_attn_step": (_c_int, [_vp] * 10 + [_c_int] * 10 + [_c_float, _c_int, _vp]),
     "gdnx_pages_workspace_bytes": (_c_ll, [_c_int] * 2),

@@ -61,25 +61,26 @@ def _check(q, k, v, lengths):
     return B, Tq, Tk, Hq, Hkv, D
 
 
-def _forward(q, k, v, window, sinks, scale, lengths, want_lse):
+def _forward(q, k, v, window, sinks, scale, lengths, want_lse, train=False):
     B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
     code = _lib.dtype_code(q.dtype)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     y = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if want_lse else None
+    low = torch.empty_like(y) if train and q.dtype == torch.bfloat16 else None      # y minus its rounding
     nws = _bytes("gdnx_win_attn_fwd_workspace_bytes", B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
     _lib.call("gdnx_win_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths), y.data_ptr(),
-              _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
+              _addr(low), _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
               sinks, scale, code)
-    return q, k, v, y, lse
+    return q, k, v, y, lse, low
 
 
 class WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, lengths):
-        q, k, v, y, lse = _forward(q, k, v, window, sinks, scale, lengths, True)
-        ctx.save_for_backward(q, k, v, lengths, y, lse)
+        q, k, v, y, lse, low = _forward(q, k, v, window, sinks, scale, lengths, True, True)
+        ctx.save_for_backward(q, k, v, lengths, y, lse, low)
         ctx.args = (window, sinks, scale)
         ctx.mark_non_differentiable(lse)
         return y, lse
@@ -87,7 +88,7 @@ class WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _):
-        q, k, v, lengths, y, lse = ctx.saved_tensors
+        q, k, v, lengths, y, lse, low = ctx.saved_tensors
         window, sinks, scale = ctx.args
         B, Tq, Hq, D = q.shape
         Tk, Hkv = k.shape[1:3]
@@ -99,7 +100,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         _need(nws >= 0, "invalid sizes")
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("gdnx_win_attn_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths),
-                  y.data_ptr(), lse.data_ptr(), dy.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                  y.data_ptr(), _addr(low), lse.data_ptr(), dy.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                   ws.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
                   sinks, scale, code)
         return dq, dk, dv, None, None, None, None
@@ -125,7 +126,7 @@ def window_attention(q, k, v, window=None, sinks=0, *, scale=None, lengths=None,
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         y, lse = WindowAttentionFunction.apply(q, k, v, window, sinks, scale, lengths)
     else:
-        y, lse = _forward(q, k, v, window, sinks, scale, lengths, return_lse)[3:]
+        y, lse = _forward(q, k, v, window, sinks, scale, lengths, return_lse)[3:5]
     return (y, lse) if return_lse else y
 
 

@@ -15,6 +15,12 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// What rounding to bf16 leaves over (0 where there is no finite rest).
+__device__ __forceinline__ float bf16_rest(float x) {
+  const float r = x - (float)(bf16)x;
+  return fabsf(r) < INFINITY ? r : 0.f;
+}
+
 // (p < 0 stands for a query that sees nothing)
 __device__ __forceinline__ bool attn_visible(int p, int j, int window, int sinks) {
   return j <= p && (p - j < window || j < sinks);

@@ -35,7 +35,10 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) win_join_ke
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
-  for (int e = 0; e < E; ++e) ((CT*)a.y)[r * D + lane * E + e] = from_f<CT>(acc[e] * inv);
+  for (int e = 0; e < E; ++e) {
+    ((CT*)a.y)[r * D + lane * E + e] = from_f<CT>(acc[e] * inv);
+    if (a.y_low) ((CT*)a.y_low)[r * D + lane * E + e] = from_f<CT>(bf16_rest(acc[e] * inv));
+  }
   if (lane == 0 && a.lse) {
     const int h = (int)(r % a.Hq);
     const long long bi = r / a.Hq;

@@ -84,14 +84,21 @@ template <int D> struct LaneMap {
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds4*)(tile + 8 * T::RB + (col0 ^ (64 * t) ^ 32)));
     return (bf16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
-  // a transposed accumulator [D][32 rows], times f, as 32 rows of bf16
-  __device__ __forceinline__ void put(char* tile, const f32x16* o, float f) const {
+  // a transposed accumulator [D][32 rows], times f, as 32 rows of bf16; low:
+  // what that rounding leaves over
+  __device__ __forceinline__ void put(char* tile, const f32x16* o, float f, bool low = false) const {
 #pragma unroll
     for (int t = 0; t < T::ND; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st4((bf16*)(tile + T::at(n, 4 * t + i) + 8 * h), o[t][4 * i] * f, o[t][4 * i + 1] * f, o[t][4 * i + 2] * f,
-            o[t][4 * i + 3] * f);
+      for (int i = 0; i < 4; ++i) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = o[t][4 * i + e] * f;
+          if (low) x[e] = bf16_rest(x[e]);
+        }
+        st4((bf16*)(tile + T::at(n, 4 * t + i) + 8 * h), x[0], x[1], x[2], x[3]);
+      }
   }
 };
 

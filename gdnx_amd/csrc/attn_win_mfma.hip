@@ -156,15 +156,22 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   if (h == 0 && a.lse && qi < a.Tq)
     a.lse[((long long)b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
   // the output by way of LDS, so that whole rows are stored
-  lm.put((wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RB, o, inv);
-  __syncthreads();
-  bf16* yb = (bf16*)a.y + (long long)b * a.Tq * a.Hq * D;
+  bf16* outs[2] = {(bf16*)a.y, (bf16*)a.y_low};
 #pragma unroll
-  for (int u = tid; u < 128 * T::UPR; u += 256) {
-    const int r = u / T::UPR, c = u % T::UPR;
-    int i, g;
-    rm.at(r, &i, &g);
-    if (i < a.Tq) *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)((r < 64 ? k0 : v0) + T::at(r & 63, c));
+  for (int m = 0; m < 2; ++m) {
+    if (!outs[m]) break;
+    if (m) __syncthreads();
+    lm.put((wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RB, o, inv, m == 1);
+    __syncthreads();
+    bf16* yb = outs[m] + (long long)b * a.Tq * a.Hq * D;
+#pragma unroll
+    for (int u = tid; u < 128 * T::UPR; u += 256) {
+      const int r = u / T::UPR, c = u % T::UPR;
+      int i, g;
+      rm.at(r, &i, &g);
+      if (i < a.Tq)
+        *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)((r < 64 ? k0 : v0) + T::at(r & 63, c));
+    }
   }
 }
 

@@ -44,6 +44,14 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += (float)gf[c][e] * (float)yf[e];
     }
+    // (with y rounded to bf16 alone, delta's error would be that of dS over again)
+    if (a.y_low)
+#pragma unroll
+      for (int c = 0; c < T::NS; ++c) {
+        const bf16x8 yf = *(const bf16x8*)((const bf16*)a.y_low + row + 16 * c + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += (float)gf[c][e] * (float)yf[e];
+      }
     delta = half_sum(delta);
     if (p >= 0) {
       lse = a.lse[srow] * kLog2e;

@@ -1212,8 +1212,8 @@ extern "C" long long gdnx_win_attn_fwd_workspace_bytes(int B, int Tq, int Tk, in
   return parts > 1 ? parts * B * Tq * Hq * (head_dim + 2) * 4 : 0;
 }
 
-extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, float* lse,
-                                 void* workspace,
+extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, void* y_low,
+                                 float* lse, void* workspace,
                                  long long q_b, long long q_t, long long q_h, long long k_b, long long k_t,
                                  long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk,
                                  int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
@@ -1224,10 +1224,11 @@ extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, co
   if (!q || !k || !v || !y) return set_error(GDNX_ERR_ARG, "q, k, v, y must be non-null");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(y))
     return set_error(GDNX_ERR_ARG, "q, k, v, y must be 16-byte aligned");
-  if (!aligned16(workspace)) return set_error(GDNX_ERR_ARG, "workspace must be 16-byte aligned");
+  if (!aligned16(workspace) || !aligned16(y_low))
+    return set_error(GDNX_ERR_ARG, "y_low and workspace must be 16-byte aligned");
   const int parts = win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
   if (parts > 1 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
-  WinAttnArgs a{q, k, v, lengths, y, lse, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv,
+  WinAttnArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv,
                 head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype,
                 group_magic(Hq / Hkv), parts, (float*)workspace};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
@@ -1239,7 +1240,7 @@ extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, co
 }
 
 extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, const int* lengths, const void* y,
-                                 const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                                 const void* y_low, const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
                                  long long q_b, long long q_t, long long q_h, long long k_b, long long k_t,
                                  long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk,
                                  int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
@@ -1248,11 +1249,11 @@ extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, co
   int rc = check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype);
   if (rc) return rc;
   if (!q || !k || !v || !y || !lse || !dy || !dq || !dk || !dv)
-    return set_error(GDNX_ERR_ARG, "all pointers but lengths must be non-null");
+    return set_error(GDNX_ERR_ARG, "all pointers but lengths and y_low must be non-null");
   if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
-  for (const void* p : {q, k, v, y, dy, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
+  for (const void* p : {q, k, v, y, y_low, dy, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
     if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
-  WinAttnBwdArgs a{q, k, v, lengths, y, lse, dy, dq, dk, dv, (float*)workspace, {q_b, q_t, q_h}, {k_b, k_t, k_h},
+  WinAttnBwdArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse, dy, dq, dk, dv, (float*)workspace, {q_b, q_t, q_h}, {k_b, k_t, k_h},
                    {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim,
                    window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype, group_magic(Hq / Hkv)};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||

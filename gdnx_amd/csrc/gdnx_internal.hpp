@@ -455,6 +455,7 @@ struct WinAttnArgs {
   const void* v;
   const int* lengths;   // [B] valid tokens of a row, or null
   void* y;
+  void* y_low;          // bf16: what rounding y left over, or null
   float* lse;
   long long qs[3], ks[3], vs[3];
   int B, Tq, Tk, Hq, Hkv, D, window, sinks;
@@ -470,6 +471,7 @@ struct WinAttnBwdArgs {
   const void* v;
   const int* lengths;
   const void* y;
+  const void* y_low;
   const float* lse;
   const void* dy;
   void* dq;

@@ -611,25 +611,29 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
  * nothing gives y = 0, lse = -infinity and no gradient.  Keys at or beyond
  * lengths[b] are never read.
  *   y   [B,Tq,Hq,D] io dtype, contiguous: softmax(scale q.k) v
+ *   y_low bf16, as y (may be null, and is not written for float32): y minus its
+ *       rounding, for the backward, whose dS would otherwise carry the rounding
+ *       of y besides its own
  *   lse [B,Hq,Tq] float32 (may be null): log of the softmax's denominator
  * workspace: gdnx_win_attn_fwd_workspace_bytes bytes (-1 if the sizes are
  * invalid; null where that is 0): few rows of queries against many keys are
  * split over the keys and joined. */
 long long gdnx_win_attn_fwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
                                             int sinks, int dtype);
-int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, float* lse,
-                      void* workspace, long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
+int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, void* y_low,
+                      float* lse, void* workspace, long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
                       long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
                       int head_dim, int window, int sinks, float scale, int dtype, void* stream);
 
-/* Its gradients from dy [B,Tq,Hq,D] (contiguous) and the forward's y and lse:
+/* Its gradients from dy [B,Tq,Hq,D] (contiguous) and the forward's y, y_low
+ * (may be null) and lse:
  * dq, dk, dv contiguous in the io dtype, dk and dv summed over a key head's
  * query heads in float32.  workspace: gdnx_win_attn_bwd_workspace_bytes (-1 if
  * the sizes are invalid). */
 long long gdnx_win_attn_bwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
                                             int sinks, int dtype);
 int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, const int* lengths, const void* y,
-                      const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                      const void* y_low, const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
                       long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
                       long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
                       int head_dim, int window, int sinks, float scale, int dtype, void* stream);

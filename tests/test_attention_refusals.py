@@ -10,12 +10,12 @@ VP = lambda x: None if x is None else ctypes.c_void_p(x)
 
 
 def _win(over, bwd=False):
-    a = dict(q=64, k=64, v=64, lengths=None, y=64, lse=64, dy=64, dq=64, dk=64, dv=64, ws=64, st=[128] * 9, B=1, Tq=8,
+    a = dict(q=64, k=64, v=64, lengths=None, y=64, low=64, lse=64, dy=64, dq=64, dk=64, dv=64, ws=64, st=[128] * 9, B=1, Tq=8,
              Tk=8, Hq=2, Hkv=1, D=64, window=0, sinks=0, scale=0.125, dt=_lib.DTYPE_BF16)
     a.update(over)
     lib = _lib.load()
     ints = [a[n] for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D", "window", "sinks")]
-    names = ("q", "k", "v", "lengths", "y", "lse") + (("dy", "dq", "dk", "dv", "ws") if bwd else ("ws",))
+    names = ("q", "k", "v", "lengths", "y", "low", "lse") + (("dy", "dq", "dk", "dv", "ws") if bwd else ("ws",))
     fn = lib.gdnx_win_attn_bwd if bwd else lib.gdnx_win_attn_fwd
     return fn(*(VP(a[n]) for n in names), *a["st"], *ints, a["scale"], a["dt"], None), lib.gdnx_last_error().decode()
 

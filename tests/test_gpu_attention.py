@@ -4,9 +4,8 @@ Tolerances (relative L2).  float32: a score is a sum of D products, wrong by
 about sqrt(D) 2^-24 of its terms, a few 1e-6 for scores of a few units, and P
 and every later sum follow: 1e-5 for y, 3e-5 for the gradients (two more
 products).  bfloat16: the output is rounded once (2^-9 at most, 1.1e-3 rms)
-and P, dS and the y in delta are operands of a further product (1.1e-3 rms
-each): sqrt(2..5) x 1.1e-3 with head room: 4e-3 for y and 8e-3 for the
-gradients.  lse is float32 in both: 1e-5 and, of bf16 inputs, the same.
+and P and dS are operands of a further product (1.1e-3 rms each):
+sqrt(2..5) x 1.1e-3 with head room: 4e-3 for y and 8e-3 for the gradients.  lse is float32 in both: 1e-5 and, of bf16 inputs, the same.
 """
 import pytest
 import torch
@@ -20,7 +19,7 @@ TOL = {torch.float32: (1e-5, 3e-5), torch.bfloat16: (4e-3, 8e-3)}
 
 
 def rel(a, b):
-    a, b = a.double().cpu(), b.double()
+    a, b = a.detach().double().cpu(), b.detach().double()
     return float((a - b).norm() / b.norm().clamp(min=1e-30)) if b.norm() > 0 else float(a.norm())
 
 
