@@ -1,5 +1,5 @@
 // Work shared out over a long axis, and its parts joined in order: the
-// forward's keys where rows are few, the dk / dv kernel's rows where a key
+// forward's and dq's keys where rows are few, the dk / dv kernel's rows where a key
 // tile is seen by many (sinks, no window).
 #pragma once
 #include "attn_common.hpp"
@@ -53,19 +53,37 @@ template <typename CT, int D> static int launch_win_join(const WinAttnArgs& a, h
   return check_launch("win_join_kernel");
 }
 
+// ---- dq: parts of a row's keys, [parts][B,Tq,Hq,D] ----
+template <typename CT> __global__ void __launch_bounds__(256) win_dq_join_kernel(WinAttnBwdArgs a) {
+  const long long n = (long long)a.B * a.Tq * a.Hq * a.D, u = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  if (u >= n) return;
+  f32x4 x = zero4();
+  for (int p = 0; p < a.dq_parts; ++p) x += *(const f32x4*)(a.part + p * n + u);
+  x *= a.scale;
+  st4((CT*)a.dq + u, x[0], x[1], x[2], x[3]);
+}
+
+template <typename CT> static int launch_dq_join(const WinAttnBwdArgs& a, hipStream_t stream) {
+  if (a.dq_parts == 1) return GDNX_OK;
+  const long long n = (long long)a.B * a.Tq * a.Hq * a.D;
+  hipLaunchKernelGGL((win_dq_join_kernel<CT>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, a);
+  return check_launch("win_dq_join_kernel");
+}
+
 // ---- dk, dv: spans of a key tile's rows ----
-// The 64-row steps that the KT keys from k0 take, cut into parts of at most
-// a.span steps each.
+// The 64-row steps that the KT keys from k0 take, cut into as few parts as
+// hold a.span steps at most, of one size (`per`).
 template <int KT> struct KeySpan {
   int i0;              // the first query
   int rows;            // rows (query, head) from there on
-  int steps, parts;
+  int steps, parts, per;
   __device__ __forceinline__ KeySpan(const WinAttnBwdArgs& a, int k0, int len) {
     const int off = a.Tk - a.Tq, p0 = max(k0, off), pe = k0 < len ? last_query<KT>(k0, len, a.window, a.sinks) : 0;
     i0 = p0 - off;
     rows = pe > p0 ? (pe - p0) * (a.Hq / a.Hkv) : 0;
     steps = (rows + 63) / 64;
     parts = max(1, (steps + a.span - 1) / a.span);
+    per = (steps + parts - 1) / parts;
   }
 };
 

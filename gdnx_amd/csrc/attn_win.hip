@@ -204,7 +204,8 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dq_f32_kernel(Win
   const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 63) / 64;
   int w = blockIdx.x;
   const int hk = w % a.Hkv; w /= a.Hkv;
-  const int b = w % a.B, tile = nt - 1 - w / a.B;
+  const int b = w % a.B; w /= a.B;
+  const int part = w % a.dq_parts, tile = nt - 1 - w / a.dq_parts;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
   const F32Rows rows(tile, wave, n, hk, G, a.g_magic, a.Tq, off, len);
   const float* kb = (const float*)a.k + b * a.ks[0] + hk * a.ks[2];
@@ -227,11 +228,12 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dq_f32_kernel(Win
     delta += __shfl_xor(delta, 32, 64);
     if (rows.p >= 0) {
       lse = a.lse[srow] * kLog2e;
-      if (g == 0) a.delta[srow] = delta;
+      if (g == 0 && part == 0) a.delta[srow] = delta;
     }
   }
   const float sc = a.scale * kLog2e;
   const KeyTiles<32> kt(rows.wg0, rows.wg1, len, a.window, a.sinks);
+  const int per = (kt.count + a.dq_parts - 1) / a.dq_parts, t0 = part * per, t1 = min(kt.count, t0 + per);
   F32Stage<D> st(tid);
   const auto load = [&](int it) {
     const int j0 = kt.start(it);
@@ -244,15 +246,15 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dq_f32_kernel(Win
   f32x4 o[T::NS];
 #pragma unroll
   for (int t = 0; t < T::NS; ++t) o[t] = zero4();
-  if (kt.count > 0) {
-    load(0);
+  if (t0 < t1) {
+    load(t0);
     st.store(smem, smem + T::WORDS);
   }
   lds_barrier();
-  for (int it = 0; it < kt.count; ++it) {
+  for (int it = t0; it < t1; ++it) {
     const int j0 = kt.start(it);
-    const float *sk = smem + (it & 1) * 2 * T::WORDS, *sv = sk + T::WORDS;
-    load(min(it + 1, kt.count - 1));
+    const float *sk = smem + ((it - t0) & 1) * 2 * T::WORDS, *sv = sk + T::WORDS;
+    load(min(it + 1, t1 - 1));
     if (rows.some(j0, a.window, a.sinks)) {
       const bool all = rows.all(j0, a.window, a.sinks);
       f32x4 ds[2];
@@ -274,11 +276,17 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dq_f32_kernel(Win
 #pragma unroll
         for (int u = 0; u < 2; ++u) mma(o[t], ld_cols<T::LD>(sk, 16 * u, 16 * t + n, g), ds[u]);
     }
-    float* next = smem + ((it + 1) & 1) * 2 * T::WORDS;
+    float* next = smem + ((it - t0 + 1) & 1) * 2 * T::WORDS;
     st.store(next, next + T::WORDS);
     lds_barrier();
   }
   if (rows.i >= a.Tq) return;
+  if (a.dq_parts > 1) {
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t)
+      *(f32x4*)(a.part + ((long long)part * a.B * a.Tq * a.Hq + r) * D + 16 * t + 4 * g) = o[t];
+    return;
+  }
 #pragma unroll
   for (int t = 0; t < T::NS; ++t) *(f32x4*)((float*)a.dq + r * D + 16 * t + 4 * g) = o[t] * a.scale;
 }
@@ -301,7 +309,7 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dkv_f32_kernel(Wi
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
   const KeySpan<KT> ks(a, k0, len);
   if (sl.part >= ks.parts) return;
-  const int t0 = sl.part * a.span * (64 / BR), t1 = min((sl.part + 1) * a.span * (64 / BR), (ks.rows + BR - 1) / BR);
+  const int t0 = sl.part * ks.per * (64 / BR), t1 = min((sl.part + 1) * ks.per * (64 / BR), (ks.rows + BR - 1) / BR);
   const int kw = k0 + wave * 16, j = kw + n;
   f32x4 kf[T::NS], vf[T::NS];
   {
@@ -463,9 +471,9 @@ template <int D> static int launch_fwd(const WinAttnArgs& a, hipStream_t stream)
 
 template <int D> static int launch_bwd(const WinAttnBwdArgs& a, hipStream_t stream) {
   const long long nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 63) / 64, heads = (long long)a.B * a.Hkv;
-  hipLaunchKernelGGL((win_dq_f32_kernel<D>), dim3((unsigned)(nt * heads)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((win_dq_f32_kernel<D>), dim3((unsigned)(nt * heads * a.dq_parts)), dim3(256), 0, stream, a);
   int rc = check_launch("win_dq_f32_kernel");
-  if (rc) return rc;
+  if (rc || (rc = launch_dq_join<float>(a, stream))) return rc;
   hipLaunchKernelGGL((win_dkv_f32_kernel<D>), dim3((unsigned)(span_slots<64>(a) * heads)), dim3(256), 0, stream, a);
   rc = check_launch("win_dkv_f32_kernel");
   return rc ? rc : launch_dkv_join<float, D, 64>(a, stream);

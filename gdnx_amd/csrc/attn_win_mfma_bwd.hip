@@ -19,7 +19,8 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 127) / 128;
   int w = blockIdx.x;
   const int hk = w % a.Hkv; w /= a.Hkv;
-  const int b = w % a.B, tile = nt - 1 - w / a.B;
+  const int b = w % a.B; w /= a.B;
+  const int part = w % a.dq_parts, tile = nt - 1 - w / a.dq_parts;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk, off = a.Tk - a.Tq;
   const RowMap rm(tile * 128, G, a.g_magic);
   const bf16* kb = (const bf16*)a.k + b * a.ks[0] + hk * a.ks[2];
@@ -55,7 +56,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
     delta = half_sum(delta);
     if (p >= 0) {
       lse = a.lse[srow] * kLog2e;
-      if (h == 0) a.delta[srow] = delta;
+      if (h == 0 && part == 0) a.delta[srow] = delta;
     }
   }
   const float sc = a.scale * kLog2e;
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   const int wv0 = rm.last(wave * 32) + off, wv1 = min(min(rm.last(wave * 32 + 31), a.Tq - 1) + off, len - 1);
   const bool rows_ok = rm.last(wave * 32 + 31) < a.Tq && rm.last(wave * 32 + 31) + off < len && wv0 >= 0;
   const KeyTiles<BK> kt(wg0, wg1, len, a.window, a.sinks);
+  const int per = (kt.count + a.dq_parts - 1) / a.dq_parts, t0 = part * per, t1 = min(kt.count, t0 + per);
 
   f32x16 o[T::ND];
 #pragma unroll
@@ -70,12 +72,12 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   const LaneMap<D> lm(lane);
   const TileLoad<D> tl(tid, wave, (int)a.ks[1], (int)a.vs[1]);
   const auto load = [&](char* tk, char* tv, int it) {
-    const int j0 = kt.start(min(it, kt.count - 1));
+    const int j0 = kt.start(min(it, t1 - 1));
     tl.load(tk, kb + j0 * a.ks[1], tv, vb + j0 * a.vs[1], len - 1 - j0);
   };
   const auto tile_step = [&](const char* tk, const char* tv, int it) {
     const int j0 = kt.start(it);
-    const bool some = it < kt.count && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    const bool some = it < t1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
     if (!some) return;
     const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
 #pragma unroll
@@ -103,15 +105,26 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
       }
     }
   };
-  if (kt.count > 0) load(k0, v0, 0);
+  if (t0 < t1) load(k0, v0, t0);
   loads_done_barrier();
-  for (int it = 0; it < kt.count; it += 2) {
+  for (int it = t0; it < t1; it += 2) {
     load(k1, v1, it + 1);
     tile_step(k0, v0, it);
     loads_done_barrier();
     load(k0, v0, it + 2);
     tile_step(k1, v1, it + 1);
     loads_done_barrier();
+  }
+  if (a.dq_parts > 1) {                    // a span of the keys: float32 sums, joined by win_dq_join_kernel
+    if (qi < a.Tq) {
+      float* po = a.part + (((long long)part * a.B + b) * a.Tq + qi) * a.Hq * D + qh * D + 4 * h;
+#pragma unroll
+      for (int t = 0; t < T::ND; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(f32x4*)(po + 32 * t + 8 * i) = (f32x4){o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+    }
+    return;
   }
   lm.put((wave < 2 ? k0 : v0) + (wave & 1) * 32 * T::RB, o, a.scale);
   __syncthreads();
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
   const KeySpan<128> ks(a, k0, len);
   if (part >= ks.parts) return;
-  const int t0 = part * a.span * (64 / BR), t1 = min((part + 1) * a.span * (64 / BR), (ks.rows + BR - 1) / BR);
+  const int t0 = part * ks.per * (64 / BR), t1 = min((part + 1) * ks.per * (64 / BR), (ks.rows + BR - 1) / BR);
 
   const int kw = k0 + wave * 32, j = kw + n;
   bf16x8 kf[T::NS];
@@ -305,9 +318,9 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
 
 template <int D> static int launch(const WinAttnBwdArgs& a, hipStream_t stream) {
   const long long heads = (long long)a.B * a.Hkv, nt = ((long long)a.Tq * (a.Hq / a.Hkv) + 127) / 128;
-  hipLaunchKernelGGL((win_dq_bf16_kernel<D>), dim3((unsigned)(nt * heads)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((win_dq_bf16_kernel<D>), dim3((unsigned)(nt * heads * a.dq_parts)), dim3(256), 0, stream, a);
   int rc = check_launch("win_dq_bf16_kernel");
-  if (rc) return rc;
+  if (rc || (rc = launch_dq_join<bf16>(a, stream))) return rc;
   hipLaunchKernelGGL((win_dkv_bf16_kernel<D>), dim3((unsigned)(span_slots<128>(a) * heads)), dim3(256), 0, stream, a);
   rc = check_launch("win_dkv_bf16_kernel");
   return rc ? rc : launch_dkv_join<bf16, D, 128>(a, stream);

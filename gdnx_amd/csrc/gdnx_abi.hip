@@ -1160,12 +1160,15 @@ static int check_strides(const long long* st, int dtype, const char* name) {
 // ceil(2^32 / G): see RowMap
 static unsigned group_magic(int G) { return G > 1 ? (unsigned)(((1ULL << 32) + G - 1) / G) : 0; }
 
-// Bytes of the spans' gradients behind delta (-1: too many).
-static long long win_bwd_part_bytes(const WinBwdPlan& p, int B, int Tk, int Hkv, int D, int dtype) {
+// Bytes of the spans' sums behind delta, dq's and then dk's and dv's in one place (-1: too many).
+static long long win_bwd_part_bytes(const WinBwdPlan& p, int dq_parts, int B, int Tq, int Tk, int Hq, int Hkv, int D,
+                                    int dtype) {
   const int KT = win_dkv_keys(dtype);
   const long long slots = (long long)p.sink_tiles * p.sink_parts + ((Tk + KT - 1) / KT - p.sink_tiles) * (long long)p.tile_parts;
   if (!prod_le(kMaxGroups / 4, {B, Hkv, slots})) return -1;
-  return p.tile_parts > 1 || (p.sink_tiles > 0 && p.sink_parts > 1) ? slots * B * Hkv * 2 * KT * D * 4 : 0;
+  const long long kv = p.tile_parts > 1 || (p.sink_tiles > 0 && p.sink_parts > 1) ? slots * B * Hkv * 2 * KT * D * 4 : 0;
+  const long long q = dq_parts > 1 ? (long long)dq_parts * B * Tq * Hq * D * 4 : 0;
+  return kv > q ? kv : q;
 }
 
 static long long win_bwd_delta_bytes(int B, int Tq, int Hq) { return ((long long)B * Tq * Hq * 4 + 255) / 256 * 256; }
@@ -1200,8 +1203,9 @@ extern "C" long long gdnx_win_attn_bwd_workspace_bytes(int B, int Tq, int Tk, in
                                                        int sinks, int dtype) {
   if (check_win(B, Tq, Tk, Hq, Hkv, head_dim, window, sinks, dtype)) return -1;
   const long long delta = win_bwd_delta_bytes(B, Tq, Hq);
-  const long long part =
-      win_bwd_part_bytes(win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks, dtype), B, Tk, Hkv, head_dim, dtype);
+  const long long part = win_bwd_part_bytes(win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks, dtype),
+                                            win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype), B, Tq, Tk, Hq,
+                                            Hkv, head_dim, dtype);
   return part < 0 ? -1 : delta + part;
 }
 
@@ -1260,7 +1264,8 @@ extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, co
       (rc = check_strides(a.vs, dtype, "v")))
     return rc;
   const WinBwdPlan p = win_attn_bwd_plan(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
-  if (win_bwd_part_bytes(p, B, Tk, Hkv, head_dim, dtype) < 0)
+  a.dq_parts = win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
+  if (win_bwd_part_bytes(p, a.dq_parts, B, Tq, Tk, Hq, Hkv, head_dim, dtype) < 0)
     return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
   a.span = p.span;
   a.tile_parts = p.tile_parts;

@@ -484,7 +484,8 @@ struct WinAttnBwdArgs {
   int dtype;
   unsigned g_magic;     // ceil(2^32 / (Hq / Hkv))
   int span, tile_parts, sink_tiles, sink_parts;     // WinBwdPlan
-  float* part;          // [B,Hkv][slots][dk, dv][tile's keys][D]: a slot is a span of a key tile's rows
+  int dq_parts;         // spans that a row's keys are cut into for dq
+  float* part;          // dq's sums, then (they are joined by then) [B,Hkv][slots][dk, dv][tile's keys][D]: a slot is a span of a key tile's rows
 };
 // How the dk / dv kernels share the rows: spans of at most `span` 64-row
 // steps; the most spans of a tile without and with sinks.
