@@ -15,41 +15,41 @@ __device__ __forceinline__ float* part_stats(const WinAttnArgs& a, int part, lon
   return a.part + (long long)a.parts * rows * a.D + 2 * (part * rows + row);
 }
 
-// One wave a row ([B,Tq,Hq]).
+// D / 4 threads a row ([B,Tq,Hq]), four columns each.
 template <typename CT, int D> __global__ void __launch_bounds__(256) win_join_kernel(WinAttnArgs a) {
-  constexpr int E = D / 64;
-  const long long rows = (long long)a.B * a.Hq * a.Tq, r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int V = D / 4;
+  const long long rows = (long long)a.B * a.Hq * a.Tq, r = (long long)blockIdx.x * (256 / V) + threadIdx.x / V;
   if (r >= rows) return;
-  const int lane = threadIdx.x & 63;
-  float mm = -INFINITY;
-  for (int i = 0; i < a.parts; ++i) mm = fmaxf(mm, part_stats(a, i, r)[0]);
-  const float ms = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  const int d = 4 * (threadIdx.x % V);
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = zero4();
+#pragma unroll 4
   for (int i = 0; i < a.parts; ++i) {
-    const float f = __builtin_amdgcn_exp2f(part_stats(a, i, r)[0] - ms);
-    ll += part_stats(a, i, r)[1] * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += part_out(a, i, r)[lane * E + e] * f;
+    const float* ml = part_stats(a, i, r);
+    const f32x4 x = *(const f32x4*)(part_out(a, i, r) + d);
+    const float mn = fmaxf(m, ml[0]), ms = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ms), g = __builtin_amdgcn_exp2f(ml[0] - ms);
+    l = l * f + ml[1] * g;
+    acc = acc * f + x * g;
+    m = mn;
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    ((CT*)a.y)[r * D + lane * E + e] = from_f<CT>(acc[e] * inv);
-    if (a.y_low) ((CT*)a.y_low)[r * D + lane * E + e] = from_f<CT>(bf16_rest(acc[e] * inv));
-  }
-  if (lane == 0 && a.lse) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  acc *= inv;
+  st4((CT*)a.y + r * D + d, acc[0], acc[1], acc[2], acc[3]);
+  if (a.y_low)
+    st4((CT*)a.y_low + r * D + d, bf16_rest(acc[0]), bf16_rest(acc[1]), bf16_rest(acc[2]), bf16_rest(acc[3]));
+  if (d == 0 && a.lse) {
     const int h = (int)(r % a.Hq);
     const long long bi = r / a.Hq;
-    a.lse[((bi / a.Tq) * a.Hq + h) * a.Tq + bi % a.Tq] = ll == 0.f ? -INFINITY : mm * kLn2 + logf(ll);
+    a.lse[((bi / a.Tq) * a.Hq + h) * a.Tq + bi % a.Tq] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
   }
 }
 
 template <typename CT, int D> static int launch_win_join(const WinAttnArgs& a, hipStream_t stream) {
   if (a.parts == 1) return GDNX_OK;
   const long long rows = (long long)a.B * a.Hq * a.Tq;
-  hipLaunchKernelGGL((win_join_kernel<CT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((win_join_kernel<CT, D>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, stream,
+                     a);
   return check_launch("win_join_kernel");
 }
 
@@ -100,36 +100,32 @@ struct SpanSlot {
   }
 };
 
-// 32 keys a workgroup: their parts summed in order.
+// A key tile's parts summed in order, four columns of dk or dv a thread.
 template <typename CT, int D, int KT> __global__ void __launch_bounds__(256) win_dkv_join_kernel(WinAttnBwdArgs a) {
-  constexpr int V = D / 4, RPW = 256 / V, BLK = KT / 32;
+  constexpr int BLK = 2 * KT * D / 1024;             // workgroups a tile
   int w = blockIdx.x;
   const int hk = w % a.Hkv; w /= a.Hkv;
   const int b = w % a.B; w /= a.B;
-  const int blk = w % BLK, kt = w / BLK;
+  const int kt = w / BLK, u = 4 * ((w % BLK) * 256 + threadIdx.x);   // of [dk, dv][KT][D]
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
   const KeySpan<KT> ks(a, kt * KT, len);
-  if (ks.parts <= 1) return;
+  const int key = kt * KT + u / D % KT, d = u % D;
+  if (ks.parts <= 1 || key >= a.Tk) return;
   const int first = kt < a.sink_tiles ? kt * a.sink_parts : a.sink_tiles * a.sink_parts + (kt - a.sink_tiles) * a.tile_parts;
-  const long long slot = ((long long)b * a.Hkv + hk) * span_slots<KT>(a) + first;
-  const int d = 4 * (threadIdx.x % V);
-  for (int r = blk * 32 + threadIdx.x / V; r < blk * 32 + 32; r += RPW) {
-    if (kt * KT + r >= a.Tk) break;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      f32x4 x = zero4();
-      for (int p = 0; p < ks.parts; ++p) x += *(const f32x4*)(a.part + ((slot + p) * 2 * KT + m * KT + r) * D + d);
-      if (m == 0) x *= a.scale;
-      st4((CT*)(m ? a.dv : a.dk) + (((long long)b * a.Tk + kt * KT + r) * a.Hkv + hk) * D + d, x[0], x[1], x[2], x[3]);
-    }
-  }
+  const float* part = a.part + (((long long)b * a.Hkv + hk) * span_slots<KT>(a) + first) * 2 * KT * D + u;
+  f32x4 x = zero4();
+#pragma unroll 4
+  for (int p = 0; p < ks.parts; ++p) x += *(const f32x4*)(part + (long long)p * 2 * KT * D);
+  const bool dk = u < KT * D;
+  if (dk) x *= a.scale;
+  st4((CT*)(dk ? a.dk : a.dv) + (((long long)b * a.Tk + key) * a.Hkv + hk) * D + d, x[0], x[1], x[2], x[3]);
 }
 
 template <typename CT, int D, int KT> static int launch_dkv_join(const WinAttnBwdArgs& a, hipStream_t stream) {
   if (a.tile_parts == 1 && (a.sink_tiles == 0 || a.sink_parts == 1)) return GDNX_OK;
   // (with a window often only the tiles with sinks have several parts)
   const long long tiles = a.tile_parts > 1 ? (a.Tk + KT - 1) / KT : a.sink_tiles;
-  hipLaunchKernelGGL((win_dkv_join_kernel<CT, D, KT>), dim3((unsigned)(tiles * (KT / 32) * a.B * a.Hkv)), dim3(256), 0,
+  hipLaunchKernelGGL((win_dkv_join_kernel<CT, D, KT>), dim3((unsigned)(tiles * (2 * KT * D / 1024) * a.B * a.Hkv)), dim3(256), 0,
                      stream, a);
   return check_launch("win_dkv_join_kernel");
 }

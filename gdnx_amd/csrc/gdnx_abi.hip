@@ -1165,7 +1165,7 @@ static long long win_bwd_part_bytes(const WinBwdPlan& p, int dq_parts, int B, in
                                     int dtype) {
   const int KT = win_dkv_keys(dtype);
   const long long slots = (long long)p.sink_tiles * p.sink_parts + ((Tk + KT - 1) / KT - p.sink_tiles) * (long long)p.tile_parts;
-  if (!prod_le(kMaxGroups / 4, {B, Hkv, slots})) return -1;
+  if (!prod_le(kMaxGroups / 32, {B, Hkv, slots})) return -1;       // (32: the join's workgroups a tile)
   const long long kv = p.tile_parts > 1 || (p.sink_tiles > 0 && p.sink_parts > 1) ? slots * B * Hkv * 2 * KT * D * 4 : 0;
   const long long q = dq_parts > 1 ? (long long)dq_parts * B * Tq * Hq * D * 4 : 0;
   return kv > q ? kv : q;
