@@ -6,6 +6,45 @@
 
 namespace gdnx {
 
+// ---- forward: rows that are gone over again ----
+// In a tile that a row sees in part, a hidden value enters its product times
+// zero, which is NaN where the value is not finite.  So a row whose output is
+// not finite is formed again, by its whole wave, from what it sees alone: 64
+// keys at a time, a lane a key for the scores and D / 64 columns for the sum.
+// Nothing of this runs while all outputs are finite.
+template <typename CT, int D, int BK> struct CarefulRow {
+  static constexpr int E = D / 64;
+  float m, l, acc[E];
+  __device__ __forceinline__ CarefulRow(const WinAttnArgs& a, const CT* q, const CT* kb, const CT* vb,
+                                        const KeyTiles<BK>& kt, int t0, int t1, int p, int lane)
+      : m(-INFINITY), l(0.f) {
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int it = t0; it < t1; ++it)
+      for (int jb = kt.start(it); jb < kt.start(it) + BK; jb += 64) {
+        const int j = jb + lane;
+        const bool vis = lane < BK && attn_visible(p, j, a.window, a.sinks);
+        float s = 0.f;
+        if (vis)
+          for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(kb[j * a.ks[1] + d]), s);
+        s = vis ? s * (a.scale * kLog2e) : -INFINITY;
+        float mx = s;
+        for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+        const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m - ms);
+        const float pr = vis ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
+        float sum = pr;
+        for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
+        m = mn;
+        l = l * f + sum;
+        for (int e = 0; e < E; ++e) acc[e] *= f;
+        for (unsigned long long seen = __ballot(vis); seen; seen &= seen - 1) {
+          const int key = __ffsll(seen) - 1;
+          const float pk = __shfl(pr, key, 64);
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(pk, to_f(vb[(jb + key) * a.vs[1] + lane * E + e]), acc[e]);
+        }
+      }
+  }
+};
+
 // ---- forward: parts of a row's keys ----
 __device__ __forceinline__ float* part_out(const WinAttnArgs& a, int part, long long row) {
   return a.part + ((long long)part * a.B * a.Hq * a.Tq + row) * a.D;
@@ -42,6 +81,40 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) win_join_ke
     const int h = (int)(r % a.Hq);
     const long long bi = r / a.Hq;
     a.lse[((bi / a.Tq) * a.Hq + h) * a.Tq + bi % a.Tq] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  }
+}
+
+// The rows of a wave in `redo` (a bit for each of its rows) formed again and
+// stored over what the workgroup has stored before its last barrier.
+template <typename CT, int D, int BK>
+__device__ __forceinline__ void careful_rows(const WinAttnArgs& a, unsigned long long redo, const RowMap& rm, int row0,
+                                             int b, int hk, int off, int part, const CT* kb, const CT* vb,
+                                             const KeyTiles<BK>& kt, int t0, int t1, int lane) {
+  constexpr int E = D / 64;
+  for (; redo; redo &= redo - 1) {
+    int i, h;
+    rm.at(row0 + __ffsll(redo) - 1, &i, &h);
+    h += hk * (a.Hq / a.Hkv);
+    const CT* q = (const CT*)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
+    const CarefulRow<CT, D, BK> c(a, q, kb, vb, kt, t0, t1, i + off, lane);
+    const long long r = ((long long)b * a.Tq + i) * a.Hq + h;
+    const float inv = c.l == 0.f ? 0.f : 1.f / c.l;
+    for (int e = 0; e < E; ++e) {
+      if (a.parts > 1) {
+        part_out(a, part, r)[lane * E + e] = c.acc[e];
+        continue;
+      }
+      ((CT*)a.y)[r * D + lane * E + e] = from_f<CT>(c.acc[e] * inv);
+      if (a.y_low) ((CT*)a.y_low)[r * D + lane * E + e] = from_f<CT>(bf16_rest(c.acc[e] * inv));
+    }
+    if (lane == 0) {
+      if (a.parts > 1) {
+        part_stats(a, part, r)[0] = c.m;
+        part_stats(a, part, r)[1] = c.l;
+      } else if (a.lse) {
+        a.lse[((long long)b * a.Hq + h) * a.Tq + i] = c.l == 0.f ? -INFINITY : c.m * kLn2 + logf(c.l);
+      }
+    }
   }
 }
 

@@ -80,7 +80,7 @@ struct F32Rows {
     rows_ok = last < Tq && last + off < len && wv0 >= 0;
   }
   __device__ __forceinline__ bool some(int j0, int window, int sinks) const {
-    return j0 <= wv1 && (j0 + 31 > wv0 - window || j0 < sinks);
+    return wv0 <= wv1 && j0 <= wv1 && (j0 + 31 > wv0 - window || j0 < sinks);
   }
   __device__ __forceinline__ bool all(int j0, int window, int sinks) const {
     return rows_ok && j0 + 31 <= wv0 && (wv1 - j0 < window || j0 + 32 <= sinks);
@@ -175,9 +175,16 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_fwd_f32_kernel(Wi
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (rows.i >= a.Tq) return;
+  // rows of the wave whose output is not finite (0 times it is NaN)
+  float rest = 0.f;
+#pragma unroll
+  for (int t = 0; t < T::NS; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rest = fmaf(o[t][e], 0.f, rest);
+  unsigned long long redo = __ballot(rows.p >= 0 && rest != 0.f);
+  redo = (redo | redo >> 16 | redo >> 32 | redo >> 48) & 0xffffu;
   const long long r = ((long long)b * a.Tq + rows.i) * a.Hq + rows.h;
-  if (a.parts > 1) {
+  if (rows.i < a.Tq && a.parts > 1) {
     float* po = part_out(a, part, r) + 4 * g;
 #pragma unroll
     for (int t = 0; t < T::NS; ++t) *(f32x4*)(po + 16 * t) = o[t];
@@ -186,13 +193,17 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_fwd_f32_kernel(Wi
       ml[0] = m;
       ml[1] = l;
     }
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  } else if (rows.i < a.Tq) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int t = 0; t < T::NS; ++t) *(f32x4*)((float*)a.y + r * D + 16 * t + 4 * g) = o[t] * inv;
-  if (g == 0 && a.lse)
-    a.lse[((long long)b * a.Hq + rows.h) * a.Tq + rows.i] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    for (int t = 0; t < T::NS; ++t) *(f32x4*)((float*)a.y + r * D + 16 * t + 4 * g) = o[t] * inv;
+    if (g == 0 && a.lse)
+      a.lse[((long long)b * a.Hq + rows.h) * a.Tq + rows.i] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  }
+  if (redo) {
+    __builtin_amdgcn_s_waitcnt(0x0070);             // (the wave's own stores come first)
+    careful_rows<float, D, 32>(a, redo, rows.rm, wave * 16, b, hk, off, part, kb, vb, kt, t0, t1, lane);
+  }
 }
 
 // dq, and delta for the dk / dv kernel

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   const auto tile_step = [&](const char* tk, const char* tv, int it) {
     const int j0 = kt.start(it);
     // whether the wave sees anything of the tile, and all of it
-    const bool some = it < t1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    const bool some = it < t1 && wv0 <= wv1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
     if (!some) return;
     const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
     f32x16 s[2];
@@ -134,6 +134,14 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
     loads_done_barrier();
   }
   l = half_sum(l);
+  // rows of the wave whose output is not finite (0 times it is NaN)
+  float rest = 0.f;
+#pragma unroll
+  for (int t = 0; t < T::ND; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) rest = fmaf(o[t][e], 0.f, rest);
+  unsigned long long redo = __ballot(p >= 0 && rest != 0.f);
+  redo = (redo | redo >> 32) & 0xffffffffu;
 
   if (a.parts > 1) {                       // a span of the keys: unnormalised, joined by win_join_kernel
     if (qi < a.Tq) {
@@ -149,6 +157,10 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
         ml[0] = m;
         ml[1] = l;
       }
+    }
+    if (redo) {
+      __builtin_amdgcn_s_waitcnt(0x0070);           // (the wave's own stores come first)
+      careful_rows<bf16, D, BK>(a, redo, rm, wave * 32, b, hk, off, part, kb, vb, kt, t0, t1, lane);
     }
     return;
   }
@@ -173,6 +185,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
         *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)((r < 64 ? k0 : v0) + T::at(r & 63, c));
     }
   }
+  if (__syncthreads_or(redo != 0) && redo) careful_rows<bf16, D, BK>(a, redo, rm, wave * 32, b, hk, off, part, kb, vb, kt, t0, t1, lane);
 }
 
 template <int D> static int launch(const WinAttnArgs& a, hipStream_t stream) {

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   };
   const auto tile_step = [&](const char* tk, const char* tv, int it) {
     const int j0 = kt.start(it);
-    const bool some = it < t1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
+    const bool some = it < t1 && wv0 <= wv1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
     if (!some) return;
     const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
 #pragma unroll

@@ -106,6 +106,29 @@ def test_padding_may_hold_anything(gpu_lib, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_token_that_is_not_finite_reaches_only_who_sees_it(gpu_lib, bad, D, dtype):
+    """Keys and values of inner tokens: later than some queries of their tile, or left behind by its window."""
+    T, W, S, at = 300, 50, 3, (1, 100, 163, 250)
+    q, k, v, _ = make(1, T, T, 4, 2, D, dtype, seed=6)
+    hide = oa.visible(T, T, W, S, T)[:, list(at)].any(1)            # queries that see one of them
+    clean = oa.attention(q, k, v, W, S)[0]
+    y0 = attention.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), window=W, sinks=S)
+    for what in "kv":
+        k2, v2 = k.clone(), v.clone()
+        for j in at:
+            (k2 if what == "k" else v2)[0, j, :, 3] = bad
+        y = attention.window_attention(q.to(DEV), k2.to(DEV), v2.to(DEV), window=W, sinks=S)
+        assert torch.isfinite(y[0, ~hide]).all()
+        assert rel(y[0, ~hide], clean[0, ~hide]) <= TOL[dtype][0]
+        if what == "v":
+            assert not torch.isfinite(y[0, hide][..., 3].float()).any()      # and who sees it gets it, in its column
+            assert rel(y[0, hide][..., 4:], clean[0, hide][..., 4:]) <= TOL[dtype][0]
+    assert rel(y0, clean) <= TOL[dtype][0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("scale", [0.02, 1.0])
 def test_scores_of_all_sizes(gpu_lib, dtype, scale):
     """A scale of 1: scores to +-40, where the running maximum does all the work.  Rounding scores of that
