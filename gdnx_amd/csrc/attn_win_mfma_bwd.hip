@@ -83,10 +83,22 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s = zero16(), dp = zero16();
+      {                                    // (operands read one ahead: left alone, right before their use)
+        bf16x8 fk[T::NS], fv[T::NS];
+        const auto fetch = [&](int c) {
+          fk[c] = lm.row(tk + u * 32 * T::RB, c);
+          fv[c] = lm.row(tv + u * 32 * T::RB, c);
+        };
+        fetch(0);
 #pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(tk + u * 32 * T::RB, c), qf[c]);
-#pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(tv + u * 32 * T::RB, c), gf[c]);
+        for (int c = 0; c < T::NS; ++c) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (c + 1 < T::NS) fetch(c + 1);
+          mma32(s, fk[c], qf[c]);
+          mma32(dp, fv[c], gf[c]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sc, -lse)) * (dp[e] - delta);
       if (!all) {
@@ -237,10 +249,22 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
     if (some) {
       const bool all = (t + 1) * BR <= ks.rows && tp0 >= kw + 31 && (tp1 - kw < a.window || kw + 32 <= a.sinks);
       f32x16 s = zero16(), dp = zero16();
+      {
+        bf16x8 fq[T::NS], fg[T::NS], fv[T::NS];
+        const auto fetch = [&](int c) {
+          fq[c] = lm.row(tq, c);
+          fg[c] = lm.row(tg, c);
+          fv[c] = lm.row(vt, c);
+        };
+        fetch(0);
 #pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(s, lm.row(tq, c), kf[c]);
-#pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(dp, lm.row(tg, c), lm.row(vt, c));
+        for (int c = 0; c < T::NS; ++c) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (c + 1 < T::NS) fetch(c + 1);
+          mma32(s, fq[c], kf[c]);
+          mma32(dp, fg[c], fv[c]);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -265,13 +289,21 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
           }
         }
       }
+      {
+        constexpr int M = 2 * T::ND;
+        bf16x8 fg[M], fq[M];
+        const auto fetch = [&](int i) {
+          fg[i] = lm.cols(tg + 16 * (i / T::ND) * T::RB, i % T::ND);
+          fq[i] = lm.cols(tq + 16 * (i / T::ND) * T::RB, i % T::ND);
+        };
+        const bf16x8 pf[2] = {acc_frag32(s, 0), acc_frag32(s, 1)}, df[2] = {acc_frag32(dp, 0), acc_frag32(dp, 1)};
+        fetch(0);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const bf16x8 pf = acc_frag32(s, c), df = acc_frag32(dp, c);
-#pragma unroll
-        for (int t2 = 0; t2 < T::ND; ++t2) {
-          mma32(ov[t2], lm.cols(tg + 16 * c * T::RB, t2), pf);
-          mma32(ok[t2], lm.cols(tq + 16 * c * T::RB, t2), df);
+        for (int i = 0; i < M; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (i + 1 < M) fetch(i + 1);
+          mma32(ov[i % T::ND], fg[i], pf[i / T::ND]);
+          mma32(ok[i % T::ND], fq[i], df[i / T::ND]);
         }
       }
     }
