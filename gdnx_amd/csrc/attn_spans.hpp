@@ -84,17 +84,33 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) win_join_ke
   }
 }
 
-// The rows of a wave in `redo` (a bit for each of its rows) formed again and
-// stored over what the workgroup has stored before its last barrier.
-template <typename CT, int D, int BK>
-__device__ __forceinline__ void careful_rows(const WinAttnArgs& a, unsigned long long redo, const RowMap& rm, int row0,
-                                             int b, int hk, int off, int part, const CT* kb, const CT* vb,
-                                             const KeyTiles<BK>& kt, int t0, int t1, int lane) {
+// The rows of the wave in `redo` (a bit for each of its WR rows) formed again
+// and stored over what the workgroup has stored before its last barrier.  All
+// of it is read and worked out anew from the kernel's arguments, the first
+// and only ones of a forward kernel of 4 WR rows a workgroup: held from the
+// kernel's start, it took registers from the main loop (5 % of its time).
+template <typename CT, int D, int BK, int WR> __device__ __forceinline__ void careful_rows(unsigned redo) {
   constexpr int E = D / 64;
+  const auto* args = (const __attribute__((address_space(4))) WinAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  int w = blockIdx.x, tid = opaque(threadIdx.x);
+  asm volatile("" : "+s"(args), "+s"(w));
+  WinAttnArgs a;
+  __builtin_memcpy(&a, (const void*)args, sizeof(a));
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = a.Hq / a.Hkv, nt = (a.Tq * G + 4 * WR - 1) / (4 * WR), off = a.Tk - a.Tq;
+  const int hk = w % a.Hkv; w /= a.Hkv;
+  const int b = w % a.B; w /= a.B;
+  const int part = w % a.parts, tile = nt - 1 - w / a.parts;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
+  const RowMap rm(tile * 4 * WR, G, a.g_magic);
+  const KeyTiles<BK> kt(rm.i0 + off, min(rm.last(4 * WR - 1), a.Tq - 1) + off, len, a.window, a.sinks);
+  const int per = (kt.count + a.parts - 1) / a.parts, t0 = part * per, t1 = min(kt.count, t0 + per);
+  const CT* kb = (const CT*)a.k + b * a.ks[0] + hk * a.ks[2];
+  const CT* vb = (const CT*)a.v + b * a.vs[0] + hk * a.vs[2];
   for (; redo; redo &= redo - 1) {
     int i, h;
-    rm.at(row0 + __ffsll(redo) - 1, &i, &h);
-    h += hk * (a.Hq / a.Hkv);
+    rm.at(wave * WR + __ffs(redo) - 1, &i, &h);
+    h += hk * G;
     const CT* q = (const CT*)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2];
     const CarefulRow<CT, D, BK> c(a, q, kb, vb, kt, t0, t1, i + off, lane);
     const long long r = ((long long)b * a.Tq + i) * a.Hq + h;

@@ -181,8 +181,8 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_fwd_f32_kernel(Wi
   for (int t = 0; t < T::NS; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) rest = fmaf(o[t][e], 0.f, rest);
-  unsigned long long redo = __ballot(rows.p >= 0 && rest != 0.f);
-  redo = (redo | redo >> 16 | redo >> 32 | redo >> 48) & 0xffffu;
+  const unsigned long long bad = __ballot(rows.p >= 0 && rest != 0.f);
+  const unsigned redo = (unsigned)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
   const long long r = ((long long)b * a.Tq + rows.i) * a.Hq + rows.h;
   if (rows.i < a.Tq && a.parts > 1) {
     float* po = part_out(a, part, r) + 4 * g;
@@ -202,7 +202,7 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_fwd_f32_kernel(Wi
   }
   if (redo) {
     __builtin_amdgcn_s_waitcnt(0x0070);             // (the wave's own stores come first)
-    careful_rows<float, D, 32>(a, redo, rows.rm, wave * 16, b, hk, off, part, kb, vb, kt, t0, t1, lane);
+    careful_rows<float, D, 32, 16>(redo);
   }
 }
 

@@ -75,11 +75,23 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
     if (!some) return;
     const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks);
     f32x16 s[2];
+    s[0] = s[1] = zero16();
+    {                                      // (operands read two ahead: left alone, right before their use)
+      bf16x8 fk[T::NS][2];
+      const auto fetch = [&](int c) {
+        fk[c][0] = lm.row(tk, c);
+        fk[c][1] = lm.row(tk + 32 * T::RB, c);
+      };
+      fetch(0);
+      fetch(1);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = zero16();
-#pragma unroll
-      for (int c = 0; c < T::NS; ++c) mma32(s[u], lm.row(tk + u * 32 * T::RB, c), qf[c]);
+      for (int c = 0; c < T::NS; ++c) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + 2 < T::NS) fetch(c + 2);
+        mma32(s[0], fk[c][0], qf[c]);
+        mma32(s[1], fk[c][1], qf[c]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (!all) {
       const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
@@ -140,9 +152,8 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   for (int t = 0; t < T::ND; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) rest = fmaf(o[t][e], 0.f, rest);
-  unsigned long long redo = __ballot(p >= 0 && rest != 0.f);
-  redo = (redo | redo >> 32) & 0xffffffffu;
-
+  const unsigned long long bad = __ballot(p >= 0 && rest != 0.f);
+  const unsigned redo = (unsigned)(bad | bad >> 32);
   if (a.parts > 1) {                       // a span of the keys: unnormalised, joined by win_join_kernel
     if (qi < a.Tq) {
       const long long r = ((long long)b * a.Tq + qi) * a.Hq + qh;
@@ -160,7 +171,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
     }
     if (redo) {
       __builtin_amdgcn_s_waitcnt(0x0070);           // (the wave's own stores come first)
-      careful_rows<bf16, D, BK>(a, redo, rm, wave * 32, b, hk, off, part, kb, vb, kt, t0, t1, lane);
+      careful_rows<bf16, D, BK, 32>(redo);
     }
     return;
   }
@@ -185,7 +196,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
         *(uint4*)(yb + ((long long)i * a.Hq + hk * G + g) * D + 8 * c) = *(const uint4*)((r < 64 ? k0 : v0) + T::at(r & 63, c));
     }
   }
-  if (__syncthreads_or(redo != 0) && redo) careful_rows<bf16, D, BK>(a, redo, rm, wave * 32, b, hk, off, part, kb, vb, kt, t0, t1, lane);
+  if (__syncthreads_or(redo != 0) && redo) careful_rows<bf16, D, BK, 32>(redo);
 }
 
 template <int D> static int launch(const WinAttnArgs& a, hipStream_t stream) {
