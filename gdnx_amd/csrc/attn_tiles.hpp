@@ -104,11 +104,13 @@ template <int D> struct LaneMap {
 
 // 64-row tiles of two matrices straight into LDS, 256 threads, 16 bytes a lane:
 // an instruction fills 1 KB in lane order, so the units' permutation is made by
-// what each lane reads.  Rows beyond the last valid one are read from it.
+// what each lane reads.  Rows beyond the last valid one are read from it (what
+// they give is masked).  Offsets within a tile are 32-bit: token strides stay
+// below 2^24 elements.
 template <int D> struct TileLoad {
   using T = Tile<D>;
   static constexpr int N = 64 * T::UPR / 256, STEP = 256 / T::UPR;
-  unsigned row, oa, ob, sa, sb, u;
+  unsigned row, sa, sb, u;
   int wave;
   __device__ __forceinline__ TileLoad(int tid, int wave_, int as, int bs) : row(tid / T::UPR), wave(wave_) {
     u = ((tid % T::UPR) ^ T::swz(row)) * 16;
@@ -135,33 +137,5 @@ __device__ __forceinline__ void loads_done_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-
-// A tile of BK rows of two matrices, by way of registers: 256 threads, rows
-// clamped to the last valid one (what lies beyond is masked).  Offsets within
-// a tile are 32-bit: token strides stay below 2^24 elements.
-template <int D, int BK> struct Stage {
-  using T = Tile<D>;
-  static constexpr int N = BK * T::UPR / 256, STEP = 256 / T::UPR;
-  u32x4 x[N], y[N];
-  int row, unit;
-  __device__ __forceinline__ Stage(int tid) : row(tid / T::UPR), unit(tid % T::UPR) {}
-  // a, b: the tile's first rows; last: the last valid row of the tile (>= 0)
-  __device__ __forceinline__ void load(const bf16* a, int as, const bf16* b, int bs, int last) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const unsigned r = min(row + i * STEP, last);
-      x[i] = *(const u32x4*)((const char*)a + (r * (unsigned)as + 8 * unit) * 2);
-      y[i] = *(const u32x4*)((const char*)b + (r * (unsigned)bs + 8 * unit) * 2);
-    }
-  }
-  __device__ __forceinline__ void store(char* ta, char* tb) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int o = T::at(row + i * STEP, unit);
-      *(u32x4*)(ta + o) = x[i];
-      *(u32x4*)(tb + o) = y[i];
-    }
-  }
-};
 
 }  // namespace gdnx
