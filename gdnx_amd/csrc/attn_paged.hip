@@ -269,35 +269,41 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
   }
 }
 
-// one wave a query head: its spans joined in order
+// A workgroup a query head: D / 4 threads take a span's four columns each, the
+// groups of them every n-th span, and are joined in order.
 template <typename CT, int D> __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
-  constexpr int BT = FragT<CT>::KSTEP, E = D / 64;
-  const long long head = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (head >= (long long)a.NS * a.Hq) return;
-  const int s = (int)(head / a.Hq), lane = threadIdx.x & 63;
+  constexpr int BT = FragT<CT>::KSTEP, V = D / 4, NG = 256 / V;
+  __shared__ __attribute__((aligned(16))) float s_acc[NG][D];
+  __shared__ float s_m[NG], s_l[NG];
+  const long long head = blockIdx.x;
+  const int s = (int)(head / a.Hq), grp = threadIdx.x / V, d = 4 * (threadIdx.x % V);
   const Seen see(a, a.slots ? a.slots[s] : s);
   const int parts = spans((see.nvis + BT - 1) / BT, a.spans);
   if (parts <= 1) return;                          // written by its workgroup
   const float* ml = a.part + (long long)a.NS * a.Hq * a.spans * D + 2 * head * a.spans;
-  float mm = -INFINITY;
-  for (int i = lane; i < parts; i += 64) mm = fmaxf(mm, ml[2 * i]);
-#pragma unroll
-  for (int x = 32; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor(mm, x, 64));
-  const float ms = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  const float* po = a.part + head * a.spans * D + lane * E;
+  const float* po = a.part + head * a.spans * D + d;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = zero4();
+  const auto add = [&](float m2, float l2, const f32x4& x) {
+    const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ms), g = __builtin_amdgcn_exp2f(m2 - ms);
+    l = l * f + l2 * g;
+    acc = acc * f + x * g;
+    m = mn;
+  };
 #pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - ms);
-    ll += ml[2 * i + 1] * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += po[(long long)i * D + e] * f;
+  for (int i = grp; i < parts; i += NG) add(ml[2 * i], ml[2 * i + 1], *(const f32x4*)(po + (long long)i * D));
+  *(f32x4*)&s_acc[grp][d] = acc;
+  if (d == 0) {
+    s_m[grp] = m;
+    s_l[grp] = l;
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  __syncthreads();
+  if (grp) return;
 #pragma unroll
-  for (int e = 0; e < E; ++e) ((CT*)a.y)[head * D + lane * E + e] = from_f<CT>(acc[e] * inv);
+  for (int g = 1; g < NG; ++g) add(s_m[g], s_l[g], *(const f32x4*)&s_acc[g][d]);
+  acc *= l == 0.f ? 0.f : 1.f / l;
+  st4((CT*)a.y + head * D + d, acc[0], acc[1], acc[2], acc[3]);
 }
 
 // Spans of a row: enough workgroups for eight a CU where the rows and heads
@@ -318,8 +324,7 @@ template <typename CT, int D> static int launch_paged(const PagedAttnArgs& a, hi
                      dim3(256), 0, stream, a);
   int rc = check_launch("paged_attn_kernel");
   if (rc || a.spans == 1) return rc;
-  hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((unsigned)(((long long)a.NS * a.Hq + 3) / 4)), dim3(256), 0, stream,
-                     a);
+  hipLaunchKernelGGL((paged_join_kernel<CT, D>), dim3((unsigned)((long long)a.NS * a.Hq)), dim3(256), 0, stream, a);
   return check_launch("paged_join_kernel");
 }
 

@@ -1309,7 +1309,7 @@ extern "C" int gdnx_paged_attn_step(const void* q, const void* k, const void* v,
     if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
   const int sp = paged_attn_spans(NS, Hq, Hkv, paged_keys(width, page, window, sinks), dtype);
   if (sp > 1 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
-  if (!prod_le(kMaxGroups, {NS, Hkv, (Hq / Hkv + 15) / 16, sp}))
+  if (!prod_le(kMaxGroups, {NS, Hkv, (Hq / Hkv + 15) / 16, sp}) || !prod_le(kMaxGroups, {NS, Hq}))
     return set_error(GDNX_ERR_SHAPE, "too many rows and heads in one call");
   int lg = 0;
   while ((1 << lg) < page) ++lg;
