@@ -5,7 +5,10 @@
 // through without a gap, x = 0 .. nvis - 1 (the sinks, then the window), so a
 // tile of keys needs no mask but its end.
 //
-// Bound by HBM: each visible key and value is read once.  A workgroup takes a
+// Bound by HBM: each visible key and value is read once.  256 rows of up to
+// 8192 tokens (16 query heads on 4, d = 128, bf16; 2.18 GB) take 400 us,
+// 5.4 TB/s; two rows of 262143 tokens (32 on 8; 1.5 GB) 263 us with the join,
+// 5.8 TB/s; a large copy reaches 5.1.  A workgroup takes a
 // span of one row's keys for one key head and up to 16 of its query heads
 // (grouped heads share what is read); its four waves take the span's tiles
 // (32 keys in bf16, 16 in float32) in turn, each with its own running
@@ -270,7 +273,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
 }
 
 // A workgroup a query head: D / 4 threads take a span's four columns each, the
-// groups of them every n-th span, and are joined in order.
+// groups of them every n-th span, and are joined in order.  (A workgroup a row
+// took 20 us for two rows of 128 spans and 32 heads, this form 7.)
 template <typename CT, int D> __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
   constexpr int BT = FragT<CT>::KSTEP, V = D / 4, NG = 256 / V;
   __shared__ __attribute__((aligned(16))) float s_acc[NG][D];
@@ -306,14 +310,23 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) paged_join_
   st4((CT*)a.y + head * D + d, acc[0], acc[1], acc[2], acc[3]);
 }
 
-// Spans of a row: enough workgroups for eight a CU where the rows and heads
-// alone do not give them, each at least four tiles long.
+// Spans of a row of `keys` visible keys.  Two workgroups a CU where the rows
+// and heads alone do not give them, each span at least four tiles; up to six a
+// CU (so that rows of unequal lengths level out) while a span keeps 32 tiles,
+// beside which a workgroup's start and its share of the join are small.  In us,
+// one span / this rule / eight a CU with at least four tiles each:
+//   256 rows up to 8192 tokens, 16/4 heads, d = 128    431 / 400 / 400
+//   2 rows of 262143 tokens, 32/8, d = 128            2937 / 263 / 268
+//   16 rows, window 4096, 16/4, d = 128                 61 /  26 /  35
+//   48 rows, window 512, 16/16, d = 64                  19 /  19 /  24
 int paged_attn_spans(int NS, int Hq, int Hkv, long long keys, int dtype) {
   const int G = Hq / Hkv, tile = dtype == GDNX_DTYPE_BF16 ? 32 : 16;
   const long long base = (long long)NS * Hkv * ((G + 15) / 16);
-  long long n = (2048 + base - 1) / base;
+  long long n = (512 + base - 1) / base, more = (1536 + base - 1) / base;
   const long long most = (keys + 4 * tile - 1) / (4 * tile);
   if (n > most) n = most;
+  if (more > keys / (32 * tile)) more = keys / (32 * tile);
+  if (n < more) n = more;
   if (n > 256) n = 256;
   return n < 1 ? 1 : (int)n;
 }

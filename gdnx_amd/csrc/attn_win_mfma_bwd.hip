@@ -9,6 +9,12 @@ namespace gdnx {
 // dQ, and delta for dK: the forward's walk over the key tiles, per 32 x 32
 // scores
 //   S^T = K Q^T,  dP^T = V dY^T,  dS^T = P^T o (dP^T - delta),  dQ^T += K^T dS^T
+// The scores are formed here and again by the dk / dv kernel, seven products in
+// place of five: one kernel for all three would add its dq tiles up with float
+// atomics, whose order changes the result, or write every tile's out.  Bound
+// like the forward (matrix units busy 43 %); B = 4, T = 4096, 16/4 heads,
+// d = 128, window 1024, 16 sinks: 227 to 254 us (445 thousand cycles; 480 with
+// operands not read ahead).
 template <int D>
 __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   using T = Tile<D>;
@@ -154,7 +160,13 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
 // dK, dV of 128 keys of one key head over a span of the rows that see them; a
 // wave owns 32 keys.  Per 32 rows
 //   S = Q K^T,  dP = dY V^T,  dV^T += dY^T P,  dK^T += Q^T dS
-// K stays in registers, V in LDS; 64 rows of Q and dY a step, double-buffered.
+// K stays in registers (the wave's 32 keys, half of what it holds are the sums),
+// V in LDS, which both together would not fit beside; 32 rows of Q and dY a
+// step, straight into LDS, double-buffered.  Bound by LDS, about half of whose
+// reads' rate it takes, and their latency: each product reads an operand, and
+// with two waves a SIMD the matrix units are busy 39 % of the cycles.  B = 4,
+// T = 4096, 16/4 heads, d = 128, window 1024, 16 sinks: 302 to 360 us (631
+// thousand cycles; 700 with operands not read ahead).
 template <int D>
 __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) {
   using T = Tile<D>;

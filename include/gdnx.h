@@ -609,7 +609,9 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
  *     j <= p,  p < lengths[b],  and  p - j < window or j < sinks
  * (lengths null: Tk; window 0: every earlier key).  A query that sees
  * nothing gives y = 0, lse = -infinity and no gradient.  Keys at or beyond
- * lengths[b] are never read.
+ * lengths[b] never enter a result; a key or value before it that is not finite
+ * reaches only the outputs of queries that see it (gradients may take it up
+ * with its tile of 64 keys).
  *   y   [B,Tq,Hq,D] io dtype, contiguous: softmax(scale q.k) v
  *   y_low bf16, as y (may be null, and is not written for float32): y minus its
  *       rounding, for the backward, whose dS would otherwise carry the rounding
