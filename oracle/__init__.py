@@ -13,6 +13,8 @@ Modules:
              GDN3 dense / bridge regime), sequential and chunked forms.
   gdn3    -- GDN3 Kronecker-residual recurrence with circular residual buffer
              and two-timescale rearrangement-SVD compaction.
+  attention -- attention with a sliding window and sinks, its gradients, and
+             a paged cache's bookkeeping.
   inputs  -- seeded synthetic input generators for the benchmark configs.
 
 Pinning status of every function is listed in each module header.
