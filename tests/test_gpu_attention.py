@@ -94,6 +94,16 @@ def test_window_attention(gpu_lib, shape, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 40, 40, 20, 1, 9, 2, None), (2, 9, 300, 150, 1, 60, 0, [300, 295]),
+                                   (1, 70, 70, 34, 2, None, 0, [66]), (1, 3, 20, 400, 2, None, 0, None)],
+                         ids=lambda s: "-".join(map(str, s[:7])))
+def test_large_groups(gpu_lib, shape, dtype):
+    """Groups that are no power of two, longer than a tile's rows, or the size of several tiles."""
+    B, Tq, Tk, Hq, Hkv, window, sinks, lengths = shape
+    check(*make(B, Tq, Tk, Hq, Hkv, 64, dtype), window, sinks, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_padding_may_hold_anything(gpu_lib, dtype):
     q, k, v, dy = make(2, 100, 100, 4, 2, 64, dtype)
     lengths = [61, 0]
@@ -328,6 +338,18 @@ def test_paged_step(gpu_lib, case, D, dtype):
     assert torch.equal(dev2[2].cpu().nan_to_num(7.0), vp.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,window", [([3000] * 40, 8, 8, None), ([2000 + 700 * r for r in range(16)], 4, 4, 1500),
+                                                ([1, 9000, 0, 40] * 8, 16, 8, None)])
+def test_paged_step_spans(gpu_lib, lens, Hq, Hkv, window):
+    """Enough rows and heads for one span or a few, whose number the table's width and not the row decides."""
+    q, kp, vp, table, ln, ks, vs = paged(lens, Hq, Hkv, 64, 64, torch.bfloat16, fill=float("nan"))
+    y = attention.paged_attention_step(q.to(DEV), None, None, *(t.to(DEV) for t in (kp, vp, table, ln)),
+                                       window=window, sinks=5)
+    ref = step_ref(q, ks, vs, window, 5)
+    tol = TOL[torch.bfloat16][0]
+    assert rel(y, ref) <= tol and rows_rel(y, ref) <= 5 * tol
+
+
 def test_paged_step_slots_missing_pages_and_odd_tables(gpu_lib):
     lens, dtype = [100, 50, 75], torch.bfloat16
     q, kp, vp, table, ln, ks, vs = paged(lens, 4, 2, 64, 16, dtype, width=4096)      # a table far wider than its rows
@@ -356,7 +378,7 @@ def test_paged_step_slots_missing_pages_and_odd_tables(gpu_lib):
 
 def test_paged_step_matches_the_prompt_form(gpu_lib):
     q, kp, vp, table, ln, ks, vs = paged([333], 8, 2, 128, 32, torch.bfloat16)
-    y = attention.paged_attention_step(*(t.to(DEV) for t in (q,)), None, None, *(t.to(DEV) for t in (kp, vp, table, ln)),
+    y = attention.paged_attention_step(q.to(DEV), None, None, *(t.to(DEV) for t in (kp, vp, table, ln)),
                                        window=100, sinks=5)
     z = attention.window_attention(q[None].to(DEV), ks[0][None].to(DEV), vs[0][None].to(DEV), window=100, sinks=5)
     assert rel(y, z[0].cpu()) <= 4e-3
