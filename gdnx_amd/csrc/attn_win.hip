@@ -440,19 +440,21 @@ static int fwd_keys(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 64 : 32; }
 int win_dkv_keys(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 128 : 64; }
 
 // Parts that the rows' keys are cut into: one, unless the workgroups would not
-// give every CU its two; then as many as do, each of at least four tiles.
-// Forward in us, uncut / cut (bf16, d = 128 unless said): 2 x 200 queries on
-// 16584 keys, 16/2 heads 297 / 77; 2048 on 16384, 16/4 344 / 297; 4096 on 4096,
-// 8/2 82 / 65; 16 on 4096, 8/8 109 / 16; float32, 200 on 8000, 8/4 762 / 89.
-// Where a row sees few tiles the join takes back what the cut gains: 1000 on
-// 9000, window 1024, 16/4, d = 64 22 / 25.
+// give every CU its two; then as many as do, each of at least four tiles (eight
+// in bf16, whose tiles take less time beside the join, unless the workgroups are very
+// few).  Forward in us, uncut / cut (bf16, d = 128 unless said): 2 x 200
+// queries on 16584 keys, 16/2 heads 297 / 77; 2048 on 16384, 16/4 344 / 297;
+// 4096 on 4096, 8/2 82 / 65; 16 on 4096, 8/8 109 / 16 (eight tiles: 21);
+// float32, 200 on 8000, 8/4 762 / 89; 512 on 512, 16/4 54 / 32 (eight: 36).
+// 2048 on 2048, window 512, 8/2 stays uncut: 18, cut by four tiles 22.
 int win_attn_fwd_parts(int B, int Tq, int Tk, int Hq, int Hkv, int window, int sinks, int dtype) {
   const int G = Hq / Hkv, R = fwd_rows(dtype);
   const long long base = (((long long)Tq * G + R - 1) / R) * B * Hkv;
   const long long span = window > 0 ? (long long)window + sinks + (R - 1) / G + 1 : Tk, keys = span < Tk ? span : Tk;
   const long long tiles = (keys + fwd_keys(dtype) - 1) / fwd_keys(dtype);
+  const int least = dtype == GDNX_DTYPE_BF16 && base > 32 ? 8 : 4;
   long long parts = 512 / base;
-  if (parts > tiles / 4) parts = tiles / 4;
+  if (parts > tiles / least) parts = tiles / least;
   return parts < 1 ? 1 : (int)parts;
 }
 
@@ -474,8 +476,11 @@ WinBwdPlan win_attn_bwd_plan(int B, int Tq, int Tk, int Hq, int Hkv, int window,
   const long long ns = sinks > 0 && win ? ((long long)sinks + KT - 1) / KT : 0;
   WinBwdPlan p;
   p.sink_tiles = (int)(ns < tiles ? ns : tiles);
-  // all heads' steps: a triangle without a window
-  const long long total = heads * (win ? (tiles - p.sink_tiles) * one + p.sink_tiles * full : tiles * full / 2);
+  // all heads' steps: a triangle without a window, with one those of the tiles or, of fewer queries, of their rows
+  long long seen = (tiles - p.sink_tiles) * one;
+  const long long rows = full * (((long long)window + KT - 1) / KT + 1);
+  if (seen > rows) seen = rows;
+  const long long total = heads * (win ? seen + p.sink_tiles * full : tiles * full / 2);
   long long span = (total + 767) / 768;
   if (span < 8) span = 8;
   if (win && one <= 2 * span) span = span > one ? span : one;
