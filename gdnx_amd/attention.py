@@ -71,8 +71,8 @@ def _forward(q, k, v, window, sinks, scale, lengths, want_lse, train=False):
     nws = _bytes("gdnx_win_attn_fwd_workspace_bytes", B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
     _lib.call("gdnx_win_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths), y.data_ptr(),
-              _addr(low), _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
-              sinks, scale, code)
+              _addr(low), _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq,
+              Hkv, D, window, sinks, scale, code)
     return q, k, v, y, lse, low
 
 

@@ -18,12 +18,13 @@ namespace gdnx {
 // change), which spares the rescaling of 64 accumulators on most tiles.
 //
 // Bound by the matrix and vector units together at the clock that the chip's
-// power leaves: the matrix units are busy 46 to 48 % of the cycles and the
-// softmax of a tile takes about as long as its products; the two waves of a
-// SIMD overlap them.  16 query heads on 4, d = 128: 16384 tokens without a window
-// 1.05 PFLOP/s; 32768 tokens, window 2048, 64 sinks 584 us, 940 TFLOP/s of
-// visible products; B = 4, T = 4096, window 1024 (a quarter of each row's tiles
-// are cut by the window or the diagonal) 160 to 200 us.
+// power leaves: the matrix units are busy 46 to 48 % of the cycles, the softmax
+// of a tile takes about as long as its products, and neither operands read
+// further ahead nor waves shifted against each other change the time.  16 query
+// heads on 4, d = 128: 16384 tokens without a window 1.05 to 1.09 PFLOP/s; 32768
+// tokens, window 2048, 64 sinks 571 to 584 us, 950 TFLOP/s of visible products;
+// B = 4, T = 4096, window 1024 (three of a row's 18 tiles are cut by the window
+// or the diagonal, or hold the sinks) 152 us, 168 to 191 with y_low and lse.
 template <int D>
 __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
   using T = Tile<D>;

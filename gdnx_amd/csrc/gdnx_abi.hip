@@ -1232,8 +1232,8 @@ extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, co
     return set_error(GDNX_ERR_ARG, "y_low and workspace must be 16-byte aligned");
   const int parts = win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
   if (parts > 1 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
-  WinAttnArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv,
-                head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype,
+  WinAttnArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse,
+                {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype,
                 group_magic(Hq / Hkv), parts, (float*)workspace};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
       (rc = check_strides(a.vs, dtype, "v")))
@@ -1244,7 +1244,8 @@ extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, co
 }
 
 extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, const int* lengths, const void* y,
-                                 const void* y_low, const float* lse, const void* dy, void* dq, void* dk, void* dv, void* workspace,
+                                 const void* y_low, const float* lse, const void* dy, void* dq, void* dk, void* dv,
+                                 void* workspace,
                                  long long q_b, long long q_t, long long q_h, long long k_b, long long k_t,
                                  long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk,
                                  int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
@@ -1257,8 +1258,8 @@ extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, co
   if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
   for (const void* p : {q, k, v, y, y_low, dy, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)workspace})
     if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
-  WinAttnBwdArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse, dy, dq, dk, dv, (float*)workspace, {q_b, q_t, q_h}, {k_b, k_t, k_h},
-                   {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim,
+  WinAttnBwdArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse, dy, dq, dk, dv,
+                   (float*)workspace, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim,
                    window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype, group_magic(Hq / Hkv)};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
       (rc = check_strides(a.vs, dtype, "v")))

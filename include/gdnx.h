@@ -603,9 +603,10 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
  *
  * Attention with a sliding window and sinks.  q [B,Tq,Hq,D], k and v
  * [B,Tk,Hkv,D] in the io dtype with any element strides (batch, token, head)
- * that are multiples of 16 bytes (a token's at most 2^24), D contiguous; Hq a multiple of Hkv, query
- * head h reading key head h / (Hq / Hkv); D = 64 or 128.  Query i stands at
- * position p = i + Tk - Tq and sees key j if
+ * that are multiples of 16 bytes (a token's at most 2^24 elements), D
+ * contiguous; Hq a multiple of Hkv, query head h reading key head
+ * h / (Hq / Hkv); D = 64 or 128.  Query i stands at position p = i + Tk - Tq
+ * and sees key j if
  *     j <= p,  p < lengths[b],  and  p - j < window or j < sinks
  * (lengths null: Tk; window 0: every earlier key).  A query that sees
  * nothing gives y = 0, lse = -infinity and no gradient.  Keys at or beyond
@@ -623,8 +624,8 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
 long long gdnx_win_attn_fwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int head_dim, int window,
                                             int sinks, int dtype);
 int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, void* y_low,
-                      float* lse, void* workspace, long long q_b, long long q_t, long long q_h, long long k_b, long long k_t, long long k_h,
-                      long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
+                      float* lse, void* workspace, long long q_b, long long q_t, long long q_h,
+                      long long k_b, long long k_t, long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
                       int head_dim, int window, int sinks, float scale, int dtype, void* stream);
 
 /* Its gradients from dy [B,Tq,Hq,D] (contiguous) and the forward's y, y_low
