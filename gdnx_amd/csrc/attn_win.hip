@@ -178,13 +178,17 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_fwd_f32_kernel(Wi
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  if (rows.p < 0) {                         // a row that sees nothing: 0 times a value that is not finite is NaN
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) o[t] = zero4();
+  }
   // rows of the wave whose output is not finite (0 times it is NaN)
   float rest = 0.f;
 #pragma unroll
   for (int t = 0; t < T::NS; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) rest = fmaf(o[t][e], 0.f, rest);
-  const unsigned long long bad = __ballot(rows.p >= 0 && rest != 0.f);
+  const unsigned long long bad = __ballot(rest != 0.f);
   const unsigned redo = (unsigned)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
   const long long r = ((long long)b * a.Tq + rows.i) * a.Hq + rows.h;
   if (rows.i < a.Tq && a.parts > 1) {

@@ -156,13 +156,17 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
     loads_done_barrier();
   }
   l = half_sum(l);
+  if (p < 0) {                             // a row that sees nothing: 0 times a value that is not finite is NaN
+#pragma unroll
+    for (int t = 0; t < T::ND; ++t) o[t] = zero16();
+  }
   // rows of the wave whose output is not finite (0 times it is NaN)
   float rest = 0.f;
 #pragma unroll
   for (int t = 0; t < T::ND; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) rest = fmaf(o[t][e], 0.f, rest);
-  const unsigned long long bad = __ballot(p >= 0 && rest != 0.f);
+  const unsigned long long bad = __ballot(rest != 0.f);
   const unsigned redo = (unsigned)(bad | bad >> 32);
   if (a.parts > 1) {                       // a span of the keys: unnormalised, joined by win_join_kernel
     if (qi < a.Tq) {

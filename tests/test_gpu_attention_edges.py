@@ -1,0 +1,50 @@
+"""Attention beside values that are not finite, padding, split keys, odd strides and the ends of the arguments' ranges.
+
+Tolerances are those of test_gpu_attention, where they are derived.
+"""
+import pytest
+import torch
+
+from gdnx_amd import attention
+from test_gpu_attention import DEV, make
+
+pytestmark = pytest.mark.gpu
+DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+HEADS = pytest.mark.parametrize("D", [64, 128])
+
+
+def ints(xs):
+    return torch.tensor(xs, dtype=torch.int32, device=DEV)
+
+
+# B, Tq, Tk, Hq, Hkv, window, sinks, lengths, tokens that are not finite (each within every row's length)
+UNSEEN = [
+    (2, 100, 100, 4, 2, 30, 4, [61, 90], (3, 59)),               # padded queries beside them
+    (2, 100, 100, 3, 1, None, 0, [70, 97], (1, 69)),
+    (1, 90, 40, 2, 1, 20, 2, None, (0, 5)),                      # queries before position 0
+    (2, 100, 3000, 4, 2, None, 0, [2950, 2925], (7, 2920)),      # keys split over several workgroups
+]
+
+
+def unseeing(case, what, bad, D, dtype):
+    """The case's inputs, k or v not finite at its tokens, and which queries see nothing."""
+    B, Tq, Tk, Hq, Hkv, _, _, lengths, at = case
+    q, k, v, dy = make(B, Tq, Tk, Hq, Hkv, D, dtype, seed=11)
+    (k if what == "k" else v)[:, list(at), :, 3] = bad
+    p = torch.arange(Tq) + Tk - Tq
+    none = (p < 0) | (p >= torch.tensor(lengths or [Tk] * B)[:, None])
+    assert none.any(1).all()
+    return [x.to(DEV).requires_grad_(True) for x in (q, k, v)], dy.to(DEV), none.to(DEV)
+
+
+@DTYPES
+@HEADS
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("case", UNSEEN, ids=lambda c: "-".join(map(str, c[:7])))
+def test_queries_that_see_nothing_give_zero_beside_what_is_not_finite(gpu_lib, case, what, bad, D, dtype):
+    W, S, lengths = case[5:8]
+    ins, _, none = unseeing(case, what, bad, D, dtype)
+    y, lse = attention.window_attention(*ins, window=W, sinks=S, lengths=None if lengths is None else ints(lengths),
+                                        return_lse=True)
+    assert (y[none] == 0).all() and (lse.transpose(1, 2)[none] == float("-inf")).all()
