@@ -299,6 +299,10 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dq_f32_kernel(Win
     lds_barrier();
   }
   if (rows.i >= a.Tq) return;
+  if (rows.p < 0) {                         // a row that sees nothing: 0 times a key that is not finite is NaN
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) o[t] = zero4();
+  }
   if (a.dq_parts > 1) {
 #pragma unroll
     for (int t = 0; t < T::NS; ++t)

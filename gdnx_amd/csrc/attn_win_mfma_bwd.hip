@@ -133,6 +133,10 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
     tile_step(k1, v1, it + 1);
     loads_done_barrier();
   }
+  if (p < 0) {                             // a row that sees nothing: 0 times a key that is not finite is NaN
+#pragma unroll
+    for (int t = 0; t < T::ND; ++t) o[t] = zero16();
+  }
   if (a.dq_parts > 1) {                    // a span of the keys: float32 sums, joined by win_dq_join_kernel
     if (qi < a.Tq) {
       float* po = a.part + (((long long)part * a.B + b) * a.Tq + qi) * a.Hq * D + qh * D + 4 * h;

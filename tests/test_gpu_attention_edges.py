@@ -48,3 +48,16 @@ def test_queries_that_see_nothing_give_zero_beside_what_is_not_finite(gpu_lib, c
     y, lse = attention.window_attention(*ins, window=W, sinks=S, lengths=None if lengths is None else ints(lengths),
                                         return_lse=True)
     assert (y[none] == 0).all() and (lse.transpose(1, 2)[none] == float("-inf")).all()
+
+
+@DTYPES
+@HEADS
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("case", UNSEEN, ids=lambda c: "-".join(map(str, c[:7])))
+def test_queries_that_see_nothing_have_no_gradient(gpu_lib, case, what, bad, D, dtype):
+    W, S, lengths = case[5:8]
+    ins, dy, none = unseeing(case, what, bad, D, dtype)
+    y = attention.window_attention(*ins, window=W, sinks=S, lengths=None if lengths is None else ints(lengths))
+    dq, = torch.autograd.grad(y, ins[:1], grad_outputs=dy)
+    assert (dq[none] == 0).all()
