@@ -26,6 +26,12 @@ __device__ __forceinline__ bool attn_visible(int p, int j, int window, int sinks
   return j <= p && (p - j < window || j < sinks);
 }
 
+// Whether a query of [off, len) sees key j: its first possible one is the nearest.
+__device__ __forceinline__ bool key_seen(int j, int off, int len, int window, int sinks) {
+  const int p = max(j, off);
+  return p < len && attn_visible(p, j, window, sinks);
+}
+
 // Key tiles of BK that queries at positions [p0, p1] see, sinks first: tile
 // `it` of `count` starts at key start(it).
 template <int BK> struct KeyTiles {

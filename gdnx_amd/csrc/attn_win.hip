@@ -422,6 +422,10 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dkv_f32_kernel(Wi
     store(si ^ 1);
     lds_barrier();
   }
+  if (!key_seen(j, off, len, a.window, a.sinks)) {   // (0 times a query or dY that is not finite is NaN)
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) ok[t] = ov[t] = zero4();
+  }
   if (ks.parts > 1) {                        // a span's sums, joined by win_dkv_join_kernel
     const long long slot = ((long long)b * a.Hkv + hk) * span_slots<KT>(a) + w;
     float* pk = a.part + (slot * 2 * KT + wave * 16 + n) * D + 4 * g;

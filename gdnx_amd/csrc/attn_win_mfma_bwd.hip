@@ -336,6 +336,10 @@ __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) 
     if (t + 1 < t1) row_step(q1, g1, q0, g0, t + 1, 1);
   }
 
+  if (!key_seen(j, off, len, a.window, a.sinks)) {    // (0 times a query or dY that is not finite is NaN)
+#pragma unroll
+    for (int t = 0; t < T::ND; ++t) ok[t] = ov[t] = zero16();
+  }
   if (ks.parts > 1) {                       // a span: float32 sums, joined by win_dkv_join_kernel
     const long long slot = ((long long)b * a.Hkv + hk) * span_slots<128>(a) + w;
     float* pk = a.part + (slot * 2 * 128 + wave * 32 + n) * D + 4 * h;

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from gdnx_amd import attention
+from oracle import attention as oa
 from test_gpu_attention import DEV, make
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +62,24 @@ def test_queries_that_see_nothing_have_no_gradient(gpu_lib, case, what, bad, D, 
     y = attention.window_attention(*ins, window=W, sinks=S, lengths=None if lengths is None else ints(lengths))
     dq, = torch.autograd.grad(y, ins[:1], grad_outputs=dy)
     assert (dq[none] == 0).all()
+
+
+@DTYPES
+@HEADS
+@pytest.mark.parametrize("case", [(2, 100, 100, 4, 2, 30, 0, [61, 90], 55),       # tokens beyond the length
+                                  (1, 200, 200, 2, 1, 40, 2, [150], 149),
+                                  (1, 20, 300, 4, 1, 50, 3, None, 10)],           # tokens that no query reaches
+                         ids=lambda c: "-".join(map(str, c[:7])))
+def test_tokens_that_nobody_sees_have_no_gradient(gpu_lib, case, D, dtype):
+    """Whatever a query of their tile holds."""
+    B, Tq, Tk, Hq, Hkv, W, S, lengths, at = case
+    q, k, v, dy = make(B, Tq, Tk, Hq, Hkv, D, dtype, seed=12)
+    seen = torch.stack([oa.visible(Tq, Tk, W, S, n).any(0) for n in lengths or [Tk] * B])
+    seen &= torch.arange(Tk) < torch.tensor(lengths or [Tk] * B)[:, None]
+    for what in ("q", "dy"):
+        q2, g2 = q.clone(), dy.clone()
+        (q2 if what == "q" else g2)[:, at, :, 5] = float("inf")
+        ins = [x.to(DEV).requires_grad_(True) for x in (q2, k, v)]
+        y = attention.window_attention(*ins, window=W, sinks=S, lengths=None if lengths is None else ints(lengths))
+        _, dk, dv = torch.autograd.grad(y, ins, grad_outputs=g2.to(DEV))
+        assert not seen.all() and (dk[~seen.to(DEV)] == 0).all() and (dv[~seen.to(DEV)] == 0).all()
