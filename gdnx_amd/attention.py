@@ -35,15 +35,22 @@ def _addr(t):
 
 
 def _rows16(t):
-    """t with D contiguous and every other stride a multiple of 16 bytes, as the
-    kernels read it (views of a fused projection are taken as they are)."""
+    """t with D contiguous and every other stride that is used a multiple of 16
+    bytes, as the kernels read it (views of a fused projection are taken as they
+    are; axes of one element may have any stride)."""
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
             return t                    # (D is 64 or 128: every row is whole units)
         unit = 16 // t.element_size()
-        if t.stride(-1) == 1 and all(s % unit == 0 for s in t.stride()[:-1]) and t.stride(1) <= 1 << 24:
+        if t.stride(-1) == 1 and all(s % unit == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape)) and (
+                t.stride(1) <= 1 << 24 or t.shape[1] == 1):
             return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _strides(t):
+    """Batch, token and head stride; none for axes of one element."""
+    return [0 if n == 1 else s for s, n in zip(t.stride()[:3], t.shape)]
 
 
 def _check(q, k, v, lengths):
@@ -71,7 +78,7 @@ def _forward(q, k, v, window, sinks, scale, lengths, want_lse, train=False):
     nws = _bytes("gdnx_win_attn_fwd_workspace_bytes", B, Tq, Tk, Hq, Hkv, D, window, sinks, code)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
     _lib.call("gdnx_win_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths), y.data_ptr(),
-              _addr(low), _addr(lse), _addr(ws), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq,
+              _addr(low), _addr(lse), _addr(ws), *_strides(q), *_strides(k), *_strides(v), B, Tq, Tk, Hq,
               Hkv, D, window, sinks, scale, code)
     return q, k, v, y, lse, low
 
@@ -101,7 +108,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         _lib.call("gdnx_win_attn_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), _addr(lengths),
                   y.data_ptr(), _addr(low), lse.data_ptr(), dy.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                  ws.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], B, Tq, Tk, Hq, Hkv, D, window,
+                  ws.data_ptr(), *_strides(q), *_strides(k), *_strides(v), B, Tq, Tk, Hq, Hkv, D, window,
                   sinks, scale, code)
         return dq, dk, dv, None, None, None, None
 

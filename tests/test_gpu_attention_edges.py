@@ -7,7 +7,7 @@ import torch
 
 from gdnx_amd import attention
 from oracle import attention as oa
-from test_gpu_attention import DEV, make
+from test_gpu_attention import DEV, TOL, make, rel
 
 pytestmark = pytest.mark.gpu
 DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -83,3 +83,29 @@ def test_tokens_that_nobody_sees_have_no_gradient(gpu_lib, case, D, dtype):
         y = attention.window_attention(*ins, window=W, sinks=S, lengths=None if lengths is None else ints(lengths))
         _, dk, dv = torch.autograd.grad(y, ins, grad_outputs=g2.to(DEV))
         assert not seen.all() and (dk[~seen.to(DEV)] == 0).all() and (dv[~seen.to(DEV)] == 0).all()
+
+
+@DTYPES
+def test_axes_of_one_element_may_have_any_stride(gpu_lib, dtype):
+    """The last token of a fused projection whose width is no multiple of 16 bytes, aligned and not; one head
+    whose stride is that of a transposed axis."""
+    T, D, width = 40, 64, 6 * 64 + 6
+    g = torch.Generator().manual_seed(13)
+    k, v = (torch.randn(1, T, 1, D, generator=g).to(dtype) for _ in range(2))
+    fused = torch.randn(1, T, width, generator=g).to(dtype)
+    for first in (0, 2):
+        x = fused.to(DEV)[..., first:first + 4 * D].unflatten(-1, (4, D))[:, -1:]
+        assert x.is_contiguous() and x.stride(1) == width
+        x.requires_grad_(True)
+        y = attention.window_attention(x, k.to(DEV), v.to(DEV), window=20, sinks=3)
+        dx, = torch.autograd.grad(y.float().sum(), x)
+        want = oa.attention(fused[..., first:first + 4 * D].unflatten(-1, (4, D))[:, -1:], k, v, 20, 3,
+                            dy=torch.ones(1, 1, 4, D))
+        assert rel(y, want[0]) <= TOL[dtype][0] and rel(dx, want[2]) <= TOL[dtype][1]
+    one = torch.randn(1, T, D, 1, generator=g).to(dtype)
+    x = one.to(DEV).transpose(2, 3)
+    assert x.is_contiguous() and x.stride(2) == 1
+    y = attention.window_attention(x, k.to(DEV), v.to(DEV), window=20, sinks=3)
+    assert rel(y, oa.attention(one.transpose(2, 3), k, v, 20, 3)[0]) <= TOL[dtype][0]
+    far = torch.randn(1, 2, (1 << 24) + 8, generator=g).to(dtype).to(DEV)[:, :1, 8:8 + D].unflatten(-1, (1, D))
+    attention.window_attention(far, k.to(DEV), v.to(DEV))      # (a stride that no token needs)
