@@ -1157,6 +1157,10 @@ static int check_strides(const long long* st, int dtype, const char* name) {
   return GDNX_OK;
 }
 
+// What the kernels get: no window is one longer than any row, and sinks beyond that are all tokens.
+static int window_arg(int window) { return window == 0 || window > kNoWindow ? kNoWindow : window; }
+static int sinks_arg(int sinks) { return sinks > kNoWindow ? kNoWindow : sinks; }
+
 // ceil(2^32 / G): see RowMap
 static unsigned group_magic(int G) { return G > 1 ? (unsigned)(((1ULL << 32) + G - 1) / G) : 0; }
 
@@ -1233,7 +1237,7 @@ extern "C" int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, co
   const int parts = win_attn_fwd_parts(B, Tq, Tk, Hq, Hkv, window, sinks, dtype);
   if (parts > 1 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
   WinAttnArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse,
-                {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype,
+                {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim, window_arg(window), sinks_arg(sinks), scale, dtype,
                 group_magic(Hq / Hkv), parts, (float*)workspace};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
       (rc = check_strides(a.vs, dtype, "v")))
@@ -1260,7 +1264,7 @@ extern "C" int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, co
     if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
   WinAttnBwdArgs a{q, k, v, lengths, y, dtype == GDNX_DTYPE_BF16 ? y_low : nullptr, lse, dy, dq, dk, dv,
                    (float*)workspace, {q_b, q_t, q_h}, {k_b, k_t, k_h}, {v_b, v_t, v_h}, B, Tq, Tk, Hq, Hkv, head_dim,
-                   window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype, group_magic(Hq / Hkv)};
+                   window_arg(window), sinks_arg(sinks), scale, dtype, group_magic(Hq / Hkv)};
   if ((rc = check_strides(a.qs, dtype, "q")) || (rc = check_strides(a.ks, dtype, "k")) ||
       (rc = check_strides(a.vs, dtype, "v")))
     return rc;
@@ -1315,7 +1319,7 @@ extern "C" int gdnx_paged_attn_step(const void* q, const void* k, const void* v,
   int lg = 0;
   while ((1 << lg) < page) ++lg;
   PagedAttnArgs a{q, k, v, k_pages, v_pages, table, lengths, slots, y, (float*)workspace, NS, rows, width, n_pages, lg,
-                  Hq, Hkv, head_dim, window == 0 || window > kNoWindow ? kNoWindow : window, sinks, scale, dtype, sp};
+                  Hq, Hkv, head_dim, window_arg(window), sinks_arg(sinks), scale, dtype, sp};
   if ((rc = paged_attn_dispatch(a, (hipStream_t)stream))) return rc;
   const FiniteBuf outs[] = {{y, (size_t)NS * Hq * head_dim, dtype}};
   return finite_outputs(outs, 1, (hipStream_t)stream);

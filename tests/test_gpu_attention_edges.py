@@ -5,7 +5,7 @@ Tolerances are those of test_gpu_attention, where they are derived.
 import pytest
 import torch
 
-from gdnx_amd import attention
+from gdnx_amd import _lib, attention
 from oracle import attention as oa
 from test_gpu_attention import DEV, TOL, make, rel
 
@@ -109,3 +109,28 @@ def test_axes_of_one_element_may_have_any_stride(gpu_lib, dtype):
     assert rel(y, oa.attention(one.transpose(2, 3), k, v, 20, 3)[0]) <= TOL[dtype][0]
     far = torch.randn(1, 2, (1 << 24) + 8, generator=g).to(dtype).to(DEV)[:, :1, 8:8 + D].unflatten(-1, (1, D))
     attention.window_attention(far, k.to(DEV), v.to(DEV))      # (a stride that no token needs)
+
+
+@DTYPES
+def test_sinks_to_the_end_of_an_int(gpu_lib, dtype):
+    """All tokens are sinks, in a C caller's natural words for it."""
+    B, T, Hq, Hkv, D, W = 1, 150, 4, 2, 64, 20
+    q, k, v, dy = (x.to(DEV) for x in make(B, T, T, Hq, Hkv, D, dtype, seed=16))
+    code = _lib.dtype_code(dtype)
+    def run(sinks):
+        y, dq, low = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
+        dk, dv = torch.empty_like(k), torch.empty_like(v)
+        lse = torch.empty(B, Hq, T, device=DEV)
+        sizes = (B, T, T, Hq, Hkv, D, W, sinks)
+        ws = [torch.empty(max(16, getattr(gpu_lib, f"gdnx_win_attn_{d}_workspace_bytes")(*sizes, code)),
+                          dtype=torch.uint8, device=DEV) for d in ("fwd", "bwd")]
+        st = [*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]]
+        p = lambda *ts: [t.data_ptr() for t in ts]
+        _lib.call("gdnx_win_attn_fwd", q.device, *p(q, k, v), None, *p(y, low, lse, ws[0]), *st, *sizes, 0.125, code)
+        _lib.call("gdnx_win_attn_bwd", q.device, *p(q, k, v), None, *p(y, low, lse, dy, dq, dk, dv, ws[1]), *st, *sizes,
+                  0.125, code)
+        return y, lse, dq, dk, dv
+    want = run(T)
+    for sinks in (1 << 30, (1 << 31) - 64, (1 << 31) - 1):
+        assert all(torch.equal(a, b) for a, b in zip(run(sinks), want)), sinks
+    assert rel(want[0], oa.attention(q, k, v)[0]) <= TOL[dtype][0]
