@@ -1168,9 +1168,12 @@ static unsigned group_magic(int G) { return G > 1 ? (unsigned)(((1ULL << 32) + G
 static long long win_bwd_part_bytes(const WinBwdPlan& p, int dq_parts, int B, int Tq, int Tk, int Hq, int Hkv, int D,
                                     int dtype) {
   const int KT = win_dkv_keys(dtype);
-  const long long slots = (long long)p.sink_tiles * p.sink_parts + ((Tk + KT - 1) / KT - p.sink_tiles) * (long long)p.tile_parts;
-  if (!prod_le(kMaxGroups / 32, {B, Hkv, slots})) return -1;       // (32: the join's workgroups a tile)
-  const long long kv = p.tile_parts > 1 || (p.sink_tiles > 0 && p.sink_parts > 1) ? slots * B * Hkv * 2 * KT * D * 4 : 0;
+  const long long tiles = (Tk + KT - 1) / KT;
+  const long long slots = (long long)p.sink_tiles * p.sink_parts + (tiles - p.sink_tiles) * p.tile_parts;
+  const long long joined = p.tile_parts > 1 ? tiles : p.sink_parts > 1 ? p.sink_tiles : 0;
+  if (!prod_le(kMaxGroups, {B, Hkv, slots})) return -1;
+  if (joined && !prod_le(kMaxGroups, {B, Hkv, joined, 2 * KT * D / 1024})) return -1;     // (the join's workgroups)
+  const long long kv = joined ? slots * B * Hkv * 2 * KT * D * 4 : 0;
   const long long q = dq_parts > 1 ? (long long)dq_parts * B * Tq * Hq * D * 4 : 0;
   return kv > q ? kv : q;
 }

@@ -134,3 +134,17 @@ def test_sinks_to_the_end_of_an_int(gpu_lib, dtype):
     for sinks in (1 << 30, (1 << 31) - 64, (1 << 31) - 1):
         assert all(torch.equal(a, b) for a, b in zip(run(sinks), want)), sinks
     assert rel(want[0], oa.attention(q, k, v)[0]) <= TOL[dtype][0]
+
+
+def test_a_backward_of_many_rows_and_heads(gpu_lib):
+    """526 thousand workgroups and 2^32 elements a tensor; all rows of the batch are alike."""
+    B, T, H, D, W = 64, 32769, 32, 64, 40
+    g = torch.Generator(device=DEV).manual_seed(20)
+    one = [torch.randn(1, T, H, D, generator=g, device=DEV).bfloat16() for _ in range(4)]
+    def run(B):
+        ins = [x.expand(B, -1, -1, -1).detach().requires_grad_(True) for x in one[:3]]
+        y = attention.window_attention(*ins, window=W)
+        return (y, *torch.autograd.grad(y, ins, grad_outputs=one[3].expand(B, -1, -1, -1).contiguous()))
+    for got, want in zip(run(B), run(1)):
+        assert rel(got[0], want[0].cpu()) <= 1e-3            # (other spans, which are summed in another order)
+        assert all(torch.equal(x, got[0]) for x in got)
