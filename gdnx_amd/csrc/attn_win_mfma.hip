@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_bf16_kernel(WinAttnArgs a) {
       if (a.scale < 0.f) qf[c] = -qf[c];
     }
   }
-  const float sc = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+  const float size = fabsf(a.scale) * kLog2e, sc = size < 1e-30f ? 1e-30f : size;      // (no number stays none)
   // positions of the workgroup's and of the wave's rows
   const int wg0 = rm.i0 + off, wg1 = min(rm.last(127), a.Tq - 1) + off;
   const int wv0 = rm.last(wave * 32) + off, wv1 = min(min(rm.last(wave * 32 + 31), a.Tq - 1) + off, len - 1);

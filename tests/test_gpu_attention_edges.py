@@ -148,3 +148,15 @@ def test_a_backward_of_many_rows_and_heads(gpu_lib):
     for got, want in zip(run(B), run(1)):
         assert rel(got[0], want[0].cpu()) <= 1e-3            # (other spans, which are summed in another order)
         assert all(torch.equal(x, got[0]) for x in got)
+
+
+@DTYPES
+def test_a_scale_that_is_no_number(gpu_lib, dtype):
+    """Gives no number, in both types, in the prompt's form and the served token's."""
+    q, k, v, _ = (x.to(DEV) for x in make(1, 40, 40, 2, 1, 64, dtype, seed=17))
+    y = attention.window_attention(q, k, v, window=9, scale=float("nan"))
+    assert torch.isnan(y).all()
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    pool = [x[0].transpose(0, 1).unsqueeze(0).contiguous() for x in (k[:, :32], v[:, :32])]
+    y = attention.paged_attention_step(q[:, 0], None, None, *pool, table, ints([32]), scale=float("nan"))
+    assert torch.isnan(y).all()
