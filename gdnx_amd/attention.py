@@ -128,7 +128,7 @@ def window_attention(q, k, v, window=None, sinks=0, *, scale=None, lengths=None,
     B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
     if B == 0 or Tq == 0 or Tk == 0:
         y = empty_result((B, Tq, Hq, D), q.dtype, q.device, q, k, v)
-        return (y, torch.full((B, Hq, Tq), float("-inf"), device=q.device)) if return_lse else y
+        return (y, torch.full((B, Hq, Tq), float("-inf"), dtype=torch.float32, device=q.device)) if return_lse else y
     scale = D ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         y, lse = WindowAttentionFunction.apply(q, k, v, window, sinks, scale, lengths)

@@ -160,3 +160,14 @@ def test_a_scale_that_is_no_number(gpu_lib, dtype):
     pool = [x[0].transpose(0, 1).unsqueeze(0).contiguous() for x in (k[:, :32], v[:, :32])]
     y = attention.paged_attention_step(q[:, 0], None, None, *pool, table, ints([32]), scale=float("nan"))
     assert torch.isnan(y).all()
+
+
+def test_empty_lse_is_float32(gpu_lib):
+    x = lambda T: torch.randn(2, T, 2, 64, device=DEV)
+    q, k = x(3), x(0)
+    torch.set_default_dtype(torch.float64)
+    try:
+        _, lse = attention.window_attention(q, k, k, return_lse=True)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert lse.dtype == torch.float32 and lse.shape == (2, 2, 3) and (lse == float("-inf")).all()
