@@ -13,6 +13,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _need, empty_result
@@ -32,6 +33,12 @@ def _bytes(query, *sizes):
 
 def _addr(t):
     return None if t is None else t.data_ptr()
+
+
+def _no_tangents(*ts):
+    if forward_ad._current_level >= 0:          # (inside dual_level() only)
+        _need(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in ts),
+              "attention has no forward-mode derivative")
 
 
 def _rows16(t):
@@ -123,8 +130,10 @@ def window_attention(q, k, v, window=None, sinks=0, *, scale=None, lengths=None,
     hold; their outputs and gradients are zero, as are those of queries before
     position 0.  scale defaults to 1/sqrt(D).  Returns y [B,Tq,Hq,D], with
     return_lse also the log-sum-exp of each query's scores [B,Hq,Tq] (float32,
-    -inf where nothing is seen, not differentiable)."""
+    -inf where nothing is seen, not differentiable).  There is no forward-mode
+    derivative and no second one."""
     window, sinks = _window(window, sinks)
+    _no_tangents(q, k, v)
     B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
     if B == 0 or Tq == 0 or Tk == 0:
         y = empty_result((B, Tq, Hq, D), q.dtype, q.device, q, k, v)
@@ -147,8 +156,10 @@ def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=Non
     token stands at position length - 1.  k, v [NS,Hkv,D] are its key and
     value, which the call also writes to their page; None where they are there
     already.  window, sinks and scale as in ``window_attention``.  Returns y
-    [NS,Hq,D] (or ``out``)."""
+    [NS,Hq,D] (or ``out``), which is not differentiable: no gradient reaches the
+    inputs."""
     window, sinks = _window(window, sinks)
+    _no_tangents(q, k, v, k_pages, v_pages)
     dev, dtype = q.device, q.dtype
     _need(q.is_cuda and q.dim() == 3, "q must be a CUDA (HIP) tensor [NS,Hq,D]")
     NS, Hq, D = q.shape

@@ -171,3 +171,19 @@ def test_empty_lse_is_float32(gpu_lib):
     finally:
         torch.set_default_dtype(torch.float32)
     assert lse.dtype == torch.float32 and lse.shape == (2, 2, 3) and (lse == float("-inf")).all()
+
+
+def test_forward_mode_is_refused(gpu_lib):
+    """There is no forward-mode derivative: an error, not a result without its tangent."""
+    q, k, v, t = make(1, 8, 8, 2, 2, 64, torch.float32, seed=18)
+    q, k, v, t = (x.to(DEV) for x in (q, k, v, t))
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        attention.window_attention(q, k, v)                          # (no tangent: as ever)
+        for n in range(3):
+            ins = [torch.autograd.forward_ad.make_dual(x, t) if i == n else x for i, x in enumerate((q, k, v))]
+            with pytest.raises(ValueError, match="forward-mode"):
+                attention.window_attention(*ins)
+        q1 = torch.autograd.forward_ad.make_dual(q[:, 0], t[:, 0])
+        with pytest.raises(ValueError, match="forward-mode"):
+            attention.paged_attention_step(q1, None, None, *(x.transpose(1, 2).contiguous() for x in (k, v)), table, ints([8]))
