@@ -30,9 +30,11 @@ __device__ const uint4 g_zero_row[32] = {};       // one row of zeros: 512 bytes
 
 struct Seen {                                     // a row's visible keys
   int len, lo, ns, nvis;
+  bool fits;                                      // whether the table has a place for the last token
   __device__ __forceinline__ Seen(const PagedAttnArgs& a, int r) {
     const long long cap = (long long)a.width << a.page_log;
     len = r >= 0 && r < a.rows ? a.lengths[r] : 0;
+    fits = len <= cap;
     len = len < 0 ? 0 : len > cap ? (int)cap : len;
     lo = len > a.window ? len - a.window : 0;
     ns = min(a.sinks, lo);
@@ -111,8 +113,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
   }
   const int* table = a.table + (long long)r * a.width;
   const long long rowb = D * (int)sizeof(CT), headb = rowb << a.page_log;
-  const char* knew = a.k ? (const char*)a.k + ((long long)s * a.Hkv + hk) * rowb : nullptr;
-  const char* vnew = a.v ? (const char*)a.v + ((long long)s * a.Hkv + hk) * rowb : nullptr;
+  // a new token without a place in the cache is neither written nor seen
+  const char* knew = a.k && see.fits ? (const char*)a.k + ((long long)s * a.Hkv + hk) * rowb : nullptr;
+  const char* vnew = a.v && see.fits ? (const char*)a.v + ((long long)s * a.Hkv + hk) * rowb : nullptr;
   // the new token goes to its page (nobody reads it there in this call)
   if (knew && span == 0 && gblk == 0 && tid < 2 * UPR) {
     const int pos = see.len - 1, pg = table[pos >> a.page_log], u = tid % UPR;
@@ -147,11 +150,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
     if (lane < BT) {
       const int x = t * BT + lane, j = x < see.ns ? x : x - see.ns + see.lo;
       long long o = -1;
-      if (x < see.nvis) {
-        if (knew && x == see.nvis - 1) o = -2;
-        else if (pg >= 0 && pg < a.n_pages)
-          o = ((long long)pg * a.Hkv + hk) * headb + (j & ((1 << a.page_log) - 1)) * rowb;
-      }
+      if (x < see.nvis && pg >= 0 && pg < a.n_pages)
+        o = knew && x == see.nvis - 1 ? -2 : ((long long)pg * a.Hkv + hk) * headb + (j & ((1 << a.page_log) - 1)) * rowb;
       off[lane] = o;
     }
     wave_lds_sync();

@@ -650,7 +650,8 @@ int gdnx_win_attn_bwd(const void* q, const void* k, const void* v, const int* le
  *   their page by the call, or both null where they are there already;
  *   k_pages, v_pages [n_pages,Hkv,page,D];  table [rows,width] int32, an entry
  *   outside [0, n_pages) meaning that the row has no such page: its tokens are
- *   not seen;  lengths [rows] int32.
+ *   not seen, and a new one is not written;  lengths [rows] int32 (beyond
+ *   width * page: the row is cut there, and the new token has no place either).
  * workspace: gdnx_paged_attn_workspace_bytes bytes (-1 if the sizes are
  * invalid; null where that is 0).  Two rows of a call must not share a slot
  * when k and v are given. */

@@ -7,7 +7,7 @@ import torch
 
 from gdnx_amd import _lib, attention
 from oracle import attention as oa
-from test_gpu_attention import DEV, TOL, make, rel
+from test_gpu_attention import DEV, TOL, make, paged, rel
 
 pytestmark = pytest.mark.gpu
 DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -187,3 +187,19 @@ def test_forward_mode_is_refused(gpu_lib):
         q1 = torch.autograd.forward_ad.make_dual(q[:, 0], t[:, 0])
         with pytest.raises(ValueError, match="forward-mode"):
             attention.paged_attention_step(q1, None, None, *(x.transpose(1, 2).contiguous() for x in (k, v)), table, ints([8]))
+
+
+@DTYPES
+def test_a_new_token_without_a_place(gpu_lib, dtype):
+    """Neither written nor seen: the call does what it does of a cache alone, and no cached token is lost."""
+    q, kp, vp, table, _, ks, vs = paged([48, 40], 4, 2, 64, 16, dtype, seed=19)
+    new = [torch.randn(2, 2, 64, generator=torch.Generator().manual_seed(n)).to(dtype).to(DEV) for n in (1, 2)]
+    gone = table.clone()
+    gone[0, 2] = -1
+    gone[1, 2] = 10 ** 6
+    for tab, lens in ((table, [49, 1000]), (gone, [48, 40])):        # longer than its table row; its page is not there
+        kd, vd, td = kp.to(DEV), vp.to(DEV), tab.to(DEV)
+        alone = attention.paged_attention_step(q.to(DEV), None, None, kd, vd, td, ints(lens))
+        y = attention.paged_attention_step(q.to(DEV), *new, kd, vd, td, ints(lens))
+        assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
+        assert torch.equal(y, alone) and torch.isfinite(y).all()
