@@ -154,10 +154,16 @@ def pages_compact(k_pages, v_pages, table, refs, out=None):
     return t_out, r_out
 
 
+def _version(t):
+    return None if t.is_inference() else t._version      # (inference tensors count no changes)
+
+
 class PagedKVCache:
-    """A page pool with its table.  Rows are named by the caller as ints (or as
-    the int32 tensor that ``rows_tensor`` made of them, so that a step's layers
-    share one upload)."""
+    """A page pool with its table.  Rows are named by the caller as ints, or as
+    the int32 tensor that ``rows_tensor`` made of them, so that a step's calls
+    share one upload; neither waits for the device (another tensor is read
+    back).  A graph captures the functions above on the cache's tensors: the
+    lengths that the cache keeps on the host do not advance with a replay."""
 
     def __init__(self, n_pages: int, page: int, Hkv: int, D: int, rows: int, max_len: int, layers: int = 1,
                  dtype=torch.bfloat16, device="cuda"):
@@ -185,6 +191,9 @@ class PagedKVCache:
         return [self._free_rows.pop() for _ in range(n)]
 
     def _check_rows(self, rows):
+        if isinstance(rows, torch.Tensor):
+            made = getattr(rows, "named_rows", None)
+            rows = made[0] if made and made[1] == _version(rows) else rows.tolist()
         rows = [int(r) for r in rows]
         free = set(self._free_rows)
         if len(set(rows)) != len(rows):
@@ -194,15 +203,33 @@ class PagedKVCache:
                 raise ValueError(f"row {r} is not allocated")
         return rows
 
+    def _upload(self, xs):
+        """A list as an int32 device tensor, by way of pinned memory (which torch
+        keeps until the copy is done), so that nothing waits."""
+        if self.device.type != "cuda" or not xs:
+            return torch.tensor(xs, dtype=torch.int32, device=self.device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("rows named as ints cannot be captured: name them by a tensor that rows_tensor made before")
+        return torch.tensor(xs, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
+
+    def _named(self, rows):
+        """The rows, checked, as a list and as a device tensor."""
+        host = self._check_rows(rows)
+        if isinstance(rows, torch.Tensor) and rows.dtype == torch.int32 and rows.device == self.table.device:
+            return host, rows
+        return host, self._upload(host)
+
     def rows_tensor(self, rows):
         """The rows as an int32 device tensor, checked (-1 is not a row here)."""
         if isinstance(rows, torch.Tensor):
             return rows
-        return torch.tensor(self._check_rows(rows), dtype=torch.int32, device=self.device)
+        host, t = self._named(rows)
+        t.named_rows = host, _version(t)
+        return t
 
     def free(self, rows) -> None:
-        rows = self._check_rows(rows)
-        pages_free(self.table, self.lengths, self.refs, self.rows_tensor(rows))
+        rows, named = self._named(rows)
+        pages_free(self.table, self.lengths, self.refs, named)
         for r in rows:
             self.lens[r] = 0
         self._free_rows.extend(rows)
@@ -221,13 +248,13 @@ class PagedKVCache:
 
     def reserve(self, rows, n_new: int = 1):
         """Room for the next n_new tokens of every row; returns start (int32 [n])."""
-        rows, n_new = self._check_rows(rows), int(n_new)
+        n_new, (rows, named) = int(n_new), self._named(rows)
         _need(n_new >= 0, "n_new must not be negative")
         for r in rows:
             if self.lens[r] + n_new > self.width * self.page:
                 raise ValueError(f"row {r}: {self.lens[r]} + {n_new} tokens, the table holds {self.width * self.page}")
         self._take(sum(-(-(self.lens[r] + n_new) // self.page) - -(-self.lens[r] // self.page) for r in rows))
-        start = pages_reserve(self.table, self.lengths, self.refs, self.rows_tensor(rows), n_new, self.page, self.status)
+        start = pages_reserve(self.table, self.lengths, self.refs, named, n_new, self.page, self.status)
         for r in rows:
             self.lens[r] += n_new
         return start
@@ -246,14 +273,15 @@ class PagedKVCache:
 
     def fork(self, parents) -> list:
         """A new row for every entry of parents (a row may be named more than once), holding what it holds."""
-        parents = [int(r) for r in parents]
+        parents = [int(r) for r in (parents.tolist() if isinstance(parents, torch.Tensor) else parents)]
         self._check_rows(set(parents))
         if len(parents) > len(self._free_rows):
             raise RuntimeError(f"page cache full: {len(parents)} rows asked, {len(self._free_rows)} free")
         self._take(sum(self.lens[r] % self.page != 0 for r in parents))
         children = self.alloc(len(parents))
-        up = torch.tensor([parents, children], dtype=torch.int32, device=self.device)
-        pages_fork(self.k_pages, self.v_pages, self.table, self.lengths, self.refs, up[0], up[1], self.status)
+        up = self._upload(parents + children)
+        pages_fork(self.k_pages, self.v_pages, self.table, self.lengths, self.refs, up[:len(parents)], up[len(parents):],
+                   self.status)
         for p, c in zip(parents, children):
             self.lens[c] = self.lens[p]
         return children
