@@ -7,7 +7,7 @@ import torch
 
 from gdnx_amd import _lib, attention
 from oracle import attention as oa
-from test_gpu_attention import DEV, TOL, make, paged, rel
+from test_gpu_attention import DEV, TOL, check, make, paged, rel
 
 pytestmark = pytest.mark.gpu
 DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -203,3 +203,45 @@ def test_a_new_token_without_a_place(gpu_lib, dtype):
         y = attention.paged_attention_step(q.to(DEV), *new, kd, vd, td, ints(lens))
         assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
         assert torch.equal(y, alone) and torch.isfinite(y).all()
+
+
+def parts(q, k, window, sinks):
+    """Workspace bytes of the forward: more than none where its keys are split."""
+    code = _lib.dtype_code(q.dtype)
+    return _lib.load().gdnx_win_attn_fwd_workspace_bytes(*q.shape[:2], k.shape[1], q.shape[2], k.shape[2], q.shape[3],
+                                                         window or 0, sinks, code)
+
+
+@DTYPES
+@HEADS
+@pytest.mark.parametrize("shape", [
+    (2, 33, 1500, 4, 2, None, 0, [1500, 1481]), (2, 33, 1500, 4, 2, None, 0, [1499, 70]),     # fewer tiles than parts
+    (1, 40, 2500, 6, 2, 1500, 70, None), (4, 130, 1200, 16, 4, None, 0, [1200, 1070, 0, 1100]),
+    (1, 1, 2000, 3, 1, None, 0, [2000])], ids=lambda s: "-".join(map(str, s[:7])) + f"-{s[7]}")
+def test_split_keys(gpu_lib, shape, D, dtype):
+    B, Tq, Tk, Hq, Hkv, window, sinks, lengths = shape
+    x = make(B, Tq, Tk, Hq, Hkv, D, dtype, seed=14)
+    assert parts(x[0], x[1], window, sinks) > 0
+    check(*x, window, sinks, lengths)
+
+
+@DTYPES
+@HEADS
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
+def test_split_keys_beside_what_is_not_finite(gpu_lib, bad, D, dtype):
+    """Inner tokens that some queries of their tile do not see: later ones, and those the window has left behind."""
+    Tq, Tk, W, S, at = 100, 2600, 2200, 3, (310, 2550)
+    q, k, v, _ = make(1, Tq, Tk, 4, 2, D, dtype, seed=15)
+    assert parts(q, k, W, S) > 0
+    hide = oa.visible(Tq, Tk, W, S, Tk)[:, list(at)].any(1)
+    want, want_lse = oa.attention(q, k, v, W, S)
+    assert hide.any() and not hide.all()
+    for what in "kv":
+        k2, v2 = k.clone(), v.clone()
+        (k2 if what == "k" else v2)[0, list(at), :, 3] = bad
+        y, lse = attention.window_attention(q.to(DEV), k2.to(DEV), v2.to(DEV), window=W, sinks=S, return_lse=True)
+        assert rel(y[0, ~hide], want[0, ~hide]) <= TOL[dtype][0]
+        assert float((lse[0][:, ~hide].cpu().double() - want_lse[0][:, ~hide]).abs().max()) <= 1e-4
+        if what == "v":
+            assert not torch.isfinite(y[0, hide][..., 3].float()).any()
+            assert rel(y[0, hide][..., 4:], want[0, hide][..., 4:]) <= TOL[dtype][0]
