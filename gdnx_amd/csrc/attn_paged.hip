@@ -20,7 +20,10 @@
 //
 // S^T = K Q^T puts a query head in a lane column: its statistics are in-lane
 // maxima and two shuffles, and its probabilities are the operand of
-// O^T = V^T P^T.  Spans are joined by a second kernel, in order.
+// O^T = V^T P^T: in bf16 they are two, the rounded value and what that leaves
+// over, since the matrix units wait for memory anyway (256 rows 384 us with one
+// operand and with two; y is 1.7e-3 from 64 bits, which is its own rounding,
+// instead of 2.2e-3).  Spans are joined by a second kernel, in order.
 #include "attn_common.hpp"
 
 namespace gdnx {
@@ -222,11 +225,21 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedAttnArgs a) {
     l = l * f + sum;
     m = mn;
     const Frag pf = acc_frag((CT*)nullptr, sx[0], sx[NU - 1]);
+    Frag pr{};                           // what rounding P to bf16 leaves over
+    if constexpr (sizeof(CT) == 2) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sx[u][e] = bf16_rest(sx[u][e]);
+      pr = acc_frag((CT*)nullptr, sx[0], sx[NU - 1]);
+    }
     wave_lds_sync();
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       o[c] *= f;
-      mma(o[c], v_frag<D>(stage, c, n, g), pf);
+      const Frag vf = v_frag<D>(stage, c, n, g);
+      mma(o[c], vf, pf);
+      if constexpr (sizeof(CT) == 2) mma(o[c], vf, pr);
     }
   }
   l += __shfl_xor(l, 16, 64);

@@ -7,7 +7,7 @@ import torch
 
 from gdnx_amd import _lib, attention
 from oracle import attention as oa
-from test_gpu_attention import DEV, TOL, check, make, paged, rel
+from test_gpu_attention import DEV, TOL, check, make, paged, rel, step_ref
 
 pytestmark = pytest.mark.gpu
 DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -245,3 +245,16 @@ def test_split_keys_beside_what_is_not_finite(gpu_lib, bad, D, dtype):
         if what == "v":
             assert not torch.isfinite(y[0, hide][..., 3].float()).any()
             assert rel(y[0, hide][..., 4:], want[0, hide][..., 4:]) <= TOL[dtype][0]
+
+
+@HEADS
+@pytest.mark.parametrize("lens,Hq,Hkv,window", [([3000, 17, 900, 2000], 16, 4, None), ([5000], 32, 8, 700),
+                                                ([100] * 20, 8, 2, None)])
+def test_a_served_token_is_rounded_once(gpu_lib, lens, Hq, Hkv, window, D):
+    """bf16: half a unit in the last place is 2^-8 of a power of two, so rounding a value m 2^e, 1 <= m < 2, is off by
+    2^-8 / sqrt(3) / m of it, in the mean over a Gaussian's values 1.66e-3; a tenth more for a sample of some thousand.
+    A probability rounded to bf16 before its product would add as much again in squares: 2.2e-3."""
+    q, kp, vp, table, _, ks, vs = paged(lens, Hq, Hkv, D, 16, torch.bfloat16, seed=21)
+    y = attention.paged_attention_step(q.to(DEV), None, None, kp.to(DEV), vp.to(DEV), table.to(DEV), ints(lens),
+                                       window=window, sinks=4)
+    assert rel(y, step_ref(q, ks, vs, window, 4)) <= 1.83e-3
