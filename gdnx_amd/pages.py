@@ -277,9 +277,10 @@ class PagedKVCache:
         self._check_rows(set(parents))
         if len(parents) > len(self._free_rows):
             raise RuntimeError(f"page cache full: {len(parents)} rows asked, {len(self._free_rows)} free")
-        self._take(sum(self.lens[r] % self.page != 0 for r in parents))
-        children = self.alloc(len(parents))
+        children = self._free_rows[::-1][:len(parents)]             # (what alloc gives)
         up = self._upload(parents + children)
+        self._take(sum(self.lens[r] % self.page != 0 for r in parents))
+        self.alloc(len(parents))
         pages_fork(self.k_pages, self.v_pages, self.table, self.lengths, self.refs, up[:len(parents)], up[len(parents):],
                    self.status)
         for p, c in zip(parents, children):

@@ -90,6 +90,9 @@ def test_rows_named_as_ints_are_not_captured(gpu_lib):
         pages.pages_reserve(c.table, c.lengths, c.refs, rt, 1, c.page, c.status)
         with pytest.raises(RuntimeError, match="captured"):
             c.reserve(rows)
+        with pytest.raises(RuntimeError, match="captured"):
+            c.fork(rows)
+    assert len(c.alloc(2)) == 2 and c.lens == [1, 1, 0, 0]      # (nothing was taken)
     for n in range(3):
         graph.replay()
         torch.cuda.synchronize()
