@@ -215,7 +215,8 @@ class PagedKVCache:
     def _named(self, rows):
         """The rows, checked, as a list and as a device tensor."""
         host = self._check_rows(rows)
-        if isinstance(rows, torch.Tensor) and rows.dtype == torch.int32 and rows.device == self.table.device:
+        if isinstance(rows, torch.Tensor) and rows.dtype == torch.int32 and rows.device == self.table.device and (
+                rows.is_contiguous()):
             return host, rows
         return host, self._upload(host)
 

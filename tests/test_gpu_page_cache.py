@@ -64,6 +64,8 @@ def test_rows_by_any_tensor(gpu_lib):
     c.reserve(rt, 3)
     c.reserve(torch.tensor(rows[:1]), 2)                 # read back, and taken in 64 bits too
     assert c.lens[rows[0]] == 5 and c.lens[rows[1]] == 3 and c.lengths.tolist() == c.lens
+    c.reserve(rt.repeat_interleave(2)[::2])              # a view with gaps
+    assert c.lengths.tolist() == c.lens == [6, 4, 0, 0]
     rt[0] = rt[1]                                        # changed since: what it was made of no longer holds
     with pytest.raises(ValueError, match="twice"):
         c.reserve(rt)
