@@ -125,13 +125,15 @@ def window_attention(q, k, v, window=None, sinks=0, *, scale=None, lengths=None,
     D 64 or 128, any strides), differentiable in q, k and v.
 
     Query i stands at position p = i + Tk - Tq and sees key j if j <= p and
-    p - j < window or j < sinks (window None: every earlier key).  lengths
+    p - j < window or j < sinks (window None or 0: every earlier key).  lengths
     (int32 [B]): tokens at or beyond a row's length are padding, whatever they
     hold; their outputs and gradients are zero, as are those of queries before
-    position 0.  scale defaults to 1/sqrt(D).  Returns y [B,Tq,Hq,D], with
-    return_lse also the log-sum-exp of each query's scores [B,Hq,Tq] (float32,
-    -inf where nothing is seen, not differentiable).  There is no forward-mode
-    derivative and no second one."""
+    position 0.  A value within the length that is not finite reaches the
+    outputs of the queries that see it, and gradients of its tile.  scale
+    defaults to 1/sqrt(D).  Returns y [B,Tq,Hq,D], with return_lse also the
+    log-sum-exp of each query's scores [B,Hq,Tq] (float32, -inf where nothing
+    is seen, not differentiable).  There is no forward-mode derivative and no
+    second one."""
     window, sinks = _window(window, sinks)
     _no_tangents(q, k, v)
     B, Tq, Tk, Hq, Hkv, D = _check(q, k, v, lengths)
@@ -155,7 +157,8 @@ def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=Non
     slots[s] (int32 [NS]; outside the table: an empty row, y = 0), or s.  The
     token stands at position length - 1.  k, v [NS,Hkv,D] are its key and
     value, which the call also writes to their page; None where they are there
-    already.  window, sinks and scale as in ``window_attention``.  Returns y
+    already; a token that has no place in the table is neither written nor seen.
+    window, sinks and scale as in ``window_attention``.  Returns y
     [NS,Hq,D] (or ``out``), which is not differentiable: no gradient reaches the
     inputs."""
     window, sinks = _window(window, sinks)

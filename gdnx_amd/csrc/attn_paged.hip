@@ -45,7 +45,8 @@ struct Seen {                                     // a row's visible keys
   }
 };
 
-// spans that a row of n key tiles is cut into: at least four tiles each
+// spans that a row of n key tiles is cut into: about four tiles each, or more (five
+// tiles are cut into three and two)
 __device__ __forceinline__ int spans(int tiles, int max_spans) { return min(max_spans, (tiles + 3) / 4); }
 
 // (a choice between pointers is read as memory of any kind, LDS included,
@@ -324,7 +325,7 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) paged_join_
 }
 
 // Spans of a row of `keys` visible keys.  Two workgroups a CU where the rows
-// and heads alone do not give them, each span at least four tiles; up to six a
+// and heads alone do not give them, each span about four tiles or more; up to six a
 // CU (so that rows of unequal lengths level out) while a span keeps 32 tiles,
 // beside which a workgroup's start and its share of the join are small.  In us,
 // one span / this rule / eight a CU with at least four tiles each:

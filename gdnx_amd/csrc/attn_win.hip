@@ -446,14 +446,14 @@ template <int D> __global__ void __launch_bounds__(256, 2) win_dkv_f32_kernel(Wi
 }
 
 // ---- shares of the work ----
-// Rows a workgroup takes in the forward, keys a tile holds, workgroups that run at once.
+// Rows a workgroup takes in the forward, keys a tile holds there and in the dk / dv kernel.
 static int fwd_rows(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 128 : 64; }
 static int fwd_keys(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 64 : 32; }
 int win_dkv_keys(int dtype) { return dtype == GDNX_DTYPE_BF16 ? 128 : 64; }
 
-// Parts that the rows' keys are cut into: one, unless the workgroups would not
-// give every CU its two; then as many as do, each of at least four tiles (eight
-// in bf16, whose tiles take less time beside the join, unless the workgroups are very
+// Parts that the rows' keys are cut into: as many as keep the workgroups within
+// two a CU (so one from 257 workgroups on), each of at least four tiles (eight in
+// bf16, whose tiles take less time beside the join, unless the workgroups are very
 // few).  Forward in us, uncut / cut (bf16, d = 128 unless said): 2 x 200
 // queries on 16584 keys, 16/2 heads 297 / 77; 2048 on 16384, 16/4 344 / 297;
 // 4096 on 4096, 8/2 82 / 65; 16 on 4096, 8/8 109 / 16 (eight tiles: 21);

@@ -12,15 +12,20 @@ namespace gdnx {
 // double-buffered, one barrier a tile (by way of registers: 1260 instead of
 // 1170 thousand cycles for the prompt below).
 //   S^T = K Q^T   a lane holds 32 scores of one row
-//   O^T += V^T P^T   the score accumulators, as bf16, are the operand
+//   O^T += V^T P^T   the score accumulators, as bf16, are the operand (their rest
+//                    as a second one would be half as many matrix instructions again:
+//                    y is 2.1e-3 to 2.3e-3 from 64 bits, 1.7e-3 of it its own rounding)
 // The running maximum is raised only when a score exceeds it by 2^8: the
 // output is then rescaled (P stays below 256, its relative rounding does not
 // change), which spares the rescaling of 64 accumulators on most tiles.
 //
-// Bound by the matrix and vector units together at the clock that the chip's
-// power leaves: the matrix units are busy 46 to 48 % of the cycles, the softmax
-// of a tile takes about as long as its products, and neither operands read
-// further ahead nor waves shifted against each other change the time.  16 query
+// Bound by the matrix and vector units, which take turns: matrix instructions
+// are in work 48 % of the cycles, other vector ones 43 %, and the two waves of a
+// SIMD hardly cover one's softmax with the other's products; neither operands
+// read further ahead nor waves shifted against each other change the time.  LDS
+// is active 25 % of the cycles by its counter; a wave of 32 rows reads an operand
+// for every product, and 64 rows a wave, which would halve that, were not tried.
+// The clock is 1.6 to 2.0 GHz under this load.  16 query
 // heads on 4, d = 128: 16384 tokens without a window 1.05 to 1.09 PFLOP/s; 32768
 // tokens, window 2048, 64 sinks 571 to 584 us, 950 TFLOP/s of visible products;
 // B = 4, T = 4096, window 1024 (three of a row's 18 tiles are cut by the window

@@ -11,10 +11,13 @@ namespace gdnx {
 //   S^T = K Q^T,  dP^T = V dY^T,  dS^T = P^T o (dP^T - delta),  dQ^T += K^T dS^T
 // The scores are formed here and again by the dk / dv kernel, seven products in
 // place of five: one kernel for all three would add its dq tiles up with float
-// atomics, whose order changes the result, or write every tile's out.  Bound
-// like the forward (matrix units busy 43 %); B = 4, T = 4096, 16/4 heads,
-// d = 128, window 1024, 16 sinks: 227 to 254 us (445 thousand cycles; 480 with
-// operands not read ahead).
+// atomics, whose order changes the result, or write every tile's out.  P and dS
+// are rounded to bf16 as the operands of the second products, as P is in the
+// forward (gradients are 2.3e-3 to 2.4e-3 from 64 bits, 1.7e-3 of it their own
+// rounding).  Bound like the forward (matrix instructions in work 43 % of the
+// cycles, other vector ones 31 %, LDS 23 %); B = 4, T = 4096, 16/4 heads, d = 128,
+// window 1024, 16 sinks: 225 to 254 us (448 thousand cycles; 480 with operands
+// not read ahead).
 template <int D>
 __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
   using T = Tile<D>;
@@ -166,11 +169,11 @@ __global__ void __launch_bounds__(256, 2) win_dq_bf16_kernel(WinAttnBwdArgs a) {
 //   S = Q K^T,  dP = dY V^T,  dV^T += dY^T P,  dK^T += Q^T dS
 // K stays in registers (the wave's 32 keys, half of what it holds are the sums),
 // V in LDS, which both together would not fit beside; 32 rows of Q and dY a
-// step, straight into LDS, double-buffered.  Bound by LDS, about half of whose
-// reads' rate it takes, and their latency: each product reads an operand, and
-// with two waves a SIMD the matrix units are busy 39 % of the cycles.  B = 4,
-// T = 4096, 16/4 heads, d = 128, window 1024, 16 sinks: 302 to 360 us (631
-// thousand cycles; 700 with operands not read ahead).
+// step, straight into LDS, double-buffered.  Bound by the latency of LDS: each
+// product reads an operand, its waves wait 47 % of their cycles, LDS is active
+// 30 % of all by its counter, and with two waves a SIMD the matrix units are busy
+// 39 %.  B = 4, T = 4096, 16/4 heads, d = 128, window 1024, 16 sinks: 302 to 360 us
+// (625 thousand cycles; 700 with operands not read ahead).
 template <int D>
 __global__ void __launch_bounds__(256, 2) win_dkv_bf16_kernel(WinAttnBwdArgs a) {
   using T = Tile<D>;

@@ -33,7 +33,7 @@ namespace {
 constexpr int PT = 1024;             // threads of the bookkeeping workgroup
 constexpr int PW = PT / 64;
 
-// Exclusive prefix sum over the workgroup; *total gets the sum.  sh: PW + 1 ints.
+// Exclusive prefix sum over the workgroup; *total gets the sum.  sh: PW ints.
 __device__ __forceinline__ int wg_scan(int x, int* sh, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int s = x;

@@ -603,16 +603,20 @@ int gdnx_rls_bwd(const float* q, const float* K, const float* V, const float* Bg
  *
  * Attention with a sliding window and sinks.  q [B,Tq,Hq,D], k and v
  * [B,Tk,Hkv,D] in the io dtype with any element strides (batch, token, head)
- * that are multiples of 16 bytes (a token's at most 2^24 elements), D
+ * that are multiples of 16 bytes (a token's at most 2^24 elements; that of an
+ * axis of one element is not used: pass 0), D
  * contiguous; Hq a multiple of Hkv, query head h reading key head
  * h / (Hq / Hkv); D = 64 or 128.  Query i stands at position p = i + Tk - Tq
  * and sees key j if
  *     j <= p,  p < lengths[b],  and  p - j < window or j < sinks
- * (lengths null: Tk; window 0: every earlier key).  A query that sees
- * nothing gives y = 0, lse = -infinity and no gradient.  Keys at or beyond
- * lengths[b] never enter a result; a key or value before it that is not finite
- * reaches only the outputs of queries that see it (gradients may take it up
- * with its tile of 64 keys).
+ * (lengths null: Tk; window 0: every earlier key; window and sinks up to
+ * 2^31 - 1).  A query that sees nothing gives y = 0, lse = -infinity and no
+ * gradient, and a key that no query sees has none, whatever the others hold; y = 0
+ * and lse = -infinity also where every visible score is -infinity.  Keys at or
+ * beyond lengths[b] never enter a result; a key or value before it that is not
+ * finite reaches only the outputs of queries that see it.  Into gradients of
+ * queries and keys that are seen, a value of q, k, v or dy within the length that
+ * is not finite may come with its tile of up to 64 rows or keys.
  *   y   [B,Tq,Hq,D] io dtype, contiguous: softmax(scale q.k) v
  *   y_low bf16, as y (may be null, and is not written for float32): y minus its
  *       rounding, for the backward, whose dS would otherwise carry the rounding
@@ -625,7 +629,8 @@ long long gdnx_win_attn_fwd_workspace_bytes(int B, int Tq, int Tk, int Hq, int H
                                             int sinks, int dtype);
 int gdnx_win_attn_fwd(const void* q, const void* k, const void* v, const int* lengths, void* y, void* y_low,
                       float* lse, void* workspace, long long q_b, long long q_t, long long q_h,
-                      long long k_b, long long k_t, long long k_h, long long v_b, long long v_t, long long v_h, int B, int Tq, int Tk, int Hq, int Hkv,
+                      long long k_b, long long k_t, long long k_h, long long v_b, long long v_t, long long v_h,
+                      int B, int Tq, int Tk, int Hq, int Hkv,
                       int head_dim, int window, int sinks, float scale, int dtype, void* stream);
 
 /* Its gradients from dy [B,Tq,Hq,D] (contiguous) and the forward's y, y_low

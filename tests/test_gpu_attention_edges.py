@@ -258,3 +258,16 @@ def test_a_served_token_is_rounded_once(gpu_lib, lens, Hq, Hkv, window, D):
     y = attention.paged_attention_step(q.to(DEV), None, None, kp.to(DEV), vp.to(DEV), table.to(DEV), ints(lens),
                                        window=window, sinks=4)
     assert rel(y, step_ref(q, ks, vs, window, 4)) <= 1.83e-3
+
+
+@DTYPES
+def test_scores_that_are_all_minus_infinity(gpu_lib, dtype):
+    q, k, v, _ = (x.to(DEV) for x in make(1, 40, 40, 2, 1, 64, dtype, seed=22))
+    q[..., 0], k[:, :20, :, 0] = 1.0, float("-inf")
+    y, lse = attention.window_attention(q, k, v, window=9, return_lse=True)
+    assert (y[:, :20] == 0).all() and (lse[..., :20] == float("-inf")).all()
+    want = oa.attention(q[:, 20:], k[:, 20:], v[:, 20:], 9)           # the others see finite ones
+    assert rel(y[:, 20:], want[0]) <= TOL[dtype][0] and torch.isfinite(lse[..., 20:]).all()
+    pool = [x[0].transpose(0, 1).unsqueeze(0).contiguous() for x in (k[:, :32], v[:, :32])]
+    y = attention.paged_attention_step(q[:, 0], None, None, *pool, torch.zeros(1, 1, dtype=torch.int32, device=DEV), ints([20]))
+    assert (y == 0).all()
