@@ -56,8 +56,12 @@ def _rows16(t):
 
 
 def _strides(t):
-    """Batch, token and head stride; none for axes of one element."""
-    return [0 if n == 1 else s for s, n in zip(t.stride()[:3], t.shape)]
+    """Batch, token and head stride; none that an axis of one element has of its own."""
+    if t.is_contiguous():
+        _, T, H, D = t.shape
+        return T * H * D, H * D, D
+    st = t.stride()
+    return st[:3] if 1 not in t.shape else [0 if n == 1 else s for s, n in zip(st[:3], t.shape)]
 
 
 def _check(q, k, v, lengths):
