@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libgdnx.so")
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F64 = 2      # gdnx_check_finite only
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _c_int, _c_ll, _vp, _c_float = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_float
 
@@ -93,6 +93,14 @@ SIGNATURES = {
     "gdnx_pages_free": (_c_int, [_vp] * 4 + [_c_int] * 4 + [_vp]),
     "gdnx_pages_trim": (_c_int, [_vp] * 4 + [_c_int] * 7 + [_vp]),
     "gdnx_pages_compact": (_c_int, [_vp] * 7 + [_c_int] * 8 + [_vp]),
+    "gdnx_pages_packed_workspace_bytes": (_c_ll, [_c_int] * 2),
+    "gdnx_pages_reserve_packed": (_c_int, [_vp] * 11 + [_c_int] * 6 + [_vp]),
+    "gdnx_pages_write_packed": (_c_int, [_vp] * 5 + [_c_ll] * 6 + [_c_int] * 7 + [_vp]),
+    "gdnx_chunk_attn": (_c_int, [_vp] * 9 + [_c_ll] * 2 + [_c_int] * 11 + [_c_float, _c_int, _vp]),
+    "gdnx_conv_fwd": (_c_int, [_vp] * 7 + [_c_ll] * 2 + [_c_int] * 7 + [_vp]),
+    "gdnx_conv_bwd_workspace_bytes": (_c_ll, [_c_int] * 5),
+    "gdnx_conv_bwd": (_c_int, [_vp] * 12 + [_c_ll] * 2 + [_c_int] * 7 + [_vp]),
+    "gdnx_conv_packed": (_c_int, [_vp] * 8 + [_c_ll] + [_c_int] * 8 + [_vp]),
 }
 
 

@@ -3,10 +3,12 @@
 ``window_attention`` is differentiable attention over a sliding window of the
 last tokens and the first few ones (sinks), for training and prompts;
 ``paged_attention_step`` serves one token per sequence from a paged key-value
-cache (``gdnx_amd.pages``) under the same visibility rule.  Grouped heads:
+cache (``gdnx_amd.pages``) under the same visibility rule, and
+``paged_attention_chunk`` packed rows of several (prompts' pieces, drafts and
+single tokens in one call).  Grouped heads:
 query head h reads key head h // (Hq // Hkv).  The kernels are
-csrc/attn_win.hip and csrc/attn_paged.hip (gdnx_win_attn_*,
-gdnx_paged_attn_step in include/gdnx.h).
+csrc/attn_win.hip, csrc/attn_paged.hip and csrc/attn_chunk.hip (gdnx_win_attn_*,
+gdnx_paged_attn_step, gdnx_chunk_attn in include/gdnx.h).
 """
 from __future__ import annotations
 
@@ -205,5 +207,57 @@ def paged_attention_step(q, k, v, k_pages, v_pages, table, lengths, *, slots=Non
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
     _lib.call("gdnx_paged_attn_step", q.device, q.data_ptr(), _addr(k), _addr(v), k_pages.data_ptr(),
               v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), _addr(slots), out.data_ptr(), _addr(ws), NS,
+              rows, width, n_pages, page, Hq, Hkv, D, window, sinks, D ** -0.5 if scale is None else float(scale), code)
+    return out
+
+
+def paged_attention_chunk(q, k_pages, v_pages, table, lengths, offsets, *, slots=None, window=None, sinks=0, scale=None,
+                          out=None):
+    """Packed new tokens of every row over its cached ones: row i has queries
+    q[offsets[i]:offsets[i+1]] (q [N,Hq,D], any token and head strides; offsets
+    int32 [n+1] as ``pages.pages_reserve_packed`` gives them; a row may have
+    none) and is table row slots[i] (int32 [n]; outside the table: an empty
+    row, y = 0), or i.
+
+    Its c tokens stand at positions length - c .. length - 1, their keys and
+    values in their pages already (``pages.pages_write_packed``); k_pages,
+    v_pages, table and lengths as in ``paged_attention_step``, window, sinks and
+    scale as in ``window_attention``.  A token before position 0, and one of a
+    row whose length does not fit the table, gives 0; a key whose page is
+    missing is not seen.  Returns y [N,Hq,D] (or ``out``, which keeps
+    what it holds behind the last row's tokens; a new tensor's rows there are not
+    initialised), which is not differentiable."""
+    window, sinks = _window(window, sinks)
+    _no_tangents(q, k_pages, v_pages)
+    dev, dtype = q.device, q.dtype
+    _need(q.is_cuda and q.dim() == 3, "q must be a CUDA (HIP) tensor [N,Hq,D]")
+    N, Hq, D = q.shape
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == D,
+          "k_pages and v_pages must share shape [n_pages,Hkv,page,D]")
+    n_pages, Hkv, page, _ = k_pages.shape
+    _need(Hkv > 0 and Hq % Hkv == 0, "query heads must be a multiple of key heads")
+    _need(table.dim() == 2 and lengths.dim() == 1 and lengths.shape[0] == table.shape[0],
+          "table must be [rows,width], lengths [rows]")
+    rows, width = table.shape
+    _need(offsets.dim() == 1 and offsets.numel() >= 1, "offsets must be [n+1]")
+    n = offsets.numel() - 1
+    for t in (table, lengths, offsets) if slots is None else (table, lengths, offsets, slots):
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == dev,
+              "table, lengths, offsets and slots must be contiguous int32 on q's device")
+    _need(n <= rows if slots is None else tuple(slots.shape) == (n,), "slots must be [n], or no more rows than the table's")
+    _need(k_pages.dtype == v_pages.dtype == dtype and k_pages.device == v_pages.device == dev
+          and k_pages.is_contiguous() and v_pages.is_contiguous(),
+          "k_pages and v_pages must be contiguous, of q's dtype and device")
+    code = _lib.dtype_code(dtype)
+    if out is None:
+        out = torch.empty(N, Hq, D, dtype=dtype, device=dev)
+    else:
+        _need(tuple(out.shape) == (N, Hq, D) and out.dtype == dtype and out.is_contiguous() and out.device == dev,
+              "out must be contiguous [N,Hq,D] of q's dtype")
+    if N == 0 or n == 0:
+        return out
+    q = _rows16(q.unsqueeze(0))[0]
+    _lib.call("gdnx_chunk_attn", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+              lengths.data_ptr(), offsets.data_ptr(), _addr(slots), out.data_ptr(), None, *_strides(q.unsqueeze(0))[1:], N, n,
               rows, width, n_pages, page, Hq, Hkv, D, window, sinks, D ** -0.5 if scale is None else float(scale), code)
     return out

@@ -1444,3 +1444,173 @@ extern "C" int gdnx_pages_compact(void* k_pages, void* v_pages, const int* table
   a.table_out = table_out; a.refs_out = refs_out; a.rows = rows; a.width = width; a.page = page;
   return pages_compact_dispatch(a, (int*)workspace, (hipStream_t)stream);
 }
+
+// ---- packed rows: new tokens over the page cache ----
+
+namespace gdnx {
+
+static int check_packed(int n, int N) {
+  if (n < 1 || n > (1 << 24) || N < 0 || N >= kNoWindow) return set_error(GDNX_ERR_SHAPE, "bad sizes n=%d N=%d", n, N);
+  return GDNX_OK;
+}
+
+}  // namespace gdnx
+
+extern "C" long long gdnx_pages_packed_workspace_bytes(int n, int n_pages) {
+  if (n < 0 || n > (1 << 24) || n_pages < 1 || n_pages > (1 << 30)) return -1;
+  return 4 * (n + 1LL + n_pages);
+}
+
+extern "C" int gdnx_pages_reserve_packed(int* table, int* lengths, int* refs, const int* slots, const int* n_new,
+                                         int* offsets, int* start, int* positions, int* places, int* status,
+                                         void* workspace, int n, int N, int rows, int width, int n_pages, int page,
+                                         void* stream) {
+  g_err[0] = 0;
+  int rc = check_pool(rows, width, n_pages, page);
+  if (rc || (rc = check_packed(n, N))) return rc;
+  if (!prod_le((1LL << 31) - 1, {n, width}) || !prod_le((1LL << 31) - 1, {n_pages, page}))
+    return set_error(GDNX_ERR_SHAPE, "n * width and n_pages * page must stay below 2^31");
+  if (!table || !lengths || !refs || !slots || !n_new || !offsets || !start || !status || (N > 0 && (!positions || !places)))
+    return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  const PagesPackedArgs a{table, lengths, refs, slots, n_new, offsets, start, positions, places, status,
+                          n, N, rows, width, n_pages, page};
+  return pages_reserve_packed_dispatch(a, (int*)workspace, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_pages_write_packed(const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                                       const int* places, long long k_l, long long k_t, long long k_h, long long v_l,
+                                       long long v_t, long long v_h, int layers, int N, int n_pages, int page, int Hkv,
+                                       int head_dim, int dtype, void* stream) {
+  g_err[0] = 0;
+  PagesArgs pool{};
+  pool.n_pages = n_pages;
+  int rc = check_pool(1, 1, n_pages, page);
+  if (rc || (rc = check_pool_data(k_pages, v_pages, layers, Hkv, page, head_dim, dtype, pool))) return rc;
+  if (N < 1 || N >= kNoWindow) return set_error(GDNX_ERR_SHAPE, "bad number of tokens %d", N);
+  if (!k_new || !v_new || !places) return set_error(GDNX_ERR_ARG, "all pointers must be non-null");
+  if (!aligned16(k_new) || !aligned16(v_new)) return set_error(GDNX_ERR_ARG, "k_new and v_new must be 16-byte aligned");
+  PagesPutArgs a{k_new, v_new, {k_l, k_t, k_h}, {v_l, v_t, v_h}, k_pages, v_pages, places, pool.page_bytes,
+                 pool.row_bytes, layers, N, n_pages, page, Hkv};
+  const int size = dtype == GDNX_DTYPE_BF16 ? 2 : 4;
+  for (long long* st : {a.ks, a.vs})
+    for (int i = 0; i < 3; ++i) {
+      if (st[i] < 0 || st[i] > (1LL << 40) || st[i] * size % 16 != 0)
+        return set_error(GDNX_ERR_SHAPE, "strides must be non-negative multiples of 16 bytes");
+      st[i] *= size;
+    }
+  if (!prod_le(kMaxGroups, {2, layers, pages_put_groups(a)}))
+    return set_error(GDNX_ERR_SHAPE, "too many tokens in one call");
+  return pages_put_dispatch(a, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_chunk_attn(const void* q, const void* k_pages, const void* v_pages, const int* table,
+                               const int* lengths, const int* offsets, const int* slots, void* y, void* workspace,
+                               long long q_t, long long q_h, int N, int n, int rows, int width, int n_pages, int page,
+                               int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
+                               void* stream) {
+  g_err[0] = 0;
+  int rc = check_attn_sizes(Hq, Hkv, head_dim, window, sinks, dtype);
+  if (rc || (rc = check_pool(rows, width, n_pages, page)) || (rc = check_packed(n, N))) return rc;
+  if (!slots && n > rows) return set_error(GDNX_ERR_SHAPE, "bad number of rows %d (table rows %d)", n, rows);
+  if (!prod_le(kNoWindow, {N, Hq}) || !prod_le(kMaxGroups * 4, {N, Hq}))
+    return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
+  if (!q || !k_pages || !v_pages || !table || !lengths || !offsets || !y)
+    return set_error(GDNX_ERR_ARG, "all pointers but slots and workspace must be non-null");
+  for (const void* p : {q, k_pages, v_pages, (const void*)y, (const void*)workspace})
+    if (!aligned16(p)) return set_error(GDNX_ERR_ARG, "tensors and workspace must be 16-byte aligned");
+  const int unit = dtype == GDNX_DTYPE_BF16 ? 8 : 4;
+  if (q_t < 0 || q_h < 0 || q_t % unit || q_h % unit || q_t > (1LL << 40) || q_h > (1LL << 40))
+    return set_error(GDNX_ERR_SHAPE, "q: strides must be non-negative multiples of 16 bytes");
+  int lg = 0;
+  while ((1 << lg) < page) ++lg;
+  if (N == 0) return GDNX_OK;
+  ChunkAttnArgs a{q, k_pages, v_pages, table, lengths, offsets, slots, y, (float*)workspace, {q_t, q_h}, N, n, rows, width,
+                  n_pages, lg, Hq, Hkv, head_dim, window_arg(window), sinks_arg(sinks), scale, dtype};
+  return chunk_attn_dispatch(a, (hipStream_t)stream);
+}
+
+// ---- short causal convolution ----
+
+namespace gdnx {
+
+static int check_conv(int B, int T, int C, int W, int wdtype, int dtype) {
+  for (int d : {wdtype, dtype})
+    if (d != GDNX_DTYPE_F32 && d != GDNX_DTYPE_BF16)
+      return set_error(GDNX_ERR_ARG, "dtype %d is not GDNX_DTYPE_F32/BF16", d);
+  if (W < 2 || W > 8) return set_error(GDNX_ERR_SHAPE, "%d taps unsupported (2 to 8)", W);
+  if (B < 1 || T < 1 || C < 1 || T >= kNoWindow || C > (1 << 24))
+    return set_error(GDNX_ERR_SHAPE, "bad sizes B=%d T=%d C=%d", B, T, C);
+  if (!prod_le(1LL << 40, {B, T, C}) || conv_groups(B, T, C, W, dtype) > kMaxGroups)
+    return set_error(GDNX_ERR_SHAPE, "too many rows, tokens and channels in one call");
+  return GDNX_OK;
+}
+
+static int check_conv_x(const void* x, const void* weight, long long x_b, long long x_t) {
+  if (!x || !weight) return set_error(GDNX_ERR_ARG, "x and weight must be non-null");
+  if (x_b < 0 || x_t < 0 || x_b > (1LL << 40) || x_t > (1LL << 40))
+    return set_error(GDNX_ERR_SHAPE, "x: strides must not be negative");
+  return GDNX_OK;
+}
+
+}  // namespace gdnx
+
+extern "C" int gdnx_conv_fwd(const void* x, const void* weight, const void* bias, const void* state, const int* lengths,
+                             void* y, void* state_out, long long x_b, long long x_t, int B, int T, int C, int W, int silu,
+                             int wdtype, int dtype, void* stream) {
+  g_err[0] = 0;
+  int rc = check_conv(B, T, C, W, wdtype, dtype);
+  if (rc || (rc = check_conv_x(x, weight, x_b, x_t))) return rc;
+  if (!y) return set_error(GDNX_ERR_ARG, "y must be non-null");
+  ConvArgs a{};
+  a.x = x; a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.y = y; a.state_out = state_out;
+  a.xs[0] = x_b; a.xs[1] = x_t; a.B = B; a.T = T; a.C = C; a.W = W; a.silu = silu != 0; a.wdtype = wdtype; a.dtype = dtype;
+  if ((rc = conv_dispatch(a, false, (hipStream_t)stream))) return rc;
+  const FiniteBuf outs[] = {{y, (size_t)B * T * C, dtype}};
+  return finite_outputs(outs, 1, (hipStream_t)stream);
+}
+
+extern "C" long long gdnx_conv_bwd_workspace_bytes(int B, int T, int C, int W, int dtype) {
+  if (check_conv(B, T, C, W, dtype, dtype)) return -1;
+  return conv_bwd_blocks(B, T, C, W, dtype) * (W + 1) * C * 4;
+}
+
+extern "C" int gdnx_conv_bwd(const void* x, const void* weight, const void* bias, const void* state, const int* lengths,
+                             const void* dy, const void* dstate_out, void* dx, void* dweight, void* dbias, void* dstate,
+                             void* workspace, long long x_b, long long x_t, int B, int T, int C, int W, int silu,
+                             int wdtype, int dtype, void* stream) {
+  g_err[0] = 0;
+  int rc = check_conv(B, T, C, W, wdtype, dtype);
+  if (rc || (rc = check_conv_x(x, weight, x_b, x_t))) return rc;
+  if (!dy || !dx || !dweight) return set_error(GDNX_ERR_ARG, "dy, dx and dweight must be non-null");
+  if (!workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  if ((uintptr_t)workspace & 3u) return set_error(GDNX_ERR_ARG, "workspace must be 4-byte aligned");
+  ConvArgs a{};
+  a.x = x; a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.dy = dy; a.dstate_out = dstate_out;
+  a.dx = dx; a.dweight = dweight; a.dbias = dbias; a.dstate = dstate; a.part = (float*)workspace;
+  a.xs[0] = x_b; a.xs[1] = x_t; a.B = B; a.T = T; a.C = C; a.W = W; a.silu = silu != 0; a.wdtype = wdtype; a.dtype = dtype;
+  if ((rc = conv_dispatch(a, true, (hipStream_t)stream))) return rc;
+  const FiniteBuf outs[] = {{dx, (size_t)B * T * C, dtype}, {dweight, (size_t)C * W, wdtype},
+                            {dbias, dbias ? (size_t)C : 0, wdtype}, {dstate, dstate ? (size_t)B * (W - 1) * C : 0, dtype}};
+  return finite_outputs(outs, 4, (hipStream_t)stream);
+}
+
+extern "C" int gdnx_conv_packed(const void* x, const int* offsets, const void* weight, const void* bias, void* pool,
+                                const int* slots, const int* to_slots, void* y, long long x_t, int N, int n, int n_slots,
+                                int C, int W, int silu, int wdtype, int dtype, void* stream) {
+  g_err[0] = 0;
+  int rc = check_conv(1, 1, C, W, wdtype, dtype);
+  if (rc || (rc = check_packed(n, N)) || (rc = check_conv_x(pool, weight, 0, x_t))) return rc;
+  if (n_slots < 1 || !prod_le(1LL << 50, {n_slots, W, C}) || !prod_le(1LL << 50, {N, C}))
+    return set_error(GDNX_ERR_SHAPE, "bad number of slots %d", n_slots);
+  if (!slots && n > n_slots) return set_error(GDNX_ERR_SHAPE, "%d rows for %d slots", n, n_slots);
+  if (!offsets && n != N) return set_error(GDNX_ERR_SHAPE, "without offsets every row has one token: n=%d N=%d", n, N);
+  if (N > 0 && (!x || !y)) return set_error(GDNX_ERR_ARG, "x and y must be non-null");
+  ConvPackedArgs p{};
+  ConvArgs& a = p.a;
+  a.x = x; a.weight = weight; a.bias = bias; a.state = pool; a.state_out = pool; a.y = y; a.xs[1] = x_t;
+  a.C = C; a.W = W; a.silu = silu != 0; a.wdtype = wdtype; a.dtype = dtype;
+  p.offsets = offsets; p.slots = slots; p.to_slots = to_slots; p.N = N; p.n = n; p.n_slots = n_slots;
+  if (conv_packed_groups(p) > kMaxGroups) return set_error(GDNX_ERR_SHAPE, "too many rows, tokens and channels in one call");
+  return conv_packed_dispatch(p, (hipStream_t)stream);
+}

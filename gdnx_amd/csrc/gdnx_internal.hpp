@@ -519,6 +519,24 @@ struct PagedAttnArgs {
 int paged_attn_spans(int NS, int Hq, int Hkv, long long keys, int dtype);
 int paged_attn_dispatch(const PagedAttnArgs& a, hipStream_t stream);
 
+// Packed new tokens over a paged key-value cache.
+struct ChunkAttnArgs {
+  const void* q;        // [N,Hq,D], strides qs (token, head)
+  const void* k_pages;  // [n_pages,Hkv,page,D]
+  const void* v_pages;
+  const int* table;     // [rows,width]
+  const int* lengths;   // [rows], the new tokens included
+  const int* offsets;   // [n + 1]
+  const int* slots;     // [n] table row of each row, or null
+  void* y;              // [N,Hq,D]
+  float* part;
+  long long qs[2];
+  int N, n, rows, width, n_pages, page_log, Hq, Hkv, D, window, sinks;
+  float scale;
+  int dtype;
+};
+int chunk_attn_dispatch(const ChunkAttnArgs& a, hipStream_t stream);
+
 // The page pool's operations.
 struct PagesArgs {
   void* k_pages;        // [layers,n_pages,Hkv,page,D]
@@ -536,6 +554,33 @@ struct PagesArgs {
   long long page_bytes;
   int row_bytes, layers, n, n_new, rows, width, n_pages, page, Hkv, window, sinks, trim;
 };
+// Rows of unlike numbers of new tokens, and the places of packed tokens.
+struct PagesPackedArgs {
+  int* table;
+  int* lengths;
+  int* refs;
+  const int* slots;     // [n]
+  const int* n_new;     // [n]
+  int* offsets;         // [n + 1]
+  int* start;           // [n]
+  int* positions;       // [N]
+  int* places;          // [N]
+  int* status;          // [2]
+  int n, N, rows, width, n_pages, page;
+};
+struct PagesPutArgs {
+  const void* k_new;    // [layers,N,Hkv,D], strides in bytes
+  const void* v_new;
+  long long ks[3], vs[3];
+  void* k_pages;
+  void* v_pages;
+  const int* places;    // [N]
+  long long page_bytes;
+  int row_bytes, layers, N, n_pages, page, Hkv;
+};
+int pages_reserve_packed_dispatch(const PagesPackedArgs& a, int* ws, hipStream_t stream);
+long long pages_put_groups(const PagesPutArgs& a);
+int pages_put_dispatch(const PagesPutArgs& a, hipStream_t stream);
 int pages_reserve_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
 int pages_fork_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
 int pages_copy_dispatch(const PagesArgs& a, const int* src, const int* dst, hipStream_t stream);
@@ -543,5 +588,39 @@ int pages_compact_dispatch(const PagesArgs& a, int* ws, hipStream_t stream);
 int pages_free_dispatch(const PagesArgs& a, hipStream_t stream);
 long long pages_write_groups(const PagesArgs& a);
 int pages_write_dispatch(const PagesArgs& a, hipStream_t stream);
+
+// Short causal convolution; x strides (batch, token) in elements, the rest contiguous.
+struct ConvArgs {
+  const void* x;         // [B,T,C]
+  const void* weight;    // [C,W] wdtype
+  const void* bias;      // [C] wdtype, or null
+  const void* state;     // [B,W-1,C], or null (zeros)
+  const int* lengths;    // [B], or null
+  void* y;
+  void* state_out;       // [B,W-1,C], or null
+  const void* dy;
+  const void* dstate_out;
+  void* dx;
+  void* dweight;         // wdtype, or null
+  void* dbias;
+  void* dstate;
+  float* part;           // [blocks][W + 1][C]
+  long long xs[2];
+  int B, T, C, W, silu, wdtype, dtype;
+  int lx_log, groups, span, blocks;     // conv_shape
+};
+// Packed rows: a.x [N,C] with token stride a.xs[1], a.state and a.state_out the pool.
+struct ConvPackedArgs {
+  ConvArgs a;
+  const int* offsets;    // [n + 1], or null (one token a row)
+  const int* slots;      // [n], or null
+  const int* to_slots;
+  int N, n, n_slots;
+};
+long long conv_bwd_blocks(int B, int T, int C, int W, int dtype);
+long long conv_groups(int B, int T, int C, int W, int dtype);
+int conv_dispatch(ConvArgs& a, bool bwd, hipStream_t stream);
+long long conv_packed_groups(const ConvPackedArgs& p);
+int conv_packed_dispatch(ConvPackedArgs& p, hipStream_t stream);
 
 }  // namespace gdnx

@@ -25,6 +25,7 @@
 // into 64 rows of 8 layers 17 us for 134 MB; writing 8 prompts of up to 1001
 // tokens into 4 layers 15 us for 66 MB; freeing 3 us.
 #include "attn_common.hpp"
+#include "packed_rows.hpp"
 
 namespace gdnx {
 
@@ -33,19 +34,19 @@ namespace {
 constexpr int PT = 1024;             // threads of the bookkeeping workgroup
 constexpr int PW = PT / 64;
 
-// Exclusive prefix sum over the workgroup; *total gets the sum.  sh: PW ints.
-__device__ __forceinline__ int wg_scan(int x, int* sh, int* total) {
+// Exclusive prefix sum over the workgroup; *total gets the sum.  sh: PW of them.
+template <typename T> __device__ __forceinline__ T wg_scan(T x, T* sh, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = x;
+  T s = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(s, off, 64);
+    const T y = __shfl_up(s, off, 64);
     if (lane >= off) s += y;
   }
   __syncthreads();                   // (sh may still be read from the call before)
   if (lane == 63) sh[wave] = s;
   __syncthreads();
-  int base = 0, all = 0;
+  T base = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < PW; ++w) {
     if (w < wave) base += sh[w];
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(PT) pages_fork_kernel(PagesArgs a, int* ws) {
     if (s < a.n && a.slots[s] != a.start[s] && row_length(a, a.start[s]) == 0) len = row_length(a, a.slots[s]);
     const bool started = len > 0 && len % a.page != 0;
     int total;
-    const int at = wg_scan(started, sh, &total);
+    const int at = wg_scan((int)started, sh, &total);
     if (s < a.n) {
       lens[s] = len;
       dst[s] = -1;
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(PT) pages_plan_kernel(PagesArgs a, int* ws) {
     const bool hole = p < used && r == 0, mover = p >= used && r != 0;
     // (a step holds both only where `used` falls into it)
     int th, tm;
-    const int ah = wg_scan(hole, sh, &th), am = wg_scan(mover, sh, &tm);
+    const int ah = wg_scan((int)hole, sh, &th), am = wg_scan((int)mover, sh, &tm);
     if (hole) dst[holes + ah] = p;
     if (mover) src[movers + am] = p;
     holes += th;
@@ -344,6 +345,164 @@ __global__ void __launch_bounds__(256) pages_write_kernel(PagesArgs a, unsigned 
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (to[e] >= 0) *(u32x4*)(pool + to[e]) = x[e];
+}
+
+// ---- packed rows of unlike lengths ----
+// The rows' tokens packed one after the other, and their pages: first a
+// workgroup's prefix sums over the rows (as in a reserve), then a thread for
+// every page that was taken and one for every packed token.
+// ws: [n + 1] first page of each row in the list (its end: how many there are), then [n_pages] free pages
+__global__ void __launch_bounds__(PT) pages_reserve_packed_kernel(PagesPackedArgs a, int* ws) {
+  __shared__ int sh[PW], s_bad;
+  __shared__ long long sl[PW];
+  int* offs = ws;
+  int* list = ws + a.n + 1;
+  if (threadIdx.x == 0) s_bad = 0;
+  PagesArgs pool{};
+  pool.lengths = a.lengths; pool.rows = a.rows; pool.width = a.width; pool.page = a.page;
+  long long tokens = 0;
+  int need = 0;
+  for (int s0 = 0; s0 < a.n; s0 += PT) {
+    const int s = s0 + threadIdx.x;
+    const int add = s < a.n ? max(a.n_new[s], 0) : 0, len = s < a.n ? row_length(pool, a.slots[s]) : -1;
+    long long sum;
+    const long long off = tokens + wg_scan((long long)add, sl, &sum);
+    tokens += sum;
+    bool bad = s < a.n && off + add > a.N;   // its last token lies behind the batch
+    int c = 0;
+    if (len >= 0) {
+      const long long want = ((long long)len + add + a.page - 1) / a.page;
+      if (want > a.width) bad = true;
+      else c = (int)want - (len + a.page - 1) / a.page;
+    }
+    int total;
+    const int at = wg_scan(c, sh, &total);
+    if (s < a.n) {
+      offs[s] = need + at;
+      a.offsets[s] = (int)min(off, (long long)a.N);
+      a.start[s] = len;
+    }
+    if (bad) atomicAdd(&s_bad, 1);
+    need += total;                           // (at most width times rows, which the host keeps under 2^31)
+  }
+  const int got = find_free(a.refs, a.n_pages, need, list, sh);
+  __syncthreads();
+  const bool fail = got < need || s_bad > 0;
+  if (threadIdx.x == 0) {
+    offs[a.n] = fail ? 0 : need;
+    a.offsets[a.n] = fail ? 0 : (int)tokens;
+    if (fail) {
+      a.status[0] = need - got;
+      a.status[1] = s_bad;
+    }
+  }
+  for (int s = threadIdx.x; s < a.n; s += PT) {
+    if (fail) {
+      a.offsets[s] = 0;
+      a.start[s] = -1;
+    } else if (a.start[s] >= 0) {
+      a.lengths[a.slots[s]] = a.start[s] + max(a.n_new[s], 0);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) pages_place_kernel(PagesPackedArgs a, const int* ws) {
+  const int *offs = ws, *list = ws + a.n + 1;
+  const int lane = threadIdx.x & 63;
+  const int base = __builtin_amdgcn_readfirstlane(blockIdx.x * 256 + (threadIdx.x & ~63)), u = base + lane;
+  // the last row that starts at or before x, from row i0 on
+  const auto find = [&](const int* starts, int x, int i0) {
+    int lo = i0, hi = a.n - 1;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      if (starts[mid] <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  };
+  const int taken = offs[a.n], tokens = a.offsets[a.n];
+  if (base < taken) {
+    const int i0 = wave_find(a.n, base, lane, [&](int i) { return (long long)offs[i]; });
+    if (u < taken) {
+      const int s = find(offs, u, max(i0, 0)), r = a.slots[s], pg = list[u];
+      a.table[(size_t)r * a.width + (a.start[s] + a.page - 1) / a.page + u - offs[s]] = pg;
+      a.refs[pg] = 1;
+    }
+  }
+  if (base >= a.N) return;
+  int pos = -1, place = -1;
+  if (base < tokens) {
+    const int i0 = wave_find(a.n, base, lane, [&](int i) { return (long long)a.offsets[i]; });
+    if (u < tokens) {
+      const int s = find(a.offsets, u, max(i0, 0)), st = a.start[s];
+      if (st >= 0) {
+        pos = st + u - a.offsets[s];
+        const int col = pos / a.page, had = (st + a.page - 1) / a.page;
+        const int pg = col < had ? a.table[(size_t)a.slots[s] * a.width + col] : list[offs[s] + col - had];
+        if (pg >= 0 && pg < a.n_pages) place = pg * a.page + pos - col * a.page;
+      }
+    }
+  }
+  if (u < a.N) {
+    a.positions[u] = pos;
+    a.places[u] = place;
+  }
+}
+
+// Packed keys and values to their places.  As pages_write_kernel: 1024 of a
+// layer's 16-byte units a workgroup, four a thread, all loaded before the first
+// is stored.
+__global__ void __launch_bounds__(256) pages_put_kernel(PagesPutArgs a, unsigned per_layer) {
+  const unsigned upr = a.row_bytes / 16, upt = a.Hkv * upr;    // units of a head's row, of a token
+  const unsigned lk = blockIdx.x / per_layer, blk = blockIdx.x % per_layer;
+  const int layer = lk >> 1;
+  const long long first = (long long)blk * 1024;
+  const int tok0 = (int)(first / upt);
+  const unsigned rem = (unsigned)(first - (long long)tok0 * upt);
+  const bool val = lk & 1;
+  const long long st = val ? a.vs[1] : a.ks[1], sh = val ? a.vs[2] : a.ks[2];
+  const char* from = (const char*)(val ? a.v_new : a.k_new) + layer * (val ? a.vs[0] : a.ks[0]);
+  char* pool = (char*)(val ? a.v_pages : a.k_pages) + (long long)layer * a.n_pages * a.page_bytes;
+  u32x4 x[4];
+  long long to[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned r = rem + e * 256 + threadIdx.x, dt = r / upt, u = r - dt * upt, h = u / upr;
+    const long long t = (long long)tok0 + dt;
+    to[e] = -1;
+    if (t >= a.N) continue;
+    const int place = a.places[t];
+    if (place < 0) continue;
+    const int pg = place / a.page, in = place - pg * a.page;
+    if (pg >= a.n_pages) continue;
+    x[e] = *(const u32x4*)(from + t * st + h * sh + (u - h * upr) * 16);
+    to[e] = pg * a.page_bytes + ((long long)h * a.page + in) * a.row_bytes + (u - h * upr) * 16;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (to[e] >= 0) *(u32x4*)(pool + to[e]) = x[e];
+}
+
+int pages_reserve_packed_dispatch(const PagesPackedArgs& a, int* ws, hipStream_t stream) {
+  hipLaunchKernelGGL(pages_reserve_packed_kernel, dim3(1), dim3(PT), 0, stream, a, ws);
+  const int rc = check_launch("pages_reserve_packed_kernel");
+  if (rc) return rc;
+  // pages that can be taken: a started page for every row besides those that the tokens fill
+  const long long full = (long long)a.N / a.page + a.n, most = full < a.n_pages ? full : a.n_pages;
+  const long long threads = most > a.N ? most : a.N;
+  if (threads == 0) return GDNX_OK;
+  hipLaunchKernelGGL(pages_place_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, (const int*)ws);
+  return check_launch("pages_place_kernel");
+}
+
+long long pages_put_groups(const PagesPutArgs& a) {
+  return ((long long)a.N * a.Hkv * (a.row_bytes / 16) + 1023) / 1024;
+}
+
+int pages_put_dispatch(const PagesPutArgs& a, hipStream_t stream) {
+  const unsigned per_layer = (unsigned)pages_put_groups(a);
+  hipLaunchKernelGGL(pages_put_kernel, dim3(per_layer * 2 * a.layers), dim3(256), 0, stream, a, per_layer);
+  return check_launch("pages_put_kernel");
 }
 
 int pages_reserve_dispatch(const PagesArgs& a, int* ws, hipStream_t stream) {

@@ -12,6 +12,8 @@ the rows' lengths on the host, and raises before a call that cannot be served.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib, attention
@@ -84,6 +86,62 @@ def pages_write(k, v, k_pages, v_pages, table, slots, start):
     _lib.call("gdnx_pages_write", table.device, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
               table.data_ptr(), slots.data_ptr(), start.data_ptr(), layers, slots.numel(), k.shape[-3],
               table.shape[0], table.shape[1], n_pages, page, Hkv, D, code)
+
+
+class PackedTokens(NamedTuple):
+    """A batch of packed rows, as ``pages_reserve_packed`` lays it out (all int32, on the device)."""
+    offsets: torch.Tensor     # [n+1] row i has tokens offsets[i] .. offsets[i+1] - 1
+    start: torch.Tensor       # [n] the rows' lengths before (-1: an empty row)
+    positions: torch.Tensor   # [tokens] a token's position in its row (-1: it has none)
+    places: torch.Tensor      # [tokens] its place in the pool, page * page size + place in the page (-1: none)
+
+
+def pages_reserve_packed(table, lengths, refs, slots, n_new, page: int, status, tokens: int) -> PackedTokens:
+    """Pages for the next n_new[i] tokens (int32 [n], on the device; below 0:
+    none) of every row slots[i] (outside the table: an empty row), whose
+    lengths grow by as much, and the packed batch that these tokens make.
+    tokens: the batch's size, which may be more than the rows' tokens (those
+    behind the last row's are nobody's).  If the pool or a table row is too
+    small for any of them, or the batch is, nothing changes, all offsets are 0,
+    start, positions and places -1, and status (int32 [2]) holds the pages
+    missing and the rows that do not fit."""
+    rows, width, n_pages = _state(table, lengths, refs)
+    _ints(table, slots, n_new, status)
+    _need(slots.dim() == 1 and n_new.shape == slots.shape and tuple(status.shape) == (2,),
+          "slots and n_new must be [n], status [2]")
+    n, tokens, dev = slots.numel(), int(tokens), table.device
+    _need(tokens >= 0, "tokens must not be negative")
+    buf = torch.empty(2 * n + 1 + 2 * tokens, dtype=torch.int32, device=dev)
+    plan = PackedTokens(buf[:n + 1], buf[n + 1:2 * n + 1], buf[2 * n + 1:2 * n + 1 + tokens], buf[2 * n + 1 + tokens:])
+    if n == 0:
+        plan.offsets.zero_()
+        buf[1:].fill_(-1)
+        return plan
+    ws = torch.empty(attention._bytes("gdnx_pages_packed_workspace_bytes", n, n_pages), dtype=torch.uint8, device=dev)
+    _lib.call("gdnx_pages_reserve_packed", dev, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), slots.data_ptr(),
+              n_new.data_ptr(), *(t.data_ptr() for t in plan), status.data_ptr(), ws.data_ptr(), n, tokens, rows, width,
+              n_pages, int(page))
+    return plan
+
+
+def pages_write_packed(k, v, k_pages, v_pages, places):
+    """Keys and values k, v [(layers,)N,Hkv,D] (any strides: views of a fused
+    projection are read as they are) of packed tokens to their places in the
+    pool (int32 [N]; outside it: not written).  No place may be named twice."""
+    layers, n_pages, Hkv, page, D, code = _pools(k_pages, v_pages, places)
+    _ints(places)
+    lead = (layers,) if k_pages.dim() == 5 else ()
+    N = places.numel()
+    _need(places.dim() == 1 and tuple(k.shape) == tuple(v.shape) == (*lead, N, Hkv, D),
+          "k and v must be [(layers,)N,Hkv,D], places [N]")
+    _need(k.dtype == v.dtype == k_pages.dtype and k.device == v.device == k_pages.device,
+          "k, v and the pages must share dtype and device")
+    if k.numel() == 0:
+        return
+    k, v = (attention._rows16(t if lead else t.unsqueeze(0)) for t in (k, v))
+    _lib.call("gdnx_pages_write_packed", places.device, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(),
+              v_pages.data_ptr(), places.data_ptr(), *attention._strides(k), *attention._strides(v), layers, N, n_pages,
+              page, Hkv, D, code)
 
 
 def pages_copy(k_pages, v_pages, src, dst):
@@ -271,6 +329,35 @@ class PagedKVCache:
         return attention.paged_attention_step(q, k, v, self.k_pages[layer], self.v_pages[layer], self.table,
                                               self.lengths, slots=self.rows_tensor(rows), window=window, sinks=sinks,
                                               scale=scale, out=out)
+
+    def reserve_packed(self, rows, n_new, tokens=None) -> PackedTokens:
+        """Room for the next n_new[i] tokens (ints) of every row, and the packed
+        batch that they make, of ``tokens`` tokens (None: as many as the rows')."""
+        n_new, (rows, named) = [int(c) for c in n_new], self._named(rows)
+        tokens = sum(n_new) if tokens is None else int(tokens)
+        _need(len(n_new) == len(rows) and min(n_new, default=0) >= 0, "n_new must name a number of tokens for every row")
+        _need(tokens >= sum(n_new), f"{sum(n_new)} tokens in a batch of {tokens}")
+        for r, c in zip(rows, n_new):
+            if self.lens[r] + c > self.width * self.page:
+                raise ValueError(f"row {r}: {self.lens[r]} + {c} tokens, the table holds {self.width * self.page}")
+        up = self._upload(n_new)
+        self._take(sum(-(-(self.lens[r] + c) // self.page) - -(-self.lens[r] // self.page) for r, c in zip(rows, n_new)))
+        plan = pages_reserve_packed(self.table, self.lengths, self.refs, named, up, self.page, self.status, tokens)
+        for r, c in zip(rows, n_new):
+            self.lens[r] += c
+        return plan
+
+    def write_packed(self, plan, k, v, layer=None) -> None:
+        """Keys and values [(layers,)N,Hkv,D] (of one layer: [N,Hkv,D]) of a packed batch to their places."""
+        kp, vp = (self.k_pages, self.v_pages) if layer is None else (self.k_pages[layer], self.v_pages[layer])
+        pages_write_packed(k, v, kp, vp, plan.places)
+
+    def chunk(self, layer: int, rows, plan, q, *, window=None, sinks=0, scale=None, out=None):
+        """One layer's attention of a packed batch's tokens (reserved and written
+        before): ``attention.paged_attention_chunk`` on the cache's tensors."""
+        return attention.paged_attention_chunk(q, self.k_pages[layer], self.v_pages[layer], self.table, self.lengths,
+                                               plan.offsets, slots=self.rows_tensor(rows), window=window, sinks=sinks,
+                                               scale=scale, out=out)
 
     def fork(self, parents) -> list:
         """A new row for every entry of parents (a row may be named more than once), holding what it holds."""

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define GDNX_ABI_VERSION 13
+#define GDNX_ABI_VERSION 14
 
 enum { GDNX_DTYPE_F32 = 0, GDNX_DTYPE_BF16 = 1, GDNX_DTYPE_F64 = 2 /* gdnx_check_finite only */ };
 
@@ -717,6 +717,84 @@ int gdnx_pages_trim(int* table, int* lengths, int* refs, const int* slots, int w
 int gdnx_pages_compact(void* k_pages, void* v_pages, const int* table, const int* refs, int* table_out,
                        int* refs_out, void* workspace, int layers, int rows, int width, int n_pages, int page,
                        int Hkv, int head_dim, int dtype, void* stream);
+
+/* ---- packed rows: new tokens of unlike numbers, without padding ----
+ *
+ * Row i of n has tokens offsets[i] .. offsets[i + 1] - 1 of a batch of N
+ * (offsets int32 [n + 1], not falling; whatever they hold, nothing outside the
+ * batch is touched).  A row may have none; tokens behind the last row's are
+ * nobody's: what the outputs hold there stays as it was.
+ *
+ * Pages for n_new[i] more tokens (below 0: none) of every row slots[i], as
+ * gdnx_pages_reserve does it, and the packed batch that they make:
+ *   offsets [n + 1];  start [n] the old lengths (-1: an empty row, whose tokens
+ *   have no place);  positions [N] a token's position in its row, places [N] its
+ *   place in the pool, page * page_size + place in the page (-1 both: a token
+ *   of an empty row or of nobody; a place also where the row lacks the page).
+ * If the pool lacks pages, a table row is too short or a row's tokens end
+ * behind the batch, nothing changes: offsets are 0, start, positions and
+ * places -1, and status holds the pages that were missing and the number of
+ * such rows.  n_pages * page must stay below 2^31.  workspace:
+ * gdnx_pages_packed_workspace_bytes(n, n_pages). */
+long long gdnx_pages_packed_workspace_bytes(int n, int n_pages);
+int gdnx_pages_reserve_packed(int* table, int* lengths, int* refs, const int* slots, const int* n_new, int* offsets,
+                              int* start, int* positions, int* places, int* status, void* workspace, int n, int N,
+                              int rows, int width, int n_pages, int page, void* stream);
+
+/* Keys and values k_new, v_new [layers,N,Hkv,D] (element strides of layer,
+ * token and head, multiples of 16 bytes; D contiguous) to places [N] of the
+ * pool (outside it: not written).  No place may be named twice. */
+int gdnx_pages_write_packed(const void* k_new, const void* v_new, void* k_pages, void* v_pages, const int* places,
+                            long long k_l, long long k_t, long long k_h, long long v_l, long long v_t, long long v_h,
+                            int layers, int N, int n_pages, int page, int Hkv, int head_dim, int dtype, void* stream);
+
+/* Attention of packed new tokens over a paged cache that holds their keys and
+ * values already.  Row i is table row r = slots[i] (slots null: i; outside
+ * [0, rows): an empty row); its c tokens stand at positions lengths[r] - c ..
+ * lengths[r] - 1, and the one at p sees key j of the row if j <= p and
+ * p - j < window (0: any) or j < sinks, and its page is in the pool.  A token
+ * that sees nothing (of an empty row, or before position 0) gives y = 0; so do
+ * all tokens of a row whose length does not fit the table.
+ * A key or value that is not finite reaches only the tokens that see it.
+ * q [N,Hq,D] with element strides (token, head) that are multiples of 16
+ * bytes, y [N,Hq,D] contiguous; pages, table and lengths as
+ * gdnx_paged_attn_step. */
+int gdnx_chunk_attn(const void* q, const void* k_pages, const void* v_pages, const int* table, const int* lengths,
+                    const int* offsets, const int* slots, void* y, void* workspace, long long q_t, long long q_h, int N,
+                    int n, int rows, int width, int n_pages, int page, int Hq, int Hkv, int head_dim, int window,
+                    int sinks, float scale, int dtype, void* stream);
+
+/* ---- short causal convolution along the tokens, W = 2 to 8 taps a channel ----
+ *
+ *   u_t = bias + sum_j weight[:, j] x_{t-W+1+j},   y_t = silu ? u_t sigmoid(u_t) : u_t
+ * x [B,T,C] in the io dtype with any element strides (batch, token), C
+ * contiguous; weight [C,W] and bias [C] (or null) in wdtype; state [B,W-1,C]
+ * (or null: zeros) the W - 1 inputs before token 0; y [B,T,C].  Tokens at or
+ * beyond lengths[b] (null: T; clamped to [0, T]) are padding, whatever they
+ * hold: their y is 0.  state_out [B,W-1,C] (or null): the W - 1 inputs before
+ * the row's end.  No pointer needs more than its element's alignment.  The
+ * backward gives dx [B,T,C] (0 in padding), dweight and dbias (or null) in
+ * wdtype, summed in float32 in a fixed order, and dstate (or null), from dy and
+ * dstate_out, the gradient of state_out (or null).  workspace:
+ * gdnx_conv_bwd_workspace_bytes (-1 if the sizes are invalid). */
+int gdnx_conv_fwd(const void* x, const void* weight, const void* bias, const void* state, const int* lengths, void* y,
+                  void* state_out, long long x_b, long long x_t, int B, int T, int C, int W, int silu, int wdtype,
+                  int dtype, void* stream);
+long long gdnx_conv_bwd_workspace_bytes(int B, int T, int C, int W, int dtype);
+int gdnx_conv_bwd(const void* x, const void* weight, const void* bias, const void* state, const int* lengths,
+                  const void* dy, const void* dstate_out, void* dx, void* dweight, void* dbias, void* dstate,
+                  void* workspace, long long x_b, long long x_t, int B, int T, int C, int W, int silu, int wdtype,
+                  int dtype, void* stream);
+
+/* The same over packed rows (offsets null: one token a row, n == N), each
+ * continuing the state in slot slots[i] of pool [n_slots,W-1,C] (slots null: i;
+ * outside the pool: an empty row, y = 0), its new state going to slot
+ * to_slots[i] (null: the same; outside the pool: nowhere).  x [N,C] with a token
+ * stride.  No slot that a row writes may be read or written by another row of
+ * the call. */
+int gdnx_conv_packed(const void* x, const int* offsets, const void* weight, const void* bias, void* pool,
+                     const int* slots, const int* to_slots, void* y, long long x_t, int N, int n, int n_slots, int C,
+                     int W, int silu, int wdtype, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -50,6 +50,36 @@ def attention(q, k, v, window=None, sinks=0, scale=None, lengths=None, dy=None):
     return (y, lse) if dy is None else (y, lse, dq, dk, dv)
 
 
+def paged_chunk(q, k_pages, v_pages, table, lengths, offsets, slots=None, window=None, sinks=0, scale=None):
+    """y [N,Hq,D] in float64 of packed new tokens over a paged cache; table, lengths, offsets and slots are
+    lists.  Tokens behind the last row are NaN."""
+    N, Hq, D = q.shape
+    n_pages, Hkv, page, _ = k_pages.shape
+    scale = D ** -0.5 if scale is None else scale
+    q, k_pages, v_pages = (x.detach().cpu().double() for x in (q, k_pages, v_pages))
+    y = torch.full_like(q, float("nan"))
+    for i in range(len(offsets) - 1):
+        t0, c = offsets[i], offsets[i + 1] - offsets[i]
+        r = i if slots is None else slots[i]
+        n = lengths[r] if 0 <= r < len(table) else 0
+        if n > len(table[0]) * page:
+            n = 0
+        for t in range(c):
+            p = n - c + t
+            seen = [j for j in range(p + 1) if (window is None or p - j < window or j < sinks)
+                    and 0 <= table[r][j // page] < n_pages] if n else []
+            y[t0 + t] = 0
+            if not seen:
+                continue
+            at = torch.tensor([table[r][j // page] for j in seen])
+            place = torch.tensor([j % page for j in seen])
+            for h in range(Hkv):
+                k, v = k_pages[at, h, place], v_pages[at, h, place]
+                g = slice(h * (Hq // Hkv), (h + 1) * (Hq // Hkv))
+                y[t0 + t, g] = torch.softmax(q[t0 + t, g] @ k.T * scale, 1) @ v
+    return y
+
+
 class Pages:
     """The cache as lists: ``rows[r]`` is the row's page numbers (None where
     trimmed), ``lens[r]`` its tokens, ``refs`` the counts, ``data[page]`` any value."""
@@ -79,6 +109,33 @@ class Pages:
             start.append(self.lens[s])
             self.lens[s] += n_new
         return start
+
+    def reserve_packed(self, slots, n_new, tokens):
+        """(offsets, start, positions, places), or None where a row, the pool or the batch is too small."""
+        n_new, here = [max(c, 0) for c in n_new], [0 <= s < len(self.rows) for s in slots]
+        need = [-(-(self.lens[s] + c) // self.page) - -(-self.lens[s] // self.page) if ok else 0
+                for s, c, ok in zip(slots, n_new, here)]
+        short = any(ok and self.lens[s] + c > self.width * self.page for s, c, ok in zip(slots, n_new, here))
+        if short or sum(need) > len(self._free()) or sum(n_new) > tokens:
+            return None
+        free, offsets, start, positions, places = self._free(), [0], [], [], []
+        for s, c, n, ok in zip(slots, n_new, need, here):
+            offsets.append(offsets[-1] + c)
+            start.append(self.lens[s] if ok else -1)
+            if not ok:
+                positions += [-1] * c
+                places += [-1] * c
+                continue
+            for _ in range(n):
+                self.rows[s].append(free.pop(0))
+                self.refs[self.rows[s][-1]] = 1
+            for p in range(self.lens[s], self.lens[s] + c):
+                pg = self.rows[s][p // self.page]
+                positions.append(p)
+                places.append(-1 if pg is None else pg * self.page + p % self.page)
+            self.lens[s] += c
+        more = [-1] * (tokens - offsets[-1])
+        return offsets, start, positions + more, places + more
 
     def fork(self, parents, children):
         """(page, copy) pairs, or None where pages are missing."""
