@@ -96,6 +96,7 @@ SIGNATURES = {
     "gdnx_pages_packed_workspace_bytes": (_c_ll, [_c_int] * 2),
     "gdnx_pages_reserve_packed": (_c_int, [_vp] * 11 + [_c_int] * 6 + [_vp]),
     "gdnx_pages_write_packed": (_c_int, [_vp] * 5 + [_c_ll] * 6 + [_c_int] * 7 + [_vp]),
+    "gdnx_chunk_attn_workspace_bytes": (_c_ll, [_c_int] * 10),
     "gdnx_chunk_attn": (_c_int, [_vp] * 9 + [_c_ll] * 2 + [_c_int] * 11 + [_c_float, _c_int, _vp]),
     "gdnx_conv_fwd": (_c_int, [_vp] * 7 + [_c_ll] * 2 + [_c_int] * 7 + [_vp]),
     "gdnx_conv_bwd_workspace_bytes": (_c_ll, [_c_int] * 5),

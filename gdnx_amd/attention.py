@@ -256,8 +256,10 @@ def paged_attention_chunk(q, k_pages, v_pages, table, lengths, offsets, *, slots
               "out must be contiguous [N,Hq,D] of q's dtype")
     if N == 0 or n == 0:
         return out
-    q = _rows16(q.unsqueeze(0))[0]
+    q = _rows16(q.unsqueeze(0))
+    nws = _bytes("gdnx_chunk_attn_workspace_bytes", N, n, width, page, Hq, Hkv, D, window, sinks, code)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
     _lib.call("gdnx_chunk_attn", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
-              lengths.data_ptr(), offsets.data_ptr(), _addr(slots), out.data_ptr(), None, *_strides(q.unsqueeze(0))[1:], N, n,
-              rows, width, n_pages, page, Hq, Hkv, D, window, sinks, D ** -0.5 if scale is None else float(scale), code)
+              lengths.data_ptr(), offsets.data_ptr(), _addr(slots), out.data_ptr(), _addr(ws), *_strides(q)[1:], N, n, rows,
+              width, n_pages, page, Hq, Hkv, D, window, sinks, D ** -0.5 if scale is None else float(scale), code)
     return out

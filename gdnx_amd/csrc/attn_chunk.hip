@@ -1,96 +1,311 @@
 // Attention of packed new tokens over a paged key-value cache (gfx950):
 // prompts' pieces, drafts and single tokens in one call.
 //
-// Row i's n new tokens stand at the last n positions of its table row (its
+//   P_j = exp(s q.k_j - lse) over the visible j,  y = sum_j P_j v_j
+//
+// Row i's c new tokens stand at the last c positions of its table row (its
 // length counts them, and their keys and values are in their pages); the one
 // at p sees key j if j <= p and p - j < window or j < sinks.  A key without a
 // page is not seen.
 //
-// The form here is the plain one: a wave takes a query head of a token, 64 keys
-// at a time, a lane a key for the scores and D / 64 columns for the sum.
-#include "attn_common.hpp"
-#include "packed_rows.hpp"
+// Two forms, by a row's (token, query head of the group) pairs.  Up to 32 of
+// them (single tokens, drafts) wait for memory: attn_chunk_short.hpp.  More
+// (prompts' pieces) are tiles of 128 (64 in float32) against tiles of keys in
+// LDS, as in windowed attention: attn_chunk_mfma.hip and below.  Both are in one
+// launch, so that rows of both kinds share the chip; where the rows' tokens
+// are is found from the offsets by the workgroups themselves, so nothing waits
+// for the host.
+#include "attn_chunk_short.hpp"
+#include "attn_f32.hpp"
 
 namespace gdnx {
 
-namespace {
+int chunk_bf16_launch(const ChunkAttnArgs& a, unsigned groups, hipStream_t stream);
 
-// A query from what it sees alone.
-template <typename CT, int D> struct ChunkRow {
-  static constexpr int E = D / 64;
-  float m, l, acc[E];
-  __device__ __forceinline__ ChunkRow(const ChunkAttnArgs& a, const CT* q, int r, int hk, int p, int len, int lane)
-      : m(-INFINITY), l(0.f) {
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    const int* table = a.table + (long long)r * a.width;
-    const int mask = (1 << a.page_log) - 1;
-    const KeyTiles<64> kt(p, p, len, a.window, a.sinks);
-    for (int it = 0; it < kt.count; ++it) {
-      const int j = kt.start(it) + lane;
-      const int pg = attn_visible(p, j, a.window, a.sinks) ? table[j >> a.page_log] : -1;
-      const bool vis = pg >= 0 && pg < a.n_pages;
-      const long long at = vis ? (((long long)pg * a.Hkv + hk) << a.page_log) + (j & mask) : 0;     // its row in the pool
-      float s = 0.f;
-      if (vis) {
-        const CT* k = (const CT*)a.k_pages + at * D;
-        for (int d = 0; d < D; ++d) s = fmaf(to_f(q[d]), to_f(k[d]), s);
+// Float32: v_mfma_f32_16x16x4_f32, a wave owns 16 rows; tiles of 32 keys by way
+// of registers into LDS, double-buffered, one barrier a tile (attn_win.hip).
+template <int D> __device__ __forceinline__ void chunk_long_f32(const ChunkAttnArgs& a, float* smem) {
+  using T = F32Tile<D>;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
+  const ChunkItem item(a, blockIdx.x);
+  const int hk = item.hk;
+  int si, first, count, tile;
+  if (!row_item(a.offsets, a.n, a.N, G, 64, item.item, lane, &si, &first, &count, &tile)) return;
+  const long long pairs = (long long)count * G;
+  if (pairs <= a.short_rows || tile * 64LL >= pairs) return;
+  ChunkSeq sq;
+  sq.find(a, si, first, count);
+  const int off = sq.off, len = sq.len;
+  const RowMap rm(tile * 64, G, a.g_magic);
+  const KeyTiles<32> kt(rm.i0 + off, min(rm.last(63), count - 1) + off, len, a.window, a.sinks);
+  const int parts = chunk_parts(kt.count, a.parts);
+  if (item.part >= parts) return;
+  const int per = (kt.count + parts - 1) / parts, t0 = item.part * per, t1 = min(kt.count, t0 + per);
+  const int* table = a.table + (long long)sq.r * a.width;
+  const int mask = (1 << a.page_log) - 1;
+  const float *kb = (const float*)a.k_pages, *vb = (const float*)a.v_pages;
+  int qi, qh;
+  rm.at(wave * 16 + n, &qi, &qh);
+  qh += hk * G;
+  const int p = qi < count ? qi + off : -1;
+  const int wv0 = rm.last(wave * 16) + off, last = rm.last(wave * 16 + 15);
+  const int wv1 = min(last, count - 1) + off;
+  const bool rows_ok = last < count && wv0 >= 0;
+  f32x4 qf[T::NS];
+  {
+    const float* qp = (const float*)a.q + (first + (p >= 0 ? qi : 0)) * a.qs[0] + (p >= 0 ? qh : 0) * a.qs[1];
+#pragma unroll
+    for (int c = 0; c < T::NS; ++c) qf[c] = *(const f32x4*)(qp + 16 * c + 4 * g);
+  }
+  const float sc = a.scale * kLog2e;
+  F32Stage<D> st(tid);
+  // the page of key j0 + lane of a tile, and (there) which of its 32 keys have one
+  const auto page_at = [&](int it) { return table[min(kt.start(min(it, t1 - 1)) + (lane & 31), len - 1) >> a.page_log]; };
+  const auto load = [&](int it, int pg) {
+    const int j0 = kt.start(min(it, t1 - 1));
+    const bool there = pg >= 0 && pg < a.n_pages;
+    const int page = there ? pg : 0;
+    st.load([&](int r, const float** x, const float** y) {
+      const int c = min(r, len - 1 - j0);
+      const long long at = ((((long long)__shfl(page, c) * a.Hkv + hk) << a.page_log) + ((j0 + c) & mask)) * D;
+      *x = kb + at;
+      *y = vb + at;
+    });
+    return (unsigned)__ballot(there);
+  };
+  f32x4 o[T::NS];
+#pragma unroll
+  for (int t = 0; t < T::NS; ++t) o[t] = zero4();
+  float m = -INFINITY, l = 0.f;
+  unsigned there = 0;
+  int pg = -1;
+  if (t0 < t1) {
+    there = load(t0, page_at(t0));
+    pg = page_at(t0 + 1);
+    st.store(smem, smem + T::WORDS);
+  }
+  lds_barrier();
+  for (int it = t0; it < t1; ++it) {
+    const int j0 = kt.start(it);
+    const float *sk = smem + ((it - t0) & 1) * 2 * T::WORDS, *sv = sk + T::WORDS;
+    const unsigned there_next = load(it + 1, pg);
+    pg = page_at(it + 2);
+    if (wv0 <= wv1 && j0 <= wv1 && (j0 + 31 > wv0 - a.window || j0 < a.sinks)) {
+      const bool all = rows_ok && j0 + 31 <= wv0 && (wv1 - j0 < a.window || j0 + 32 <= a.sinks) && there == ~0u;
+      const unsigned lv = there >> (4 * g);
+      f32x4 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = zero4();
+#pragma unroll
+        for (int c = 0; c < T::NS; ++c) mma(s[u], ld_frag(sk + (16 * u + n) * T::LD + 16 * c, g), qf[c]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[u][e] = all || ((lv >> (16 * u + e) & 1) && attn_visible(p, j0 + 16 * u + 4 * g + e, a.window, a.sinks))
+                        ? s[u][e] * sc : -INFINITY;
       }
-      s = vis ? s * (a.scale * kLog2e) : -INFINITY;
-      float mx = s;
-      for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
-      const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m - ms);
-      const float pr = vis ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
-      float sum = pr;
-      for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
-      m = mn;
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
+      const float f = exp2f(m - ms);
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[u][e] = exp2f(s[u][e] - ms);
+          sum += s[u][e];
+        }
       l = l * f + sum;
-      for (int e = 0; e < E; ++e) acc[e] *= f;
-      for (unsigned long long seen = __ballot(vis); seen; seen &= seen - 1) {
-        const int key = __ffsll(seen) - 1;
-        const float pk = __shfl(pr, key, 64);
-        const CT* v = (const CT*)a.v_pages + __shfl(at, key, 64) * D;
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(pk, to_f(v[lane * E + e]), acc[e]);
+      m = mn;
+#pragma unroll
+      for (int t = 0; t < T::NS; ++t) {
+        o[t] *= f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) mma(o[t], ld_cols<T::LD>(sv, 16 * u, 16 * t + n, g), s[u]);
       }
     }
+    float* next = smem + ((it - t0 + 1) & 1) * 2 * T::WORDS;
+    st.store(next, next + T::WORDS);
+    lds_barrier();
+    there = there_next;
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (p < 0) {                              // a row that sees nothing: 0 times a value that is not finite is NaN
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) o[t] = zero4();
+  }
+  // rows of the wave whose output is not finite (0 times it is NaN)
+  float rest = 0.f;
+#pragma unroll
+  for (int t = 0; t < T::NS; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rest = fmaf(o[t][e], 0.f, rest);
+  const unsigned long long bad = __ballot(rest != 0.f);
+  const unsigned redo = (unsigned)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffffu;
+  const long long r = (long long)(first + qi) * a.Hq + qh;
+  if (qi < count && parts > 1) {
+    float* po = long_out(a, item.part, r) + 4 * g;
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) *(f32x4*)(po + 16 * t) = o[t];
+    if (g == 0) {
+      float* ml = long_stats(a, item.part, r);
+      ml[0] = m;
+      ml[1] = l;
+    }
+  } else if (qi < count) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int t = 0; t < T::NS; ++t) *(f32x4*)((float*)a.y + r * D + 16 * t + 4 * g) = o[t] * inv;
+  }
+  if (redo) {
+    __builtin_amdgcn_s_waitcnt(0x0070);             // (the wave's own stores come first)
+    chunk_redo<float, D, 32, 16>(redo);
+  }
+}
+
+template <int D> __global__ void __launch_bounds__(256, 2) chunk_f32_kernel(ChunkAttnArgs a) {
+  constexpr int WORDS = F32Tile<D>::WORDS;
+  __shared__ __attribute__((aligned(16))) float smem[4 * WORDS];       // two buffers of K, V
+  __shared__ ChunkShortShared<float> sh;
+  const int n_long = a.items * a.parts * a.Hkv;
+  if ((int)blockIdx.x < n_long) chunk_long_f32<D>(a, smem);
+  else chunk_short<float, D>(a, blockIdx.x - n_long, [&](int v) { return (char*)(smem + v * WORDS); }, sh);
+}
+
+// Running joins of (maximum, sum, output) triples.
+struct ChunkJoin {
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float m2, float l2, const f32x4& x) {
+    const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ms), g = __builtin_amdgcn_exp2f(m2 - ms);
+    l = l * f + l2 * g;
+    acc = acc * f + x * g;
+    m = mn;
+  }
+  template <typename CT> __device__ __forceinline__ void store(CT* y) const {
+    const f32x4 o = acc * (l == 0.f ? 0.f : 1.f / l);
+    st4(y, o[0], o[1], o[2], o[3]);
   }
 };
 
-}  // namespace
-
-template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_attn_kernel(ChunkAttnArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long long u = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = (int)(u % a.Hq), t = (int)(u / a.Hq);
-  if (t >= a.N) return;
-  const int i = wave_find(a.n, t, lane, [&](int i) { return (long long)packed_offset(a.offsets, i, a.N); });
-  if (i < 0) return;
-  const int first = packed_offset(a.offsets, i, a.N), count = packed_offset(a.offsets, i + 1, a.N) - first;
-  if (t - first >= count) return;                  // behind the last row
-  const int r = a.slots ? a.slots[i] : i;
-  const long long cap = (long long)a.width << a.page_log;
-  int len = r >= 0 && r < a.rows ? a.lengths[r] : 0;
-  len = len < 0 || len > cap ? 0 : len;
-  const int p = len - count + t - first;
-  CT* y = (CT*)a.y + ((long long)t * a.Hq + h) * D + lane * E;
-  if (len == 0 || p < 0) {
-    for (int e = 0; e < E; ++e) y[e] = from_f<CT>(0.f);
+// Parts and spans joined in order.  Long rows: D / 4 threads a pair, a quarter
+// of an item's pairs a workgroup.  Short rows: a workgroup a pair, its groups
+// of D / 4 threads every n-th span.
+constexpr int kJoinSplit = 4;
+template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkAttnArgs a) {
+  constexpr int V = D / 4, NG = 256 / V, R = sizeof(CT) == 2 ? 128 : 64, BK = R / 2;
+  __shared__ __attribute__((aligned(16))) float s_acc[NG][D];
+  __shared__ float s_m[NG], s_l[NG];
+  const int G = a.Hq / a.Hkv, grp = threadIdx.x / V, d = 4 * (threadIdx.x % V), lane = threadIdx.x & 63;
+  int w = blockIdx.x;
+  const int n_long = a.parts > 1 ? a.items * a.Hkv * kJoinSplit : 0;
+  ChunkSeq s;
+  if (w < n_long) {
+    const int quarter = w % kJoinSplit; w /= kJoinSplit;
+    const int hk = w % a.Hkv;
+    int i, first, count, tile;
+    if (!row_item(a.offsets, a.n, a.N, G, R, w / a.Hkv, lane, &i, &first, &count, &tile)) return;
+    const long long pairs = (long long)count * G;
+    if (pairs <= a.short_rows || (long long)tile * R >= pairs) return;
+    s.find(a, i, first, count);
+    const RowMap rm(tile * R, G, a.g_magic);
+    const KeyTiles<BK> kt(rm.i0 + s.off, min(rm.last(R - 1), count - 1) + s.off, s.len, a.window, a.sinks);
+    const int parts = chunk_parts(kt.count, a.parts);
+    if (parts == 1) return;                        // written by its workgroup
+    for (int q = quarter * (R / kJoinSplit) + grp; q < (quarter + 1) * (R / kJoinSplit); q += NG) {
+      int qi, h;
+      rm.at(q, &qi, &h);
+      if (qi >= count) continue;
+      const long long row = (long long)(first + qi) * a.Hq + hk * G + h;
+      ChunkJoin j;
+#pragma unroll 4
+      for (int x = 0; x < parts; ++x) {
+        const float* ml = long_stats(a, x, row);
+        j.add(ml[0], ml[1], *(const f32x4*)(long_out(a, x, row) + d));
+      }
+      j.store((CT*)a.y + row * D + d);
+    }
     return;
   }
-  const ChunkRow<CT, D> c(a, (const CT*)a.q + t * a.qs[0] + h * a.qs[1], r, h / (a.Hq / a.Hkv), p, len, lane);
-  const float inv = c.l == 0.f ? 0.f : 1.f / c.l;
-  for (int e = 0; e < E; ++e) y[e] = from_f<CT>(c.acc[e] * inv);
+  w -= n_long;
+  const int q = w % kChunkShort, hk = w / kChunkShort % a.Hkv, i = w / kChunkShort / a.Hkv;
+  const int first = packed_offset(a.offsets, i, a.N), count = packed_offset(a.offsets, i + 1, a.N) - first;
+  if (count <= 0 || (long long)count * G > a.short_rows || q >= count * G) return;
+  s.find(a, i, first, count);
+  const ChunkSeen see(a, s);
+  constexpr int BT = FragT<CT>::KSTEP;
+  const int spans = chunk_spans((see.nvis + BT - 1) / BT, a.spans);
+  if (spans <= 1) return;                          // written by its workgroup
+  const long long row = ((long long)i * a.Hkv + hk) * kChunkShort + q;
+  ChunkJoin j;
+#pragma unroll 4
+  for (int x = grp; x < spans; x += NG) {
+    const float* ml = short_stats(a, row, x);
+    j.add(ml[0], ml[1], *(const f32x4*)(short_out(a, row, x) + d));
+  }
+  *(f32x4*)&s_acc[grp][d] = j.acc;
+  if (d == 0) {
+    s_m[grp] = j.m;
+    s_l[grp] = j.l;
+  }
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int x = 1; x < NG; ++x) j.add(s_m[x], s_l[x], *(const f32x4*)&s_acc[x][d]);
+  j.store((CT*)a.y + ((long long)(first + q / G) * a.Hq + hk * G + q % G) * D + d);
 }
 
-template <typename CT, int D> static int launch(const ChunkAttnArgs& a, hipStream_t stream) {
-  const long long groups = ((long long)a.N * a.Hq + 3) / 4;
-  hipLaunchKernelGGL((chunk_attn_kernel<CT, D>), dim3((unsigned)groups), dim3(256), 0, stream, a);
-  return check_launch("chunk_attn_kernel");
+// How the rows share the work.  Their lengths are on the device, so the
+// numbers of workgroups come from the batch's size and from the longest row that the
+// table can hold (or the window); what a row does not need ends at once.
+void chunk_attn_plan(ChunkAttnArgs& a) {
+  const long long G = a.Hq / a.Hkv, R = a.dtype == GDNX_DTYPE_BF16 ? 128 : 64, pairs = a.N * G;
+  long long keys = (long long)a.width << a.page_log;
+  // a single row goes the long way whatever it holds; rows are all short if all tokens make but one short row
+  a.short_rows = a.n == 1 && pairs > kChunkShort ? 0 : kChunkShort;
+  a.items = 0;
+  a.parts = 1;
+  a.spans = 0;
+  if (pairs > a.short_rows) {
+    a.items = (int)(pairs / R + a.n);
+    const long long win = (long long)a.window + a.sinks + R / G + 1, span = win < keys ? win : keys;
+    const long long most = pairs / (a.short_rows + 1);                      // long rows there can be
+    const long long tiles = (pairs / R + (a.n < most ? a.n : most)) * a.Hkv;
+    long long parts = 512 / (tiles ? tiles : 1);
+    if (parts > span / (R / 2) / 8) parts = span / (R / 2) / 8;
+    a.parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
+  }
+  if (a.short_rows) {
+    const long long win = (long long)a.window + a.sinks + kChunkShort;
+    a.spans = paged_attn_spans(a.n, a.Hkv, a.Hkv, win < keys ? win : keys, a.dtype);
+  }
+}
+
+template <typename CT, int D> static int join(const ChunkAttnArgs& a, hipStream_t stream) {
+  const long long groups = (a.parts > 1 ? (long long)a.items * a.Hkv * kJoinSplit : 0) +
+                           (a.spans > 1 ? (long long)a.n * a.Hkv * kChunkShort : 0);
+  if (groups == 0) return GDNX_OK;
+  hipLaunchKernelGGL((chunk_join_kernel<CT, D>), dim3((unsigned)groups), dim3(256), 0, stream, a);
+  return check_launch("chunk_join_kernel");
 }
 
 int chunk_attn_dispatch(const ChunkAttnArgs& a, hipStream_t stream) {
-  if (a.dtype == GDNX_DTYPE_BF16) return a.D == 128 ? launch<bf16, 128>(a, stream) : launch<bf16, 64>(a, stream);
-  return a.D == 128 ? launch<float, 128>(a, stream) : launch<float, 64>(a, stream);
+  const unsigned groups = (unsigned)((long long)a.items * a.parts * a.Hkv + (long long)a.n * a.Hkv * a.spans);
+  int rc;
+  if (a.dtype == GDNX_DTYPE_BF16) {
+    if ((rc = chunk_bf16_launch(a, groups, stream))) return rc;
+    return a.D == 128 ? join<bf16, 128>(a, stream) : join<bf16, 64>(a, stream);
+  }
+  if (a.D == 128) hipLaunchKernelGGL((chunk_f32_kernel<128>), dim3(groups), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((chunk_f32_kernel<64>), dim3(groups), dim3(256), 0, stream, a);
+  if ((rc = check_launch("chunk_f32_kernel"))) return rc;
+  return a.D == 128 ? join<float, 128>(a, stream) : join<float, 64>(a, stream);
 }
 
 }  // namespace gdnx

@@ -1504,17 +1504,56 @@ extern "C" int gdnx_pages_write_packed(const void* k_new, const void* v_new, voi
   return pages_put_dispatch(a, (hipStream_t)stream);
 }
 
+namespace gdnx {
+
+// Sizes of a chunk call; fills what the plan needs and the plan itself.
+static int check_chunk(ChunkAttnArgs& a, int N, int n, int width, int page, int Hq, int Hkv, int D, int window, int sinks,
+                       int dtype) {
+  int rc = check_attn_sizes(Hq, Hkv, D, window, sinks, dtype);
+  if (rc || (rc = check_pool(1, width, 1, page)) || (rc = check_packed(n, N))) return rc;
+  if (!prod_le(kNoWindow, {N, Hq})) return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
+  a.N = N; a.n = n; a.width = width; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.dtype = dtype;
+  a.window = window_arg(window);
+  a.sinks = sinks_arg(sinks);
+  a.page_log = 0;
+  while ((1 << a.page_log) < page) ++a.page_log;
+  a.g_magic = group_magic(Hq / Hkv);
+  chunk_attn_plan(a);
+  // workgroups of the two kinds and of their joins
+  if (!prod_le(kMaxGroups / 2, {a.items, Hkv, a.parts > 4 ? a.parts : 4}) ||
+      !prod_le(kMaxGroups / 2, {n, Hkv, a.spans > kChunkShort ? a.spans : kChunkShort}))
+    return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
+  return GDNX_OK;
+}
+
+// Floats of the long rows' parts, then of the short rows' spans.
+static long long chunk_part_floats(const ChunkAttnArgs& a) {
+  return a.parts > 1 ? (long long)a.parts * a.N * a.Hq * (a.D + 2) : 0;
+}
+static long long chunk_span_floats(const ChunkAttnArgs& a) {
+  return a.spans > 1 ? (long long)a.n * a.Hkv * kChunkShort * a.spans * (a.D + 2) : 0;
+}
+
+}  // namespace gdnx
+
+extern "C" long long gdnx_chunk_attn_workspace_bytes(int N, int n, int width, int page, int Hq, int Hkv, int head_dim,
+                                                     int window, int sinks, int dtype) {
+  ChunkAttnArgs a{};
+  if (check_chunk(a, N, n, width, page, Hq, Hkv, head_dim, window, sinks, dtype)) return -1;
+  return 4 * (chunk_part_floats(a) + chunk_span_floats(a));
+}
+
 extern "C" int gdnx_chunk_attn(const void* q, const void* k_pages, const void* v_pages, const int* table,
                                const int* lengths, const int* offsets, const int* slots, void* y, void* workspace,
                                long long q_t, long long q_h, int N, int n, int rows, int width, int n_pages, int page,
                                int Hq, int Hkv, int head_dim, int window, int sinks, float scale, int dtype,
                                void* stream) {
   g_err[0] = 0;
-  int rc = check_attn_sizes(Hq, Hkv, head_dim, window, sinks, dtype);
-  if (rc || (rc = check_pool(rows, width, n_pages, page)) || (rc = check_packed(n, N))) return rc;
+  ChunkAttnArgs a{};
+  int rc = check_chunk(a, N, n, width, page, Hq, Hkv, head_dim, window, sinks, dtype);
+  if (rc || (rc = check_pool(rows, width, n_pages, page))) return rc;
   if (!slots && n > rows) return set_error(GDNX_ERR_SHAPE, "bad number of rows %d (table rows %d)", n, rows);
-  if (!prod_le(kNoWindow, {N, Hq}) || !prod_le(kMaxGroups * 4, {N, Hq}))
-    return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
+  if (N == 0) return GDNX_OK;
   if (!q || !k_pages || !v_pages || !table || !lengths || !offsets || !y)
     return set_error(GDNX_ERR_ARG, "all pointers but slots and workspace must be non-null");
   for (const void* p : {q, k_pages, v_pages, (const void*)y, (const void*)workspace})
@@ -1522,11 +1561,11 @@ extern "C" int gdnx_chunk_attn(const void* q, const void* k_pages, const void* v
   const int unit = dtype == GDNX_DTYPE_BF16 ? 8 : 4;
   if (q_t < 0 || q_h < 0 || q_t % unit || q_h % unit || q_t > (1LL << 40) || q_h > (1LL << 40))
     return set_error(GDNX_ERR_SHAPE, "q: strides must be non-negative multiples of 16 bytes");
-  int lg = 0;
-  while ((1 << lg) < page) ++lg;
-  if (N == 0) return GDNX_OK;
-  ChunkAttnArgs a{q, k_pages, v_pages, table, lengths, offsets, slots, y, (float*)workspace, {q_t, q_h}, N, n, rows, width,
-                  n_pages, lg, Hq, Hkv, head_dim, window_arg(window), sinks_arg(sinks), scale, dtype};
+  const long long parts = chunk_part_floats(a);
+  if (parts + chunk_span_floats(a) > 0 && !workspace) return set_error(GDNX_ERR_WORKSPACE, "workspace must be non-null");
+  a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.table = table; a.lengths = lengths; a.offsets = offsets;
+  a.slots = slots; a.y = y; a.part = (float*)workspace; a.span_part = (float*)workspace + parts;
+  a.qs[0] = q_t; a.qs[1] = q_h; a.rows = rows; a.n_pages = n_pages; a.scale = scale;
   return chunk_attn_dispatch(a, (hipStream_t)stream);
 }
 

@@ -529,12 +529,19 @@ struct ChunkAttnArgs {
   const int* offsets;   // [n + 1]
   const int* slots;     // [n] table row of each row, or null
   void* y;              // [N,Hq,D]
-  float* part;
+  float* part;          // long rows' parts [parts][N*Hq][D], [parts][N*Hq][2] maximum (log2) and sum
+  float* span_part;     // short rows' spans [n*Hkv*kChunkShort][spans][D], then [..][spans][2]
   long long qs[2];
   int N, n, rows, width, n_pages, page_log, Hq, Hkv, D, window, sinks;
   float scale;
   int dtype;
+  unsigned g_magic;     // ceil(2^32 / (Hq / Hkv))
+  int short_rows;       // rows of at most so many (token, head of the group) pairs go the short way
+  int items, parts;     // long rows: work items a key head, most parts of their keys
+  int spans;            // short rows: most spans of their keys (0: no row can be short)
 };
+constexpr int kChunkShort = 32;
+void chunk_attn_plan(ChunkAttnArgs& a);      // from the sizes: short_rows, items, parts, spans
 int chunk_attn_dispatch(const ChunkAttnArgs& a, hipStream_t stream);
 
 // The page pool's operations.

@@ -758,7 +758,10 @@ int gdnx_pages_write_packed(const void* k_new, const void* v_new, void* k_pages,
  * A key or value that is not finite reaches only the tokens that see it.
  * q [N,Hq,D] with element strides (token, head) that are multiples of 16
  * bytes, y [N,Hq,D] contiguous; pages, table and lengths as
- * gdnx_paged_attn_step. */
+ * gdnx_paged_attn_step.  workspace: gdnx_chunk_attn_workspace_bytes bytes (-1 if
+ * the sizes are invalid; null where that is 0). */
+long long gdnx_chunk_attn_workspace_bytes(int N, int n, int width, int page, int Hq, int Hkv, int head_dim, int window,
+                                          int sinks, int dtype);
 int gdnx_chunk_attn(const void* q, const void* k_pages, const void* v_pages, const int* table, const int* lengths,
                     const int* offsets, const int* slots, void* y, void* workspace, long long q_t, long long q_h, int N,
                     int n, int rows, int width, int n_pages, int page, int Hq, int Hkv, int head_dim, int window,
