@@ -188,26 +188,45 @@ struct ChunkJoin {
     acc = acc * f + x * g;
     m = mn;
   }
+  // every `step`-th of n, four asked for at a time (the last again where there are no four)
+  template <typename S, typename O>
+  __device__ __forceinline__ void take(int n, int from, int step, const S& stats, const O& out) {
+    for (int x0 = from; x0 < n; x0 += 4 * step) {
+      float ml[4][2];
+      f32x4 o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = min(x0 + e * step, n - 1);
+        ml[e][0] = stats(x)[0];
+        ml[e][1] = stats(x)[1];
+        o[e] = *(const f32x4*)out(x);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (x0 + e * step < n) add(ml[e][0], ml[e][1], o[e]);
+    }
+  }
   template <typename CT> __device__ __forceinline__ void store(CT* y) const {
     const f32x4 o = acc * (l == 0.f ? 0.f : 1.f / l);
     st4(y, o[0], o[1], o[2], o[3]);
   }
 };
 
-// Parts and spans joined in order.  Long rows: D / 4 threads a pair, a quarter
-// of an item's pairs a workgroup.  Short rows: a workgroup a pair, its groups
-// of D / 4 threads every n-th span.
-constexpr int kJoinSplit = 4;
+// Parts and spans joined in order.  Long rows: D / 4 threads a pair, one pair
+// after the other only where the items are many (200 tokens on 16384 in 16 parts:
+// four pairs 39 us, one 7).  Short rows: so many groups of D / 4 threads a pair that each has about four
+// spans; with many rows a workgroup takes all pairs of one (256 single tokens, a
+// workgroup a possible pair: 54 us, most of it workgroups without work).
 template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkAttnArgs a) {
   constexpr int V = D / 4, NG = 256 / V, R = sizeof(CT) == 2 ? 128 : 64, BK = R / 2;
   __shared__ __attribute__((aligned(16))) float s_acc[NG][D];
   __shared__ float s_m[NG], s_l[NG];
   const int G = a.Hq / a.Hkv, grp = threadIdx.x / V, d = 4 * (threadIdx.x % V), lane = threadIdx.x & 63;
   int w = blockIdx.x;
-  const int n_long = a.parts > 1 ? a.items * a.Hkv * kJoinSplit : 0;
+  const int n_long = a.parts > 1 ? a.items * a.Hkv * a.join_split : 0;
   ChunkSeq s;
   if (w < n_long) {
-    const int quarter = w % kJoinSplit; w /= kJoinSplit;
+    const int q0 = w % a.join_split * (R / a.join_split) + grp, q1 = q0 - grp + R / a.join_split; w /= a.join_split;
     const int hk = w % a.Hkv;
     int i, first, count, tile;
     if (!row_item(a.offsets, a.n, a.N, G, R, w / a.Hkv, lane, &i, &first, &count, &tile)) return;
@@ -218,47 +237,48 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
     const KeyTiles<BK> kt(rm.i0 + s.off, min(rm.last(R - 1), count - 1) + s.off, s.len, a.window, a.sinks);
     const int parts = chunk_parts(kt.count, a.parts);
     if (parts == 1) return;                        // written by its workgroup
-    for (int q = quarter * (R / kJoinSplit) + grp; q < (quarter + 1) * (R / kJoinSplit); q += NG) {
+    for (int q = q0; q < q1; q += NG) {
       int qi, h;
       rm.at(q, &qi, &h);
-      if (qi >= count) continue;
+      if (qi >= count) return;
       const long long row = (long long)(first + qi) * a.Hq + hk * G + h;
       ChunkJoin j;
-#pragma unroll 4
-      for (int x = 0; x < parts; ++x) {
-        const float* ml = long_stats(a, x, row);
-        j.add(ml[0], ml[1], *(const f32x4*)(long_out(a, x, row) + d));
-      }
+      j.take(parts, 0, 1, [&](int x) { return long_stats(a, x, row); }, [&](int x) { return long_out(a, x, row) + d; });
       j.store((CT*)a.y + row * D + d);
     }
     return;
   }
   w -= n_long;
-  const int q = w % kChunkShort, hk = w / kChunkShort % a.Hkv, i = w / kChunkShort / a.Hkv;
+  // `share` groups of threads take a pair's spans, 256 / V / share pairs a workgroup at a time
+  const int share = min(a.join_share, NG), step = NG / share, blocks = a.join_blocks;
+  const int block = w % blocks; w /= blocks;
+  const int hk = w % a.Hkv, i = w / a.Hkv;
   const int first = packed_offset(a.offsets, i, a.N), count = packed_offset(a.offsets, i + 1, a.N) - first;
-  if (count <= 0 || (long long)count * G > a.short_rows || q >= count * G) return;
+  if (count <= 0 || (long long)count * G > a.short_rows || block * step >= count * G) return;
   s.find(a, i, first, count);
   const ChunkSeen see(a, s);
   constexpr int BT = FragT<CT>::KSTEP;
   const int spans = chunk_spans((see.nvis + BT - 1) / BT, a.spans);
   if (spans <= 1) return;                          // written by its workgroup
-  const long long row = ((long long)i * a.Hkv + hk) * kChunkShort + q;
-  ChunkJoin j;
-#pragma unroll 4
-  for (int x = grp; x < spans; x += NG) {
-    const float* ml = short_stats(a, row, x);
-    j.add(ml[0], ml[1], *(const f32x4*)(short_out(a, row, x) + d));
+  for (int q0 = block * step; q0 < count * G; q0 += blocks * step) {
+    const int q = q0 + grp / share, part = grp % share;
+    const long long row = ((long long)i * a.Hkv + hk) * kChunkShort + q;
+    ChunkJoin j;
+    if (q < count * G) j.take(spans, part, share, [&](int x) { return short_stats(a, row, x); },
+                              [&](int x) { return short_out(a, row, x) + d; });
+    if (share > 1) {
+      __syncthreads();
+      *(f32x4*)&s_acc[grp][d] = j.acc;
+      if (d == 0) {
+        s_m[grp] = j.m;
+        s_l[grp] = j.l;
+      }
+      __syncthreads();
+      if (part == 0)
+        for (int x = 1; x < share; ++x) j.add(s_m[grp + x], s_l[grp + x], *(const f32x4*)&s_acc[grp + x][d]);
+    }
+    if (part == 0 && q < count * G) j.store((CT*)a.y + ((long long)(first + q / G) * a.Hq + hk * G + q % G) * D + d);
   }
-  *(f32x4*)&s_acc[grp][d] = j.acc;
-  if (d == 0) {
-    s_m[grp] = j.m;
-    s_l[grp] = j.l;
-  }
-  __syncthreads();
-  if (grp) return;
-#pragma unroll
-  for (int x = 1; x < NG; ++x) j.add(s_m[x], s_l[x], *(const f32x4*)&s_acc[x][d]);
-  j.store((CT*)a.y + ((long long)(first + q / G) * a.Hq + hk * G + q % G) * D + d);
 }
 
 // How the rows share the work.  Their lengths are on the device, so the
@@ -275,21 +295,27 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
   if (pairs > a.short_rows) {
     a.items = (int)(pairs / R + a.n);
     const long long win = (long long)a.window + a.sinks + R / G + 1, span = win < keys ? win : keys;
-    const long long most = pairs / (a.short_rows + 1);                      // long rows there can be
-    const long long tiles = (pairs / R + (a.n < most ? a.n : most)) * a.Hkv;
-    long long parts = 512 / (tiles ? tiles : 1);
+    const long long most = pairs / (a.short_rows + 1), rows = a.n < most ? a.n : most;      // long rows there can be
+    const long long tiles = ((pairs + R - 1) / R + (rows - 1) / 2) * a.Hkv;
+    long long parts = (a.n == 1 ? 512 : 1024) / (tiles ? tiles : 1);
+    if (parts > 4096 / ((long long)a.items * a.Hkv)) parts = 4096 / ((long long)a.items * a.Hkv);
     if (parts > span / (R / 2) / 8) parts = span / (R / 2) / 8;
     a.parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
+    a.join_split = (long long)a.items * a.Hkv >= 256 ? 4 : (int)(R * a.D / 1024);      // workgroups an item
   }
   if (a.short_rows) {
     const long long win = (long long)a.window + a.sinks + kChunkShort;
     a.spans = paged_attn_spans(a.n, a.Hkv, a.Hkv, win < keys ? win : keys, a.dtype);
+    const int groups = 1024 / a.D;                       // of a join's workgroup
+    a.join_share = 1;
+    while (a.join_share < groups && 4 * a.join_share < a.spans) a.join_share *= 2;
+    a.join_blocks = (long long)a.n * a.Hkv >= 512 ? 1 : (kChunkShort + groups / a.join_share - 1) / (groups / a.join_share);
   }
 }
 
 template <typename CT, int D> static int join(const ChunkAttnArgs& a, hipStream_t stream) {
-  const long long groups = (a.parts > 1 ? (long long)a.items * a.Hkv * kJoinSplit : 0) +
-                           (a.spans > 1 ? (long long)a.n * a.Hkv * kChunkShort : 0);
+  const long long groups = (a.parts > 1 ? (long long)a.items * a.Hkv * a.join_split : 0) +
+                           (a.spans > 1 ? (long long)a.n * a.Hkv * a.join_blocks : 0);
   if (groups == 0) return GDNX_OK;
   hipLaunchKernelGGL((chunk_join_kernel<CT, D>), dim3((unsigned)groups), dim3(256), 0, stream, a);
   return check_launch("chunk_join_kernel");

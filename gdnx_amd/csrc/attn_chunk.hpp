@@ -23,13 +23,14 @@ struct ChunkSeq {
 };
 
 // Where a workgroup stands among the long rows' work: key heads fastest (a
-// head's tiles share an XCD's L2 where 8 divides the heads), then the parts.
+// head's tiles share an XCD's L2 where 8 divides the heads), then the parts; a
+// row's last tiles, which see most keys, first.
 struct ChunkItem {
   int hk, part, item;
   __device__ __forceinline__ ChunkItem(const ChunkAttnArgs& a, int w) {
     hk = w % a.Hkv; w /= a.Hkv;
     part = w % a.parts;
-    item = w / a.parts;
+    item = a.items - 1 - w / a.parts;
   }
 };
 

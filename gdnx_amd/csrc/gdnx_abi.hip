@@ -1520,7 +1520,7 @@ static int check_chunk(ChunkAttnArgs& a, int N, int n, int width, int page, int 
   a.g_magic = group_magic(Hq / Hkv);
   chunk_attn_plan(a);
   // workgroups of the two kinds and of their joins
-  if (!prod_le(kMaxGroups / 2, {a.items, Hkv, a.parts > 4 ? a.parts : 4}) ||
+  if (!prod_le(kMaxGroups / 2, {a.items, Hkv, a.parts > 16 ? a.parts : 16}) ||
       !prod_le(kMaxGroups / 2, {n, Hkv, a.spans > kChunkShort ? a.spans : kChunkShort}))
     return set_error(GDNX_ERR_SHAPE, "too many rows, heads and tokens in one call");
   return GDNX_OK;

@@ -539,6 +539,8 @@ struct ChunkAttnArgs {
   int short_rows;       // rows of at most so many (token, head of the group) pairs go the short way
   int items, parts;     // long rows: work items a key head, most parts of their keys
   int spans;            // short rows: most spans of their keys (0: no row can be short)
+  int join_split;       // long rows' join: workgroups an item
+  int join_share, join_blocks;      // short rows' join: groups of threads a pair, workgroups a row and key head
 };
 constexpr int kChunkShort = 32;
 void chunk_attn_plan(ChunkAttnArgs& a);      // from the sizes: short_rows, items, parts, spans
