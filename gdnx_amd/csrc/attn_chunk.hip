@@ -8,8 +8,8 @@
 // at p sees key j if j <= p and p - j < window or j < sinks.  A key without a
 // page is not seen.
 //
-// Two forms, by a row's (token, query head of the group) pairs.  Up to 32 of
-// them (single tokens, drafts) wait for memory: attn_chunk_short.hpp.  More
+// Two forms, by a row's (token, query head of the group) pairs.  Up to 32 (16 in
+// float32) of them (single tokens, drafts) wait for memory: attn_chunk_short.hpp.  More
 // (prompts' pieces) are tiles of 128 (64 in float32) against tiles of keys in
 // LDS, as in windowed attention: attn_chunk_mfma.hip and below.  Both are in one
 // launch, so that rows of both kinds share the chip; where the rows' tokens
@@ -39,7 +39,7 @@ template <int D> __device__ __forceinline__ void chunk_long_f32(const ChunkAttnA
   const int off = sq.off, len = sq.len;
   const RowMap rm(tile * 64, G, a.g_magic);
   const KeyTiles<32> kt(rm.i0 + off, min(rm.last(63), count - 1) + off, len, a.window, a.sinks);
-  const int parts = chunk_parts(kt.count, a.parts);
+  const int parts = chunk_parts(a, kt.count);
   if (item.part >= parts) return;
   const int per = (kt.count + parts - 1) / parts, t0 = item.part * per, t1 = min(kt.count, t0 + per);
   const int* table = a.table + (long long)sq.r * a.width;
@@ -235,7 +235,7 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
     s.find(a, i, first, count);
     const RowMap rm(tile * R, G, a.g_magic);
     const KeyTiles<BK> kt(rm.i0 + s.off, min(rm.last(R - 1), count - 1) + s.off, s.len, a.window, a.sinks);
-    const int parts = chunk_parts(kt.count, a.parts);
+    const int parts = chunk_parts(a, kt.count);
     if (parts == 1) return;                        // written by its workgroup
     for (int q = q0; q < q1; q += NG) {
       int qi, h;
@@ -284,13 +284,23 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
 // How the rows share the work.  Their lengths are on the device, so the
 // numbers of workgroups come from the batch's size and from the longest row that the
 // table can hold (or the window); what a row does not need ends at once.
+//
+// Long rows' keys are cut into parts where the tiles do not give every CU its
+// two workgroups (one row), or twice that (several, whose lengths differ, so that
+// parts level out: three pieces of 1024 on up to 8192 tokens 255 us uncut, 187
+// in two, 202 in three), but into no more than 4096 workgroups, most of which have
+// no work where rows are short (256 single tokens: 418 us, with 11600 of them, 402).
+// A part has four tiles at least, eight where the tiles are many already; in us,
+// eight / four: 8 x 9 tokens on 2000, 16/4 heads, 30.6 / 20.7; 12 float32 rows with a
+// window of 512 27.8 / 17.5; 4 x 512 on 500 43.9 / 48.8.
 void chunk_attn_plan(ChunkAttnArgs& a) {
   const long long G = a.Hq / a.Hkv, R = a.dtype == GDNX_DTYPE_BF16 ? 128 : 64, pairs = a.N * G;
   long long keys = (long long)a.width << a.page_log;
   // a single row goes the long way whatever it holds; rows are all short if all tokens make but one short row
-  a.short_rows = a.n == 1 && pairs > kChunkShort ? 0 : kChunkShort;
+  const int short_pairs = chunk_short_pairs(a.dtype == GDNX_DTYPE_BF16 ? 2 : 4);
+  a.short_rows = a.n == 1 && pairs > short_pairs ? 0 : short_pairs;
   a.items = 0;
-  a.parts = 1;
+  a.parts = a.least = 1;
   a.spans = 0;
   if (pairs > a.short_rows) {
     a.items = (int)(pairs / R + a.n);
@@ -299,7 +309,8 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
     const long long tiles = ((pairs + R - 1) / R + (rows - 1) / 2) * a.Hkv;
     long long parts = (a.n == 1 ? 512 : 1024) / (tiles ? tiles : 1);
     if (parts > 4096 / ((long long)a.items * a.Hkv)) parts = 4096 / ((long long)a.items * a.Hkv);
-    if (parts > span / (R / 2) / 8) parts = span / (R / 2) / 8;
+    a.least = tiles > 192 ? 8 : 4;
+    if (parts > span / (R / 2) / a.least) parts = span / (R / 2) / a.least;
     a.parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
     a.join_split = (long long)a.items * a.Hkv >= 256 ? 4 : (int)(R * a.D / 1024);      // workgroups an item
   }
@@ -309,7 +320,7 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
     const int groups = 1024 / a.D;                       // of a join's workgroup
     a.join_share = 1;
     while (a.join_share < groups && 4 * a.join_share < a.spans) a.join_share *= 2;
-    a.join_blocks = (long long)a.n * a.Hkv >= 512 ? 1 : (kChunkShort + groups / a.join_share - 1) / (groups / a.join_share);
+    a.join_blocks = (long long)a.n * a.Hkv >= 512 ? 1 : (short_pairs + groups / a.join_share - 1) / (groups / a.join_share);
   }
 }
 

@@ -34,8 +34,8 @@ struct ChunkItem {
   }
 };
 
-// Parts that an item of `tiles` key tiles is cut into: of eight tiles at least.
-__device__ __forceinline__ int chunk_parts(int tiles, int most) { return max(1, min(most, tiles / 8)); }
+// Parts that an item of `tiles` key tiles is cut into.
+__device__ __forceinline__ int chunk_parts(const ChunkAttnArgs& a, int tiles) { return max(1, min(a.parts, tiles / a.least)); }
 
 // A short row's visible keys, counted through without a gap: the sinks, then
 // from the first key that its first token's window holds on.
@@ -135,7 +135,7 @@ template <typename CT, int D, int BK, int WR> __device__ __forceinline__ void ch
   s.find(a, i, first, count);
   const RowMap rm(tile * 4 * WR, G, a.g_magic);
   const KeyTiles<BK> kt(rm.i0 + s.off, min(rm.last(4 * WR - 1), count - 1) + s.off, s.len, a.window, a.sinks);
-  const int parts = chunk_parts(kt.count, a.parts), per = (kt.count + parts - 1) / parts;
+  const int parts = chunk_parts(a, kt.count), per = (kt.count + parts - 1) / parts;
   const int t0 = it.part * per, t1 = min(kt.count, t0 + per);
   for (; redo; redo &= redo - 1) {
     int qi, h;

@@ -74,7 +74,7 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
   // positions of the workgroup's rows
   const int wg0 = rm.i0 + off, wg1 = min(rm.last(127), count - 1) + off;
   const KeyTiles<BK> kt(wg0, wg1, len, a.window, a.sinks);
-  const int parts = chunk_parts(kt.count, a.parts);
+  const int parts = chunk_parts(a, kt.count);
   if (item.part >= parts) return;
   const int per = (kt.count + parts - 1) / parts, t0 = item.part * per, t1 = min(kt.count, t0 + per);
   const int* table = a.table + (long long)sq.r * a.width;

@@ -537,12 +537,14 @@ struct ChunkAttnArgs {
   int dtype;
   unsigned g_magic;     // ceil(2^32 / (Hq / Hkv))
   int short_rows;       // rows of at most so many (token, head of the group) pairs go the short way
-  int items, parts;     // long rows: work items a key head, most parts of their keys
+  int items, parts;     // long rows: work items a key head, most parts of their keys,
+  int least;            // of so many tiles at least
   int spans;            // short rows: most spans of their keys (0: no row can be short)
   int join_split;       // long rows' join: workgroups an item
   int join_share, join_blocks;      // short rows' join: groups of threads a pair, workgroups a row and key head
 };
-constexpr int kChunkShort = 32;
+constexpr int kChunkShort = 32;      // the most pairs of a short row
+__host__ __device__ constexpr int chunk_short_pairs(int value_bytes) { return value_bytes == 2 ? kChunkShort : 16; }
 void chunk_attn_plan(ChunkAttnArgs& a);      // from the sizes: short_rows, items, parts, spans
 int chunk_attn_dispatch(const ChunkAttnArgs& a, hipStream_t stream);
 
