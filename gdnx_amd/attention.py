@@ -37,10 +37,10 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _no_tangents(*ts):
+def _no_tangents(*ts, what="attention"):
     if forward_ad._current_level >= 0:          # (inside dual_level() only)
         _need(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in ts),
-              "attention has no forward-mode derivative")
+              f"{what} has no forward-mode derivative")
 
 
 def _rows16(t):

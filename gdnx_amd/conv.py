@@ -23,20 +23,21 @@ def _weight(x, weight, bias):
     C = x.shape[-1]
     if weight.dim() == 3 and weight.shape[1] == 1:      # as a depthwise library convolution keeps it
         weight = weight[:, 0]
-    _need(weight.dim() == 2 and weight.shape[0] == C, f"weight must be [C,W] (or [C,1,W]) with C = {C}")
-    _need(2 <= weight.shape[1] <= 8, f"{weight.shape[1]} taps: 2 to 8 are supported")
-    _need(weight.dtype in (x.dtype, torch.float32) and weight.device == x.device,
+    _need(weight.dim() == 2 and weight.shape[0] == C, "weight must be [C,W] (or [C,1,W]), C being x's channels")
+    W, dtype = weight.shape[1], weight.dtype
+    _need(2 <= W <= 8, "2 to 8 taps are supported")
+    _need((dtype == torch.float32 or dtype == x.dtype) and weight.device == x.device,
           "weight must be float32 or of x's dtype, on x's device")
     if bias is not None:
-        _need(tuple(bias.shape) == (C,) and bias.dtype == weight.dtype and bias.device == x.device,
+        _need(bias.dim() == 1 and bias.shape[0] == C and bias.dtype == dtype and bias.device == x.device,
               "bias must be [C] of weight's dtype on x's device")
         bias = bias.contiguous()
-    return weight.contiguous(), bias, weight.shape[1], _lib.dtype_code(weight.dtype)
+    return weight.contiguous(), bias, W, _lib.dtype_code(dtype)
 
 
 def _silu(activation):
-    _need(activation in ("silu", None), f'activation must be "silu" or None, got {activation!r}')
-    return int(activation == "silu")
+    _need(activation == "silu" or activation is None, 'activation must be "silu" or None')
+    return int(activation is not None)
 
 
 def _channels(t):
@@ -44,46 +45,54 @@ def _channels(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _bt_strides(x):
+    """Batch and token stride; none that an axis of one element has of its own."""
+    B, T, _ = x.shape
+    b, t, _ = x.stride()
+    return b if B > 1 else 0, t if T > 1 else 0
+
+
 class CausalConvFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, silu, want_state):
-        y, last = _forward(x, weight, bias, state, lengths, silu, want_state)
-        ctx.save_for_backward(x, weight, bias, state, lengths)
-        ctx.silu = silu
+        y, last, kept = _forward(x, weight, bias, state, lengths, silu, want_state)
+        ctx.save_for_backward(*kept, lengths)
+        ctx.args = silu, weight.shape
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
-        x, weight, bias, state, lengths = ctx.saved_tensors
-        xc = _channels(x)
-        w, b, W, wcode = _weight(x, weight, bias)
+        x, w, b, state, lengths = ctx.saved_tensors
+        silu, shape = ctx.args
         B, T, C = x.shape
-        code = _lib.dtype_code(x.dtype)
+        W, code = w.shape[1], _lib.dtype_code(x.dtype)
         dy = torch.zeros(B, T, C, dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
         dlast = None if dlast is None else dlast.contiguous()
-        state = None if state is None else state.contiguous()
         dx, dw = torch.empty(B, T, C, dtype=x.dtype, device=x.device), torch.empty_like(w)
         db = None if b is None else torch.empty_like(b)
         dstate = None if state is None else torch.empty_like(state)
         ws = torch.empty(_bytes("gdnx_conv_bwd_workspace_bytes", B, T, C, W, code), dtype=torch.uint8, device=x.device)
-        _lib.call("gdnx_conv_bwd", x.device, xc.data_ptr(), w.data_ptr(), _addr(b), _addr(state), _addr(lengths),
+        st = _bt_strides(x)
+        _lib.call("gdnx_conv_bwd", x.device, x.data_ptr(), w.data_ptr(), _addr(b), _addr(state), _addr(lengths),
                   dy.data_ptr(), _addr(dlast), dx.data_ptr(), dw.data_ptr(), _addr(db), _addr(dstate), ws.data_ptr(),
-                  *xc.stride()[:2], B, T, C, W, ctx.silu, wcode, code)
-        return dx, dw.view(weight.shape), db, dstate, None, None, None
+                  st[0], st[1], B, T, C, W, silu, _lib.dtype_code(w.dtype), code)
+        return dx, dw.view(shape), db, dstate, None, None, None
 
 
 def _forward(x, weight, bias, state, lengths, silu, want_state):
+    """y, the state handed on (or None), and the inputs as the kernels read them."""
     weight, bias, W, wcode = _weight(x, weight, bias)
     x = _channels(x)
     B, T, C = x.shape
     state = None if state is None else state.contiguous()
     y = torch.empty(B, T, C, dtype=x.dtype, device=x.device)
     last = torch.empty(B, W - 1, C, dtype=x.dtype, device=x.device) if want_state else None
+    st = _bt_strides(x)
     _lib.call("gdnx_conv_fwd", x.device, x.data_ptr(), weight.data_ptr(), _addr(bias), _addr(state), _addr(lengths),
-              y.data_ptr(), _addr(last), *x.stride()[:2], B, T, C, W, silu, wcode, _lib.dtype_code(x.dtype))
-    return y, last
+              y.data_ptr(), _addr(last), st[0], st[1], B, T, C, W, silu, wcode, _lib.dtype_code(x.dtype))
+    return y, last, (x, weight, bias, state)
 
 
 def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=None, return_state=False):
@@ -98,7 +107,7 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
     and gradients are zero.  Returns y [B,T,C], with return_state also the last
     W - 1 inputs before each row's end [B,W-1,C].  There is no forward-mode
     derivative and no second one."""
-    _no_tangents(x, weight, bias, state)
+    _no_tangents(x, weight, bias, state, what="the convolution")
     _need(x.is_cuda and x.dim() == 3, "x must be a CUDA (HIP) tensor [B,T,C]")
     _lib.dtype_code(x.dtype)
     silu, (B, T, C) = _silu(activation), x.shape
@@ -116,36 +125,37 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
     elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in srcs):
         y, last = CausalConvFunction.apply(x, weight, bias, state, lengths, silu, return_state)
     else:
-        y, last = _forward(x, weight, bias, state, lengths, silu, return_state)
+        y, last, _ = _forward(x, weight, bias, state, lengths, silu, return_state)
     return (y, last) if return_state else y
 
 
-def _slots(slots, n, x, name):
+def _slots(slots, n, x):
     if slots is not None:
-        _need(tuple(slots.shape) == (n,) and slots.dtype == torch.int32 and slots.is_contiguous()
-              and slots.device == x.device, f"{name} must be contiguous int32 [n] on x's device")
+        _need(slots.dim() == 1 and slots.shape[0] == n and slots.dtype == torch.int32 and slots.is_contiguous()
+              and slots.device == x.device, "slots and to_slots must be contiguous int32 [n] on x's device")
 
 
 def _packed(x, offsets, n, pool, weight, bias, slots, to_slots, activation, out):
-    _no_tangents(x, weight, bias, pool)
+    _no_tangents(x, weight, bias, pool, what="the convolution")
     _need(x.is_cuda and x.dim() == 2, "x must be a CUDA (HIP) tensor [tokens,C]")
     code, silu, (N, C) = _lib.dtype_code(x.dtype), _silu(activation), x.shape
     weight, bias, W, wcode = _weight(x, weight, bias)
-    _need(pool.dim() == 3 and tuple(pool.shape[1:]) == (W - 1, C) and pool.dtype == x.dtype and pool.device == x.device
+    _need(pool.dim() == 3 and pool.shape[1] == W - 1 and pool.shape[2] == C and pool.dtype == x.dtype and pool.device == x.device
           and pool.is_contiguous(), "pool must be contiguous [n_slots,W-1,C] of x's dtype on x's device")
-    _slots(slots, n, x, "slots")
-    _slots(to_slots, n, x, "to_slots")
+    _slots(slots, n, x)
+    _slots(to_slots, n, x)
     _need(slots is not None or n <= pool.shape[0], "more rows than the pool has slots: name their slots")
     if out is None:
         out = torch.empty(N, C, dtype=x.dtype, device=x.device)
     else:
-        _need(tuple(out.shape) == (N, C) and out.dtype == x.dtype and out.is_contiguous() and out.device == x.device,
-              "out must be contiguous, of x's shape, dtype and device")
+        _need(tuple(out.shape) == (N, C) and out.dtype == x.dtype and out.is_contiguous() and out.device == x.device
+              and (N == 0 or out.data_ptr() != x.data_ptr()),
+              "out must be contiguous, of x's shape, dtype and device, and not x")
     if n == 0 or C == 0 or pool.shape[0] == 0:
         return out.zero_() if pool.shape[0] == 0 else out
     x = _channels(x)
     _lib.call("gdnx_conv_packed", x.device, x.data_ptr(), _addr(offsets), weight.data_ptr(), _addr(bias),
-              pool.data_ptr(), _addr(slots), _addr(to_slots), out.data_ptr(), x.stride(0), N, n, pool.shape[0], C, W,
+              pool.data_ptr(), _addr(slots), _addr(to_slots), out.data_ptr(), x.stride(0) if N > 1 else 0, N, n, pool.shape[0], C, W,
               silu, wcode, code)
     return out
 

@@ -20,6 +20,11 @@ of a state pool in HBM, and three state kinds are kept:
     one row block per slot, so a sequence's compactions do not depend on the
     other sequences in its batch.
 
+With ``conv=(channels, taps)`` a slot also holds the last inputs of the short
+convolution before the recurrence (gdn3/gdn3_upgrade.py:760-762), which
+``convolve`` continues for single tokens, equal prompts and packed rows of unlike
+lengths.
+
 ``step`` advances one token for a batch whose rows name their slots (-1: an
 empty row, y = 0); sequences join and leave without moving states.  The
 arithmetic is the HIP kernels'; the pool gathers and scatters of a prefill
@@ -29,6 +34,7 @@ from __future__ import annotations
 
 import torch
 
+from . import conv as _conv
 from . import gdn3, ops
 
 KINDS = ("dense", "chan", "gdn3")
@@ -37,7 +43,7 @@ KINDS = ("dense", "chan", "gdn3")
 class DecodeStateCache:
     def __init__(self, n_slots: int, H: int, M: int, D: int, device="cuda", kind: str = "dense", *,
                  R: int = 4, P: int = 16, factors=None, slow_decay: float = 0.97, compact_every=None,
-                 compact_mode: str = "svd"):
+                 compact_mode: str = "svd", conv=None, conv_dtype=torch.bfloat16):
         if kind not in KINDS:
             raise ValueError(f"kind must be one of {KINDS}, got {kind!r}")
         if kind == "chan" and M != 1:
@@ -62,6 +68,10 @@ class DecodeStateCache:
             self.pos = [0] * n_slots          # tokens each slot has seen
         else:
             self.pool = torch.zeros(n_slots, H, M, D, D, dtype=torch.float32, device=self.device)
+        self.conv_pool = None
+        if conv is not None:
+            channels, taps = conv
+            self.conv_pool = torch.zeros(n_slots, taps - 1, channels, dtype=conv_dtype, device=self.device)
 
     # ---- slots ----
     def alloc(self, n: int = 1) -> list:
@@ -93,6 +103,8 @@ class DecodeStateCache:
                 self.pos[s] = 0
         else:
             self.pool.index_fill_(0, idx, 0.0)
+        if self.conv_pool is not None:
+            self.conv_pool.index_fill_(0, idx, 0.0)
 
     def state(self, slot: int):
         """The state of one slot (views): S [H, M, D, D], or (A, B, U, Vb)
@@ -187,3 +199,23 @@ class DecodeStateCache:
         return ops.delta_decode_step_slots(q.contiguous(), k.contiguous(), v.contiguous(), a_e.float().contiguous(),
                                            a_w.float().contiguous(), log_g.float().contiguous(), self.pool, st,
                                            out=out)
+
+    def convolve(self, slots, x, weight, bias=None, *, offsets=None, activation="silu", out=None):
+        """The short convolution (``conv.causal_conv_packed``) of the rows' next
+        tokens, continuing and advancing the inputs that the slots hold (-1: an
+        empty row, y = 0): x [n,C] one token a row, [n,T,C] T of each, or with
+        offsets (int32 [n+1], on the device) packed rows [N,C].  Returns y in x's shape."""
+        if self.conv_pool is None:
+            raise ValueError("the cache was made without a convolution (conv=(channels, taps))")
+        st, n = self._slot_tensor(slots), len(slots)
+        if offsets is not None:
+            return _conv.causal_conv_packed(x, offsets, self.conv_pool, weight, bias, slots=st, activation=activation,
+                                            out=out)
+        if x.shape[0] != n:
+            raise ValueError(f"{x.shape[0]} rows for {n} slots")
+        if x.dim() == 2:
+            return _conv.causal_conv_step(x, self.conv_pool, weight, bias, slots=st, activation=activation, out=out)
+        offsets = torch.arange(n + 1, dtype=torch.int32, device=self.device) * x.shape[1]
+        y = _conv.causal_conv_packed(x.reshape(-1, x.shape[-1]), offsets, self.conv_pool, weight, bias, slots=st,
+                                     activation=activation, out=None if out is None else out.view(-1, x.shape[-1]))
+        return y.view(x.shape)

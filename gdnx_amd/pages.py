@@ -101,8 +101,8 @@ def pages_reserve_packed(table, lengths, refs, slots, n_new, page: int, status, 
     none) of every row slots[i] (outside the table: an empty row), whose
     lengths grow by as much, and the packed batch that these tokens make.
     tokens: the batch's size, which may be more than the rows' tokens (those
-    behind the last row's are nobody's).  If the pool or a table row is too
-    small for any of them, or the batch is, nothing changes, all offsets are 0,
+    behind the last row's are nobody's).  No row may be named twice.  If the pool
+    or a table row is too small for any of them, or the batch is, nothing changes, all offsets are 0,
     start, positions and places -1, and status (int32 [2]) holds the pages
     missing and the rows that do not fit."""
     rows, width, n_pages = _state(table, lengths, refs)

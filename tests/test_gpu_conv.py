@@ -262,3 +262,41 @@ def test_graph_and_other_stream(gpu_lib):
         want = step(pools[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(*pools), turn
+
+
+@pytest.mark.parametrize("C", [4096, 37])
+def test_more_than_2_to_the_31_elements(gpu_lib, C):
+    """Forward, backward and a packed call whose last rows lie beyond 32-bit offsets, against the same rows alone."""
+    T, W = (1 << 31) // C + 1000, 4
+    x = torch.zeros(1, T, C, dtype=torch.bfloat16, device=DEV)
+    tail = torch.randn(1, 300, C, device=DEV).bfloat16()
+    x[:, -300:] = tail
+    w = torch.randn(C, W, device=DEV)
+    x.requires_grad_(True)
+    y = conv.causal_conv(x, w)
+    dy = torch.zeros_like(y)
+    dy[:, -300:] = torch.randn(1, 300, C, device=DEV).bfloat16()
+    dx, = torch.autograd.grad(y, x, dy)
+    small = tail.clone().requires_grad_(True)
+    ys = conv.causal_conv(small, w)
+    dxs, = torch.autograd.grad(ys, small, dy[:, -300:].contiguous())
+    assert torch.equal(y[:, -300:], ys) and torch.equal(dx[:, -300:], dxs) and not dx[:, -400:-303].any()
+    del dx, dy, y
+    pool = torch.zeros(3, W - 1, C, dtype=torch.bfloat16, device=DEV)
+    off = torch.tensor([0, 5, T - 200, T], dtype=torch.int32, device=DEV)
+    y = conv.causal_conv_packed(x.detach()[0], off, pool, w)
+    assert torch.equal(y[T - 300:T - 200], ys[0, :100])
+    assert torch.equal(y[T - 200:], conv.causal_conv(tail[:, 100:], w)[0]) and torch.equal(pool[2], tail[0, -3:])
+
+
+def test_refuses_what_it_has_no_derivative_for(gpu_lib):
+    x, w = torch.randn(1, 5, 8, device=DEV, requires_grad=True), torch.randn(8, 4, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError, match="the convolution has no forward-mode derivative"):
+            conv.causal_conv(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()), w)
+    g, = torch.autograd.grad(conv.causal_conv(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+    with pytest.raises(ValueError, match="and not x"):
+        p = torch.zeros(5, 3, 8, device=DEV)
+        conv.causal_conv_step(x.detach()[0], p, w, out=x.detach()[0])

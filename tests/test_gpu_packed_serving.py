@@ -1,0 +1,52 @@
+"""The operators of a packed step together: the example, and the convolution of a decode-state cache."""
+import importlib.util
+import os
+import sys
+
+import pytest
+import torch
+
+from gdnx_amd import conv
+from gdnx_amd.decode_cache import DecodeStateCache
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_packed_serving_example(gpu_lib):
+    spec = importlib.util.spec_from_file_location("packed_serving", os.path.join(ROOT, "examples", "packed_serving.py"))
+    ex = importlib.util.module_from_spec(spec)
+    try:
+        spec.loader.exec_module(ex)
+    finally:
+        sys.path.remove(os.path.join(ROOT, "examples"))
+    # bf16 layers: each rounds its output once (2e-3 relative) and the served form sums in another order
+    assert ex.main(lengths=(90, 17, 130), piece=32, steps=9) < 1e-2
+
+
+@pytest.mark.parametrize("kind,M", [("dense", 1), ("gdn3", 2)])
+def test_cache_convolution(gpu_lib, kind, M):
+    """Equal prompts, packed pieces and single tokens continue one another; slots come back empty."""
+    n, C, W, T = 3, 40, 4, 12
+    x, w = torch.randn(n, T, C, device="cuda").bfloat16(), torch.randn(C, W, device="cuda")
+    b = torch.randn(C, device="cuda")
+    whole = conv.causal_conv(x, w, b)
+    cache = DecodeStateCache(5, 2, M, 64, kind=kind, conv=(C, W))
+    slots = cache.alloc(n)[::-1]
+    got = [cache.convolve(slots, x[:, :5], w, b)]
+    off = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda")
+    got.append(cache.convolve(slots, x[:, 5:7].reshape(-1, C), w, b, offsets=off).view(n, 2, C))
+    for t in range(7, T):
+        got.append(cache.convolve(slots, x[:, t], w, b)[:, None])
+    assert torch.equal(torch.cat(got, 1), whole)
+    assert (cache.convolve([slots[0], -1], x[:2, 0], w, b)[1] == 0).all()
+    assert (cache.conv_pool[slots] != 0).any()
+    cache.free(slots)
+    cache.alloc(5)
+    assert (cache.conv_pool == 0).all()
+    with pytest.raises(ValueError, match="twice"):
+        cache.convolve([1, 1], x[:2, 0], w, b)
+    with pytest.raises(ValueError, match="rows for"):
+        cache.convolve([1, 2], x[:, 0], w, b)
+    with pytest.raises(ValueError, match="without a convolution"):
+        DecodeStateCache(2, 1, 1, 64).convolve([0], x[:1, 0], w, b)
