@@ -252,8 +252,8 @@ def paged_attention_chunk(q, k_pages, v_pages, table, lengths, offsets, *, slots
     if out is None:
         out = torch.empty(N, Hq, D, dtype=dtype, device=dev)
     else:
-        _need(tuple(out.shape) == (N, Hq, D) and out.dtype == dtype and out.is_contiguous() and out.device == dev,
-              "out must be contiguous [N,Hq,D] of q's dtype")
+        _need(tuple(out.shape) == (N, Hq, D) and out.dtype == dtype and out.is_contiguous() and out.device == dev
+              and (N == 0 or out.data_ptr() != q.data_ptr()), "out must be contiguous [N,Hq,D] of q's dtype, and not q")
     if N == 0 or n == 0:
         return out
     q = _rows16(q.unsqueeze(0))

@@ -211,8 +211,8 @@ class DecodeStateCache:
         if offsets is not None:
             return _conv.causal_conv_packed(x, offsets, self.conv_pool, weight, bias, slots=st, activation=activation,
                                             out=out)
-        if x.shape[0] != n:
-            raise ValueError(f"{x.shape[0]} rows for {n} slots")
+        if x.dim() not in (2, 3) or x.shape[0] != n:
+            raise ValueError(f"x must be [n,C] or [n,T,C] (or packed, with offsets): {x.shape[0]} rows for {n} slots")
         if x.dim() == 2:
             return _conv.causal_conv_step(x, self.conv_pool, weight, bias, slots=st, activation=activation, out=out)
         offsets = torch.arange(n + 1, dtype=torch.int32, device=self.device) * x.shape[1]

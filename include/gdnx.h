@@ -757,7 +757,7 @@ int gdnx_pages_write_packed(const void* k_new, const void* v_new, void* k_pages,
  * all tokens of a row whose length does not fit the table.
  * A key or value that is not finite reaches only the tokens that see it.
  * q [N,Hq,D] with element strides (token, head) that are multiples of 16
- * bytes, y [N,Hq,D] contiguous; pages, table and lengths as
+ * bytes, y [N,Hq,D] contiguous and not q's memory; pages, table and lengths as
  * gdnx_paged_attn_step.  workspace: gdnx_chunk_attn_workspace_bytes bytes (-1 if
  * the sizes are invalid; null where that is 0). */
 long long gdnx_chunk_attn_workspace_bytes(int N, int n, int width, int page, int Hq, int Hkv, int head_dim, int window,

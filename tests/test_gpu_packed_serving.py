@@ -6,7 +6,7 @@ import sys
 import pytest
 import torch
 
-from gdnx_amd import conv
+from gdnx_amd import attention, conv
 from gdnx_amd.decode_cache import DecodeStateCache
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +50,19 @@ def test_cache_convolution(gpu_lib, kind, M):
         cache.convolve([1, 2], x[:, 0], w, b)
     with pytest.raises(ValueError, match="without a convolution"):
         DecodeStateCache(2, 1, 1, 64).convolve([0], x[:1, 0], w, b)
+
+
+def test_refuses_what_would_be_read_wrongly(gpu_lib):
+    """Heads beside the channels of a prompt; attention over its own queries' memory."""
+    cache = DecodeStateCache(3, 1, 1, 64, conv=(64, 4))
+    x, w = torch.randn(2, 5, 3, 64, device="cuda").bfloat16(), torch.randn(64, 4, device="cuda")
+    before = cache.conv_pool.clone()
+    with pytest.raises(ValueError, match="x must be"):
+        cache.convolve([0, 1], x, w)
+    assert torch.equal(cache.conv_pool, before)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, pool = torch.randn(4, 1, 64, device="cuda").bfloat16(), torch.zeros(2, 1, 16, 64, device="cuda").bfloat16()
+    kept = q.clone()
+    with pytest.raises(ValueError, match="and not q"):
+        attention.paged_attention_chunk(q, pool, pool, i32([[0]]), i32([4]), i32([0, 4]), out=q)
+    assert torch.equal(q, kept)
