@@ -4,7 +4,11 @@
 // waves take in turn, a tile of 32 (16 in float32) each, straight to registers
 // as the served step does (attn_paged.hip): bound by memory, each visible key and
 // value is read once for all pairs.  Spans of long rows are joined by a second
-// kernel, in order.
+// kernel, in order.  Few rows wait for one lookup after the other (offsets and
+// slot, length, page, keys), so queries are asked for after the first page and masks
+// are formed where a tile needs them: 8 rows of 5 tokens on up to 2000, 16/4 heads,
+// 13.3 us (16.2 with every tile masked and rescaled, and the waves' join by
+// straight rows in LDS).
 #pragma once
 #include "attn_chunk.hpp"
 #include "attn_paged.hpp"
@@ -30,9 +34,9 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
   const int span = w % a.spans; w /= a.spans;
   const int hk = w % a.Hkv, i = w / a.Hkv;
   const int first = packed_offset(a.offsets, i, a.N), count = packed_offset(a.offsets, i + 1, a.N) - first;
-  if (count <= 0 || (long long)count * G > a.short_rows) return;
-  ChunkSeq s;
+  ChunkSeq s;                                                     // (looked up beside the offsets, not after them)
   s.find(a, i, first, count);
+  if (count <= 0 || (long long)count * G > a.short_rows) return;
   const ChunkSeen see(a, s);
   const int rows = count * G, blocks = (rows + 15) / 16;
   const int tiles = (see.nvis + BT - 1) / BT, parts = chunk_spans(tiles, a.spans);
@@ -55,6 +59,9 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
   const long long rowb = D * (int)sizeof(CT), headb = rowb << a.page_log;
   const int per = (tiles + parts - 1) / parts, t0 = span * per, t1 = min(tiles, t0 + per);
 
+  const auto page_of = [&](int x) { return x < see.nvis ? table[see.key(x) >> a.page_log] : -1; };
+  int t = t0 + wave;
+  int pg = t < t1 && lane < BT ? page_of(t * BT + lane) : -1;
   Frag qf[NB][NKS];
   int pos[NB];
 #pragma unroll
@@ -67,9 +74,9 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
     for (int c = 0; c < NKS; ++c) {
       if (there) qf[b][c] = *(const Frag*)((const CT*)a.q + (first + qi) * a.qs[0] + h * a.qs[1] + (4 * c + g) * EPU);
       else qf[b][c] = Frag{};
+      if (a.scale < 0.f) qf[b][c] = -qf[b][c];
     }
   }
-  const auto page_of = [&](int x) { return x < see.nvis ? table[see.key(x) >> a.page_log] : -1; };
   Frag kr[NU][NKS];
   u32x4 vr[NV];
   bool live[NU];                       // whether the lane's keys of the tile are there
@@ -100,7 +107,7 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
     }
   };
 
-  const float sc = a.scale * kLog2e;
+  const float size = fabsf(a.scale) * kLog2e, sc = size < 1e-30f ? 1e-30f : size;      // (no number stays none)
   f32x4 o[NB][NT];
   float m[NB], l[NB];
 #pragma unroll
@@ -110,9 +117,8 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
     m[b] = -INFINITY;
     l[b] = 0.f;
   }
-  int t = t0 + wave;
-  if (t < t1) load(t, lane < BT ? page_of(t * BT + lane) : -1);
-  int pg = t + 4 < t1 && lane < BT ? page_of((t + 4) * BT + lane) : -1;
+  if (t < t1) load(t, pg);
+  pg = t + 4 < t1 && lane < BT ? page_of((t + 4) * BT + lane) : -1;
   for (; t < t1; t += 4) {
     f32x4 sx[NB][NU];
 #pragma unroll
@@ -128,19 +134,24 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
     wave_lds_sync();
 #pragma unroll
     for (int i = 0; i < NV; ++i) *(u32x4*)((char*)stage + (i * 64 + lane) * 16) = vr[i];
-    // which keys of the lane's accumulator rows are seen: lane 4 g + e has key 16 u + 4 g + e
-    // (a single token sees all that are there)
+    // whether all the tokens see all of the tile (a single one what is there); else which keys of the lane's
+    // accumulator rows are seen: lane 4 g + e has key 16 u + 4 g + e
+    const int k0 = see.key(t * BT), k1 = see.key(t * BT + BT - 1);
+    bool all = count == 1 || (k1 <= s.off && (s.off + count - 1 - k0 < a.window || k1 < a.sinks));
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const unsigned long long lv = __ballot(live[u]) >> (4 * g);
+    for (int u = 0; u < NU; ++u) all = all && __all(live[u]);
+    if (!all) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = see.key(t * BT + 16 * u + 4 * g + e);
+      for (int u = 0; u < NU; ++u) {
+        const unsigned long long lv = __ballot(live[u]) >> (4 * g);
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-          if (b < blocks)
-            sx[b][u][e] = (lv >> e & 1) && (count == 1 || attn_visible(pos[b], j, a.window, a.sinks)) ? sx[b][u][e] * sc
-                                                                                                       : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const int j = see.key(t * BT + 16 * u + 4 * g + e);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            if (b < blocks)
+              sx[b][u][e] = (lv >> e & 1) && (count == 1 || attn_visible(pos[b], j, a.window, a.sinks)) ? sx[b][u][e] : -INFINITY;
+        }
       }
     }
     if (t + 4 < t1) {
@@ -148,7 +159,6 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
       pg = t + 8 < t1 && lane < BT ? page_of((t + 8) * BT + lane) : -1;
     }
     Frag pf[NB], pr[NB];                 // P, and what rounding it to bf16 leaves over
-    float f[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
       if (b < blocks) {
@@ -158,19 +168,22 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sx[b][u][e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[b], mx), ms = mn == -INFINITY ? 0.f : mn;
-        f[b] = __builtin_amdgcn_exp2f(m[b] - ms);
-        float sum = 0.f;
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sc;
+        if (__any(mx > m[b] + 8.f)) {        // (raised by steps of 2^8)
+          const float mn = fmaxf(m[b], mx), f = __builtin_amdgcn_exp2f(m[b] - (mn == -INFINITY ? 0.f : mn));
+          m[b] = mn;
+          l[b] *= f;
+#pragma unroll
+          for (int c = 0; c < NT; ++c) o[b][c] *= f;
+        }
+        const float ms = m[b] == -INFINITY ? 0.f : m[b];
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            sx[b][u][e] = __builtin_amdgcn_exp2f(sx[b][u][e] - ms);
-            sum += sx[b][u][e];
+            sx[b][u][e] = __builtin_amdgcn_exp2f(fmaf(sx[b][u][e], sc, -ms));
+            l[b] += sx[b][u][e];
           }
-        l[b] = l[b] * f[b] + sum;
-        m[b] = mn;
         pf[b] = acc_frag((CT*)nullptr, sx[b][0], sx[b][NU - 1]);
         if constexpr (sizeof(CT) == 2) {
 #pragma unroll
@@ -187,7 +200,6 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
 #pragma unroll
       for (int b = 0; b < NB; ++b)
         if (b < blocks) {
-          o[b][c] *= f[b];
           mma(o[b][c], vf, pf[b]);
           if constexpr (sizeof(CT) == 2) mma(o[b][c], vf, pr[b]);
         }
@@ -206,12 +218,12 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
       }
     }
   wave_lds_sync();
-  float* so = (float*)buf(wave);
+  float* so = (float*)buf(wave);         // a row's 16-byte units by an xor, so that 16 rows are stored without a bank conflict
 #pragma unroll
   for (int b = 0; b < NB; ++b)
     if (b < blocks) {
 #pragma unroll
-      for (int c = 0; c < NT; ++c) *(f32x4*)&so[(16 * b + n) * D + 16 * c + 4 * g] = o[b][c];
+      for (int c = 0; c < NT; ++c) *(f32x4*)&so[(16 * b + n) * D + 4 * ((4 * c + g) ^ n)] = o[b][c];
     }
   __syncthreads();
   for (int u = tid; u < rows * (D / 4); u += 256) {
@@ -226,7 +238,7 @@ __device__ __forceinline__ void chunk_short(const ChunkAttnArgs& a, int w, const
     for (int v = 0; v < 4; ++v) {
       const float f = __builtin_amdgcn_exp2f(sh.m[v][q] - ms);
       ll += sh.l[v][q] * f;
-      acc += *(const f32x4*)&((const float*)buf(v))[q * D + d] * f;
+      acc += *(const f32x4*)&((const float*)buf(v))[q * D + (d ^ 4 * (q & 15))] * f;
     }
     if (fmaf(acc[0], 0.f, fmaf(acc[1], 0.f, fmaf(acc[2], 0.f, acc[3] * 0.f))) != 0.f) atomicOr(&sh.bad, 1u << q);
     int qi, h;
