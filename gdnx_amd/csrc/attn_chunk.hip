@@ -56,9 +56,12 @@ template <int D> __device__ __forceinline__ void chunk_long_f32(const ChunkAttnA
   {
     const float* qp = (const float*)a.q + (first + (p >= 0 ? qi : 0)) * a.qs[0] + (p >= 0 ? qh : 0) * a.qs[1];
 #pragma unroll
-    for (int c = 0; c < T::NS; ++c) qf[c] = *(const f32x4*)(qp + 16 * c + 4 * g);
+    for (int c = 0; c < T::NS; ++c) {
+      qf[c] = *(const f32x4*)(qp + 16 * c + 4 * g);
+      if (a.scale < 0.f) qf[c] = -qf[c];
+    }
   }
-  const float sc = a.scale * kLog2e;
+  const float size = fabsf(a.scale) * kLog2e, sc = size < 1e-30f ? 1e-30f : size;      // (no number stays none)
   F32Stage<D> st(tid);
   // the page of key j0 + lane of a tile, and (there) which of its 32 keys have one
   const auto page_at = [&](int it) { return table[min(kt.start(min(it, t1 - 1)) + (lane & 31), len - 1) >> a.page_log]; };
@@ -93,40 +96,46 @@ template <int D> __device__ __forceinline__ void chunk_long_f32(const ChunkAttnA
     pg = page_at(it + 2);
     if (wv0 <= wv1 && j0 <= wv1 && (j0 + 31 > wv0 - a.window || j0 < a.sinks)) {
       const bool all = rows_ok && j0 + 31 <= wv0 && (wv1 - j0 < a.window || j0 + 32 <= a.sinks) && there == ~0u;
-      const unsigned lv = there >> (4 * g);
       f32x4 s[2];
+      s[0] = s[1] = zero4();
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = zero4();
+      for (int c = 0; c < T::NS; ++c)
 #pragma unroll
-        for (int c = 0; c < T::NS; ++c) mma(s[u], ld_frag(sk + (16 * u + n) * T::LD + 16 * c, g), qf[c]);
+        for (int u = 0; u < 2; ++u) mma(s[u], ld_frag(sk + (16 * u + n) * T::LD + 16 * c, g), qf[c]);
+      if (!all) {
+        const int d = p - j0 - 4 * g, ds = a.sinks - j0 - 4 * g;
+        const unsigned lv = there >> (4 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s[u][e] = all || ((lv >> (16 * u + e) & 1) && attn_visible(p, j0 + 16 * u + 4 * g + e, a.window, a.sinks))
-                        ? s[u][e] * sc : -INFINITY;
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = 16 * u + e;
+            s[u][e] = (c <= d) & ((d - c < a.window) | (c < ds)) & (lv >> c & 1) ? s[u][e] : -INFINITY;
+          }
       }
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                        fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
-      const float f = exp2f(m - ms);
-      float sum = 0.f;
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sc;
+      if (__any(mx > m + 8.f)) {             // (raised by steps of 2^8)
+        const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < T::NS; ++t) o[t] *= f;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[u][e] = exp2f(s[u][e] - ms);
-          sum += s[u][e];
+          s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], sc, -ms));
+          l += s[u][e];
         }
-      l = l * f + sum;
-      m = mn;
 #pragma unroll
-      for (int t = 0; t < T::NS; ++t) {
-        o[t] *= f;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) mma(o[t], ld_cols<T::LD>(sv, 16 * u, 16 * t + n, g), s[u]);
-      }
+        for (int t = 0; t < T::NS; ++t) mma(o[t], ld_cols<T::LD>(sv, 16 * u, 16 * t + n, g), s[u]);
     }
     float* next = smem + ((it - t0 + 1) & 1) * 2 * T::WORDS;
     st.store(next, next + T::WORDS);
@@ -310,6 +319,10 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
     long long parts = (a.n == 1 ? 512 : 1024) / (tiles ? tiles : 1);
     if (parts > 4096 / ((long long)a.items * a.Hkv)) parts = 4096 / ((long long)a.items * a.Hkv);
     a.least = tiles > 192 ? 8 : 4;
+#ifdef LEASTF
+    if (a.dtype != GDNX_DTYPE_BF16) a.least = LEASTF;
+#endif
+
     if (parts > span / (R / 2) / a.least) parts = span / (R / 2) / a.least;
     a.parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
     a.join_split = (long long)a.items * a.Hkv >= 256 ? 4 : (int)(R * a.D / 1024);      // workgroups an item
