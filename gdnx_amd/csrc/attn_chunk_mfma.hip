@@ -11,36 +11,28 @@ namespace {
 // from the table): lane x holds the page of key j0 + x, or of the last one.  An
 // instruction fills `ROWS` tokens, which lie in one page where it has so many:
 // its place is then a scalar, 32-bit offsets are the lanes'.  (By lane
-// exchanges throughout, 2048 tokens on 30001 in pages of 16 took 767 us, of 128 673.)
-template <int D> struct PagedTileLoad {
+// exchanges throughout, as SMALL pages need it, 2048 tokens on 30001 took 673 us;
+// 580 with scalar places, 555 with the matrix instructions' priority below.)
+template <int D, bool SMALL> struct PagedTileLoad {
   using T = Tile<D>;
   static constexpr int N = 64 * T::UPR / 256, STEP = 256 / T::UPR, ROWS = 64 / T::UPR;
   unsigned row, u;
-  int wave, log;
-  __device__ __forceinline__ PagedTileLoad(int tid, int wave_, int log_) : row(tid / T::UPR), wave(wave_), log(log_) {
+  int wave, mask;
+  __device__ __forceinline__ PagedTileLoad(int tid, int wave_, int log) : row(tid / T::UPR), wave(wave_), mask((1 << log) - 1) {
     u = ((tid % T::UPR) ^ T::swz(row)) * 16;
   }
-  __device__ __forceinline__ void load(char* tk, const char* k, char* tv, const char* v, long long page_bytes, int pg, int j0,
-                                       int last) const {
+  __device__ __forceinline__ void load(char* tk, const char* k, char* tv, const char* v, long long page, int j0, int last) const {
     typedef __attribute__((address_space(1))) void* G;
     typedef __attribute__((address_space(3))) void* L;
-    const int mask = (1 << log) - 1;
-    if (1 << log >= ROWS) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const long long at = __builtin_amdgcn_readlane(pg, i * STEP + wave * ROWS) * page_bytes;
-        const unsigned in = ((j0 + min((int)row + i * STEP, last)) & mask) * T::RB + u;
-        __builtin_amdgcn_global_load_lds((G)(k + at + in), (L)(tk + i * 4096 + wave * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((G)(v + at + in), (L)(tv + i * 4096 + wave * 1024), 16, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = min((int)row + i * STEP, last);
-        const long long at = __shfl(pg, r) * page_bytes + (((j0 + r) & mask) * T::RB + u);
-        __builtin_amdgcn_global_load_lds((G)(k + at), (L)(tk + i * 4096 + wave * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((G)(v + at), (L)(tv + i * 4096 + wave * 1024), 16, 0, 0);
-      }
+    for (int i = 0; i < N; ++i) {
+      const int r = min((int)row + i * STEP, last), x = i * STEP + wave * ROWS;
+      const unsigned in = ((j0 + r) & mask) * T::RB + u;
+      long long at;
+      if constexpr (SMALL) at = __shfl(page, r);
+      else at = (long long)__builtin_amdgcn_readlane((int)(page >> 32), x) << 32 | (unsigned)__builtin_amdgcn_readlane((int)page, x);
+      __builtin_amdgcn_global_load_lds((G)(k + at + in), (L)(tk + i * 4096 + wave * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((G)(v + at + in), (L)(tv + i * 4096 + wave * 1024), 16, 0, 0);
     }
   }
 };
@@ -53,7 +45,7 @@ template <int D> struct PagedTileLoad {
 // form of win_fwd_bf16_kernel (attn_win_mfma.hip): S^T = K Q^T, a lane holding 32
 // scores of one row; O^T += V^T P^T.  The page of a tile's keys is looked up
 // two tiles ahead.
-template <int D>
+template <int D, bool SMALL>
 __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64 * Tile<D>::RB], char (&v0)[64 * Tile<D>::RB],
                                            char (&k1)[64 * Tile<D>::RB], char (&v1)[64 * Tile<D>::RB]) {
   using T = Tile<D>;
@@ -106,13 +98,13 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
   float m = -INFINITY, l = 0.f;
 
   const LaneMap<D> lm(lane);
-  const PagedTileLoad<D> tl(tid, wave, a.page_log);
+  const PagedTileLoad<D, SMALL> tl(tid, wave, a.page_log);
   const auto page_at = [&](int it) { return table[min(kt.start(min(it, t1 - 1)) + lane, len - 1) >> a.page_log]; };
   // asks for a tile; which of its keys are there
   const auto load = [&](char* tk, char* tv, int it, int pg) {
     const int j0 = kt.start(min(it, t1 - 1));
     const bool there = pg >= 0 && pg < a.n_pages;
-    tl.load(tk, kb, tv, vb, page_bytes, there ? pg : 0, j0, len - 1 - j0);
+    tl.load(tk, kb, tv, vb, (there ? pg : 0) * page_bytes, j0, len - 1 - j0);
     return __ballot(there);
   };
   const auto tile_step = [&](const char* tk, const char* tv, int it, unsigned long long there) {
@@ -120,6 +112,10 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
     // whether the wave sees anything of the tile, and all of it
     const bool some = it < t1 && wv0 <= wv1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
     if (!some) return;
+    // Matrix instructions go before the other wave's vector instructions, and a tile's exponentials are through before its
+    // second products, so that the two waves of a SIMD take turns: 2048 tokens on 30001 582 -> 555 us, 1024 on 8192
+    // 92 -> 90, 8192 on 8192 777 -> 774, 4096 on none 97 -> 102 (16/4 heads, d = 128).
+    __builtin_amdgcn_s_setprio(1);
     const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks) && there == ~0ULL;
     f32x16 s[2];
     s[0] = s[1] = zero16();
@@ -140,6 +136,7 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     if (!all) {
       const int d = p - j0 - 4 * h, ds = a.sinks - j0 - 4 * h;
       const unsigned long long lv = there >> (4 * h);
@@ -174,6 +171,9 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
         sum += s[u][e];
       }
     l += sum;
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -182,6 +182,8 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
 #pragma unroll
         for (int t = 0; t < T::ND; ++t) mma32(o[t], lm.cols(tv + (32 * u + 16 * c) * T::RB, t), pf);
       }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
   };
   if (t0 < t1) {
     unsigned long long there0 = load(k0, v0, t0, page_at(t0)), there1;
@@ -248,20 +250,26 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
   if (__syncthreads_or(redo != 0) && redo) chunk_redo<bf16, D, BK, 32>(redo);
 }
 
-template <int D> __global__ void __launch_bounds__(256, 2) chunk_bf16_kernel(ChunkAttnArgs a) {
+template <int D, bool SMALL> __global__ void __launch_bounds__(256, 2) chunk_bf16_kernel(ChunkAttnArgs a) {
   constexpr int BYTES = 64 * Tile<D>::RB;
   // two buffers of K and V, each a variable of its own: what is read from one
   // then does not wait for the loads into the other
   __shared__ __attribute__((aligned(16))) char k0[BYTES], v0[BYTES], k1[BYTES], v1[BYTES];
   __shared__ ChunkShortShared<bf16> sh;
   const int n_long = a.items * a.parts * a.Hkv;
-  if ((int)blockIdx.x < n_long) chunk_long<D>(a, k0, v0, k1, v1);
+  if ((int)blockIdx.x < n_long) chunk_long<D, SMALL>(a, k0, v0, k1, v1);
   else chunk_short<bf16, D>(a, blockIdx.x - n_long, [&](int v) { return v == 0 ? k0 : v == 1 ? v0 : v == 2 ? k1 : v1; }, sh);
 }
 
+template <int D> static void launch(const ChunkAttnArgs& a, unsigned groups, hipStream_t stream) {
+  if (1 << a.page_log < PagedTileLoad<D, false>::ROWS)
+    hipLaunchKernelGGL((chunk_bf16_kernel<D, true>), dim3(groups), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((chunk_bf16_kernel<D, false>), dim3(groups), dim3(256), 0, stream, a);
+}
+
 int chunk_bf16_launch(const ChunkAttnArgs& a, unsigned groups, hipStream_t stream) {
-  if (a.D == 128) hipLaunchKernelGGL((chunk_bf16_kernel<128>), dim3(groups), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((chunk_bf16_kernel<64>), dim3(groups), dim3(256), 0, stream, a);
+  if (a.D == 128) launch<128>(a, groups, stream);
+  else launch<64>(a, groups, stream);
   return check_launch("chunk_bf16_kernel");
 }
 
