@@ -296,12 +296,12 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
 //
 // Long rows' keys are cut into parts where the tiles do not give every CU its
 // two workgroups (one row), or twice that (several, whose lengths differ, so that
-// parts level out: three pieces of 1024 on up to 8192 tokens 255 us uncut, 187
-// in two, 202 in three), but into no more than 4096 workgroups, most of which have
+// parts level out: three pieces up to 1024 on up to 8192 tokens 265 us with the join uncut,
+// 220 in two, 200 in three, 204 in four), but into no more than 4096 workgroups, most of which have
 // no work where rows are short (256 single tokens: 418 us, with 11600 of them, 402).
-// A part has four tiles at least, eight where the tiles are many already; in us,
-// eight / four: 8 x 9 tokens on 2000, 16/4 heads, 30.6 / 20.7; 12 float32 rows with a
-// window of 512 27.8 / 17.5; 4 x 512 on 500 43.9 / 48.8.
+// A part has four tiles at least, eight where the tiles are many already; in us with the
+// join, eight / four: 8 x 9 tokens on 2000, 16/4 heads, 37 / 25; 12 float32 rows with a
+// window of 512 29 / 21; 4 x 512 on 500 46 / 50.
 void chunk_attn_plan(ChunkAttnArgs& a) {
   const long long G = a.Hq / a.Hkv, R = a.dtype == GDNX_DTYPE_BF16 ? 128 : 64, pairs = a.N * G;
   long long keys = (long long)a.width << a.page_log;
