@@ -319,7 +319,6 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
     long long parts = (a.n == 1 ? 512 : 1024) / (tiles ? tiles : 1);
     if (parts > 4096 / ((long long)a.items * a.Hkv)) parts = 4096 / ((long long)a.items * a.Hkv);
     a.least = tiles > 192 ? 8 : 4;
-
     if (parts > span / (R / 2) / a.least) parts = span / (R / 2) / a.least;
     a.parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
     a.join_split = (long long)a.items * a.Hkv >= 256 ? 4 : (int)(R * a.D / 1024);      // workgroups an item
