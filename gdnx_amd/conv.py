@@ -106,7 +106,9 @@ def causal_conv(x, weight, bias=None, *, activation="silu", state=None, lengths=
     or beyond a row's length are padding, whatever they hold; their outputs
     and gradients are zero.  Returns y [B,T,C], with return_state also the last
     W - 1 inputs before each row's end [B,W-1,C].  There is no forward-mode
-    derivative and no second one."""
+    derivative and no second one.  A step captured in a HIP graph takes leaves
+    of its own (detached): autograd waits for the stream of an eager graph that
+    still holds the same ones, which a capture does not allow."""
     _no_tangents(x, weight, bias, state, what="the convolution")
     _need(x.is_cuda and x.dim() == 3, "x must be a CUDA (HIP) tensor [B,T,C]")
     _lib.dtype_code(x.dtype)

@@ -66,3 +66,31 @@ def test_refuses_what_would_be_read_wrongly(gpu_lib):
     with pytest.raises(ValueError, match="and not q"):
         attention.paged_attention_chunk(q, pool, pool, i32([[0]]), i32([4]), i32([0, 4]), out=q)
     assert torch.equal(q, kept)
+
+
+def test_calls_on_two_streams_at_once(gpu_lib):
+    """Long and short rows with parts and spans, a training step of the convolution: each call has a workspace of its own."""
+    g = torch.Generator().manual_seed(3)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    kp, vp = (torch.randn(80, 2, 64, 64, generator=g).bfloat16().to("cuda") for _ in range(2))
+    table, off, lens = i32([list(range(40)), list(range(40, 80))]), i32([0, 3, 203]), i32([2500, 2400])
+    qs = [torch.randn(203, 8, 64, generator=g).bfloat16().to("cuda") for _ in range(2)]
+    xs = [torch.randn(2, 400, 256, generator=g).bfloat16().to("cuda") for _ in range(2)]
+    w = torch.randn(256, 4, generator=g).to("cuda")
+    def both(i):
+        y = attention.paged_attention_chunk(qs[i], kp, vp, table, lens, off)
+        x, wl = xs[i].detach().requires_grad_(True), w.detach().requires_grad_(True)
+        z = conv.causal_conv(x, wl)
+        return (y, z.detach(), *torch.autograd.grad(z, (x, wl), xs[1 - i]))
+    want = [both(0), both(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for turn in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(turn, want[i]))
