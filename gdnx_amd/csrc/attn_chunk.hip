@@ -31,9 +31,7 @@ template <int D> __device__ __forceinline__ void chunk_long_f32(const ChunkAttnA
   const ChunkItem item(a, blockIdx.x);
   const int hk = item.hk;
   int si, first, count, tile;
-  if (!row_item(a.offsets, a.n, a.N, G, 64, item.item, lane, &si, &first, &count, &tile)) return;
-  const long long pairs = (long long)count * G;
-  if (pairs <= a.short_rows || tile * 64LL >= pairs) return;
+  if (!chunk_item(a, G, 64, item.item, lane, &si, &first, &count, &tile)) return;
   ChunkSeq sq;
   sq.find(a, si, first, count);
   const int off = sq.off, len = sq.len;
@@ -238,9 +236,7 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
     const int q0 = w % a.join_split * (R / a.join_split) + grp, q1 = q0 - grp + R / a.join_split; w /= a.join_split;
     const int hk = w % a.Hkv;
     int i, first, count, tile;
-    if (!row_item(a.offsets, a.n, a.N, G, R, w / a.Hkv, lane, &i, &first, &count, &tile)) return;
-    const long long pairs = (long long)count * G;
-    if (pairs <= a.short_rows || (long long)tile * R >= pairs) return;
+    if (!chunk_item(a, G, R, w / a.Hkv, lane, &i, &first, &count, &tile)) return;
     s.find(a, i, first, count);
     const RowMap rm(tile * R, G, a.g_magic);
     const KeyTiles<BK> kt(rm.i0 + s.off, min(rm.last(R - 1), count - 1) + s.off, s.len, a.window, a.sinks);
@@ -297,8 +293,8 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
 // Long rows' keys are cut into parts where the tiles do not give every CU its
 // two workgroups (one row), or twice that (several, whose lengths differ, so that
 // parts level out: three pieces up to 1024 on up to 8192 tokens 265 us with the join uncut,
-// 220 in two, 200 in three, 204 in four), but into no more than 4096 workgroups, most of which have
-// no work where rows are short (256 single tokens: 418 us, with 11600 of them, 402).
+// 220 in two, 200 in three, 204 in four), but into no more than 4096 workgroups, many of which have
+// no work where rows are short (256 single tokens, rows by places: 402 us, 418 with 11600 of them).
 // A part has four tiles at least, eight where the tiles are many already; in us with the
 // join, eight / four: 8 x 9 tokens on 2000, 16/4 heads, 37 / 25; 12 float32 rows with a
 // window of 512 29 / 21; 4 x 512 on 500 46 / 50.
@@ -312,9 +308,9 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
   a.parts = a.least = 1;
   a.spans = 0;
   if (pairs > a.short_rows) {
-    a.items = (int)(pairs / R + a.n);
     const long long win = (long long)a.window + a.sinks + R / G + 1, span = win < keys ? win : keys;
     const long long most = pairs / (a.short_rows + 1), rows = a.n < most ? a.n : most;      // long rows there can be
+    a.items = (int)(pairs / R + (a.n > kChunkListed ? a.n : rows));
     const long long tiles = ((pairs + R - 1) / R + (rows - 1) / 2) * a.Hkv;
     long long parts = (a.n == 1 ? 512 : 1024) / (tiles ? tiles : 1);
     if (parts > 4096 / ((long long)a.items * a.Hkv)) parts = 4096 / ((long long)a.items * a.Hkv);

@@ -34,6 +34,49 @@ struct ChunkItem {
   }
 };
 
+// The long row and its tile of T pairs that an item is; false: none.  Up to
+// kChunkListed rows, items are the long rows' tiles one after the other: the
+// wave counts them through, a lane four rows, all asked for at once.  Beyond, row_item's
+// places, most of which are empty where rows are short (61 single tokens on up to 8192:
+// 118 us with the join by places, 111 by the list; 1000 rows on up to 1000, counted in
+// steps of 64, 221, by places 198).
+__device__ __forceinline__ bool chunk_item(const ChunkAttnArgs& a, int G, int T, int item, int lane, int* row, int* first,
+                                           int* count, int* tile) {
+  if (a.n > kChunkListed) {
+    if (!row_item(a.offsets, a.n, a.N, G, T, item, lane, row, first, count, tile)) return false;
+    const long long pairs = (long long)*count * G;
+    return pairs > a.short_rows && (long long)*tile * T < pairs;
+  }
+  int o[5], c[4], t[4], sum = 0;
+#pragma unroll
+  for (int e = 0; e < 5; ++e) o[e] = packed_offset(a.offsets, min(4 * lane + e, a.n), a.N);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    c[e] = max(o[e + 1] - o[e], 0);                  // (none behind the last row)
+    const int pairs = c[e] * G;
+    t[e] = pairs > a.short_rows ? (pairs + T - 1) / T : 0;
+    sum += t[e];
+  }
+  const int end = wave_scan(sum);
+  const unsigned long long behind = __ballot(end > item);
+  if (!behind) return false;
+  const int l = __ffsll(behind) - 1;
+  item -= __builtin_amdgcn_readlane(end - sum, l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int tiles = __builtin_amdgcn_readlane(t[e], l);
+    if (item < tiles) {
+      *row = 4 * l + e;
+      *first = __builtin_amdgcn_readlane(o[e], l);
+      *count = __builtin_amdgcn_readlane(c[e], l);
+      *tile = item;
+      return true;
+    }
+    item -= tiles;
+  }
+  return false;
+}
+
 // Parts that an item of `tiles` key tiles is cut into.
 __device__ __forceinline__ int chunk_parts(const ChunkAttnArgs& a, int tiles) { return max(1, min(a.parts, tiles / a.least)); }
 
@@ -130,7 +173,7 @@ template <typename CT, int D, int BK, int WR> __device__ __forceinline__ void ch
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
   const ChunkItem it(a, w);
   int i, first, count, tile;
-  if (!row_item(a.offsets, a.n, a.N, G, 4 * WR, it.item, lane, &i, &first, &count, &tile)) return;
+  if (!chunk_item(a, G, 4 * WR, it.item, lane, &i, &first, &count, &tile)) return;
   ChunkSeq s;
   s.find(a, i, first, count);
   const RowMap rm(tile * 4 * WR, G, a.g_magic);

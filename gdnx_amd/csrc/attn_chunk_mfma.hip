@@ -56,9 +56,7 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
   const ChunkItem item(a, blockIdx.x);
   const int hk = item.hk;
   int si, first, count, tile;
-  if (!row_item(a.offsets, a.n, a.N, G, 128, item.item, lane, &si, &first, &count, &tile)) return;
-  const long long pairs = (long long)count * G;
-  if (pairs <= a.short_rows || tile * 128LL >= pairs) return;
+  if (!chunk_item(a, G, 128, item.item, lane, &si, &first, &count, &tile)) return;
   ChunkSeq sq;
   sq.find(a, si, first, count);
   const int off = sq.off, len = sq.len;

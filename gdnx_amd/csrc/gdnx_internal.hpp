@@ -544,6 +544,7 @@ struct ChunkAttnArgs {
   int join_share, join_blocks;      // short rows' join: groups of threads a pair, workgroups a row and key head
 };
 constexpr int kChunkShort = 32;      // the most pairs of a short row
+constexpr int kChunkListed = 256;    // the most rows whose long ones are counted through
 __host__ __device__ constexpr int chunk_short_pairs(int value_bytes) { return value_bytes == 2 ? kChunkShort : 16; }
 void chunk_attn_plan(ChunkAttnArgs& a);      // from the sizes: short_rows, items, parts, spans
 int chunk_attn_dispatch(const ChunkAttnArgs& a, hipStream_t stream);

@@ -23,6 +23,25 @@ template <typename F> __device__ __forceinline__ int wave_find(int n, long long 
   return -1;
 }
 
+// x of another lane, 0 where there is none or its row of 16 is not in ROWS.
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ long long dpp(long long x) {
+  return (long long)dpp<CTRL, ROWS>((int)(x >> 32)) << 32 | (unsigned)dpp<CTRL, ROWS>((int)x);
+}
+// Inclusive prefix sum over the wave: within rows of 16, then their last
+// lanes' sums to the rows behind.
+template <typename T> __device__ __forceinline__ T wave_scan(T x) {
+  x += dpp<0x111, 0xf>(x);           // row_shr 1, 2, 4, 8
+  x += dpp<0x112, 0xf>(x);
+  x += dpp<0x114, 0xf>(x);
+  x += dpp<0x118, 0xf>(x);
+  x += dpp<0x142, 0xa>(x);           // row_bcast 15, 31
+  x += dpp<0x143, 0xc>(x);
+  return x;
+}
+
 // Rows cut into tiles of T units, a token being G of them: row i owns the work
 // items from offsets[i] G / T + i on (floor), which are as many as its tiles at
 // least and one for an empty row; N G / T + n items cover every row, whatever

@@ -182,6 +182,18 @@ def test_many_rows(gpu_lib, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [130, 1100])
+def test_long_rows_among_many(gpu_lib, n, dtype):
+    """Long rows first, last and between short and empty ones, of one tile, of several and of a pair more than a tile."""
+    past, counts = [(11 * i) % 40 for i in range(n)], [(0, 1, 2, 1)[i % 4] for i in range(n)]
+    for i, c in ((0, 70), (63, 33), (64, 129), (n // 2, 17), (n - 1, 65)):
+        counts[i] = c
+    b = Batch(past, counts, 4, 2, 64, 16, dtype)
+    close(b.run(), b.want(), dtype)
+    close(b.run(window=20, sinks=2), b.want(window=20, sinks=2), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (50, 3)])
 def test_prompt_in_pieces_is_the_whole(gpu_lib, dtype, window, sinks):
     """Two prompts of unlike lengths taken in by pieces beside each other, against windowed attention over each."""
