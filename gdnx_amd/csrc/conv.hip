@@ -13,9 +13,9 @@
 // Bound by memory and by the vector units, which are busy 63 % of the forward's
 // cycles and 66 % of the backward's (26 instructions a value, its exponential
 // and reciprocal at a quarter of the rate): 4 x 4096 tokens, 6144 channels, bf16 on four
-// taps 83 us forward (402 MB, 4.8 TB/s; a large copy reaches 5.3) and 141
-// backward (604 MB, 4.3 TB/s).  A serving step of 2.8 thousand packed tokens 16 us
-// (70 MB), three single tokens 4.8 us.
+// taps 75 to 83 us forward (402 MB, 4.8 to 5.4 TB/s; a large copy reaches 5.2) and 141
+// backward (604 MB, 4.3 TB/s).  A serving step of 2.4 thousand packed tokens 16 us
+// (64 MB), three single tokens 4.8 us.
 #include <type_traits>
 
 #include "gdnx_internal.hpp"
