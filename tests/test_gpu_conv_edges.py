@@ -1,0 +1,58 @@
+"""The short convolution where its kernels' forms part: every number of taps, lanes on whole and on split channels, packed
+rows with and without an activation, filters of either type; and beside values that are not finite.  Tolerances as in
+test_gpu_conv.py, whose bounds hold for up to eight taps."""
+import pytest
+import torch
+
+from gdnx_amd import conv
+from oracle import conv as oc
+from test_gpu_conv import DEV, check, make, rel, tol
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [
+    # B, T, C, W, lengths: spans of 8 to 64 tokens, whose edges W - 1 tokens reach over
+    (2, 130, 520, 2, [130, 65]),
+    (3, 70, 36, 2, None),
+    (2, 90, 260, 3, [0, 90]),
+    (2, 200, 264, 5, [200, 131]),
+    (2, 140, 136, 6, [140, 9]),
+    (1, 131, 1032, 7, None),
+    (1, 150, 70, 8, [150]),
+    (2, 97, 520, 8, [97, 96]),
+], ids=lambda s: "-".join(map(str, s[:4])))
+def test_every_number_of_taps(gpu_lib, shape, dtype):
+    B, T, C, W, lengths = shape
+    check(make(B, T, C, W, dtype), lengths)
+    check(make(B, T, C, W, dtype, dtype, bias=False, state=False), lengths, silu=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("silu", [True, False])
+@pytest.mark.parametrize("C", [43, 528])
+@pytest.mark.parametrize("W", [2, 3, 4, 5, 6, 7, 8])
+def test_packed_forms(gpu_lib, W, C, silu, dtype):
+    counts = [5, 0, 1, 40, 9, 7, 1]
+    n, N = len(counts), sum(counts)
+    off = [sum(counts[:i]) for i in range(n + 1)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    for wdtype, bias in ((torch.float32, True), (dtype, False)):
+        g = torch.Generator().manual_seed(W)
+        x, pool = torch.randn(N, C, generator=g).to(dtype), torch.randn(2 * n + 1, W - 1, C, generator=g).to(dtype)
+        w, b = torch.randn(C, W, generator=g).to(wdtype), torch.randn(C, generator=g).to(wdtype)
+        slots, to = torch.randperm(2 * n + 1, generator=g).tolist()[:n], None
+        want, wpool = oc.causal_conv_packed(x.double(), off, pool.double(), w.double(), b.double() if bias else None, slots,
+                                            to, silu)
+        p = pool.to(DEV)
+        kw = dict(slots=i32(slots), activation="silu" if silu else None)
+        y = conv.causal_conv_packed(x.to(DEV), i32(off), p, w.to(DEV), b.to(DEV) if bias else None, **kw)
+        assert torch.equal(p.double().cpu(), wpool)
+        assert rel(y, want) <= tol(dtype, 3e-6)
+        # a token a row is the same row by row, bit for bit
+        p1, p2 = pool.to(DEV), pool.to(DEV)
+        args = w.to(DEV), b.to(DEV) if bias else None
+        one = conv.causal_conv_step(x[:n].to(DEV), p1, *args, **kw)
+        assert torch.equal(one, conv.causal_conv_packed(x[:n].to(DEV), i32(list(range(n + 1))), p2, *args, **kw))
+        assert torch.equal(p1, p2)
