@@ -1,0 +1,34 @@
+"""Packed rows over the page cache: values that are not finite in rows of both kinds, whole and cut into parts and spans."""
+import pytest
+import torch
+
+from test_gpu_chunk import DEV, Batch, close
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what,value", [("v", float("nan")), ("v", float("inf")), ("k", float("nan"))])
+@pytest.mark.parametrize("past,counts", [([64, 3], [5, 4]), ([1500, 900], [5, 4]), ([1500, 900], [1, 5]),
+                                         ([1500, 3], [90, 20]), ([1500, 900], [90, 5])],
+                         ids=["short", "spans", "single", "parts", "both"])
+def test_what_is_not_finite_reaches_those_that_see_it(gpu_lib, past, counts, what, value, D, dtype):
+    """Among the cached tokens, the new ones, and where the window leaves it behind between one new token and the next."""
+    for window, sinks, back in ((None, 0, 40), (None, 0, 0), (None, 0, -1), (None, 0, 1 - counts[0]), (24, 2, 22), (24, 2, 30),
+                                (24, 2, past[0] - 1)):
+        at = past[0] - back                                # its position in the first row
+        b = Batch(past, counts, 4, 2, D, 16, dtype)
+        if at >= b.lens[0]:
+            continue
+        plain = b.run(window=window, sinks=sinks)
+        pool = b.vp if what == "v" else b.kp
+        pool[b.table[b.slots[0]][at // 16], 1, at % 16, 5] = value
+        y = b.run(window=window, sinks=sinks)
+        p = torch.arange(past[0], past[0] + counts[0], device=DEV)
+        sees = (at <= p) & ((p - at < (window or 1 << 20)) | (at < sinks))
+        hit = torch.zeros(sum(counts), 4, D, dtype=torch.bool, device=DEV)
+        columns = slice(5, 6) if what == "v" else slice(None)
+        hit[:counts[0]][sees, 2:, columns] = True
+        assert torch.equal(~torch.isfinite(y), hit), (window, back)
+        close(torch.where(hit, plain, y), plain.double().cpu(), dtype)
