@@ -278,9 +278,10 @@ template <typename CT, int W, int V, bool WIDE> __global__ void __launch_bounds_
             du[e] *= s * fmaf(v[e], fmaf(-kLn2 * kLn2, s, kLn2 * kLn2), kLn2);
           }
         }
-      } else {                                   // (behind the row: u may be no number)
+      } else {                                   // (behind the row: nothing, where 0 times a tap or an input may be NaN)
         zero_chan<V>(x[0]);
-        zero_chan<V>(du);
+        zero_chan<V>(acc[0]);
+        return;
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) {

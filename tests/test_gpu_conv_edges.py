@@ -56,3 +56,41 @@ def test_packed_forms(gpu_lib, W, C, silu, dtype):
         one = conv.causal_conv_step(x[:n].to(DEV), p1, *args, **kw)
         assert torch.equal(one, conv.causal_conv_packed(x[:n].to(DEV), i32(list(range(n + 1))), p2, *args, **kw))
         assert torch.equal(p1, p2)
+
+
+def _grads(ins, lengths, silu):
+    leaves = {n: t.to(DEV).requires_grad_(True) for n, t in ins.items()}
+    y, last = conv.causal_conv(leaves["x"], leaves["weight"], leaves["bias"], activation="silu" if silu else None,
+                               state=leaves["state"], lengths=torch.tensor(lengths, dtype=torch.int32, device=DEV),
+                               return_state=True)
+    g = torch.Generator().manual_seed(5)
+    dy, dlast = (torch.randn(t.shape, generator=g).to(t.dtype).to(DEV) for t in (y, last))
+    return dict(zip(leaves, torch.autograd.grad((y, last), list(leaves.values()), (dy, dlast)))), dlast
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("C", [24, 520])
+def test_gradients_take_nothing_from_behind_a_rows_end(gpu_lib, C, dtype):
+    """Beside inputs, states and filters that are not finite: a token behind the end adds nothing, not zero times something."""
+    lengths, end = [40, 0, 21], 21
+    ins = make(3, 40, C, 4, dtype)
+    for silu in (False, True):
+        plain, dlast = _grads(ins, lengths, silu)
+        bad = dict(ins, state=ins["state"].clone())
+        bad["state"][1] = float("nan")                       # of a row without tokens: it is handed on, and that is all
+        got, _ = _grads(bad, lengths, silu)
+        assert all(torch.equal(got[n], plain[n]) for n in plain)
+        assert torch.equal(got["state"][1], dlast[1])
+    plain, _ = _grads(ins, lengths, False)
+    bad = dict(ins, x=ins["x"].clone())
+    bad["x"][2, end - 1] = float("inf")                      # a row's last token meets the newest tap alone
+    got, _ = _grads(bad, lengths, False)
+    assert torch.equal(got["weight"][:, :3], plain["weight"][:, :3]) and not torch.isfinite(got["weight"][:, 3]).any()
+    assert all(torch.equal(got[n], plain[n]) for n in ("x", "bias", "state"))
+    bad = dict(ins, weight=ins["weight"].clone())
+    bad["weight"][:, 0] = float("inf")                       # the oldest tap reaches the tokens W - 1 before another
+    got, _ = _grads(bad, lengths, False)
+    for b, n in enumerate(lengths):
+        assert (got["x"][b, n:] == 0).all()
+        assert torch.equal(got["x"][b, max(n - 3, 0):n], plain["x"][b, max(n - 3, 0):n])
+        assert not torch.isfinite(got["x"][b, :max(n - 3, 0)]).any()
