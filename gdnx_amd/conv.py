@@ -153,8 +153,10 @@ def _packed(x, offsets, n, pool, weight, bias, slots, to_slots, activation, out)
         _need(tuple(out.shape) == (N, C) and out.dtype == x.dtype and out.is_contiguous() and out.device == x.device
               and (N == 0 or out.data_ptr() != x.data_ptr()),
               "out must be contiguous, of x's shape, dtype and device, and not x")
-    if n == 0 or C == 0 or pool.shape[0] == 0:
-        return out.zero_() if pool.shape[0] == 0 else out
+    if n == 0 or C == 0:
+        return out
+    if pool.shape[0] == 0:                              # every row is an empty one, of a pool that is only looked at
+        pool, slots, to_slots = torch.zeros(1, W - 1, C, dtype=x.dtype, device=x.device), torch.full_like(slots, -1), None
     x = _channels(x)
     _lib.call("gdnx_conv_packed", x.device, x.data_ptr(), _addr(offsets), weight.data_ptr(), _addr(bias),
               pool.data_ptr(), _addr(slots), _addr(to_slots), out.data_ptr(), x.stride(0) if N > 1 else 0, N, n, pool.shape[0], C, W,

@@ -94,3 +94,15 @@ def test_gradients_take_nothing_from_behind_a_rows_end(gpu_lib, C, dtype):
         assert (got["x"][b, n:] == 0).all()
         assert torch.equal(got["x"][b, max(n - 3, 0):n], plain["x"][b, max(n - 3, 0):n])
         assert not torch.isfinite(got["x"][b, :max(n - 3, 0)]).any()
+
+
+def test_pool_without_slots(gpu_lib):
+    """All rows are empty ones: y = 0 for their tokens, and what lies behind the last row's stays."""
+    x, w = torch.randn(6, 8, device=DEV), torch.randn(8, 4, device=DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    pool, slots = torch.zeros(0, 3, 8, device=DEV), i32([0, -1, 5])
+    for to in (None, i32([0, 0, 1])):
+        out = torch.full((6, 8), 7.0, device=DEV)
+        y = conv.causal_conv_packed(x, i32([0, 2, 2, 4]), pool, w, slots=slots, to_slots=to, out=out)
+        assert y is out and (out[:4] == 0).all() and (out[4:] == 7).all()
+        assert (conv.causal_conv_step(x[:3], pool, w, slots=slots, to_slots=to) == 0).all()
