@@ -1526,9 +1526,9 @@ static int check_chunk(ChunkAttnArgs& a, int N, int n, int width, int page, int 
   return GDNX_OK;
 }
 
-// Floats of the long rows' parts, then of the short rows' spans.
+// Floats of the long rows' parts (rounded up to 16 bytes, in units of which both are read), then of the short rows' spans.
 static long long chunk_part_floats(const ChunkAttnArgs& a) {
-  return a.parts > 1 ? (long long)a.parts * a.N * a.Hq * (a.D + 2) : 0;
+  return a.parts > 1 ? ((long long)a.parts * a.N * a.Hq * (a.D + 2) + 3) / 4 * 4 : 0;
 }
 static long long chunk_span_floats(const ChunkAttnArgs& a) {
   return a.spans > 1 ? (long long)a.n * a.Hkv * kChunkShort * a.spans * (a.D + 2) : 0;

@@ -32,3 +32,12 @@ def test_what_is_not_finite_reaches_those_that_see_it(gpu_lib, past, counts, wha
         hit[:counts[0]][sees, 2:, columns] = True
         assert torch.equal(~torch.isfinite(y), hit), (window, back)
         close(torch.where(hit, plain, y), plain.double().cpu(), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Hq", [1, 3])
+def test_odd_parts_before_spans(gpu_lib, Hq, dtype):
+    """An odd number of tokens, heads and parts of long rows, beside short rows in several spans."""
+    for past in (800, 1100):
+        b = Batch([past, past - 30, past - 7], [41, 1, 1], Hq, Hq, 64, 16, dtype)
+        close(b.run(), b.want(), dtype)

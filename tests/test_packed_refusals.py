@@ -131,3 +131,14 @@ def test_python_refuses():
         pages.pages_reserve_packed(i[None], i, i, i, i, 16, i[:2], 4)
     with pytest.raises(ValueError, match="k_pages and v_pages"):
         pages.pages_write_packed(q, q, q, q, i)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_chunk_workspace_is_whole_units_of_16_bytes(dt):
+    """Parts of long rows lie before spans of short ones, which are read 16 bytes at a time."""
+    size = _lib.load().gdnx_chunk_attn_workspace_bytes
+    for N in (43, 45, 129, 2049):
+        for n in (1, 2, 3):
+            for width in (40, 50, 63, 200):
+                for Hq in (1, 3):
+                    assert size(N, n, width, 16, Hq, Hq, 64, 0, 0, dt) % 16 == 0
