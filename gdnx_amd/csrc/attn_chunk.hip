@@ -301,12 +301,11 @@ template <typename CT, int D> __global__ void __launch_bounds__(256) chunk_join_
 void chunk_attn_plan(ChunkAttnArgs& a) {
   const long long G = a.Hq / a.Hkv, R = a.dtype == GDNX_DTYPE_BF16 ? 128 : 64, pairs = a.N * G;
   long long keys = (long long)a.width << a.page_log;
-  // a single row goes the long way whatever it holds; rows are all short if all tokens make but one short row
-  const int short_pairs = chunk_short_pairs(a.dtype == GDNX_DTYPE_BF16 ? 2 : 4);
-  a.short_rows = a.n == 1 && pairs > short_pairs ? 0 : short_pairs;
+  // A single row too may hold fewer tokens than the batch has places: one on 30001 cached takes 22 us alone and 23 in a batch
+  // of 2048 (515 where a single row went the long way whatever it held).  Rows are all short if all tokens make but one short row.
+  const int short_pairs = a.short_rows = chunk_short_pairs(a.dtype == GDNX_DTYPE_BF16 ? 2 : 4);
   a.items = 0;
   a.parts = a.least = 1;
-  a.spans = 0;
   if (pairs > a.short_rows) {
     const long long win = (long long)a.window + a.sinks + R / G + 1, span = win < keys ? win : keys;
     const long long most = pairs / (a.short_rows + 1), rows = a.n < most ? a.n : most;      // long rows there can be
@@ -319,14 +318,12 @@ void chunk_attn_plan(ChunkAttnArgs& a) {
     a.parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
     a.join_split = (long long)a.items * a.Hkv >= 256 ? 4 : (int)(R * a.D / 1024);      // workgroups an item
   }
-  if (a.short_rows) {
-    const long long win = (long long)a.window + a.sinks + kChunkShort;
-    a.spans = paged_attn_spans(a.n, a.Hkv, a.Hkv, win < keys ? win : keys, a.dtype);
-    const int groups = 1024 / a.D;                       // of a join's workgroup
-    a.join_share = 1;
-    while (a.join_share < groups && 4 * a.join_share < a.spans) a.join_share *= 2;
-    a.join_blocks = (long long)a.n * a.Hkv >= 512 ? 1 : (short_pairs + groups / a.join_share - 1) / (groups / a.join_share);
-  }
+  const long long win = (long long)a.window + a.sinks + kChunkShort;
+  a.spans = paged_attn_spans(a.n, a.Hkv, a.Hkv, win < keys ? win : keys, a.dtype);
+  const int groups = 1024 / a.D;                       // of a join's workgroup
+  a.join_share = 1;
+  while (a.join_share < groups && 4 * a.join_share < a.spans) a.join_share *= 2;
+  a.join_blocks = (long long)a.n * a.Hkv >= 512 ? 1 : (short_pairs + groups / a.join_share - 1) / (groups / a.join_share);
 }
 
 template <typename CT, int D> static int join(const ChunkAttnArgs& a, hipStream_t stream) {

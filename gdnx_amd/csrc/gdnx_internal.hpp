@@ -539,7 +539,7 @@ struct ChunkAttnArgs {
   int short_rows;       // rows of at most so many (token, head of the group) pairs go the short way
   int items, parts;     // long rows: work items a key head, most parts of their keys,
   int least;            // of so many tiles at least
-  int spans;            // short rows: most spans of their keys (0: no row can be short)
+  int spans;            // short rows: most spans of their keys
   int join_split;       // long rows' join: workgroups an item
   int join_share, join_blocks;      // short rows' join: groups of threads a pair, workgroups a row and key head
 };

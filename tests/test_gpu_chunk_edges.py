@@ -41,3 +41,19 @@ def test_odd_parts_before_spans(gpu_lib, Hq, dtype):
     for past in (800, 1100):
         b = Batch([past, past - 30, past - 7], [41, 1, 1], Hq, Hq, 64, 16, dtype)
         close(b.run(), b.want(), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (300, 5)])
+@pytest.mark.parametrize("past,count", [(1500, 1), (0, 1), (2000, 4), (40, 3)])
+def test_a_short_row_in_a_batch_of_a_fixed_size(gpu_lib, past, count, window, sinks, dtype):
+    """Alone or before tokens of nobody it is the same row, served the same way: equal bit for bit."""
+    b = Batch([past], [count], 4, 2, 64, 16, dtype)
+    alone = b.run(window=window, sinks=sinks)
+    close(alone, b.want(window=window, sinks=sinks), dtype)
+    for N in (17, 300, 2048):
+        q = torch.full((N, 4, 64), float("nan"), device=DEV).to(dtype)
+        q[:count] = b.q.to(DEV)
+        out = torch.full((N, 4, 64), 5.0, device=DEV).to(dtype)
+        y = b.run(q, window=window, sinks=sinks, out=out)
+        assert torch.equal(y[:count], alone) and (y[count:] == 5).all(), N
