@@ -110,7 +110,7 @@ class GdnxError(RuntimeError):
 
 
 class GdnxNonFinite(GdnxError):
-    """A recurrence's outputs held NaN or infinity (GDNX_ERR_NONFINITE, only
+    """A call's outputs held NaN or infinity (GDNX_ERR_NONFINITE, only
     with set_check_finite(True)): the counterpart of the reference trainer's
     guard that drops such a step (train/train_gdn3_distill.py:329-354)."""
 
@@ -150,9 +150,9 @@ def check(rc: int, what: str) -> None:
 
 def set_check_finite(on: bool) -> bool:
     """Turn the library's non-finite checking on or off (process-wide;
-    gdnx_set_check_finite).  When on, every recurrence call scans its outputs
-    and synchronises its stream, raising GdnxNonFinite on NaN or infinity.
-    Returns the previous setting."""
+    gdnx_set_check_finite).  When on, every recurrence, attention and convolution
+    call scans its outputs and synchronises its stream, raising GdnxNonFinite on
+    NaN or infinity.  Returns the previous setting."""
     return bool(load().gdnx_set_check_finite(1 if on else 0))
 
 

@@ -5,7 +5,7 @@
 // train/train_gdn3_distill.py:329-354).  The ABI's entry points are
 // asynchronous, so detecting a NaN or an infinity in their outputs needs a
 // device-side scan and a host read.  That is opt-in: with
-// gdnx_set_check_finite(1) the recurrence entry points scan what they wrote,
+// gdnx_set_check_finite(1) the entry points that compute scan what they wrote,
 // synchronise their stream and return GDNX_ERR_NONFINITE when any value is
 // NaN or infinite; gdnx_check_finite scans one buffer on demand.  Off (the
 // default), nothing is added to the launch sequence.
@@ -51,11 +51,17 @@ __device__ __forceinline__ bool finite_of<double>(double x) {
   return isfinite(x);
 }
 
-// any non-finite element of x[0, n) sets *flag
+// any non-finite element of x[0, n) sets *flag; offsets given: of its packed rows' tokens, `run` elements each
 template <typename T>
-__global__ void __launch_bounds__(256) finite_scan_kernel(const T* __restrict__ x, long long n, unsigned* flag) {
+__global__ void __launch_bounds__(256) finite_scan_kernel(const T* __restrict__ x, long long n, const int* offsets, int rows,
+                                                          long long run, unsigned* flag) {
   bool bad = false;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256)
+  long long first = 0;
+  if (offsets) {
+    first = max(offsets[0], 0) * run;
+    n = min(n, max(offsets[rows], 0) * run);
+  }
+  for (long long i = first + (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256)
     bad |= !finite_of(x[i]);
   if (bad) flag[0] = 1u;
 }
@@ -122,13 +128,12 @@ static int finite_check_word(const FiniteBuf* bufs, int nbuf, hipStream_t stream
     if (!b.p || b.n == 0) continue;
     const long long nb = ((long long)b.n + 255) / 256;
     const dim3 grid((unsigned)(nb < 4096 ? nb : 4096));
-    if (b.dtype == GDNX_DTYPE_BF16)
-      hipLaunchKernelGGL(finite_scan_kernel<bf16>, grid, dim3(256), 0, stream, (const bf16*)b.p, (long long)b.n, flag);
-    else if (b.dtype == GDNX_DTYPE_F64)
-      hipLaunchKernelGGL(finite_scan_kernel<double>, grid, dim3(256), 0, stream, (const double*)b.p, (long long)b.n,
-                         flag);
-    else
-      hipLaunchKernelGGL(finite_scan_kernel<float>, grid, dim3(256), 0, stream, (const float*)b.p, (long long)b.n, flag);
+    const auto scan = [&](auto kernel, auto* x) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, (long long)b.n, b.offsets, b.rows, (long long)b.run, flag);
+    };
+    if (b.dtype == GDNX_DTYPE_BF16) scan(finite_scan_kernel<bf16>, (const bf16*)b.p);
+    else if (b.dtype == GDNX_DTYPE_F64) scan(finite_scan_kernel<double>, (const double*)b.p);
+    else scan(finite_scan_kernel<float>, (const float*)b.p);
     if ((rc = check_launch("finite_scan_kernel"))) return rc;
   }
   unsigned host = 0;

@@ -1566,7 +1566,9 @@ extern "C" int gdnx_chunk_attn(const void* q, const void* k_pages, const void* v
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.table = table; a.lengths = lengths; a.offsets = offsets;
   a.slots = slots; a.y = y; a.part = (float*)workspace; a.span_part = (float*)workspace + parts;
   a.qs[0] = q_t; a.qs[1] = q_h; a.rows = rows; a.n_pages = n_pages; a.scale = scale;
-  return chunk_attn_dispatch(a, (hipStream_t)stream);
+  if ((rc = chunk_attn_dispatch(a, (hipStream_t)stream))) return rc;
+  const FiniteBuf outs[] = {{y, (size_t)N * Hq * head_dim, dtype, offsets, n, (size_t)Hq * head_dim}};
+  return finite_outputs(outs, 1, (hipStream_t)stream);
 }
 
 // ---- short causal convolution ----
@@ -1605,8 +1607,8 @@ extern "C" int gdnx_conv_fwd(const void* x, const void* weight, const void* bias
   a.x = x; a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.y = y; a.state_out = state_out;
   a.xs[0] = x_b; a.xs[1] = x_t; a.B = B; a.T = T; a.C = C; a.W = W; a.silu = silu != 0; a.wdtype = wdtype; a.dtype = dtype;
   if ((rc = conv_dispatch(a, false, (hipStream_t)stream))) return rc;
-  const FiniteBuf outs[] = {{y, (size_t)B * T * C, dtype}};
-  return finite_outputs(outs, 1, (hipStream_t)stream);
+  const FiniteBuf outs[] = {{y, (size_t)B * T * C, dtype}, {state_out, state_out ? (size_t)B * (W - 1) * C : 0, dtype}};
+  return finite_outputs(outs, 2, (hipStream_t)stream);
 }
 
 extern "C" long long gdnx_conv_bwd_workspace_bytes(int B, int T, int C, int W, int dtype) {
@@ -1651,5 +1653,7 @@ extern "C" int gdnx_conv_packed(const void* x, const int* offsets, const void* w
   a.C = C; a.W = W; a.silu = silu != 0; a.wdtype = wdtype; a.dtype = dtype;
   p.offsets = offsets; p.slots = slots; p.to_slots = to_slots; p.N = N; p.n = n; p.n_slots = n_slots;
   if (conv_packed_groups(p) > kMaxGroups) return set_error(GDNX_ERR_SHAPE, "too many rows, tokens and channels in one call");
-  return conv_packed_dispatch(p, (hipStream_t)stream);
+  if ((rc = conv_packed_dispatch(p, (hipStream_t)stream))) return rc;
+  const FiniteBuf outs[] = {{y, (size_t)N * C, dtype, offsets, n, (size_t)C}};
+  return finite_outputs(outs, 1, (hipStream_t)stream);
 }

@@ -104,7 +104,10 @@ struct ChanBwdArgs {
 struct FiniteBuf {
   const void* p;
   size_t n;
-  int dtype;   // GDNX_DTYPE_*
+  int dtype;                    // GDNX_DTYPE_*
+  const int* offsets = nullptr; // packed rows (on the device): only tokens offsets[0] .. offsets[rows] - 1 are looked at,
+  int rows = 0;
+  size_t run = 0;               // of so many elements each
 };
 bool check_finite_on();
 int finite_check(const FiniteBuf* bufs, int nbuf, hipStream_t stream);

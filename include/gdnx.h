@@ -43,14 +43,16 @@ const char* gdnx_last_error(void);
 /* Non-finite checking, the counterpart of the reference trainer's NaN/inf
  * guard (train/train_gdn3_distill.py:329-354), which drops a step whose loss
  * or gradient norm is not finite.  Off by default.  When on (process-wide),
- * the recurrence entry points (delta, per-channel, GDN3 and RLS forwards and
- * backwards, the decode steps) scan the outputs they wrote, synchronise their
- * stream and return GDNX_ERR_NONFINITE if any is NaN or infinite.  Returns
- * the previous setting.  Limits while on: each checked call holds one of 64
- * per-device flag words until its stream has synchronised (a 65th concurrent
- * checked call on a device returns GDNX_ERR_HIP), and a checked call on a
- * stream under HIP graph capture returns GDNX_ERR_ARG (the check reads the
- * flag back and synchronises, which capture forbids). */
+ * the entry points that compute (delta, per-channel, GDN3 and RLS forwards and
+ * backwards, the decode steps, attention, the short convolution) scan the
+ * outputs they wrote (packed rows': the tokens offsets[0] .. offsets[n] - 1;
+ * no state pool), synchronise their stream and return GDNX_ERR_NONFINITE if
+ * any is NaN or infinite.  Returns the previous setting.  Limits while on:
+ * each checked call holds one of 64 per-device flag words until its stream has
+ * synchronised (a 65th concurrent checked call on a device returns
+ * GDNX_ERR_HIP), and a checked call on a stream under HIP graph capture returns
+ * GDNX_ERR_ARG (the check reads the flag back and synchronises, which capture
+ * forbids). */
 int gdnx_set_check_finite(int on);
 
 /* Scans x[0, n) (GDNX_DTYPE_F32, _BF16 or _F64) on the stream and waits for

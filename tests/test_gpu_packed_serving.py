@@ -94,3 +94,52 @@ def test_calls_on_two_streams_at_once(gpu_lib):
     for i in range(2):
         for turn in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(turn, want[i]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_outputs_that_are_not_finite_are_reported(gpu_lib, dtype):
+    """With checking on: what the calls wrote, and not what lies behind the last row's tokens."""
+    from gdnx_amd import _lib
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    r = lambda *s: torch.randn(*s, device="cuda").to(dtype)  # noqa: E731
+    nan = float("nan")
+    kp, vp, table, lens = r(8, 1, 16, 64), r(8, 1, 16, 64), i32([[0, 1, 2, 3], [4, 5, 6, 7]]), i32([40, 60])
+    w, x = torch.randn(12, 4, device="cuda"), r(2, 9, 12)
+    def chunk(counts, v, spare):                         # `spare` tokens of nobody before and behind the rows'
+        N, end = sum(counts) + 2 * spare, sum(counts) + spare
+        q = torch.full((N, 2, 64), nan, device="cuda").to(dtype)
+        q[spare:end] = r(sum(counts), 2, 64)
+        return attention.paged_attention_chunk(q, kp, v, table, lens, i32([spare, spare + counts[0], end]),
+                                               out=torch.full_like(q, nan))
+    def packed(x, spare, pool):
+        none = torch.full((spare, 12), nan, device="cuda").to(dtype)
+        x = torch.cat([none, x, none])
+        return conv.causal_conv_packed(x, i32([spare, spare + 4, spare + 9]), pool, w, out=torch.full_like(x, nan))
+    bad_v, bad_x, bad_state = vp.clone(), x.clone(), torch.zeros(2, 3, 12, device="cuda").to(dtype)
+    bad_v[6, 0, 11, 3] = nan                             # position 43 of the second row
+    bad_x[0, 3, 5] = float("inf")
+    bad_state[1, 2, 4] = nan
+    pool = lambda: torch.zeros(2, 3, 12, device="cuda").to(dtype)  # noqa: E731
+    prev = _lib.set_check_finite(True)
+    try:
+        for counts in ([1, 1], [3, 20], [40, 30], [0, 5]):
+            for spare in (0, 7):
+                chunk(counts, vp, spare)
+                with pytest.raises(_lib.GdnxNonFinite):
+                    chunk(counts, bad_v, spare)
+        for spare in (0, 7):
+            packed(x[0], spare, pool())
+            with pytest.raises(_lib.GdnxNonFinite):
+                packed(bad_x[0], spare, pool())
+        conv.causal_conv_step(x[:, 0], pool(), w)
+        with pytest.raises(_lib.GdnxNonFinite):
+            conv.causal_conv_step(bad_x[:, 3], pool(), w)
+        lengths = i32([9, 0])                            # a row without tokens hands its state on
+        conv.causal_conv(x, w, state=pool(), lengths=lengths, return_state=True)
+        conv.causal_conv(x, w, state=bad_state, lengths=lengths)
+        with pytest.raises(_lib.GdnxNonFinite):
+            conv.causal_conv(x, w, state=bad_state, lengths=lengths, return_state=True)
+    finally:
+        _lib.set_check_finite(prev)
+    chunk([1, 1], bad_v, 0)                              # off: no word of it
+    torch.cuda.synchronize()
