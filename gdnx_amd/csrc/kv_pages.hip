@@ -4,6 +4,7 @@
 // that none of it waits for the host and all of it can be captured.
 //
 //   reserve  a row of length n gets the pages of tokens n .. n + n_new - 1
+//            (for pages that its entries still name, those are given back)
 //   fork     a child row shares its parent's full pages (a reference more)
 //            and gets a copy of the started one
 //   free     a row's references are given back (trim: those of the pages that
@@ -164,6 +165,15 @@ __device__ __forceinline__ int row_length(const PagesArgs& a, int r) {
   return len >= 0 && len <= (long long)a.width * a.page ? len : -1;
 }
 
+// A taken page into a row's entry.  Where the caller has lowered the row's
+// length the entry may still name the page that it had: that one is given back.
+__device__ __forceinline__ void put_page(int* entry, int pg, int* refs, int n_pages) {
+  const int old = *entry;
+  *entry = pg;
+  refs[pg] = 1;
+  if (old >= 0 && old < n_pages) atomicSub(&refs[old], 1);
+}
+
 }  // namespace
 
 // ws: [n] first page of each row in the list, then [n_pages] free pages
@@ -210,11 +220,7 @@ __global__ void __launch_bounds__(PT) pages_reserve_kernel(PagesArgs a, int* ws)
     }
     const int have = (len + a.page - 1) / a.page;
     const int cnt = (int)(((long long)len + a.n_new + a.page - 1) / a.page) - have, at = offs[s];
-    for (int c = lane; c < cnt; c += 64) {
-      const int pg = list[at + c];
-      a.table[(size_t)r * a.width + have + c] = pg;
-      a.refs[pg] = 1;
-    }
+    for (int c = lane; c < cnt; c += 64) put_page(&a.table[(size_t)r * a.width + have + c], list[at + c], a.refs, a.n_pages);
     if (lane == 0) {
       a.start[s] = len;
       a.lengths[r] = len + a.n_new;
@@ -256,8 +262,7 @@ __global__ void __launch_bounds__(PT) pages_fork_kernel(PagesArgs a, int* ws) {
     const int len = lens[s];
     if (len <= 0 || len % a.page == 0) continue;
     const int pg = list[offs[s]], full = len / a.page, from = a.table[(size_t)a.slots[s] * a.width + full];
-    a.table[(size_t)a.start[s] * a.width + full] = pg;
-    a.refs[pg] = 1;
+    put_page(&a.table[(size_t)a.start[s] * a.width + full], pg, a.refs, a.n_pages);
     src[s] = from;
     if (from >= 0 && from < a.n_pages) dst[s] = pg;
   }
@@ -312,9 +317,10 @@ __global__ void __launch_bounds__(256) pages_share_kernel(PagesArgs a, const int
   const int* tp = a.table + (size_t)a.slots[s] * a.width;
   int* tc = a.table + (size_t)child * a.width;
   for (int i = threadIdx.x; i < full; i += 256) {
-    const int pg = tp[i];
+    const int pg = tp[i], old = tc[i];
     tc[i] = pg;
     if (pg >= 0 && pg < a.n_pages) atomicAdd(&a.refs[pg], 1);
+    if (old >= 0 && old < a.n_pages) atomicSub(&a.refs[old], 1);      // (put_page)
   }
   if (threadIdx.x == 0) a.lengths[child] = len;
 }
@@ -501,9 +507,8 @@ __global__ void __launch_bounds__(256) pages_place_kernel(PagesPackedArgs a, con
   if (base < taken) {
     const int s = row_of(offs);
     if (u < taken) {
-      const int r = a.slots[s], pg = list[u];
-      a.table[(size_t)r * a.width + ((a.start[s] + mask) >> lg) + u - offs[s]] = pg;
-      a.refs[pg] = 1;
+      const int col = ((a.start[s] + mask) >> lg) + u - offs[s];
+      put_page(&a.table[(size_t)a.slots[s] * a.width + col], list[u], a.refs, a.n_pages);
     }
   }
   if (base >= a.N) return;

@@ -5,7 +5,10 @@ values; a table [rows, width] says which pages hold a row's tokens (one table
 for all layers), ``lengths`` how many there are, ``refs`` how many rows use a
 page (0: free).  All of it is on the device, and so is the bookkeeping
 (csrc/kv_pages.hip): nothing here waits for the host, and pages are taken
-lowest index first, so results do not depend on timing.
+lowest index first, so results do not depend on timing.  Tokens are taken back by
+lowering a row's length, not below what it shares with a fork: the pages behind
+it stay the row's until it is freed, or until a reserve that comes to their
+entries gives them back for the ones that it takes.
 
 The functions work on the tensors; ``PagedKVCache`` keeps them together with
 the rows' lengths on the host, and raises before a call that cannot be served.
@@ -221,7 +224,8 @@ class PagedKVCache:
     the int32 tensor that ``rows_tensor`` made of them, so that a step's calls
     share one upload; neither waits for the device (another tensor is read
     back).  A graph captures the functions above on the cache's tensors: the
-    lengths that the cache keeps on the host do not advance with a replay."""
+    lengths that the cache keeps on the host do not advance with a replay.  Lengths
+    are not lowered here: tokens that may have to go again are tried on a fork."""
 
     def __init__(self, n_pages: int, page: int, Hkv: int, D: int, rows: int, max_len: int, layers: int = 1,
                  dtype=torch.bfloat16, device="cuda"):

@@ -677,6 +677,11 @@ int gdnx_paged_attn_step(const void* q, const void* k, const void* v, void* k_pa
  * call (free and trim: it may).  status [2] int32 is written only by a
  * reserve or fork that could not be served and then changed nothing else:
  * the pages that were missing, and the rows whose table row is too short.
+ * An entry in [0, n_pages) is a reference, also behind its row's length: the
+ * caller may lower a length to take tokens back (not below what the row shares
+ * with a fork, whose pages would be written), and the pages behind it stay the
+ * row's until it is freed or a reserve or fork comes to their entries, which
+ * takes free pages for them and gives the old ones back.
  * workspace: gdnx_pages_workspace_bytes(n, n_pages). */
 long long gdnx_pages_workspace_bytes(int n, int n_pages);
 
