@@ -36,6 +36,7 @@ import torch
 
 from . import conv as _conv
 from . import gdn3, ops
+from .ops import tensor_version, upload_ints
 
 KINDS = ("dense", "chan", "gdn3")
 
@@ -113,17 +114,36 @@ class DecodeStateCache:
             return self.A[slot], self.B[slot], self.U[slot], self.Vb[slot]
         return self.pool[slot]
 
-    def _slot_tensor(self, slots):
-        """The slots as an int32 device tensor, after checking on the host that
-        no live slot is named twice (two rows advancing one state would race in
-        the kernels).  A tensor is read back for the check (one sync)."""
-        host = [int(s) for s in (slots.tolist() if isinstance(slots, torch.Tensor) else slots)]
+    def _named(self, slots):
+        """The slots as ints and as an int32 device tensor, after checking on the
+        host that no live slot is named twice (two rows advancing one state would
+        race in the kernels).  Ints are uploaded without a wait; a tensor that
+        slots_tensor did not make, or that was written since, is read back."""
+        tensor = isinstance(slots, torch.Tensor)
+        made = getattr(slots, "named_slots", None)
+        host = made[0] if made and made[1] == tensor_version(slots) else slots.tolist() if tensor else slots
+        host = [int(s) for s in host]
         live = [s for s in host if 0 <= s < self.n_slots]
         if len(set(live)) != len(live):
             raise ValueError(f"slots {host} name a slot twice (rows sharing a slot would race)")
+        if tensor:
+            return host, slots.to(device=self.device, dtype=torch.int32).contiguous()
+        return host, upload_ints(host, self.device, "slots named as ints cannot be captured: name them by a tensor that "
+                                 "slots_tensor made before")
+
+    def _slot_tensor(self, slots):
+        return self._named(slots)[1]
+
+    def slots_tensor(self, slots):
+        """The slots (ints; -1: an empty row) as an int32 device tensor for ``step``
+        and ``convolve``: calls that name it share one upload, do not wait for the
+        device and can be captured (of the gdn3 kind ``convolve`` alone: the
+        positions of a step are on the host)."""
         if isinstance(slots, torch.Tensor):
-            return slots.to(device=self.device, dtype=torch.int32).contiguous()
-        return torch.as_tensor(host, dtype=torch.int32, device=self.device)
+            return slots
+        host, t = self._named(slots)
+        t.named_slots = host, tensor_version(t)
+        return t
 
     # ---- compute ----
     def prefill(self, slots, q, k, v, a_e, a_w, log_g):
@@ -178,11 +198,10 @@ class DecodeStateCache:
         chan: the same with log_g [NS,H,M,D] (M = 1).  gdn3: q, k, v
         [NS,H,(M,)D], a_e = b_gates, a_w = w_gates ([NS,H,M] or [NS,H,M,D]),
         log_g = the multiplicative decay [NS,H,M].  Returns y [NS,H,M,D]."""
-        st = self._slot_tensor(slots)
+        host, st = self._named(slots)
         if self.kind == "gdn3":
-            host = st.tolist() if isinstance(slots, torch.Tensor) else [int(s) for s in slots]
-            pos = torch.tensor([self.pos[s] if 0 <= s < self.n_slots else 0 for s in host], dtype=torch.int32,
-                               device=self.device)
+            pos = upload_ints([self.pos[s] if 0 <= s < self.n_slots else 0 for s in host], self.device,
+                              "a gdn3 step cannot be captured: the slots' positions are on the host")
             with torch.no_grad():
                 y = gdn3.gdn3_decode_step(q, k, v, a_e, a_w, log_g, (self.A, self.B, self.U, self.Vb), pos,
                                           R=self.R, P=self.P, factors=self.factors, slow_decay=self.slow_decay,
@@ -204,7 +223,8 @@ class DecodeStateCache:
         """The short convolution (``conv.causal_conv_packed``) of the rows' next
         tokens, continuing and advancing the inputs that the slots hold (-1: an
         empty row, y = 0): x [n,C] one token a row, [n,T,C] T of each, or with
-        offsets (int32 [n+1], on the device) packed rows [N,C].  Returns y in x's shape."""
+        offsets (int32 [n+1], on the device) packed rows [N,C].  Returns y in x's
+        shape.  It does not wait for the device (slots a tensor: ``slots_tensor``)."""
         if self.conv_pool is None:
             raise ValueError("the cache was made without a convolution (conv=(channels, taps))")
         st, n = self._slot_tensor(slots), len(slots)

@@ -29,6 +29,22 @@ def empty_result(shape, dtype, device, *srcs):
     return z
 
 
+def upload_ints(xs, device, captured):
+    """A list as an int32 tensor on ``device``, by way of pinned memory (which torch
+    keeps until the copy is done), so that nothing waits.  A captured copy would be
+    of memory that is used again: it raises ``captured``."""
+    if device.type != "cuda" or not xs:
+        return torch.tensor(xs, dtype=torch.int32, device=device)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(captured)
+    return torch.tensor(xs, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
+
+
+def tensor_version(t):
+    """Changes when t is written (inference tensors count no changes: None)."""
+    return None if t.is_inference() else t._version
+
+
 def _check_dense(q, k, v, a_e, a_w, log_g):
     _need(q.is_cuda, "gdnx ops need CUDA (HIP) tensors")
     _need(q.dim() == 4 and q.shape == k.shape == v.shape, "q, k, v must share shape [B,T,H,D]")

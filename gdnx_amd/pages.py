@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, attention
-from .ops import _need
+from .ops import _need, tensor_version, upload_ints
 
 
 def _ints(*ts):
@@ -215,10 +215,6 @@ def pages_compact(k_pages, v_pages, table, refs, out=None):
     return t_out, r_out
 
 
-def _version(t):
-    return None if t.is_inference() else t._version      # (inference tensors count no changes)
-
-
 class PagedKVCache:
     """A page pool with its table.  Rows are named by the caller as ints, or as
     the int32 tensor that ``rows_tensor`` made of them, so that a step's calls
@@ -255,7 +251,7 @@ class PagedKVCache:
     def _check_rows(self, rows):
         if isinstance(rows, torch.Tensor):
             made = getattr(rows, "named_rows", None)
-            rows = made[0] if made and made[1] == _version(rows) else rows.tolist()
+            rows = made[0] if made and made[1] == tensor_version(rows) else rows.tolist()
         rows = [int(r) for r in rows]
         free = set(self._free_rows)
         if len(set(rows)) != len(rows):
@@ -266,13 +262,8 @@ class PagedKVCache:
         return rows
 
     def _upload(self, xs):
-        """A list as an int32 device tensor, by way of pinned memory (which torch
-        keeps until the copy is done), so that nothing waits."""
-        if self.device.type != "cuda" or not xs:
-            return torch.tensor(xs, dtype=torch.int32, device=self.device)
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("rows named as ints cannot be captured: name them by a tensor that rows_tensor made before")
-        return torch.tensor(xs, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
+        return upload_ints(xs, self.device,
+                           "rows named as ints cannot be captured: name them by a tensor that rows_tensor made before")
 
     def _named(self, rows):
         """The rows, checked, as a list and as a device tensor."""
@@ -287,7 +278,7 @@ class PagedKVCache:
         if isinstance(rows, torch.Tensor):
             return rows
         host, t = self._named(rows)
-        t.named_rows = host, _version(t)
+        t.named_rows = host, tensor_version(t)
         return t
 
     def free(self, rows) -> None:

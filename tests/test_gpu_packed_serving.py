@@ -143,3 +143,82 @@ def test_outputs_that_are_not_finite_are_reported(gpu_lib, dtype):
         _lib.set_check_finite(prev)
     chunk([1, 1], bad_v, 0)                              # off: no word of it
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("kind,M", [("dense", 2), ("chan", 1), ("gdn3", 2)])
+def test_a_served_step_does_not_wait_for_the_device(gpu_lib, kind, M, mode):
+    n, H, D, C = 3, 2, 64, 40
+    with mode():
+        z = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+        cache = DecodeStateCache(4, H, M, D, kind=kind, conv=(C, 4), P=16)
+        x, w, off = z(n, C, t=torch.bfloat16), z(C, 4), z(n + 1, t=torch.int32)
+        io = torch.float32 if kind == "chan" else torch.bfloat16
+        qkv, gates = [z(n, H, D, t=io) for _ in range(3)], [z(n, H, M) for _ in range(2)]
+        decay = z(n, H, M, D) if kind == "chan" else z(n, H, M)
+        slots = [2, 0, -1]
+        torch.cuda.set_sync_debug_mode("error")              # (a cache may wait while it is made)
+        try:
+            for named in (slots, tuple(slots), cache.slots_tensor(slots), cache.slots_tensor(slots)):
+                cache.convolve(named, x, w)
+                cache.convolve(named, x[:, None].expand(n, 5, C), w)
+                cache.convolve(named, x, w, offsets=off)
+                cache.step(named, *qkv, *gates, decay)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        if kind == "gdn3":
+            assert cache.pos == [4, 0, 4, 0]
+
+
+def test_slots_by_any_tensor(gpu_lib):
+    cache = DecodeStateCache(4, 1, 1, 64, conv=(8, 4))
+    x, w = torch.randn(2, 8, device="cuda").bfloat16(), torch.randn(8, 4, device="cuda")
+    st = cache.slots_tensor([2, 1])
+    assert st.tolist() == [2, 1] and st.dtype == torch.int32 and cache.slots_tensor(st) is st
+    a = cache.convolve(st, x, w)
+    cache.conv_pool.zero_()
+    for named in (torch.tensor([2, 1]), torch.tensor([2, 1], device="cuda"), st.repeat_interleave(2)[::2]):
+        assert torch.equal(cache.convolve(named, x, w), a)          # read back, and taken in 64 bits too
+        cache.conv_pool.zero_()
+    st[0] = 1                                                       # written since: what it was made of no longer holds
+    with pytest.raises(ValueError, match="twice"):
+        cache.convolve(st, x, w)
+    own = torch.tensor([0, 3], dtype=torch.int32, device="cuda")    # a caller's buffer is read at every call
+    with torch.inference_mode():
+        own = own.clone()
+        cache.convolve(own, x, w)
+        own[0] = 3
+        with pytest.raises(ValueError, match="twice"):
+            cache.convolve(own, x, w)
+
+
+@pytest.mark.parametrize("kind", ["dense", "gdn3"])
+def test_a_caches_convolution_is_captured(gpu_lib, kind):
+    """By the slots' tensor; ints, whose upload would be of memory that is used again, are refused before anything moves."""
+    n, C, W = 3, 24, 4
+    caches = [DecodeStateCache(5, 1, 1, 64, kind=kind, conv=(C, W)) for _ in range(2)]
+    st = [c.slots_tensor([4, 0, 2]) for c in caches]
+    x, w = torch.zeros(n, C, device="cuda").bfloat16(), torch.randn(C, W, device="cuda")
+    off = torch.tensor([0, 2, 2, 3], dtype=torch.int32, device="cuda")
+    step = lambda c, s: (c.convolve(s, x, w, offsets=off), c.convolve(s, x, w), c.convolve(s, x[:, None], w))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(DecodeStateCache(5, 1, 1, 64, kind=kind, conv=(C, W)), st[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[1], st[1])
+        with pytest.raises(RuntimeError, match="captured"):
+            caches[1].convolve([4, 0, 2], x, w)
+        if kind == "gdn3":
+            z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+            with pytest.raises(RuntimeError, match="captured"):
+                caches[1].step(st[1], z(n, 1, 64), z(n, 1, 64), z(n, 1, 64), z(n, 1, 1), z(n, 1, 1), z(n, 1, 1))
+    for turn in range(4):
+        x.copy_(torch.randn(n, C, device="cuda"))
+        graph.replay()
+        want = step(caches[0], st[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+        assert torch.equal(caches[0].conv_pool, caches[1].conv_pool)
