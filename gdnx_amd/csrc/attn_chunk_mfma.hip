@@ -11,8 +11,8 @@ namespace {
 // from the table): lane x holds the page of key j0 + x, or of the last one.  An
 // instruction fills `ROWS` tokens, which lie in one page where it has so many:
 // its place is then a scalar, 32-bit offsets are the lanes'.  (By lane
-// exchanges throughout, as SMALL pages need it, 2048 tokens on 30001 took 673 us;
-// 580 with scalar places, 555 with the matrix instructions' priority below.)
+// exchanges throughout, as SMALL pages need it, the kernel took 673 us for 2048
+// tokens on 30001 where scalar places took 580, in turn on one card.)
 template <int D, bool SMALL> struct PagedTileLoad {
   using T = Tile<D>;
   static constexpr int N = 64 * T::UPR / 256, STEP = 256 / T::UPR, ROWS = 64 / T::UPR;
@@ -45,6 +45,13 @@ template <int D, bool SMALL> struct PagedTileLoad {
 // form of win_fwd_bf16_kernel (attn_win_mfma.hip): S^T = K Q^T, a lane holding 32
 // scores of one row; O^T += V^T P^T.  The page of a tile's keys is looked up
 // two tiles ahead.
+//
+// P is rounded to bf16 for the second product, as there (its sum is of the values
+// before): y is 2.0e-3 to 2.3e-3 from 64 bits, of which 1.7e-3 are its own rounding.
+// A third product of what that rounding leaves over, which short rows have for
+// nothing (they wait for memory), takes the whole call from 537 to 716 us for 2048
+// tokens on 30001, 225 to 258 for three pieces beside 61 single tokens, and 107 to 134 for
+// 4096 tokens on none.
 template <int D, bool SMALL>
 __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64 * Tile<D>::RB], char (&v0)[64 * Tile<D>::RB],
                                            char (&k1)[64 * Tile<D>::RB], char (&v1)[64 * Tile<D>::RB]) {
@@ -111,8 +118,9 @@ __device__ __forceinline__ void chunk_long(const ChunkAttnArgs& a, char (&k0)[64
     const bool some = it < t1 && wv0 <= wv1 && j0 <= wv1 && (j0 + BK - 1 > wv0 - a.window || j0 < a.sinks);
     if (!some) return;
     // Matrix instructions go before the other wave's vector instructions, and a tile's exponentials are through before its
-    // second products, so that the two waves of a SIMD take turns: 2048 tokens on 30001 582 -> 555 us, 1024 on 8192
-    // 92 -> 90, 8192 on 8192 777 -> 774, 4096 on none 97 -> 102 (16/4 heads, d = 128).
+    // second products, so that the two waves of a SIMD take turns.  The kernel in us, in turn on one card (others take
+    // 540 to 576 for the first): 2048 tokens on 30001 582 -> 555, 1024 on 8192 92 -> 90, 8192 on 8192 777 -> 774, 4096 on
+    // none 97 -> 102 (16/4 heads, d = 128).
     __builtin_amdgcn_s_setprio(1);
     const bool all = rows_ok && j0 + BK - 1 <= wv0 && (wv1 - j0 < a.window || j0 + BK <= a.sinks) && there == ~0ULL;
     f32x16 s[2];

@@ -616,9 +616,9 @@ struct ConvArgs {
   const void* dy;
   const void* dstate_out;
   void* dx;
-  void* dweight;         // wdtype, or null
-  void* dbias;
-  void* dstate;
+  void* dweight;         // wdtype
+  void* dbias;           // wdtype, or null
+  void* dstate;          // or null
   float* part;           // [blocks][W + 1][C]
   long long xs[2];
   int B, T, C, W, silu, wdtype, dtype;
