@@ -57,3 +57,20 @@ def test_a_short_row_in_a_batch_of_a_fixed_size(gpu_lib, past, count, window, si
         out = torch.full((N, 4, 64), 5.0, device=DEV).to(dtype)
         y = b.run(q, window=window, sinks=sinks, out=out)
         assert torch.equal(y[:count], alone) and (y[count:] == 5).all(), N
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [3, 400])
+def test_a_batch_whose_first_tokens_are_nobodys(gpu_lib, n, dtype):
+    """Offsets may begin anywhere: long, short and empty rows behind 37 tokens that no row has."""
+    past, counts = [(11 * i) % 40 for i in range(n)], [(1, 0, 2)[i % 3] for i in range(n)]
+    counts[0], counts[n // 2] = 70, 19
+    b = Batch(past, counts, 4, 2, 64, 16, dtype)
+    want, N = b.want(window=30, sinks=2), b.q.shape[0]
+    b.offsets = [37 + o for o in b.offsets]
+    q = torch.full((37 + N + 5, 4, 64), float("nan"), device=DEV).to(dtype)
+    q[37:37 + N] = b.q.to(DEV)
+    out = torch.full_like(q, 5.0)
+    b.run(q, window=30, sinks=2, out=out)
+    assert (out[:37] == 5).all() and (out[37 + N:] == 5).all()
+    close(out[37:37 + N], want, dtype)

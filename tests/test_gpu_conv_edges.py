@@ -106,3 +106,18 @@ def test_pool_without_slots(gpu_lib):
         y = conv.causal_conv_packed(x, i32([0, 2, 2, 4]), pool, w, slots=slots, to_slots=to, out=out)
         assert y is out and (out[:4] == 0).all() and (out[4:] == 7).all()
         assert (conv.causal_conv_step(x[:3], pool, w, slots=slots, to_slots=to) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_batch_whose_first_tokens_are_nobodys(gpu_lib, dtype):
+    counts, C, lead = [5, 0, 1, 70, 9], 520, 37
+    n, N = len(counts), sum(counts)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    off = [sum(counts[:i]) for i in range(n + 1)]
+    x, w, pool = torch.randn(lead + N + 3, C, device=DEV).to(dtype), torch.randn(C, 4, device=DEV), torch.randn(n, 3, C, device=DEV)
+    p1, p2 = pool.to(dtype, copy=True), pool.to(dtype, copy=True)
+    want = conv.causal_conv_packed(x[lead:lead + N], i32(off), p1, w)
+    out = torch.full_like(x, 5.0)
+    conv.causal_conv_packed(x, i32([lead + o for o in off]), p2, w, out=out)
+    assert torch.equal(out[lead:lead + N], want) and torch.equal(p1, p2)
+    assert (out[:lead] == 5).all() and (out[lead + N:] == 5).all()
